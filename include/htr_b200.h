@@ -290,6 +290,53 @@ int htr_dec_swiglu(const void* gate_up, void* out, int rows, int intermediate, h
 int htr_dec_rope_attention(const void* qkv, const int64_t* pos, const float* cosv, const float* sinv, void* k_cache, void* v_cache,
                            void* out, int q_heads, int kv_heads, int head_dim, int capacity, int* status, htr_stream_t stream);
 
+/* Serving many sequences from a paged 8-bit cache (no counterpart in the reference, whose serving stack owns its caches).  A layer's
+ * cache is keys and values [pages][kv_heads][page_size][head_dim] in e4m3 with float32 scales [pages][kv_heads], powers of two (the
+ * value of an element is element * scale); page_size 16, 32, 64 or 128, head_dim 64 or 128.  A request's page j is table entry
+ * tables[request * table_stride + j]; slot = page * page_size + place in the page.  Indices live in device memory, so the kernels
+ * check them: what lies outside is neither read nor written and ORs a bit into *status (device int, may be NULL).
+ *
+ * htr_page_plan: one step's tables and slots from lengths[requests] (tokens in the cache) and added[requests] (tokens that the step adds;
+ * 0: none; negative: the request is over and its pages come back).  A request that grows gets the pages it lacks, in the order of the
+ * requests, first from those that came back in this step, then from the top of free_pages[0..*count).  Outputs: starts[requests + 1] (first
+ * token of a request in the step's token arrays), positions and slots[max_tokens] (-1: not written, and behind the last token), seen[requests] (tokens
+ * in the cache after the step of a request that adds some, else 0), lengths_out, *count_out; tables and free_pages are updated in place.
+ * lengths_out and count_out may be lengths and count.  A request that cannot be served keeps its length, its tokens get -1:
+ * status 1 (no pages left: it and later ones that need pages), 2 (its table is full), 4 (a length that is negative or beyond the
+ * table), 8 (more tokens than max_tokens: requests that begin or end beyond).  At most 8192 requests. */
+int htr_page_plan(const int* lengths, const int* added, int requests, int* tables, int64_t table_stride, int table_width, int* free_pages,
+                  int pages, const int* count, int page_size, int max_tokens, int* starts, int* positions, int* slots, int* seen,
+                  int* lengths_out, int* count_out, int* status, htr_stream_t stream);
+/* Rotary embedding (interleaved pairs, angles cosv / sinv[angle_rows][head_dim / 2]) of the q and k parts of qkv[tokens][(q_heads + 2 * kv_heads) *
+ * head_dim] (bf16 or fp16, rows row_stride elements apart, a multiple of 8); q -> q_out[tokens][q_heads][head_dim], k and v -> the cache at slots[token].
+ * A page's scale is the smallest power of two (2^-100 at least) under which all of its tokens lie within e4m3; it begins anew with the
+ * page's first place and grows with later ones, and then the older tokens are rescaled.  Infinities become the largest value, NaN
+ * stays.  Tokens of one page are neighbours and in order, as htr_page_plan lays them out.  A token with slot -1 is not written and its
+ * q row is zero; so is one whose slot or position lies outside (status 16). */
+int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* positions, const int* slots, int tokens, const float* cosv,
+                     const float* sinv, int angle_rows, int q_heads, int kv_heads, int head_dim, void* k_cache, void* v_cache,
+                     float* k_scale, float* v_scale, int pages, int page_size, void* q_out, int* status, htr_stream_t stream);
+/* out[t][head] = softmax(scale * q[t][head] . K) V over the cache, grouped-query and causal: of the tokens [starts[r], starts[r + 1]) of
+ * request r the i-th stands at position seen[r] - n + i (n of them) and sees the positions up to its own; a token that sees nothing gets
+ * zeros.  q and out [tokens][q_heads][head_dim], bf16 or fp16; rows behind starts[requests] are left as they are.  max_new: the largest
+ * n.  A table entry that is no page hides its tokens (status 32).  The workspace needs no preparation. */
+size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new);
+int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts, const int* seen, int requests, const int* tables,
+                        int64_t table_stride, int table_width, const void* k_cache, const void* v_cache, const float* k_scale,
+                        const float* v_scale, int pages, int page_size, int q_heads, int kv_heads, int head_dim, int max_new,
+                        float scale, void* out, int* status, void* workspace, size_t workspace_bytes, htr_stream_t stream);
+int htr_paged_last_cuda_error(void);
+
+/* One token per row of logits[rows][vocab] (rows row_stride elements apart, any of HTR_DTYPE_*; vocab <= 2^20) from a uniform number u[row] in
+ * [0, 1).  Tokens are ordered by logit, ties by index; w = exp((logit - largest) / temperature).  Kept is the shortest of: the first top_k
+ * (<= 0: all); the shortest beginning of those with at least top_p of their weight (>= 1: all); those with w >= min_p (<= 0: all); at
+ * least one token.  The token is the first, by index, at which the running weight of the kept exceeds u times their sum, and
+ * logprobs[row] (may be NULL) the logarithm of its share.  temperature <= 0: the largest logit's first index, 0.  A logit of -infinity
+ * or NaN is never chosen; a row without another gives -1 and NaN.  Settings are arrays of one value per row, or NULL: 1, all, all, all. */
+int htr_sample(const void* logits, int dtype, int64_t row_stride, int rows, int vocab, const float* u, const float* temperature,
+               const int* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs, htr_stream_t stream);
+int htr_sample_last_cuda_error(void);
+
 /* Encoder-side search: tail-biting Viterbi over the bit-shift trellis, one tile per row of x[B][T] with weights w[B][T]
  * (float32, T <= 256; the encoder uses T = 256).  Replaces htr/reference.py:7-50 (viterbi) and the CUDA module of
  * htr/vit_v2.py:28-73 (built there for sm_86 / sm_120 only), the callable behind the reference's encode.VITERBI hook

@@ -1,0 +1,522 @@
+"""Page plans, the paged 8-bit cache and attention over it, against plain evaluations in 64 bits and in lists."""
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+E4M3 = torch.float8_e4m3fn
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ---- plan_step ------------------------------------------------------------------------------------------------------
+
+
+def plan_by_hand(lengths, new, tables, free, count, page, T):
+    """The same step in lists; `tables` (rows of page lists, -1 where none) and `free` are changed."""
+    width, back, status = len(tables[0]), [], 0
+    for r, (n, a) in enumerate(zip(lengths, new)):
+        if a < 0 and 0 <= n <= width * page:
+            back += tables[r][:-(-n // page)]
+    supply = back + free[:count][::-1]
+    starts, positions, slots, seen, after, at, taken = [0], [], [], [], [], 0, 0
+    for r, (n, a) in enumerate(zip(lengths, new)):
+        ok = a > 0
+        if not 0 <= n <= width * page:
+            status, ok = status | 4, False
+        if at + max(a, 0) > T:
+            status, ok = status | 8, False
+        if ok and n + a > width * page:
+            status, ok = status | 2, False
+        need = -(-(n + a) // page) - -(-n // page) if ok else 0
+        if need:
+            if taken + need > len(supply):
+                status, ok = status | 1, False
+                taken = len(supply) + 1                      # later requests that need pages get none either
+            else:
+                tables[r][-(-n // page):-(-n // page) + need] = supply[taken:taken + need]
+                taken += need
+        for i in range(max(a, 0)):
+            if at + i < T:
+                p = n + i
+                positions.append(p if ok else -1)
+                slots.append(tables[r][p // page] * page + p % page if ok else -1)
+        at += max(a, 0)
+        starts.append(min(at, T))
+        seen.append(n + a if ok else 0)
+        after.append(0 if a < 0 else n + a if ok else n)
+    if taken > len(supply):                                  # what was served before pages ran out
+        taken = sum(-(-s // page) - -(-n // page) for s, n in zip(seen, lengths) if s)
+    left = back[taken:]
+    free[count:count + len(left)] = left
+    positions += [-1] * (T - len(positions))
+    slots += [-1] * (T - len(slots))
+    return starts, positions, slots, seen, after, count + len(back) - taken, status
+
+
+def check_plan(lengths, new, tables, free, count, page, T, pad=0):
+    from htr_b200 import paged
+
+    R, width = len(lengths), len(tables[0])
+    dev_tables = torch.full((R, width + pad), -7, dtype=torch.int32, device=DEV)[:, :width]
+    dev_tables.copy_(ints(tables))
+    dev_free, status = ints(free), ints([0])
+    plan = paged.plan_step(ints(lengths), ints(new), dev_tables, dev_free, ints([count]), page, T, status=status)
+    want = plan_by_hand(lengths, new, tables, free, count, page, T)
+    for name, w in zip(("starts", "positions", "slots", "seen", "lengths"), want):
+        assert getattr(plan, name).tolist() == w, name
+    assert plan.count.tolist() == [want[5]] and status.tolist() == [want[6]]
+    assert dev_tables.tolist() == tables
+    assert dev_free.tolist()[:want[5]] == free[:want[5]]
+    return want
+
+
+def a_state(g, R, width, page, spare, most):
+    lengths = [int(torch.randint(0, most + 1, (1,), generator=g)) for _ in range(R)]
+    used = [-(-n // page) for n in lengths]
+    total = sum(used) + spare
+    ids = torch.randperm(total, generator=g).tolist()
+    tables, at = [], 0
+    for u in used:
+        tables.append(ids[at:at + u] + [-1] * (width - u))
+        at += u
+    return lengths, tables, ids[at:] + [-1] * at, spare
+
+
+@gpu
+@pytest.mark.parametrize("R,page,most,spare,T", ((1, 16, 0, 3, 40), (3, 16, 50, 20, 60), (33, 64, 500, 30, 2000), (513, 32, 200, 700, 9000), (2000, 128, 300, 100, 1500),
+                                                 (8192, 16, 20, 4000, 30000)))
+@pytest.mark.parametrize("kind", ("tokens", "mixed", "scarce"))
+def test_plan_against_lists(R, page, most, spare, T, kind):
+    g = torch.Generator().manual_seed(R + page)
+    width = -(-(most + 130) // page)
+    lengths, tables, free, count = a_state(g, R, width, page, spare, most)
+    if kind == "tokens":
+        new = [1] * R
+    else:
+        new = [int(torch.randint(-1, 2 if i % 3 else 120, (1,), generator=g)) for i in range(R)]
+    if kind == "scarce":
+        count = min(count, 2)
+    check_plan(lengths, new, tables, free, count, page, T, pad=3)
+
+
+@gpu
+def test_plan_refuses_what_does_not_fit():
+    page = 16
+    free = [9, 8, 7, 6, -1, -1, -1, -1, -1, -1]
+    tables = [[0, 1, -1], [2, -1, -1], [3, 4, 5], [-1, -1, -1]]
+    assert check_plan([32, 5, 40, 0], [17, 12, 9, 3], [t[:] for t in tables], free[:], 4, page, 64)[-1] == 2           # two tables are full
+    assert check_plan([32, 5, 40, 0], [16, 30, 8, 3], [t[:] for t in tables], free[:], 2, page, 64)[-1] == 1           # no pages left
+    assert check_plan([32, 5, 40, 0], [16, 30, -1, 3], [t[:] for t in tables], free[:], 0, page, 64)[-1] == 1          # ... but for those that come back
+    assert check_plan([-3, 5, 49, 0], [1, 2, -1, 3], [t[:] for t in tables], free[:], 4, page, 64)[-1] == 4            # impossible lengths
+    assert check_plan([3, 5, 40, 0], [1, 2, 5, 3], [t[:] for t in tables], free[:], 4, page, 7)[-1] == 8               # more tokens than announced
+    assert check_plan([3, 5, 40, 0], [0, 0, 0, 0], [t[:] for t in tables], free[:], 4, page, 0)[-1] == 0               # nothing to do
+
+
+@gpu
+@pytest.mark.parametrize("captured", (False, True))
+def test_pages_are_conserved_over_many_steps(captured):
+    """A server's life on the buffers of one cache, updated in place: no page is ever held twice or lost."""
+    from htr_b200 import paged
+
+    R, page, pages, most = 40, 16, 200, 300
+    cache = paged.PagedCache(1, 1, 64, pages, page, R, most, DEV)
+    g = torch.Generator().manual_seed(1)
+    new = ints([0] * R)
+    cache.plan(new, 700)
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cache.plan(new, 700)
+    held = 0
+    for step in range(60):
+        a = torch.where(torch.rand(R, generator=g) < 0.08, -1, torch.where(torch.rand(R, generator=g) < 0.15, torch.randint(0, 60, (R,), generator=g), 1))
+        new.copy_(a.to(torch.int32))
+        before = cache.lengths.tolist()
+        if captured:
+            graph.replay()
+        else:
+            cache.plan(new, 700)
+        lengths, tables, n = cache.lengths.tolist(), cache.tables.tolist(), int(cache.count)
+        used = [p for r in range(R) for p in tables[r][:-(-lengths[r] // page)]]
+        assert sorted(used + cache.free.tolist()[:n]) == list(range(pages))
+        assert all(x == (0 if y < 0 else b + y) or x == b for x, y, b in zip(lengths, a.tolist(), before))
+        held = max(held, len(used))
+    assert held > pages // 2
+
+
+# ---- rope_append ----------------------------------------------------------------------------------------------------
+
+
+def angles(rows, D):
+    a = torch.arange(rows, device=DEV).double()[:, None] * 1.0e4 ** -(torch.arange(0, D, 2, device=DEV).double() / D)
+    return a.cos().float(), a.sin().float()
+
+
+def rotated(x, cos, sin):
+    a, b = x[..., ::2], x[..., 1::2]
+    return torch.stack((a * cos - b * sin, a * sin + b * cos), -1).flatten(-2)
+
+
+def empty_cache(pages, hkv, page, D, fill=0x7F):
+    """A cache of bytes that would show (0x7F is NaN) wherever something is read that was never written."""
+    from htr_b200 import paged
+
+    k = torch.full((pages, hkv, page, D), fill, dtype=torch.uint8, device=DEV).view(E4M3)
+    s = torch.full((pages, hkv), 2.0 ** 20, device=DEV)
+    return paged.LayerCache(k, k.clone(), s, s.clone())
+
+
+def wanted_exponent(most):
+    e = -100
+    while most > 448.0 * 2.0 ** e:
+        e += 1
+    return e
+
+
+def check_append(dtype, D, page, hq, hkv, steps, size=1.0, pages=40, slack=0):
+    """Runs steps = [(tokens of request 0, of request 1, ...), ...] and checks the cache's contents after each of them."""
+    from htr_b200 import paged
+
+    R = len(steps[0])
+    cache, g = empty_cache(pages, hkv, page, D), torch.Generator(device=DEV).manual_seed(D + page + hq)
+    width = pages // R
+    tables = torch.randperm(pages, generator=torch.Generator().manual_seed(3))[:R * width].view(R, width)
+    cos, sin = angles(width * page, D)
+    have = [0] * R
+    truth = [[[] for _ in range(R)] for _ in range(2)]           # exact k and v of every request
+    growths = {}
+    for adds in steps:
+        T = sum(adds)
+        pos = [have[r] + i for r in range(R) for i in range(adds[r])]
+        row = [r for r in range(R) for _ in range(adds[r])]
+        slots = [int(tables[r, p // page]) * page + p % page for r, p in zip(row, pos)]
+        wide = torch.randn(T, (hq + 2 * hkv) * D + slack, device=DEV, generator=g) * size * torch.exp(torch.randn(T, 1, device=DEV, generator=g))
+        x = wide.to(dtype)[:, :(hq + 2 * hkv) * D]
+        q = paged.rope_append(x, ints(pos), ints(slots), cos, sin, cache, hq)
+        y = x.double().reshape(T, hq + 2 * hkv, D)
+        c, s = (t.double()[torch.tensor(pos, device=DEV)][:, None] for t in (cos, sin))
+        qw, kw = rotated(y[:, :hq], c, s), rotated(y[:, hq:hq + hkv], c, s)
+        # float32 rotation: three roundings relative to the terms, then one to the output's type (half a step) or, near zero, its smallest steps
+        terms = rotated(y[:, :hq].abs(), c.abs(), -s.abs()).abs() + rotated(y[:, :hq].abs(), c.abs(), s.abs()).abs()
+        assert ((q.double() - qw).abs() <= torch.finfo(dtype).eps / 2 * qw.abs() + 3 * 2.0 ** -24 * terms + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all()
+        for r in range(R):
+            at = [i for i in range(T) if row[i] == r]
+            truth[0][r] += list(kw[at])
+            truth[1][r] += list(y[at, hq + hkv:])
+            have[r] += adds[r]
+        for part, (data, scale) in enumerate(((cache.k, cache.k_scale), (cache.v, cache.v_scale))):
+            for r in range(R):
+                for j in range(-(-have[r] // page)):
+                    exact = torch.stack(truth[part][r][j * page:(j + 1) * page])
+                    id = int(tables[r, j])
+                    got = data[id, :, :exact.shape[0]].double().transpose(0, 1) * scale[id].double()[None, :, None]
+                    sc = scale[id].double()
+                    for h in range(hkv):
+                        e = wanted_exponent(float(exact[:, h].abs().max().float()))
+                        assert float(sc[h]) == 2.0 ** e, (float(sc[h]), e)
+                        if growths.get((part, id, h), e) != e:
+                            growths[part, id, h, "n"] = growths.get((part, id, h, "n"), 0) + 1
+                        growths[part, id, h] = e
+                    # half a step of e4m3 (2^-4), or of its subnormals (2^-10 of the scale), once when written and once each time that the scale grew, the
+                    # later ones in steps at most half as large as the last: below 2^-9 in all; the float32 rotation before it is 2^-20 of that
+                    bound = torch.maximum(2.0 ** -4 * exact.abs(), 2.0 ** -9 * sc[None, :, None].expand_as(exact)) * (1 + 2.0 ** -12)
+                    assert ((got - exact).abs() <= bound).all(), float(((got - exact).abs() / bound).max())
+                    stale = data[id].view(torch.uint8)[:, exact.shape[0]:]
+                    assert (stale == 0x7F).all()                 # places behind the last token are left as they were
+    return sum(v for k, v in growths.items() if k[-1] == "n")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,page,hq,hkv", ((128, 16, 4, 2), (64, 64, 3, 3), (128, 128, 5, 1), (64, 32, 16, 1)))
+def test_cache_holds_what_was_appended(dtype, D, page, hq, hkv):
+    check_append(dtype, D, page, hq, hkv, [(3, 1, 0, page + 5), (1, 0, 2 * page, 1), (0, 1, 1, 1), (2 * page, page - 2, 1, 1)])
+
+
+@gpu
+def test_cache_filled_token_by_token():
+    grown = check_append(torch.bfloat16, 64, 16, 2, 2, [(1, 1)] * 40, slack=8)
+    assert grown > 10                                            # scales grew under older tokens
+
+
+@gpu
+@pytest.mark.parametrize("size", (2.0 ** -30, 2.0 ** 30))
+def test_scales_far_from_one(size):
+    check_append(torch.bfloat16, 128, 32, 4, 1, [(40, 3), (1, 1), (1, 1)], size=size)
+
+
+@gpu
+def test_special_values_and_tokens_outside():
+    from htr_b200 import paged
+
+    D, page, hq, hkv = 64, 16, 2, 1
+    cache, (cos, sin) = empty_cache(4, hkv, page, D, fill=0), angles(32, D)
+    x = torch.ones(7, 4 * D, dtype=torch.bfloat16, device=DEV)
+    x[1, 3 * D] = float("inf")
+    x[2, 3 * D + 1] = float("nan")
+    x[3, 3 * D + 2] = float("-inf")
+    x[4:] = 5.0
+    x[5] = 0.0
+    status = ints([0])
+    # tokens 0 to 3 on page 1; 4: not served; 5: zeros on page 2; 6: a slot behind the cache
+    q = paged.rope_append(x, ints([0, 1, 2, 3, -1, 0, 0]), ints([16, 17, 18, 19, -1, 32, 64]), cos, sin, cache, hq, status=status)
+    assert int(status) == 16
+    assert (q[4] == 0).all() and (q[6] == 0).all() and (q[:4] != 0).any()
+    s = cache.v_scale[1, 0].item()
+    assert s == 2.0 ** -8                                        # the finite values alone: 1 <= 448 * 2^-8
+    v = cache.v.float()[1, 0] * s
+    assert v[1, 0] == 448 * s and v[2, 1].isnan() and v[3, 2] == -448 * s and (v[0] == 1).all() and v[2, 0] == 1
+    assert cache.v_scale[2, 0].item() == 2.0 ** -100 and (cache.v.float()[2, 0, 0] == 0).all()
+    assert (cache.k.view(torch.uint8)[0] == 0).all() and (cache.k.view(torch.uint8)[3] == 0).all()
+    status.zero_()
+    paged.rope_append(x[:2], ints([32, -5]), ints([0, 1]), cos, sin, cache, hq, status=status)        # positions without angles
+    assert int(status) == 16 and (cache.k.view(torch.uint8)[0] == 0).all()
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------
+
+
+def filled(dtype, D, page, hq, hkv, have, adds, seed=0, pages=None, spread=0):
+    """Queries and a cache for requests with have[r] + adds[r] tokens; what is not a token's is NaN."""
+    g = torch.Generator(device=DEV).manual_seed(seed + D + page)
+    R, seen = len(have), [h + a for h, a in zip(have, adds)]
+    used = [-(-max(s, 0) // page) for s in seen]
+    pages = pages or sum(used) + 2
+    cache = empty_cache(pages, hkv, page, D)
+    ids = torch.randperm(pages, generator=torch.Generator().manual_seed(seed))
+    tables, at = torch.full((R, max(used) + 2), -1, dtype=torch.int32), 0
+    for r in range(R):
+        tables[r, :used[r]] = ids[at:at + used[r]]
+        for j in range(used[r]):
+            n, id = min(page, seen[r] - j * page), int(ids[at + j])
+            for data, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+                data[id, :, :n] = (torch.randn(hkv, n, D, device=DEV, generator=g) * 100).clamp(-448, 448).to(E4M3)
+                scale[id] = 2.0 ** (torch.randint(-1 - spread, 2 + spread, (hkv,), device=DEV, generator=g) - 7).float()
+        at += used[r]
+    q = (torch.randn(sum(adds), hq, D, device=DEV, generator=g) * 2).to(dtype)
+    starts = [0]
+    for a in adds:
+        starts.append(starts[-1] + a)
+    return q, ints(starts), ints(seen), tables.to(DEV), cache
+
+
+def attend_exactly(q, starts, seen, tables, cache, scale):
+    """In 64 bits: the result, and the sum of p |v|, to which the roundings of the probabilities are relative."""
+    hq, hkv, page, D = q.shape[1], cache.k.shape[1], cache.k.shape[2], cache.k.shape[3]
+    out, spread = torch.zeros(q.shape, dtype=torch.double, device=DEV), torch.zeros(q.shape, dtype=torch.double, device=DEV)
+    for r in range(seen.numel()):
+        s, e, n = int(starts[r]), int(starts[r + 1]), int(seen[r])
+        if e == s or n <= 0:
+            continue
+        ids = tables[r, :-(-n // page)].long()
+        for h in range(hq):
+            k, v = ((c[ids, h * hkv // hq].double() * f[ids, h * hkv // hq].double()[:, None, None]).reshape(-1, D)[:n]
+                    for c, f in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+            at = torch.arange(n - (e - s), n, device=DEV)
+            hide = torch.arange(n, device=DEV)[None] > at[:, None]
+            p = (q[s:e, h].double() @ k.T * scale).masked_fill(hide, float("-inf")).softmax(-1)
+            p = torch.where(at[:, None] < 0, 0.0, p)
+            v = torch.where(hide.all(0)[:, None], 0.0, v)
+            out[s:e, h], spread[s:e, h] = p @ v, p @ v.abs()
+    return out, spread
+
+
+def check_attention(q, starts, seen, tables, cache, max_new, scale=None, **kw):
+    from htr_b200 import paged
+
+    got = paged.attention(q, starts, seen, tables, cache, max_new, scale=scale, **kw)
+    want, spread = attend_exactly(q, starts, seen, tables, cache, q.shape[2] ** -0.5 if scale is None else scale)
+    n = int(starts[-1])
+    # half a step of the output; 2^-11 for each probability (fp16); 2^-11 for the float32 scores: D terms of |q k| * scale up to about 40 in
+    # sum, 2^-24 each time the sum is rounded (128 * 40 * 2^-24 = 2^-11.7), and for the exponentials (2^-21)
+    bound = torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -10 * spread + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+    off = (got.double() - want).abs()[:n]
+    assert (off <= bound[:n]).all(), float((off / bound[:n]).max())
+    return got
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,page,hq,hkv", ((128, 64, 8, 2), (64, 16, 6, 2), (128, 16, 5, 5), (64, 128, 24, 1), (128, 32, 16, 1)))
+@pytest.mark.parametrize("have,adds", (((0, 14, 15, 16, 130, 77), (1, 1, 1, 1, 1, 0)), ((0, 1, 60, 5, 200), (1, 3, 5, 0, 2)), ((0, 63, 100), (70, 1, 33)), ((517,), (1,)),
+                                       ((300, 0, 45), (260, 129, 200))))
+def test_attention(dtype, D, page, hq, hkv, have, adds):
+    check_attention(*filled(dtype, D, page, hq, hkv, have, adds), max_new=max(adds))
+
+
+@gpu
+@pytest.mark.parametrize("adds", ((1, 1), (2, 30), (150, 3)))
+def test_attention_scales_that_differ_and_its_own_scale(adds):
+    q, starts, seen, tables, cache = filled(torch.bfloat16, 128, 16, 4, 2, (100, 333), adds, spread=5)
+    check_attention(q, starts, seen, tables, cache, max(adds), scale=0.01)
+    cache.v_scale.mul_(2.0 ** 40)
+    check_attention(q, starts, seen, tables, cache, max(adds), scale=0.01)
+    cache.v_scale.mul_(2.0 ** -90)
+    check_attention(q, starts, seen, tables, cache, max(adds), scale=0.01)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_attention_over_long_sequences(dtype):
+    check_attention(*filled(dtype, 128, 64, 4, 1, (20011, 3, 9000), (1, 1, 1)), max_new=1)
+    check_attention(*filled(dtype, 64, 128, 4, 2, (6000, 1), (40, 300)), max_new=300)
+
+
+@gpu
+def test_rows_that_see_nothing_and_rows_behind_the_last():
+    q, starts, seen, tables, cache = filled(torch.bfloat16, 64, 16, 4, 2, (20, 3, 0, 30), (2, 5, 3, 140))
+    seen[1], seen[2] = 2, 0                                      # three of the five tokens stand before the first position; not served
+    big = torch.cat([q, torch.ones_like(q[:4])])
+    out = torch.full_like(big, 7.0)
+    got = check_attention(big, starts, seen, tables, cache, 140, out=out)
+    assert got is out and (got[2:5] == 0).all() and (got[7:10] == 0).all() and (got[150:] == 7).all() and (got[5:7] != 0).any()
+    one = torch.full_like(big, 7.0)
+    check_attention(big, ints([0, 0, 0, 0, 0]), seen, tables, cache, 1, out=one)
+    assert (one == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("adds", ((1, 1), (40, 1)))
+def test_table_entries_that_are_no_page_hide_their_tokens(adds):
+    from htr_b200 import paged
+
+    q, starts, seen, tables, cache = filled(torch.bfloat16, 64, 16, 2, 1, (100, 64), adds)
+    status = ints([0])
+    want = paged.attention(q, starts, seen, tables, cache, max(adds), status=status).clone()
+    assert int(status) == 0
+    tables[0, 2], tables[1, :] = 1 << 30, -1
+    got = paged.attention(q, starts, seen, tables, cache, max(adds), status=status)
+    assert int(status) == 32 and torch.isfinite(got).all() and (got[int(starts[1]):] == 0).all() and not torch.equal(got, want)
+
+
+@gpu
+def test_pages_beyond_four_gigabytes():
+    from htr_b200 import paged
+
+    hkv, page, D, pages = 8, 128, 128, 36000                     # 4.7 GB of keys
+    k = torch.empty(pages, hkv, page, D, dtype=torch.uint8, device=DEV).view(E4M3)
+    cache = paged.LayerCache(k, torch.empty_like(k), torch.empty(pages, hkv, device=DEV), torch.empty(pages, hkv, device=DEV))
+    ids = [35999, 0, 34000]
+    for x in (0, 1):
+        for id in ids:
+            cache[x][id] = (torch.randn(hkv, page, D, device=DEV) * 90).to(E4M3)
+            cache[2 + x][id] = 2.0 ** -7
+    q = torch.randn(1, 8, D, device=DEV).bfloat16()
+    check_attention(q, ints([0, 1]), ints([300]), ints([ids]), cache, 1)
+    qkv = torch.randn(2, 24 * D, device=DEV).bfloat16()[:, :8 * D + 16 * D]
+    cos, sin = angles(400, D)
+    paged.rope_append(qkv, ints([300, 301]), ints([34000 * page + 44, 34000 * page + 45]), cos, sin, cache, 8)
+    got = cache.v[34000, :, 44:46].double() * cache.v_scale[34000].double()[:, None, None]
+    want = qkv.double().view(2, 24, D)[:, 16:].transpose(0, 1)
+    assert ((got - want).abs() <= torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -9 * cache.v_scale[34000].double()[:, None, None])).all()
+
+
+@gpu
+@pytest.mark.parametrize("adds", ((1, 1, 1), (90, 1, 200)))
+def test_two_graphs_and_another_stream(adds):
+    """Captured calls keep no buffers in common with one another or with eager ones: replayed at the same time they give what each gives alone."""
+    from htr_b200 import paged
+
+    sets = [filled(torch.bfloat16, 128, 16, 8, 2, have, adds, seed=s) for s, have in enumerate(((3000, 1, 50), (40, 2500, 700)))]
+    want = [paged.attention(*x, max(adds)).clone() for x in sets]
+    graphs, outs = [], []
+    for x in sets:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged.attention(*x, max(adds)))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for o in outs:
+            o.fill_(9)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = paged.attention(*sets[0], max(adds))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)) and torch.equal(eager, want[0])
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------------
+
+
+def test_no_cpu_path():
+    from htr_b200 import _lib, paged
+
+    i = torch.zeros(1, dtype=torch.int32)
+    k = torch.zeros(1, 1, 16, 64, dtype=torch.uint8).view(E4M3)
+    cache = paged.LayerCache(k, k, torch.ones(1, 1), torch.ones(1, 1))
+    for call in (lambda: paged.plan_step(i, i, i[None], i, i, 16, 1), lambda: paged.rope_append(torch.zeros(1, 192).bfloat16(), i, i, torch.ones(1, 32), torch.ones(1, 32), cache, 1),
+                 lambda: paged.attention(torch.zeros(1, 1, 64).bfloat16(), torch.zeros(2, dtype=torch.int32), i, i[None], cache, 1)):
+        with pytest.raises(_lib.HTRError, match="no CPU path"):
+            call()
+
+
+def test_status_codes_without_a_gpu():
+    import ctypes
+
+    from htr_b200 import _lib
+
+    L, f = _lib.lib, ctypes.c_float(1.0)
+    p = 16                                                       # an address that the checks before a launch look at and nothing reads
+
+    def plan(R=4, stride=3, width=3, pages=8, page=16, T=9, at=p):
+        return L.htr_page_plan(at, p, R, p, stride, width, p, pages, p, page, T, p, p, p, p, p, p, None, None)
+
+    assert [plan(R=0), plan(stride=2), plan(width=0), plan(pages=0), plan(page=24), plan(page=256), plan(T=-1)] == [-2] * 7
+    assert [plan(R=8193), plan(pages=1 << 28), plan(stride=1 << 28, width=1 << 28), plan(T=(1 << 31) - 1)] == [-8] * 4
+    assert plan(at=None) == -5
+
+    def append(dt=0, stride=6 * 64, T=2, rows=9, hq=4, hkv=1, D=64, pages=8, page=16, at=p):
+        return L.htr_paged_append(at, dt, stride, p, p, T, p, p, rows, hq, hkv, D, p, p, p, p, pages, page, p, None, None)
+
+    assert append(dt=2) == -3
+    assert [append(stride=6 * 64 - 8), append(stride=6 * 64 + 4), append(T=-1), append(rows=0), append(hq=0), append(hkv=0), append(D=96), append(pages=0), append(page=8)] == [-2] * 9
+    assert append(pages=1 << 28) == -8 and append(T=0, at=None) == 0 and append(at=None) == -5 and append(at=24) == -6
+
+    def attend(dt=0, T=3, R=2, stride=3, width=3, pages=8, page=16, hq=4, hkv=2, D=64, most=1, at=p, work=p, size=1 << 40):
+        return L.htr_paged_attention(at, dt, T, p, p, R, p, stride, width, p, p, p, p, pages, page, hq, hkv, D, most, f, p, None, work, size, None)
+
+    assert attend(dt=2) == -3
+    assert [attend(T=-1), attend(R=0), attend(stride=2), attend(page=17), attend(hq=5), attend(hkv=0), attend(D=32), attend(most=0)] == [-2] * 8
+    assert [attend(R=8193), attend(pages=1 << 28), attend(most=1 << 30)] == [-8] * 3
+    assert attend(T=0, at=None) == 0 and attend(at=None) == -5 and attend(at=24) == -6
+
+
+@gpu
+def test_refusals():
+    from htr_b200 import _lib, paged
+
+    q, starts, seen, tables, cache = filled(torch.bfloat16, 64, 16, 4, 2, (20, 3), (1, 1))
+    cos, sin = angles(64, 64)
+    good = dict(qkv=torch.zeros(2, 8 * 64, dtype=torch.bfloat16, device=DEV), positions=ints([20, 3]), slots=ints([0, 16]), cos=cos, sin=sin, cache=cache, q_heads=4)
+    paged.rope_append(**good)
+    bad_cache = [cache._replace(k=cache.k.float()), cache._replace(v=cache.v[:1]), cache._replace(k=cache.k.transpose(1, 2)), cache._replace(k_scale=cache.k_scale.half()),
+                 cache._replace(v_scale=cache.v_scale[:1]), cache._replace(k=cache.k[:, :, :8], v=cache.v[:, :, :8]), cache._replace(k=cache.k.cpu())]
+    for change in (dict(qkv=good["qkv"].float()), dict(qkv=good["qkv"][:, :-64]), dict(qkv=good["qkv"][0]), dict(positions=ints([1])), dict(slots=good["slots"].long()),
+                   dict(cos=cos[:, :16]), dict(sin=sin.double()), dict(cos=cos[:3]), dict(q_heads=0), *[dict(cache=c) for c in bad_cache]):
+        with pytest.raises(_lib.HTRError):
+            paged.rope_append(**{**good, **change})
+    good = dict(q=q, starts=starts, seen=seen, tables=tables, cache=cache, max_new=1)
+    paged.attention(**good)
+    for change in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(starts=starts[:2]), dict(seen=seen.long()), dict(tables=tables[:1]), dict(tables=tables.t().contiguous().t()),
+                   dict(max_new=0), dict(out=torch.empty_like(q)[:1]), dict(out=torch.empty_like(q).half()), dict(status=torch.zeros(1, device=DEV)), *[dict(cache=c) for c in bad_cache]):
+        with pytest.raises(_lib.HTRError):
+            paged.attention(**{**good, **change})
+    assert paged.attention(q[:0], ints([0, 0, 0]), seen, tables, cache, 1).shape == (0, 4, 64)
+    good = dict(lengths=ints([3, 4]), new=ints([1, 1]), tables=tables, free=ints([5, 6]), count=ints([2]), page_size=16, max_tokens=4)
+    paged.plan_step(**good)
+    for change in (dict(lengths=ints([3])), dict(new=ints([1, 1]).long()), dict(tables=tables.long()), dict(tables=tables[0]), dict(count=ints([1, 2])), dict(page_size=20),
+                   dict(max_tokens=-1), dict(lengths_out=ints([1])), dict(count_out=ints([1, 1])), dict(free=ints([])), dict(status=ints([0, 0]))):
+        with pytest.raises(_lib.HTRError):
+            paged.plan_step(**{**good, **change})
+    for args in ((1, 1, 96, 4, 16, 1, 64), (1, 1, 64, 4, 20, 1, 64), (0, 1, 64, 4, 16, 1, 64), (1, 1, 64, 0, 16, 1, 64)):
+        with pytest.raises(_lib.HTRError):
+            paged.PagedCache(*args, DEV)
