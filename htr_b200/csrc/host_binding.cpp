@@ -22,6 +22,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
 #include <vector>
 
@@ -48,6 +49,11 @@ struct Entry {
   decltype(&htr_dec_rope_attention) rope_attention;
   decltype(&htr_dec_add_rmsnorm) add_rmsnorm;
   decltype(&htr_dec_swiglu) swiglu;
+  decltype(&htr_page_plan) page_plan;
+  decltype(&htr_paged_append) paged_append;
+  decltype(&htr_paged_attention) paged_attention;
+  decltype(&htr_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
+  decltype(&htr_sample) sample;
 } g_lib = {};
 
 // ---- workspaces: buffers that ops.py owns (one per device, stream and kind); this table only remembers where they are
@@ -518,6 +524,172 @@ PyObject* py_decoder_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(y));
 }
 
+// ---- serving many sequences (htr_b200/paged.py, sampling.py): a step's plan, append and attention are 2 to 5 us of GPU each for a few sequences,
+// and 20 to 27 us of host work in Python and ctypes
+
+// an optional tensor of `count` elements; false for what is neither None nor such a tensor
+bool optional_of(PyObject* o, const at::Device& dev, at::ScalarType type, int64_t count, void** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = tensor(o);
+  if (!vector_of(t, dev, type) || t->numel() != count) return false;
+  *out = t->data_ptr();
+  return true;
+}
+
+bool table_of(const at::Tensor* t, const at::Device& dev, int64_t requests, int64_t* stride) {
+  if (!t || t->scalar_type() != at::kInt || t->device() != dev || t->dim() != 2 || t->size(0) != requests || t->size(1) < 1 || t->size(1) > (1 << 30) ||
+      t->stride(1) != 1)
+    return false;
+  *stride = std::max(t->stride(0), t->size(1));
+  return requests == 1 || t->stride(0) >= t->size(1);
+}
+
+// a layer's cache: (k, v, k_scale, v_scale)
+struct Cache {
+  void *k, *v;
+  float *ks, *vs;
+  int pages, heads, page, dim;
+};
+bool cache_of(PyObject* o, const at::Device& dev, Cache* c) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const at::Tensor* t[4];
+  for (int i = 0; i < 4; ++i)
+    if (!(t[i] = tensor(PyTuple_GET_ITEM(o, i))) || !plain(*t[i], dev, i < 2 ? at::kFloat8_e4m3fn : at::kFloat)) return false;
+  if (t[0]->dim() != 4 || t[1]->sizes() != t[0]->sizes() || t[0]->size(0) > (1 << 30) || t[0]->size(1) > (1 << 30)) return false;
+  for (int i = 2; i < 4; ++i)
+    if (t[i]->dim() != 2 || t[i]->size(0) != t[0]->size(0) || t[i]->size(1) != t[0]->size(1)) return false;
+  if (t[0]->size(2) > 128 || t[0]->size(3) > 128) return false;
+  *c = {t[0]->data_ptr(), t[1]->data_ptr(), t[2]->data_ptr<float>(), t[3]->data_ptr<float>(), (int)t[0]->size(0), (int)t[0]->size(1),
+        (int)t[0]->size(2), (int)t[0]->size(3)};
+  return true;
+}
+
+// plan_step(lengths, new, tables, free, count, page_size, max_tokens, lengths_out, count_out, status): the six tensors of a StepPlan
+PyObject* py_plan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) return none();
+  const at::Tensor *lengths = tensor(a[0]), *added = tensor(a[1]), *tables = tensor(a[2]), *pool = tensor(a[3]), *count = tensor(a[4]);
+  int page, T;
+  int64_t stride;
+  void *lengths_out, *count_out, *status;
+  if (!lengths || !lengths->is_cuda()) return none();
+  const at::Device where = lengths->device();
+  const int64_t R = lengths->numel();
+  if (!vector_of(lengths, where, at::kInt) || !vector_of(added, where, at::kInt) || added->numel() != R || !vector_of(pool, where, at::kInt) ||
+      !vector_of(count, where, at::kInt) || count->numel() != 1 || R < 1 || R > 8192 || pool->numel() > (1 << 30) || !table_of(tables, where, R, &stride))
+    return none();
+  if (!int_of(a[5], &page) || !int_of(a[6], &T) || T < 0 || !optional_of(a[7], where, at::kInt, R, &lengths_out) ||
+      !optional_of(a[8], where, at::kInt, 1, &count_out) || !optional_of(a[9], where, at::kInt, 1, &status))
+    return none();
+  const int dev = lengths->get_device();
+  OnDevice on(dev);
+  const auto ints = [&](int64_t size) { return at::detail::empty_cuda({size}, at::kInt, where, std::nullopt); };
+  at::Tensor out[6] = {ints(R + 1), ints(T), ints(T), ints(R), lengths_out ? at::Tensor() : ints(R), count_out ? at::Tensor() : ints(1)};
+  if (!lengths_out) lengths_out = out[4].data_ptr();
+  if (!count_out) count_out = out[5].data_ptr();
+  if (g_lib.page_plan(lengths->const_data_ptr<int>(), added->const_data_ptr<int>(), (int)R, tables->data_ptr<int>(), stride, (int)tables->size(1),
+                      pool->data_ptr<int>(), (int)pool->numel(), count->const_data_ptr<int>(), page, T, out[0].data_ptr<int>(), out[1].data_ptr<int>(),
+                      out[2].data_ptr<int>(), out[3].data_ptr<int>(), static_cast<int*>(lengths_out), static_cast<int*>(count_out),
+                      static_cast<int*>(status), c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+    return none();
+  PyObject* all = PyTuple_New(6);
+  if (!all) return nullptr;
+  for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(all, i, out[i].defined() ? THPVariable_Wrap(std::move(out[i])) : Py_NewRef(a[3 + i]));
+  return all;
+}
+
+// rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status): the rotated queries
+PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8) return none();
+  const at::Tensor *x = tensor(a[0]), *pos = tensor(a[1]), *slots = tensor(a[2]), *cosv = tensor(a[3]), *sinv = tensor(a[4]);
+  Cache c;
+  int hq;
+  void* status;
+  if (!x || !x->is_cuda() || x->dim() != 2 || x->stride(1) != 1) return none();
+  const at::Device where = x->device();
+  const int64_t T = x->size(0), cols = x->size(1);
+  if (!cache_of(a[5], where, &c) || !int_of(a[6], &hq) || hq < 1 || cols != ((int64_t)hq + 2 * (int64_t)c.heads) * c.dim || T < 1 || T > (1 << 30)) return none();
+  if (!vector_of(pos, where, at::kInt) || pos->numel() != T || !vector_of(slots, where, at::kInt) || slots->numel() != T || !cosv || !sinv ||
+      !plain(*cosv, where, at::kFloat) || !plain(*sinv, where, at::kFloat) || cosv->dim() != 2 || cosv->sizes() != sinv->sizes() ||
+      cosv->size(1) != c.dim / 2 || cosv->size(0) > (1 << 30) || !optional_of(a[7], where, at::kInt, 1, &status))
+    return none();
+  const int64_t stride = T == 1 ? cols : x->stride(0);
+  const int dt = dtype_code(x->scalar_type()), dev = x->get_device();
+  OnDevice on(dev);
+  at::Tensor q = at::detail::empty_cuda({T, (int64_t)hq, (int64_t)c.dim}, x->scalar_type(), where, std::nullopt);
+  if (g_lib.paged_append(x->const_data_ptr(), dt, stride, pos->const_data_ptr<int>(), slots->const_data_ptr<int>(), (int)T, cosv->const_data_ptr<float>(),
+                         sinv->const_data_ptr<float>(), (int)cosv->size(0), hq, c.heads, c.dim, c.k, c.v, c.ks, c.vs, c.pages, c.page, q.data_ptr(),
+                         static_cast<int*>(status), c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+    return none();
+  return THPVariable_Wrap(std::move(q));
+}
+
+// attention(q, starts, seen, tables, cache, max_new, scale, out, status)
+PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 9) return none();
+  const at::Tensor *q = tensor(a[0]), *starts = tensor(a[1]), *seen = tensor(a[2]), *tables = tensor(a[3]);
+  Cache c;
+  int most;
+  int64_t stride;
+  double scale;
+  void* status;
+  if (!q || !q->is_cuda() || q->dim() != 3 || !q->is_contiguous()) return none();
+  const at::Device where = q->device();
+  const int64_t T = q->size(0), hq = q->size(1), R = seen ? seen->numel() : 0;
+  if (!cache_of(a[4], where, &c) || q->size(2) != c.dim || T < 1 || T > (1 << 30) || hq > (1 << 20) || R < 1 || R > 8192) return none();
+  if (!vector_of(starts, where, at::kInt) || starts->numel() != R + 1 || !vector_of(seen, where, at::kInt) || !table_of(tables, where, R, &stride) ||
+      !int_of(a[5], &most) || most < 1 || !optional_of(a[8], where, at::kInt, 1, &status))
+    return none();
+  if (a[6] == Py_None) scale = 1.0 / std::sqrt((double)c.dim);
+  else if (!float_of(a[6], &scale)) return none();
+  const int dt = dtype_code(q->scalar_type()), dev = q->get_device();
+  most = (int)std::min<int64_t>(most, T);
+  OnDevice on(dev);
+  at::Tensor y, work;
+  if (a[7] == Py_None) {
+    y = at::detail::empty_cuda(q->sizes(), q->scalar_type(), where, std::nullopt);
+  } else {
+    const at::Tensor* o = tensor(a[7]);
+    if (!o || !plain(*o, where, q->scalar_type()) || o->sizes() != q->sizes()) return none();
+    y = *o;
+  }
+  const size_t need = g_lib.paged_attention_workspace_bytes((int)T, (int)R, (int)hq, c.heads, c.dim, most);
+  if (need) work = at::detail::empty_cuda({(int64_t)need}, at::kByte, where, std::nullopt);
+  if (g_lib.paged_attention(q->const_data_ptr(), dt, (int)T, starts->const_data_ptr<int>(), seen->const_data_ptr<int>(), (int)R, tables->const_data_ptr<int>(),
+                            stride, (int)tables->size(1), c.k, c.v, c.ks, c.vs, c.pages, c.page, (int)hq, c.heads, c.dim, most, (float)scale, y.data_ptr(),
+                            static_cast<int*>(status), need ? work.data_ptr() : nullptr, need, c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+    return none();
+  if (a[7] != Py_None) return Py_NewRef(a[7]);
+  return THPVariable_Wrap(std::move(y));
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p): (tokens, logprobs); settings are tensors or None
+PyObject* py_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) return none();
+  const at::Tensor *x = tensor(a[0]), *u = tensor(a[1]);
+  if (!x || !x->is_cuda() || x->dim() != 2) return none();
+  const at::Device where = x->device();
+  const int64_t R = x->size(0), V = x->size(1);
+  const int dt = dtype_code(x->scalar_type());
+  if (dt < 0 || R < 1 || R > (1 << 30) || V < 1 || V > (1 << 20) || (V > 1 && x->stride(1) != 1) || (R > 1 && x->stride(0) < V)) return none();
+  if (!vector_of(u, where, at::kFloat) || u->numel() != R) return none();
+  void* set[4];
+  for (int i = 0; i < 4; ++i)
+    if (!optional_of(a[2 + i], where, i == 1 ? at::kInt : at::kFloat, R, &set[i])) return none();
+  const int dev = x->get_device();
+  OnDevice on(dev);
+  at::Tensor tokens = at::detail::empty_cuda({R}, at::kLong, where, std::nullopt), logprobs = at::detail::empty_cuda({R}, at::kFloat, where, std::nullopt);
+  if (g_lib.sample(x->const_data_ptr(), dt, std::max(R > 1 ? x->stride(0) : V, V), (int)R, (int)V, u->const_data_ptr<float>(), static_cast<float*>(set[0]),
+                   static_cast<int*>(set[1]), static_cast<float*>(set[2]), static_cast<float*>(set[3]), tokens.data_ptr<int64_t>(),
+                   logprobs.data_ptr<float>(), c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+    return none();
+  PyObject* both = PyTuple_New(2);
+  if (!both) return nullptr;
+  PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(tokens)));
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(logprobs)));
+  return both;
+}
+
 // set_workspace(kind, device index, stream, buffer): the buffer that calls on this device and stream use from now on
 PyObject* py_set_workspace(PyObject*, PyObject* args) {
   int kind, device;
@@ -562,7 +734,14 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   g_lib.rope_attention = reinterpret_cast<decltype(g_lib.rope_attention)>(at_name("htr_dec_rope_attention"));
   g_lib.add_rmsnorm = reinterpret_cast<decltype(g_lib.add_rmsnorm)>(at_name("htr_dec_add_rmsnorm"));
   g_lib.swiglu = reinterpret_cast<decltype(g_lib.swiglu)>(at_name("htr_dec_swiglu"));
-  if (!g_lib.linear_workspace_bytes || !g_lib.linear_gemm_workspace_bytes || !g_lib.add_rmsnorm || !g_lib.swiglu || !g_lib.rope_cache || !g_lib.attention || !g_lib.rope_attention || !g_lib.linear_routed || !g_lib.linear_routed_gemm || !g_lib.route_plan_bytes || !g_lib.route_plan || !g_lib.moe_weighted_sum ||
+  g_lib.page_plan = reinterpret_cast<decltype(g_lib.page_plan)>(at_name("htr_page_plan"));
+  g_lib.paged_append = reinterpret_cast<decltype(g_lib.paged_append)>(at_name("htr_paged_append"));
+  g_lib.paged_attention = reinterpret_cast<decltype(g_lib.paged_attention)>(at_name("htr_paged_attention"));
+  g_lib.paged_attention_workspace_bytes =
+      reinterpret_cast<decltype(g_lib.paged_attention_workspace_bytes)>(at_name("htr_paged_attention_workspace_bytes"));
+  g_lib.sample = reinterpret_cast<decltype(g_lib.sample)>(at_name("htr_sample"));
+  if (!g_lib.page_plan || !g_lib.paged_append || !g_lib.paged_attention || !g_lib.paged_attention_workspace_bytes || !g_lib.sample ||
+      !g_lib.linear_workspace_bytes || !g_lib.linear_gemm_workspace_bytes || !g_lib.add_rmsnorm || !g_lib.swiglu || !g_lib.rope_cache || !g_lib.attention || !g_lib.rope_attention || !g_lib.linear_routed || !g_lib.linear_routed_gemm || !g_lib.route_plan_bytes || !g_lib.route_plan || !g_lib.moe_weighted_sum ||
       !g_lib.linear_gemm_padded || !g_lib.route_rows || !g_lib.linear_ex || !g_lib.linear_gemm || !g_lib.linear_padded || !g_lib.linear_fused) {
     PyErr_SetString(PyExc_ImportError, "bind: an entry point of libhtr_b200 is missing");
     return nullptr;
@@ -592,6 +771,10 @@ PyMethodDef g_methods[] = {
     fast<py_route_plan>("route_plan"),
     fast<py_moe_weighted_sum>("moe_weighted_sum"),
     fast<py_decoder_step>("decoder_step"),
+    fast<py_plan_step>("plan_step"),
+    fast<py_rope_append>("rope_append"),
+    fast<py_attention>("attention"),
+    fast<py_sample>("sample"),
     {"set_workspace", py_set_workspace, METH_VARARGS, nullptr},
     {"bind", py_bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},

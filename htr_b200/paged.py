@@ -12,10 +12,11 @@ import typing
 
 import torch
 
-from . import _lib, ops
+from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
+_host = _lib.host
 _HALF = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -84,6 +85,9 @@ def plan_step(lengths, new, tables, free, count, page_size, max_tokens, lengths_
     A request that cannot be served keeps its length and its tokens get -1; status [1], if given, then gets a bit: 1 no pages left (this request
     and later ones that need pages), 2 its table is full, 4 its length is negative or beyond its table, 8 tokens beyond max_tokens."""
     what = "plan_step"
+    plan = _host.plan_step(lengths, new, tables, free, count, page_size, max_tokens, lengths_out, count_out, status)    # the usual case; None: whatever it does not take
+    if plan is not None:
+        return StepPlan._make(plan)
     if not lengths.is_cuda:
         raise _lib.HTRError("plan_step has no CPU path: tensors must live on a CUDA device")
     dev, R, T = lengths.device, lengths.numel(), int(max_tokens)
@@ -121,6 +125,9 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None):
     page's first place, and where a later token makes it grow the older ones are rescaled.  Infinities are held as the largest value, NaN as NaN.
     A token with slot -1 is not written and its query is zero; so is one whose slot or position lies outside the buffers (status 16)."""
     what = "rope_append"
+    q = _host.rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status)
+    if q is not None:
+        return q
     if not qkv.is_cuda:
         raise _lib.HTRError("rope_append has no CPU path: tensors must live on a CUDA device")
     dev = qkv.device
@@ -157,6 +164,9 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     Returns `out`, or a new tensor like q; its rows behind starts[-1] are left as they are.  A table entry that is no page hides its
     tokens (status 32)."""
     what = "attention"
+    y = _host.attention(q, starts, seen, tables, cache, max_new, scale, out, status)
+    if y is not None:
+        return y
     if not q.is_cuda:
         raise _lib.HTRError("attention has no CPU path: tensors must live on a CUDA device")
     dev, R = q.device, seen.numel()

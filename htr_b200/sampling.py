@@ -21,6 +21,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
 
     Settings are None, one number for all rows, or a CUDA tensor of one value per row (float32; int32 for top_k).  Rows may be strided.
     The choice is reproducible to the bit: weights are added as 64-bit integers."""
+    both = _lib.host.sample(logits, u, temperature, top_k, top_p, min_p)     # the usual case; None: whatever it does not take
+    if both is not None:
+        return both
     if not logits.is_cuda:
         raise _lib.HTRError("sample has no CPU path: tensors must live on a CUDA device")
     if logits.dtype not in ops._DTYPES or logits.dim() != 2:
