@@ -409,33 +409,47 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
 
 // ---- attention over the cache -----------------------------------------------------------------------------------------------------
 //
-// The query heads of one key/value head and a request's tokens of this step are rows of one product, 16 at a time (row = token * group
-// + head), on warp-level matrix instructions m16n8k16.  A warp takes 16 cached tokens at a time, for itself alone: the dimensions that
-// a product sums over and the columns of a result may be taken in any order, so that every lane loads whole 16-byte pieces of the
-// cache's rows straight into the fragments of K^T (lane g, c: token g, dimensions 16 c ...) and of V (tokens 2 c, 2 c + 1, ...,
-// dimensions 16 g ...), and e4m3 becomes fp16, which holds it exactly, in registers.
+// What bounds it for single tokens: the cache's bytes.  The query heads of one key/value head and a request's tokens of this step are the
+// rows of one product, 8 or 16 at a time (row = token * group + head), on warp-level matrix instructions m16n8k16 with the cache as the
+// 16-row operand (S^T = K Q^T, O^T = V^T P^T), so that 8 rows fill a tile.  A warp takes 16 cached tokens at a time for itself alone, with
+// the next 16 in flight in its registers.  The dimensions that a product sums over and the rows of a result may be taken in any order, so
+// every lane (g = lane / 4, c = lane % 4) loads whole 16-byte pieces of the cache's rows straight into fragments: of K those of the tokens g
+// and g + 8 at dimensions 16 c ..., of V those of the tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 at dimensions 16 g ...; e4m3 becomes fp16, which
+// holds it exactly, on the way.  No shared memory, no barrier until a warp's tokens are through.
+//
+// The work is cut evenly, whatever the requests' lengths: a flat list of units of 64 tokens (of every request, row tile and key/value
+// head) in equal runs over the thread blocks.  A tile that lies in one run is finished there; of a tile that is cut every thread
+// block leaves its part (maximum, sum, result) in the workspace, and a second launch joins them in the order of the tokens.
+//
 // Queries are fp16 under a power of two per row (bf16 keeps all its bits: 29 binades of normal fp16 below the row's largest element).
 // Probabilities are rounded to fp16, relative to the contribution that they make: the scale of the values' page is part of the exponent
-// (P' = 2^(s + log2 scale - m)), and the sum of the probabilities takes it out again.  2^-12 each, averaged over the tokens: below the
-// rounding of the output.  Maxima, sums and results are float32.
+// (P' = 2^(s + log2 scale - m)), and the sum of the probabilities takes it out again.  2^-11 each at most, averaged over the tokens: below
+// the rounding of the output.  m follows the largest exponent only when that grows by 2^14 (P' stays below 2^14, sums are float32).
 
 struct AttentionArgs {
   const void* q;
   const int *starts, *seen, *tables;
   long long table_stride;
-  int width, requests, tokens, q_heads, kv_heads, group;
+  int width, requests, tokens, q_heads, kv_heads, group, max_new;
   const uint8_t *k_cache, *v_cache;
   const float *k_scale, *v_scale;
   int pages, shift;
   float scale;                                             // of the scores, times log2(e)
   void* out;
   int* status;
+  float* parts;                                            // two per thread block: rows x (D results, maximum, sum)
+  int4* cuts;                                              // per thread block, of the tile that begins in its run and goes beyond it: see below
 };
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8x8 matrix of fp16, a row per four lanes
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -447,122 +461,79 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-constexpr int kAttWarps = 4;
+constexpr int kAttWarps = 4, kAttThreads = kAttWarps * 32, kUnit = kAttWarps * 16;   // tokens of a unit
 constexpr float kNone = -__builtin_huge_valf();
+// thread blocks per SM, by the registers that the tiles in flight and the results need
+template <int D, int NT>
+constexpr int kAttBlocks = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttWarps * 32) paged_attention_kernel(const AttentionArgs a) {
-  constexpr int kSteps = D / 16, kCols = D / 8;            // k-steps of a score; 8-column tiles of the result = dimensions of a lane
-  __shared__ float s_o[kAttWarps][16][D + 1];
-  __shared__ float s_m[kAttWarps][16], s_l[kAttWarps][16];
-  pdl_enter();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int r = blockIdx.z, kvh = blockIdx.y;
-  const int start = a.starts[r], n = min(a.starts[r + 1], a.tokens) - start, seen = a.seen[r];
-  const int row0 = blockIdx.x * 16, rows = n * a.group;
-  if (start < 0 || row0 >= rows) return;
-  const int last = min(row0 + 15, rows - 1) / a.group;     // of the tile's tokens: it sees the most
-  const int end = min(max(seen - n + last + 1, 0), (int)min((long long)a.width << a.shift, 0x7FFFFFFFLL));
-  // queries
-  uint32_t qf[kSteps][4];
-  float row_scale[2];
-  int row_end[2];                                          // tokens that a row sees
+// a row of queries as the right operand: fragments of rows g + 8 * tile, their scale (times that of the scores), for this lane's rows 2 c, 2 c + 1
+template <typename T, int D, int NT>
+struct Rows {
+  uint32_t q[D / 16][NT][2];
+  float scale[NT][2];
+  int end[NT][2];                                          // tokens that a row sees
+  __device__ __forceinline__ void load(const AttentionArgs& a, int start, int n, int seen, int row0, int kvh, int lane) {
+    const int g = lane >> 2, c = lane & 3, rows = n * a.group;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int row = row0 + g + 8 * x, i = row / a.group;
-    const bool ok = row < rows;
-    row_end[x] = ok ? seen - n + i + 1 : 0;
-    const T* src = static_cast<const T*>(a.q) + ((size_t)(start + i) * a.q_heads + (size_t)kvh * a.group + (row - i * a.group)) * D;
-    float v[kSteps][4];
-    float most = 0.f;
+    for (int t = 0; t < NT; ++t) {
+      const int row = row0 + 8 * t + g, i = row / a.group;
+      const bool ok = row < rows;
+      const T* src = static_cast<const T*>(a.q) + ((size_t)(start + i) * a.q_heads + (size_t)kvh * a.group + (row - i * a.group)) * D;
+      float v[D / 16][4], most = 0.f;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {                     // step k: dimensions 64 (k / 4) + 16 c + 4 (k % 4) ...
-      uint2 raw = {0, 0};
-      if (ok) raw = *reinterpret_cast<const uint2*>(src + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
-      const float2 lo = Half<T>::wide(raw.x), hi = Half<T>::wide(raw.y);
-      v[k][0] = lo.x; v[k][1] = lo.y; v[k][2] = hi.x; v[k][3] = hi.y;
+      for (int k = 0; k < D / 16; ++k) {                   // step k: dimensions 64 (k / 4) + 16 c + 4 (k % 4) ...
+        uint2 raw = {0, 0};
+        if (ok) raw = *reinterpret_cast<const uint2*>(src + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
+        const float2 lo = Half<T>::wide(raw.x), hi = Half<T>::wide(raw.y);
+        v[k][0] = lo.x; v[k][1] = lo.y; v[k][2] = hi.x; v[k][3] = hi.y;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[k][j]));
-    }
-    most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 2));
-    int e = 0;
-    if (sizeof(T) == 2 && most > 0.f && most <= 3.402823466e38f) e = min(max(14 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
-    const float up = exp2i(e);
-    row_scale[x] = exp2i(-e) * a.scale;
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      qf[k][x] = pack_half(v[k][0] * up, v[k][1] * up);
-      qf[k][2 + x] = pack_half(v[k][2] * up, v[k][3] * up);
-    }
-  }
-  float o[kCols][4];
-#pragma unroll
-  for (int j = 0; j < kCols; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
-  const int* table = a.tables + r * a.table_stride;
-  bool bad = false;
-  for (int at = warp * 16; at < end; at += kAttWarps * 16) {
-    const int id = table[at >> a.shift];
-    if (id < 0 || id >= a.pages) {                         // no such page: its tokens are not seen
-      bad = true;
-      continue;
-    }
-    const size_t unit = (size_t)id * a.kv_heads + kvh;
-    const size_t base = ((unit << a.shift) + (at & ((1 << a.shift) - 1))) * D;
-    const float ks = a.k_scale[unit], vs = a.v_scale[unit];
-    const float lv = log2f(vs), inv = 1.f / vs;
-    float s[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(a.k_cache + base + (size_t)(8 * t + g) * D + 64 * i + 16 * c);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mma_16816(s[t], qf[4 * i + j], from_e4m3(w[j] & 0xFFFFu), from_e4m3(w[j] >> 16));
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[k][j]));
       }
-    }
-    float p[2][4];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float most = kNone;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float& v = s[t][2 * x + y];
-          v = at + 8 * t + 2 * c + y < row_end[x] ? v * (row_scale[x] * ks) + lv : kNone;
-          most = fmaxf(most, v);
-        }
       most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 1));
       most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 2));
-      const float now = fmaxf(m[x], most), from = now == kNone ? 0.f : now;
-      const float keep = exp2_fast(m[x] - from);
-      m[x] = now;
-      l[x] *= keep;
+      int e = 0;
+      if (most > 0.f && most <= 3.402823466e38f) e = min(max(14 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
+      const float up = exp2i(e);
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        o[j][2 * x] *= keep;
-        o[j][2 * x + 1] *= keep;
+      for (int k = 0; k < D / 16; ++k) {
+        q[k][t][0] = pack_half(v[k][0] * up, v[k][1] * up);
+        q[k][t][1] = pack_half(v[k][2] * up, v[k][3] * up);
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float e = exp2_fast(s[t][2 * x + y] - from);
-          p[t][2 * x + y] = e;
-          l[x] += e * inv;
-        }
+      for (int y = 0; y < 2; ++y) {                        // of the rows in which this lane holds scores
+        const int mine = 2 * c + y;
+        scale[t][y] = exp2i(-__shfl_sync(htr::kFullWarp, e, 4 * mine)) * a.scale;
+        const int at = row0 + 8 * t + mine;
+        end[t][y] = at < rows ? seen - n + at / a.group + 1 : 0;
+      }
     }
-    const uint32_t pf[4] = {pack_half(p[0][0], p[0][1]), pack_half(p[0][2], p[0][3]), pack_half(p[1][0], p[1][1]), pack_half(p[1][2], p[1][3])};
-    uint32_t v[4][kCols / 4];
+  }
+};
+
+// what a warp has in flight: 16 tokens of keys and values of one page
+template <int D>
+struct Tile {
+  uint4 k[2][D / 64];
+  uint32_t v[4][D / 32];
+  float ks, vs;
+  bool real;
+  __device__ __forceinline__ void load(const AttentionArgs& a, int id, int at, int kvh, int lane, bool& bad) {
+    real = id >= 0 && id < a.pages;
+    if (!real) {                                           // no such page: its tokens are not seen
+      bad = true;
+      return;
+    }
+    const int g = lane >> 2, c = lane & 3;
+    const size_t unit = (size_t)id * a.kv_heads + kvh, base = ((unit << a.shift) + (at & ((1 << a.shift) - 1))) * D;
+    const uint8_t *kp = a.k_cache + base + (size_t)g * D + 16 * c, *vp = a.v_cache + base + (size_t)(2 * c) * D + D / 8 * g;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) k[t][i] = *reinterpret_cast<const uint4*>(kp + 8 * t * D + 64 * i);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int token = 2 * c + (x & 1) + 8 * (x >> 1);
-      const uint8_t* src = a.v_cache + base + (size_t)token * D + kCols * g;
-      const bool real = at + token < end;                  // behind the request's tokens lies what an earlier one left
+      const uint8_t* src = vp + ((x & 1) + 8 * (x >> 1)) * D;
       if constexpr (D == 128) {
         const uint4 raw = *reinterpret_cast<const uint4*>(src);
         v[x][0] = raw.x; v[x][1] = raw.y; v[x][2] = raw.z; v[x][3] = raw.w;
@@ -570,56 +541,331 @@ __global__ void __launch_bounds__(kAttWarps * 32) paged_attention_kernel(const A
         const uint2 raw = *reinterpret_cast<const uint2*>(src);
         v[x][0] = raw.x; v[x][1] = raw.y;
       }
-#pragma unroll
-      for (int j = 0; j < kCols / 4; ++j)
-        if (!real) v[x][j] = 0;
     }
+    ks = a.k_scale[unit];
+    vs = a.v_scale[unit];
+  }
+};
+
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {   // 0xFF where a byte is one of e4m3's NaN
+  return __vcmpeq4(v & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+}
+
+// running softmax of a warp: results O^T (dimension D/8 g + 2 j + i / 2, rows 2 c + i % 2), maximum and sum of this lane's rows
+template <int D, int NT>
+struct Running {
+  float o[D / 16][NT][4], m[NT][2], l[NT][2];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < kCols / 4; ++j) {
-      const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5140), a1 = __byte_perm(v[0][j], v[1][j], 0x7362);
-      const uint32_t b0 = __byte_perm(v[2][j], v[3][j], 0x5140), b1 = __byte_perm(v[2][j], v[3][j], 0x7362);
-      mma_16816(o[4 * j], pf, from_e4m3(a0 & 0xFFFFu), from_e4m3(b0 & 0xFFFFu));
-      mma_16816(o[4 * j + 1], pf, from_e4m3(a0 >> 16), from_e4m3(b0 >> 16));
-      mma_16816(o[4 * j + 2], pf, from_e4m3(a1 & 0xFFFFu), from_e4m3(b1 & 0xFFFFu));
-      mma_16816(o[4 * j + 3], pf, from_e4m3(a1 >> 16), from_e4m3(b1 >> 16));
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) o[j][t][0] = o[j][t][1] = o[j][t][2] = o[j][t][3] = 0.f;
+      m[t][0] = m[t][1] = kNone;
+      l[t][0] = l[t][1] = 0.f;
     }
   }
-  if (bad && a.status && lane == 0) atomicOr(a.status, 32);
-  // ---- the warps' parts
+  // 16 tokens from `at` on; `least`: tokens that every row sees, `end`: that some row sees
+  template <typename R>
+  __device__ __forceinline__ void add(Tile<D>& x, const R& rows, int at, int least, int end, int lane) {
+    if (!x.real) return;
+    const int g = lane >> 2, c = lane & 3;
+    float s[NT][4];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    l[x] += __shfl_xor_sync(htr::kFullWarp, l[x], 1);
-    l[x] += __shfl_xor_sync(htr::kFullWarp, l[x], 2);
-    if (c == 0) {
-      s_m[warp][g + 8 * x] = m[x];
-      s_l[warp][g + 8 * x] = l[x];
+    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const uint32_t a[4] = {x.k[0][i].x, x.k[0][i].y, x.k[0][i].z, x.k[0][i].w}, b[4] = {x.k[1][i].x, x.k[1][i].y, x.k[1][i].z, x.k[1][i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a0 = from_e4m3(a[j] & 0xFFFFu), a1 = from_e4m3(b[j] & 0xFFFFu), a2 = from_e4m3(a[j] >> 16), a3 = from_e4m3(b[j] >> 16);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_16816(s[t], a0, a1, a2, a3, rows.q[4 * i + j][t][0], rows.q[4 * i + j][t][1]);
+      }
+    }
+    const float lv = __log2f(x.vs), inv = __fdividef(1.f, x.vs);       // of a power of two: exact
+    const bool edge = at + 16 > least;
+    bool grows = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {                        // token g + 8 (i / 2), row 2 c + i % 2
+        const float v = fmaf(s[t][i], rows.scale[t][i & 1] * x.ks, lv);
+        s[t][i] = edge && at + g + 8 * (i >> 1) >= rows.end[t][i & 1] ? kNone : v;
+        grows |= s[t][i] > m[t][i & 1] + 14.f;
+      }
+    if (__any_sync(htr::kFullWarp, grows)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float most = fmaxf(s[t][y], s[t][2 + y]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, d));
+          const float now = fmaxf(m[t][y], most - 6.f);
+          const float keep = now == kNone ? 1.f : exp2_fast(m[t][y] - now);
+          m[t][y] = now;
+          l[t][y] *= keep;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            o[j][t][y] *= keep;
+            o[j][t][2 + y] *= keep;
+          }
+        }
+    }
+    uint32_t p[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = exp2_fast(s[t][i] - (m[t][i & 1] == kNone ? 0.f : m[t][i & 1]));
+        l[t][i & 1] = fmaf(e[i], inv, l[t][i & 1]);
+      }
+      p[t][0] = transposed(pack_half(e[0], e[1]));
+      p[t][1] = transposed(pack_half(e[2], e[3]));
+    }
+    if (edge) {                                            // tokens that some row or none sees: a NaN there is not for the others
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int token = at + 2 * c + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          if (token >= end) x.v[i][j] = 0;                 // behind the request's tokens lies what an earlier one left
+          if (token >= least) any |= nan_bytes(x.v[i][j]);
+        }
+      }
+      if (__any_sync(htr::kFullWarp, any != 0)) spread_nan(x, rows, at, least, lane);
     }
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {                      // column 2 c + y of tile j: dimension kCols (2 c + y) + j
-      s_o[warp][g + 8 * x][kCols * (2 * c) + j] = o[j][2 * x];
-      s_o[warp][g + 8 * x][kCols * (2 * c + 1) + j] = o[j][2 * x + 1];
+    for (int j = 0; j < D / 32; ++j) {
+      const uint32_t a0 = __byte_perm(x.v[0][j], x.v[1][j], 0x5140), a1 = __byte_perm(x.v[0][j], x.v[1][j], 0x7362);
+      const uint32_t b0 = __byte_perm(x.v[2][j], x.v[3][j], 0x5140), b1 = __byte_perm(x.v[2][j], x.v[3][j], 0x7362);
+      const uint32_t f[8] = {from_e4m3(a0 & 0xFFFFu), from_e4m3(a0 >> 16), from_e4m3(b0 & 0xFFFFu), from_e4m3(b0 >> 16),
+                             from_e4m3(a1 & 0xFFFFu), from_e4m3(a1 >> 16), from_e4m3(b1 & 0xFFFFu), from_e4m3(b1 >> 16)};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        mma_16816(o[2 * j][t], f[0], f[1], f[2], f[3], p[t][0], p[t][1]);
+        mma_16816(o[2 * j + 1][t], f[4], f[5], f[6], f[7], p[t][0], p[t][1]);
+      }
     }
+  }
+  // A NaN among the values of a token that not every row sees would reach them all as 0 * NaN: it is taken out of the fragments and given
+  // to the rows that see it.  The values are spread over the lanes by token, the results by row, both by dimension.
+  template <typename R>
+  __device__ __forceinline__ void spread_nan(Tile<D>& x, const R& rows, int at, int least, int lane) {
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int place = (i & 1) + 8 * (i >> 1);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint32_t mine = at + 2 * c + place >= least ? nan_bytes(x.v[i][j]) : 0;
+        x.v[i][j] &= ~mine;
+#pragma unroll
+        for (int from = 0; from < 4; ++from) {
+          const uint32_t b = __shfl_sync(htr::kFullWarp, mine, (lane & ~3) | from);
+          const int token = at + 2 * from + place;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)                      // dimension 4 j + d of this lane's D / 8: tile 2 j + d / 2, half d % 2
+            if (b >> (8 * d) & 1)
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  if (token < rows.end[t][y]) o[2 * j + (d >> 1)][t][2 * (d & 1) + y] = __int_as_float(0x7FC00000);
+        }
+      }
+    }
+  }
+};
+
+// units of a request: every row tile and key/value head has as many as its tokens fill, at least one (which writes the zeros)
+struct Span {
+  int start, n, seen, rows, units;
+  long long total;
+  __device__ __forceinline__ Span(const AttentionArgs& a, int r, int tile_rows) {
+    start = max(a.starts[r], 0);
+    n = max(min(a.starts[r + 1], a.tokens) - start, 0);
+    seen = min(max(a.seen[r], 0), a.width << a.shift);
+    rows = min(n, a.max_new) * a.group;
+    units = max((seen + kUnit - 1) / kUnit, 1);
+    total = (long long)((rows + tile_rows - 1) / tile_rows) * units * a.kv_heads;
+  }
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attention_kernel(const AttentionArgs a) {
+  constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
+  __shared__ float s_o[kAttWarps][kRows][D + 4];
+  __shared__ float s_m[kAttWarps][kRows], s_l[kAttWarps][kRows];
+  __shared__ long long s_sum[kAttWarps], s_at;
+  __shared__ int s_r;
+  pdl_enter();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  if (tid == 0) a.cuts[blockIdx.x] = {0, 0, 0, 0};
+  // ---- this thread block's run of units
+  const int each = (a.requests + kAttThreads - 1) / kAttThreads, first = min(tid * each, a.requests), last = min(first + each, a.requests);
+  long long mine = 0;
+  for (int r = first; r < last; ++r) mine += Span(a, r, kRows).total;
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(htr::kFullWarp, sum, o);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 31) s_sum[warp] = sum;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kAttWarps; ++w) {
+    if (w < warp) sum += s_sum[w];
+    total += s_sum[w];
+  }
+  const long long share = max((total + gridDim.x - 1) / gridDim.x, 1LL), from = blockIdx.x * share, to = min(from + share, total);
+  if (from >= to) return;
+  sum -= mine;
+  if (sum <= from && from < sum + mine) {
+    int r = first;
+    for (;; ++r) {
+      const long long x = Span(a, r, kRows).total;
+      if (from < sum + x) break;
+      sum += x;
+    }
+    s_r = r;
+    s_at = from - sum;
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < 16 * (D / 2); x += kAttWarps * 32) {
-    const int row = x / (D / 2), d = x % (D / 2) * 2;
-    if (row0 + row >= rows) continue;
-    float most = kNone;
-#pragma unroll
-    for (int w = 0; w < kAttWarps; ++w) most = fmaxf(most, s_m[w][row]);
-    const float from = most == kNone ? 0.f : most;
-    float sum = 0.f, y0 = 0.f, y1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < kAttWarps; ++w) {
-      const float f = exp2_fast(s_m[w][row] - from);
-      sum += f * s_l[w][row];
-      y0 += f * s_o[w][row][d];
-      y1 += f * s_o[w][row][d + 1];
+  int r = s_r;
+  long long skip = s_at, left = to - from;
+  bool bad = false;
+  for (int segment = 0; left > 0; ++segment) {
+    const Span x(a, r, kRows);
+    if (skip >= x.total) {
+      skip -= x.total;
+      ++r;
+      --segment;
+      continue;
     }
-    const float by = sum == 0.f ? 0.f : 1.f / sum;         // a row that sees nothing: zeros
+    const int item = (int)(skip / x.units), u0 = (int)(skip % x.units), u1 = (int)min((long long)x.units, u0 + left);
+    const int kvh = item % a.kv_heads, row0 = item / a.kv_heads * kRows, rows = min(x.rows - row0, kRows);
+    const int last_token = (row0 + rows - 1) / a.group;
+    const int least = max(x.seen - x.n + row0 / a.group + 1, 0), end = max(x.seen - x.n + last_token + 1, 0);
+    Rows<T, D, NT> q;
+    q.load(a, x.start, x.n, x.seen, row0, kvh, lane);
+    Running<D, NT> run;
+    run.clear();
+    // ---- the tokens of this warp: the next 16 and the page after them are on their way while 16 are worked on
+    const int* table = a.tables + r * a.table_stride;
+    const int stop = min(u1 * kUnit, end);
+    int at = u0 * kUnit + warp * 16;
+    int id = at < stop ? table[at >> a.shift] : 0, next_id = at + kUnit < stop ? table[(at + kUnit) >> a.shift] : 0;
+    Tile<D> now, next;
+    if (at < stop) now.load(a, id, at, kvh, lane, bad);
+    while (at < stop) {
+      if (at + kUnit < stop) {
+        id = next_id;
+        if (at + 2 * kUnit < stop) next_id = table[(at + 2 * kUnit) >> a.shift];
+        next.load(a, id, at + kUnit, kvh, lane, bad);
+      }
+      run.add(now, q, at, least, end, lane);
+      at += kUnit;
+      if (at >= stop) break;
+      if (at + kUnit < stop) {
+        id = next_id;
+        if (at + 2 * kUnit < stop) next_id = table[(at + 2 * kUnit) >> a.shift];
+        now.load(a, id, at + kUnit, kvh, lane, bad);
+      }
+      run.add(next, q, at, least, end, lane);
+      at += kUnit;
+    }
+    // ---- the warps' parts
+    if (segment) __syncthreads();                          // those of the last tile have been read
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float l = run.l[t][y];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(htr::kFullWarp, l, o);
+        const int row = 8 * t + 2 * c + y;
+        if (g == 0) {
+          s_m[warp][row] = run.m[t][y];
+          s_l[warp][row] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+          *reinterpret_cast<float2*>(&s_o[warp][row][D / 8 * g + 2 * j]) = make_float2(run.o[j][t][y], run.o[j][t][2 + y]);
+      }
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == x.units;
+    float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPart;
+    for (int z = tid; z < kRows * (D / 4); z += kAttThreads) {
+      const int row = z / (D / 4), d = z % (D / 4) * 4;
+      if (row >= rows) continue;
+      float most = kNone;
+#pragma unroll
+      for (int w = 0; w < kAttWarps; ++w) most = fmaxf(most, s_m[w][row]);
+      float l = 0.f;
+      float4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kAttWarps; ++w) {
+        const float f = most == kNone ? 1.f : exp2_fast(s_m[w][row] - most);
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
+        l = fmaf(f, s_l[w][row], l);
+        y.x = fmaf(f, v.x, y.x); y.y = fmaf(f, v.y, y.y); y.z = fmaf(f, v.z, y.z); y.w = fmaf(f, v.w, y.w);
+      }
+      if (whole) {
+        const float by = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing: zeros
+        const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
+        T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
+        *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};
+      } else {
+        *reinterpret_cast<float4*>(part + row * D + d) = y;
+        if (d == 0) {
+          part[kRows * D + row] = most;
+          part[kRows * D + kRows + row] = l;
+        }
+      }
+    }
+    if (!whole && u0 == 0 && tid == 0) {                   // it begins here and ends elsewhere: request, item, parts, place of the first
+      const long long beyond = x.units - u1;
+      a.cuts[blockIdx.x] = {r, item, 1 + (int)((beyond + share - 1) / share), segment != 0};
+    }
+    skip += u1 - u0;
+    left -= u1 - u0;
+  }
+  if (bad && a.status && lane == 0) atomicOr(a.status, 32);
+}
+
+// Joins the parts of the tiles that were cut: a thread block per run of the launch before.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const AttentionArgs a) {
+  constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
+  pdl_enter();
+  const int4 cut = a.cuts[blockIdx.x];
+  if (cut.z == 0) return;
+  const Span x(a, cut.x, kRows);
+  const int kvh = cut.y % a.kv_heads, row0 = cut.y / a.kv_heads * kRows, rows = min(x.rows - row0, kRows);
+  const float *head = a.parts + ((size_t)blockIdx.x * 2 + cut.w) * kPart, *tail = a.parts + (size_t)blockIdx.x * 2 * kPart;
+  for (int z = threadIdx.x; z < rows * (D / 4); z += kAttThreads) {
+    const int row = z / (D / 4), d = z % (D / 4) * 4;
+    float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
+    float4 y = *reinterpret_cast<const float4*>(head + row * D + d);
+#pragma unroll 4
+    for (int i = 1; i < cut.z; ++i) {
+      const float* part = tail + (size_t)i * 2 * kPart;
+      const float pm = part[kRows * D + row], pl = part[kRows * D + kRows + row];
+      const float4 v = *reinterpret_cast<const float4*>(part + row * D + d);
+      const float now = fmaxf(m, pm), f = now == kNone ? 1.f : exp2_fast(m - now), h = now == kNone ? 1.f : exp2_fast(pm - now);
+      m = now;
+      l = l * f + pl * h;
+      y.x = y.x * f + v.x * h; y.y = y.y * f + v.y * h; y.z = y.z * f + v.z * h; y.w = y.w * f + v.w * h;
+    }
+    const float by = l == 0.f ? 0.f : 1.f / l;
     const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
-    T* dst = static_cast<T*>(a.out) + ((size_t)(start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
-    *reinterpret_cast<uint32_t*>(dst) = Half<T>::narrow(y0 * by, y1 * by);
+    T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
+    *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};
   }
 }
 
@@ -632,11 +878,32 @@ int page_shift(int page_size) {
   return -1;
 }
 
+int device_sms() {
+  static int cache[64] = {0};
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
+  if (dev >= 0 && dev < 64) cache[dev] = v;
+  return v;
+}
+
+int attention_blocks(int head_dim, int tiles) {            // what the GPU holds at a time
+  return device_sms() * (head_dim == 128 ? (tiles == 1 ? kAttBlocks<128, 1> : kAttBlocks<128, 2>) : tiles == 1 ? kAttBlocks<64, 1> : kAttBlocks<64, 2>);
+}
+int attention_tiles(int group, int max_new) { return (long long)group * max_new <= 8 ? 1 : 2; }
+
+template <typename T, int D, int NT>
+int attention_run(const AttentionArgs& a, cudaStream_t st) {
+  const dim3 grid(attention_blocks(D, NT)), block(kAttThreads);
+  const int rc = launch(paged_attention_kernel<T, D, NT>, grid, block, 1, 0, st, a);
+  return rc != HTR_OK ? rc : launch(paged_attention_join_kernel<T, D, NT>, grid, block, 1, 0, st, a);
+}
+
 template <typename T>
 int attention_of(const AttentionArgs& a, int head_dim, int max_new, cudaStream_t st) {
-  const dim3 grid((unsigned)(((long long)max_new * a.group + 15) / 16), a.kv_heads, a.requests);
-  return head_dim == 128 ? launch(paged_attention_kernel<T, 128>, grid, dim3(kAttWarps * 32), 1, 0, st, a)
-                         : launch(paged_attention_kernel<T, 64>, grid, dim3(kAttWarps * 32), 1, 0, st, a);
+  if (attention_tiles(a.group, max_new) == 1) return head_dim == 128 ? attention_run<T, 128, 1>(a, st) : attention_run<T, 64, 1>(a, st);
+  return head_dim == 128 ? attention_run<T, 128, 2>(a, st) : attention_run<T, 64, 2>(a, st);
 }
 
 template <typename T>
@@ -697,7 +964,12 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
   return dtype == HTR_DTYPE_BF16 ? append_of<__nv_bfloat16>(a, head_dim, grid, st) : append_of<__half>(a, head_dim, grid, st);
 }
 
-size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new) { return 0; }
+size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new) {
+  if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_new < 1 || (head_dim != 64 && head_dim != 128)) return 0;
+  const int tiles = attention_tiles(q_heads / kv_heads, max_new);
+  const size_t rows = 8 * tiles;
+  return attention_blocks(head_dim, tiles) * (2 * rows * (head_dim + 2) * sizeof(float) + sizeof(int4));
+}
 
 int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts, const int* seen, int requests, const int* tables,
                         int64_t table_stride, int table_width, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
@@ -709,14 +981,17 @@ int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts,
       q_heads % kv_heads || pages < 1 || shift < 0 || max_new < 1)
     return HTR_ERR_BAD_SHAPE;
   if (requests > 8192 || kv_heads > 16384 || q_heads > 16384 || tokens > 1 << 30 || (int64_t)max_new * (q_heads / kv_heads) > 1 << 30 ||
-      (int64_t)pages << shift > 0x7FFFFFFF || (int64_t)table_width << shift > 0x7FFFFFFF)
+      (int64_t)pages << shift > 0x7FFFFFFF || (int64_t)table_width << shift > 1 << 30)
     return HTR_ERR_TOO_LARGE;
   if (tokens == 0) return HTR_OK;
   if (!q || !starts || !seen || !tables || !k_cache || !v_cache || !k_scale || !v_scale || !out) return HTR_ERR_NULL;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return HTR_ERR_ALIGNMENT;
-  const AttentionArgs a = {q, starts, seen, tables, table_stride, table_width, requests, tokens, q_heads, kv_heads, q_heads / kv_heads,
+  if (!workspace || workspace_bytes < htr_paged_attention_workspace_bytes(tokens, requests, q_heads, kv_heads, head_dim, max_new)) return HTR_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return HTR_ERR_ALIGNMENT;
+  int4* cuts = static_cast<int4*>(workspace);
+  const AttentionArgs a = {q, starts, seen, tables, table_stride, table_width, requests, tokens, q_heads, kv_heads, q_heads / kv_heads, max_new,
                            static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), k_scale, v_scale, pages, shift,
-                           scale * 1.4426950408889634f, out, status};
+                           scale * 1.4426950408889634f, out, status, reinterpret_cast<float*>(cuts + attention_blocks(head_dim, attention_tiles(q_heads / kv_heads, max_new))), cuts};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == HTR_DTYPE_BF16 ? attention_of<__nv_bfloat16>(a, head_dim, max_new, st) : attention_of<__half>(a, head_dim, max_new, st);
 }

@@ -380,6 +380,25 @@ def test_rows_that_see_nothing_and_rows_behind_the_last():
 
 
 @gpu
+@pytest.mark.parametrize("adds", ((3, 1), (9, 2), (100, 1)))
+def test_a_nan_reaches_only_those_that_see_it(adds):
+    """Keys and values of a step's later tokens, and all behind the last, may be NaN: earlier tokens do not see them."""
+    q, starts, seen, tables, cache = filled(torch.bfloat16, 128, 16, 8, 2, (40, 17), adds)
+    from htr_b200 import paged
+
+    want = paged.attention(q, starts, seen, tables, cache, max(adds))
+    at, n = 40 + adds[0] - 2, adds[0]                            # the last token but one of request 0
+    page = int(tables[0, at // 16])
+    cache.v.view(torch.uint8)[page, 1, at % 16, 5] = 0xFF
+    cache.k.view(torch.uint8)[page, 0, at % 16, 77] = 0x7F
+    got = paged.attention(q, starts, seen, tables, cache, max(adds))
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[n - 2:n, :4] = True                                      # a NaN key takes the whole result of its heads
+    hit[n - 2:n, 4:, 5] = True                                   # a NaN value its dimension
+    assert torch.equal(got.isnan(), hit) and torch.equal(got[~hit], want[~hit])
+
+
+@gpu
 @pytest.mark.parametrize("adds", ((1, 1), (40, 1)))
 def test_table_entries_that_are_no_page_hide_their_tokens(adds):
     from htr_b200 import paged
