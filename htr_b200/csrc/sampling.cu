@@ -35,7 +35,7 @@ constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8, kBins = 2048;
 constexpr double kOne = 4398046511104.0;                   // 2^42: sums of up to 2^20 weights fit in 62 bits
 using u64 = unsigned long long;
-constexpr u64 kMark = 1ull << 63;                          // on the one message of a cluster that counts
+constexpr uint32_t kNegative = 0x7FFFFFFFu - 0x3B800000u;   // the key of -2^-8
 
 // unsigned order of floats; NaN and -infinity are 0, below everything that can be chosen
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -50,23 +50,67 @@ struct Logit {
   static constexpr int kBytes = DT == HTR_DTYPE_F32 ? 4 : 2;
   // keys of two different logits are at least 2^kGap apart
   static constexpr int kGap = DT == HTR_DTYPE_F32 ? 0 : DT == HTR_DTYPE_BF16 ? 16 : 13;
-  static __device__ __forceinline__ float wide(uint16_t raw) {
-    return DT == HTR_DTYPE_BF16 ? __uint_as_float((uint32_t)raw << 16) : __half2float(*reinterpret_cast<const __half*>(&raw));
+  static constexpr uint32_t kLowest = DT == HTR_DTYPE_F32 ? 0xFF800000u : DT == HTR_DTYPE_BF16 ? 0xFF80u : 0xFC00u;     // -infinity
+  // logit j of a vector of 16 bytes
+  static __device__ __forceinline__ float at(const uint4& v, int j) {
+    const int x = DT == HTR_DTYPE_F32 ? j : j >> 1;
+    const uint32_t w = x == 0 ? v.x : x == 1 ? v.y : x == 2 ? v.z : v.w;
+    if (DT == HTR_DTYPE_F32) return __uint_as_float(w);
+    if (DT == HTR_DTYPE_BF16) return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return j & 1 ? __high2float(h) : __low2float(h);
   }
-  static __device__ __forceinline__ uint32_t key(const char* row, int i) {
-    if (DT == HTR_DTYPE_F32) return key_of(reinterpret_cast<const float*>(row)[i]);
-    return key_of(wide(reinterpret_cast<const uint16_t*>(row)[i]));
+  // the largest of a vector, NaN left aside
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    if constexpr (DT == HTR_DTYPE_F32) {
+      return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else if constexpr (DT == HTR_DTYPE_BF16) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+      const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      return fmaxf(f.x, f.y);
+    } else {
+      const __half2* h = reinterpret_cast<const __half2*>(&v);
+      const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      return fmaxf(f.x, f.y);
+    }
+  }
+  // the key in [low, high], of which there is one: logits of 16 bits end in zeros, keys of negative ones in ones
+  static __device__ __forceinline__ uint32_t only(uint32_t low, uint32_t high) {
+    const uint32_t rest = (1u << kGap) - 1, positive = high & ~rest;
+    return high >= 0x80000000u && positive >= low ? positive : ((min(high, 0x7FFFFFFFu) + 1) & ~rest) - 1;
   }
 };
 
+// 2^42 exp((logit - max) / temperature) to the nearest integer, by a table of 2^(j / 64) and a polynomial of the fourth degree between its
+// entries (the table-driven exponential of Tang, 1989): off by 2^-44 of the largest weight before it is rounded.  The double exp of the
+// math library is right to its last bit and took most of a sample's time.
 struct Weigh {
-  double max, inv;
+  double max, by;                                          // by = 64 log2(e) / temperature
+  bool infinite;
+  const double* table;
+  uint32_t top_key;
+  const u64* known;                                        // bf16: of the 2048 values from the largest on and as many from -2^-8 on; or none
   __device__ __forceinline__ u64 operator()(uint32_t key) const {
-    if (key == 0) return 0;
-    const double x = (double)logit_of(key);
-    if (x == max) return (u64)kOne;
-    if (isinf(max)) return 0;
-    return (u64)rint(exp((x - max) * inv) * kOne);
+    if (known) {
+      if (top_key - key < (uint32_t)kBins << 16) return known[(top_key - key) >> 16];
+      if (kNegative - key < (uint32_t)kBins << 16) return known[kBins + ((kNegative - key) >> 16)];
+    }
+    return computed(key);
+  }
+  __device__ __forceinline__ u64 computed(uint32_t key) const {
+    if (infinite) return key == top_key ? (u64)kOne : 0;
+    constexpr double kShift = 6755399441055744.0;          // 1.5 * 2^52: its low word then holds the rounded sum
+    const double d = (double)logit_of(key) - max, z = fma(d, by, kShift);
+    const int k = __double2loint(z);
+    if (__double2hiint(z) < 0x4337FFFF || k < -45 * 64 || key == 0) return 0;
+    const double r = fma(d, by, -(z - kShift)), t = table[k & 63];
+    // 2^(r / 64) = 1 + r (c1 + r (c2 + ...)), c_i = (ln 2 / 64)^i / i!
+    double p = fma(r, 5.732851688640402e-10, 2.1173137155464774e-07);
+    p = fma(r, p, 5.864904955056169e-05);
+    p = fma(r, p, 1.0830424696249145e-02);
+    const double w = fma(t * r, p, t);                     // [2^(k / 64)] without its whole power
+    const double v = __hiloint2double(__double2hiint(w) + ((k >> 6) + 42) * (1 << 20), __double2loint(w));
+    return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;     // 2^52 + v: v to the nearest integer
   }
 };
 
@@ -95,17 +139,21 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
   return v;
 }
 
+template <int DT>
 struct Shared {
+  u64 known[DT == HTR_DTYPE_BF16 ? 2 * kBins : 2];
   unsigned count[kBins], lo[kBins], hi[kBins];             // of a range of keys: tokens, and their weight in two words
-  u64 red[2][kWarps];
+  u64 red[2][kWarps], ahead[2][kWarps];                    // of the warps: what each has, and what those before it have
+  double table[64];
   u64 mail[2][4];                                          // what the thread blocks of a cluster tell one another, in turns
+  u64 told[4];                                             // what its first warp tells a thread block
 };
 
 template <typename V>
 __device__ __forceinline__ V remote(const V* mine, unsigned rank) {
   uint32_t at;
   V v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
   if constexpr (sizeof(V) == 8) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
   else asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
@@ -113,343 +161,370 @@ __device__ __forceinline__ V remote(const V* mine, unsigned rank) {
 
 // A cluster of thread blocks per row, each with a contiguous slice of it, which it reads from memory once, into shared memory (rows too
 // long for that are read again from L2).
-// What bounds it: the passes over a slice (an exponential in double for every token that a sum needs) and the exchanges between thread
-// blocks, about 1 us each, not the bytes.  So:
-//  * a border is found by histograms over ranges of keys (the bits of the logits in their order): 2048 bins, first over the tokens
-//    within 12 nats of the largest, where borders usually lie, then inside the bin that holds the border until it holds one value:
-//    one or two passes for 16-bit logits, two or three for float32, and exponentials only for the tokens inside the range;
-//  * thread blocks meet in shared memory of the cluster: sums of bins are split among them, and each tells only a total.
+// What bounds it: instructions of the passes over a slice, and the exchanges between thread blocks (about 1 us each), not the bytes.  So:
+//  * a border is found by histograms over ranges of keys (the bits of the logits in their order), 2048 bins at a time, then inside the bin that
+//    holds the border until a bin is one value.  Counts alone are enough where bins are single values from the start (16-bit logits:
+//    the upper 16 binades of bf16 and as many negative ones): a bin weighs its count times one exponential.  Other tokens need an
+//    exponential each, float32 ones above all, whose first range is the 12 nats below the largest, where borders usually lie;
+//  * eight logits are compared with the lower end of a range at once: most passes meet few that matter;
+//  * thread blocks meet in shared memory of the cluster: bins are split among them, each tells only totals, and the first warp of each
+//    does the arithmetic of an exchange for all (64-bit scans in all 32 warps had been most of a small row's instructions).
 template <int DT>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, int per, int staged) {
   using L = Logit<DT>;
-  extern __shared__ __align__(16) char stage[];
-  __shared__ Shared s;
+  constexpr int kVec = 16 / L::kBytes;
+  extern __shared__ __align__(16) char smem[];
+  Shared<DT>& s = *reinterpret_cast<Shared<DT>*>(smem);
+  char* stage = smem + sizeof(Shared<DT>);
+  static_assert(sizeof(Shared<DT>) % 16 == 0, "the row's slice behind it is read in vectors");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned rank, size;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-  const int r = blockIdx.x / size, begin = min((int)rank * per, a.vocab), n = min(begin + per, a.vocab) - begin;
+  const int r = blockIdx.x / size, begin = min((int)rank * per, a.vocab), n = min(begin + per, a.vocab) - begin, vectors = (n + kVec - 1) / kVec;
   const char* src = static_cast<const char*>(a.logits) + ((size_t)r * a.row_stride + begin) * L::kBytes;
-  int turn = 0;                                            // of s.mail: a message is written over two exchanges later, when all have read it
+  const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  const float t = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
+  const int k = a.top_k ? a.top_k[r] : 0;
+  const float u = fminf(fmaxf(a.u[r], 0.f), 0.99999994f);
   const auto barrier = [&] {
     if (size > 1) htr::cluster_sync();
     else __syncthreads();
   };
-  // ---- the largest, and the first index that has it
-  u64 top = 0;
-  const auto look = [&](uint32_t key, int i) {
-    const u64 v = (u64)key << 32 | (0xFFFFFFFFu - (unsigned)(begin + i));
-    top = v > top ? v : top;
-  };
-  constexpr int kVec = 16 / L::kBytes;
-  const int whole = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / kVec : 0;
-#pragma unroll 4
-  for (int x = tid; x < whole; x += kThreads) {
-    const uint4 raw = reinterpret_cast<const uint4*>(src)[x];
-    if (staged) reinterpret_cast<uint4*>(stage)[x] = raw;
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  // kVec logits; -infinity behind the last
+  const auto from_memory = [&](int x) {
+    if (aligned && (x + 1) * kVec <= n) return reinterpret_cast<const uint4*>(src)[x];
+    uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (DT == HTR_DTYPE_F32) {
-        look(key_of(__uint_as_float(w[j])), 4 * x + j);
+        const int i = 4 * x + j;
+        w[j] = i < n ? reinterpret_cast<const uint32_t*>(src)[i] : L::kLowest;
       } else {
-        look(key_of(L::wide((uint16_t)w[j])), 8 * x + 2 * j);
-        look(key_of(L::wide((uint16_t)(w[j] >> 16))), 8 * x + 2 * j + 1);
+        const int i = 8 * x + 2 * j;
+        const uint16_t* at = reinterpret_cast<const uint16_t*>(src) + i;
+        w[j] = (i < n ? at[0] : L::kLowest) | (uint32_t)(i + 1 < n ? at[1] : L::kLowest) << 16;
       }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  const auto fetch = [&](int x) { return staged ? reinterpret_cast<const uint4*>(stage)[x] : from_memory(x); };
+  int turn = 0;                                            // of s.mail: a message is written over two exchanges later, when all have read it
+  // ---- the largest
+  float most = -__builtin_huge_valf();
+#pragma unroll 2
+  for (int x = tid; x < vectors; x += kThreads) {
+    const uint4 w = from_memory(x);
+    if (staged) reinterpret_cast<uint4*>(stage)[x] = w;
+    most = fmaxf(most, L::largest(w));
   }
-#pragma unroll 4
-  for (int i = whole * kVec + tid; i < n; i += kThreads) {
-    if constexpr (DT == HTR_DTYPE_F32) {
-      const float f = reinterpret_cast<const float*>(src)[i];
-      if (staged) reinterpret_cast<float*>(stage)[i] = f;
-      look(key_of(f), i);
-    } else {
-      const uint16_t raw = reinterpret_cast<const uint16_t*>(src)[i];
-      if (staged) reinterpret_cast<uint16_t*>(stage)[i] = raw;
-      look(key_of(L::wide(raw)), i);
+  if (tid < 64) s.table[tid] = exp2(tid / 64.0);
+  if (tid == 64) s.mail[0][3] = s.mail[1][3] = 0;
+  // of all threads of the cluster: the largest of a 32-bit value
+  const auto largest_of = [&](uint32_t v) {
+    v = __reduce_max_sync(htr::kFullWarp, v);
+    if (lane == 0) s.red[0][warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+      v = __reduce_max_sync(htr::kFullWarp, (uint32_t)s.red[0][lane]);
+      if (lane == 0) s.mail[turn][0] = v;
     }
-  }
-  if (staged) src = stage;
+    barrier();
+    v = __reduce_max_sync(htr::kFullWarp, lane < size ? (uint32_t)remote(&s.mail[turn][0], lane) : 0u);
+    turn ^= 1;
+    return v;
+  };
+  const uint32_t top_key = largest_of(key_of(most));
+  if (top_key == 0 || !(t > 0.f)) {                        // nothing to choose from; greedy: the first index that has it
+    uint32_t at = 0xFFFFFFFFu;
+    for (int x = tid; x < vectors && top_key; x += kThreads) {
+      const uint4 w = fetch(x);
+      if (key_of(L::largest(w)) != top_key) continue;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const u64 v = __shfl_xor_sync(htr::kFullWarp, top, o);
-    top = v > top ? v : top;
-  }
-  if (lane == 0) s.red[0][warp] = top;
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) top = s.red[0][w] > top ? s.red[0][w] : top;
-  if (tid == 0) s.mail[turn][0] = top;
-  barrier();
-  for (unsigned c = 0; c < size; ++c) {
-    const u64 v = remote(&s.mail[turn][0], c);
-    top = v > top ? v : top;
-  }
-  turn ^= 1;
-  const uint32_t top_key = (uint32_t)(top >> 32);
-  const float t = a.temperature ? a.temperature[r] : 1.f;
-  if (top_key == 0 || !(t > 0.f)) {                        // nothing to choose from; greedy
+      for (int j = kVec - 1; j >= 0; --j)
+        if (key_of(L::at(w, j)) == top_key) at = min(at, (uint32_t)(begin + x * kVec + j));
+    }
+    at = ~largest_of(~at);
     if (tid == 0 && rank == 0) {
-      a.tokens[r] = top_key == 0 ? -1 : (long long)(0xFFFFFFFFu - (uint32_t)top);
+      a.tokens[r] = top_key == 0 ? -1 : (long long)at;
       if (a.logprobs) a.logprobs[r] = top_key == 0 ? __int_as_float(0x7FC00000) : 0.f;
     }
     barrier();                                             // no thread block leaves while another reads its memory
     return;
   }
-  const Weigh weigh = {(double)logit_of(top_key), 1.0 / (double)t};
-  const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
+  Weigh weigh = {(double)logit_of(top_key), 64 * 1.4426950408889634 / (double)t, isinf(logit_of(top_key)) != 0, s.table, top_key, nullptr};
   const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
-  const double bound = least > 0.f ? (double)fminf(least, 1.f) * kOne : 0.0;
-  // ---- the border: keys above `high` are kept, and of those in [low, high], which are all equal, the first `ties`
+  const u64 bound = least > 0.f ? (u64)ceil((double)fminf(least, 1.f) * kOne) : 0;
+  if constexpr (DT == HTR_DTYPE_BF16) {
+    if (!by_k) {                                           // all tokens will be weighed: their values are fewer
+      for (int b = tid; b < 2 * kBins; b += kThreads) {
+        const uint32_t from = b < kBins ? top_key : kNegative, step = (uint32_t)(b & (kBins - 1)) << 16;
+        s.known[b] = from > step ? weigh.computed(from - step) : 0;
+      }
+      weigh.known = s.known;
+      __syncthreads();
+    }
+  }
+  // ---- the border: keys above `high` are kept, and of the `tied` tokens in [low, high], which are all equal, the first `ties`
   uint32_t low = 0, high = 0;
-  unsigned ties = 0xFFFFFFFFu;
-  // sums of the cluster, of two values of every thread
-  const auto sum_all = [&](u64& x, u64& y) {
-    x = warp_sum(x);
-    y = warp_sum(y);
-    if (lane == 0) {
-      s.red[0][warp] = x;
-      s.red[1][warp] = y;
-    }
-    __syncthreads();
-    if (warp == 0) {
-      x = warp_sum(s.red[0][lane]);
-      y = warp_sum(s.red[1][lane]);
-      if (lane == 0) {
-        s.mail[turn][0] = x;
-        s.mail[turn][1] = y;
+  unsigned ties = 0xFFFFFFFFu, tied = 0;
+  u64 mark = 0;                                            // of the message, one of the cluster's, that tells a border: counts them
+  // finds the border at which the tokens reach `count`, or their weight `part` of that of all that have been kept so far
+  const auto find = [&](bool counts, u64 count, float part) {
+    u64 above = 0, target = count;
+    uint32_t hi = top_key, lo = 0;
+    for (bool first = true;; first = false) {
+      if (first) {                                         // 16-bit logits: as many values as there are bins
+        lo = L::kGap ? (hi > (uint32_t)(kBins - 1) << L::kGap ? hi - ((uint32_t)(kBins - 1) << L::kGap) : 0)
+                     : key_of((float)(weigh.max - 12.0 * (double)t));
+        lo = max(weigh.infinite ? hi : lo, low);
       }
-    }
-    barrier();
-    x = y = 0;
-    for (unsigned c = 0; c < size; ++c) {
-      x += remote(&s.mail[turn][0], c);
-      y += remote(&s.mail[turn][1], c);
-    }
-    turn ^= 1;
-  };
-  // the border at which the tokens, or their weight, reach `target`
-  const auto find = [&](bool counts, u64 target) {
-    u64 above = 0;
-    uint32_t hi = top_key, lo = max(key_of((float)(weigh.max - 12.0 * (double)t)), low);
-    if (isinf(weigh.max) || lo > hi) lo = hi;
-    for (;;) {
-      int shift = 32 - __clz(hi - lo) - 11;                // at most kBins bins
-      if (shift < 0) shift = 0;
-      if (hi - lo >> shift >= kBins) ++shift;
-      for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
+      const int shift = max(21 - __clz(hi - lo), 0);       // at most kBins bins
+      const bool single = L::kGap && shift <= L::kGap;     // bins are single values
+      const bool sums = first && !counts;                  // the weight of all is needed
+      const bool below = sums && L::kGap == 16;            // the negative values from -2^-8 to -2^8 have bins too, in s.hi
+      for (int b = tid; b < kBins; b += kThreads) {
+        s.count[b] = s.hi[b] = 0;
+        if (!single) s.lo[b] = 0;
+      }
       __syncthreads();
-#pragma unroll 4
-      for (int i = tid; i < n; i += kThreads) {
-        const uint32_t key = L::key(src, i);
-        if (key < lo || key > hi) continue;
-        const int b = (hi - key) >> shift;
-        atomicAdd(&s.count[b], 1u);
-        if (!counts) {
-          const u64 w = weigh(key);
-          const unsigned x = (unsigned)w, was = atomicAdd(&s.lo[b], x), y = (unsigned)(w >> 32) + (was + x < x);
-          if (y) atomicAdd(&s.hi[b], y);
+      u64 rest = 0;                                        // the weight of tokens without a bin
+      const uint32_t from_key = sums ? low : lo;
+      const float from = from_key < 0x00800000u ? -3.402823466e38f : logit_of(from_key);
+      for (int x = tid; x < vectors; x += kThreads) {
+        const uint4 w = fetch(x);
+        if (!(L::largest(w) >= from)) continue;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const uint32_t key = key_of(L::at(w, j));
+          if (key > hi || key < from_key || key == 0) continue;
+          if (key >= lo) {
+            const int b = (hi - key) >> shift;
+            atomicAdd(&s.count[b], 1u);
+            if (counts || single) continue;
+            const u64 v = weigh(key);
+            const unsigned y = (unsigned)v, was = atomicAdd(&s.lo[b], y), z = (unsigned)(v >> 32) + (was + y < y);
+            if (z) atomicAdd(&s.hi[b], z);
+          } else if (below && single && kNegative - key < (uint32_t)kBins << 16) {
+            atomicAdd(&s.hi[(kNegative - key) >> 16], 1u);
+          } else {
+            rest += weigh(key);
+          }
         }
       }
       barrier();
-      // this thread block's share of the bins, over the cluster
-      const int share = kBins / size, b = rank * share + tid;
-      u64 value = 0, tokens = 0;
-      if (tid < share)
-        for (unsigned c = 0; c < size; ++c) {
-          const unsigned m = remote(&s.count[b], c);
-          tokens += m;
-          value += counts ? m : (u64)remote(&s.hi[b], c) << 32;
-          if (!counts) value += remote(&s.lo[b], c);
+      // this thread block's share of the bins, over the cluster: one or two for each of its first threads
+      const int share = kBins / size, each = share > kThreads ? 2 : 1, b0 = rank * share + each * tid;
+      u64 value[2] = {0, 0}, end = 0;
+      unsigned tokens[2] = {0, 0};
+      if (warp * 32 * each < share) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (j >= each) continue;
+          const int b = b0 + j;
+          unsigned more = 0;
+          u64 mass = 0;
+#pragma unroll
+          for (int c = 0; c < kMaxCluster; ++c)
+            if (c < (int)size) {
+              tokens[j] += remote(&s.count[b], c);
+              if (counts) continue;
+              if (single) {
+                if (below) more += remote(&s.hi[b], c);
+              } else {
+                mass += ((u64)remote(&s.hi[b], c) << 32) + remote(&s.lo[b], c);
+              }
+            }
+          if (single && !counts) {
+            const uint32_t top_of = hi - ((uint32_t)b << shift);
+            if (tokens[j]) mass = tokens[j] * weigh(L::only(top_of - min((1u << shift) - 1, top_of), top_of));
+            if (more) rest += more * weigh(kNegative - ((uint32_t)b << 16));
+          }
+          value[j] = counts ? tokens[j] : mass;
         }
-      // (with one thread block a thread takes two bins)
-      u64 value2 = 0, tokens2 = 0;
-      if (share > kThreads) {
-        const int b0 = 2 * tid;
-        tokens = s.count[b0];
-        value = counts ? tokens : ((u64)s.hi[b0] << 32) + s.lo[b0];
-        tokens2 = s.count[b0 + 1];
-        value2 = counts ? tokens2 : ((u64)s.hi[b0 + 1] << 32) + s.lo[b0 + 1];
+        end = warp_scan(value[0] + value[1], lane);
       }
-      u64 end = warp_scan(value + value2, lane);
       if (lane == 31) s.red[0][warp] = end;
-      __syncthreads();
-      u64 before = 0, total = 0;
-      {
-        const u64 v = s.red[0][lane], e = warp_scan(v, lane);
-        before = __shfl_sync(htr::kFullWarp, e - v, warp);
-        total = __shfl_sync(htr::kFullWarp, e, 31);
+      if (sums) {
+        rest = warp_sum(rest);
+        if (lane == 0) s.red[1][warp] = rest;
       }
-      if (tid == 0) s.mail[turn][0] = total;
+      __syncthreads();
+      if (warp == 0) {
+        const u64 v = s.red[0][lane], e = warp_scan(v, lane);
+        s.ahead[0][lane] = e - v;
+        rest = sums ? warp_sum(s.red[1][lane]) : 0;
+        if (lane == 31) {
+          s.mail[turn][0] = e;
+          s.mail[turn][1] = rest;
+        }
+      }
       barrier();
-      u64 all = above;
-      for (unsigned c = 0; c < size; ++c) {
-        const u64 v = remote(&s.mail[turn][0], c);
-        if (c < rank) before += v;
-        all += v;
+      if (warp == 0) {
+        const u64 v = lane < size ? remote(&s.mail[turn][0], lane) : 0, before = warp_sum(lane < rank ? v : 0), all = warp_sum(v);
+        rest = sums ? warp_sum(lane < size ? remote(&s.mail[turn][1], lane) : 0) : 0;
+        if (lane == 0) {
+          s.told[0] = above + before;
+          s.told[1] = above + all;
+          s.told[2] = above + all + rest;
+        }
       }
       turn ^= 1;
+      __syncthreads();
+      const u64 all = s.told[1];
+      if (sums) {
+        u64 kept = s.told[2];
+        if (tied > ties) kept -= (u64)(tied - ties) * weigh(L::only(low, high));
+        target = max(part_of(kept, part, true), (u64)1);
+      }
       if (all < target) {                                  // the border lies below this range
         above = all;
-        if (lo <= low || lo == 0) {                        // (a target that rounding puts beyond everything: all are kept)
-          return;
-        }
+        if (lo <= low) return;                             // (nothing is left: all that was kept is)
         hi = lo - 1;
         lo = low;
         continue;
       }
-      before += above + end - value - value2;
-      if (before < target && before + value + value2 >= target) {
-        const bool second = before + value < target;
-        const int at = share > kThreads ? 2 * tid + second : b;
-        const u64 from = second ? before + value : before;
-        s.mail[turn][0] = at;
-        s.mail[turn][1] = from;
-        s.mail[turn][2] = second ? value2 : value;
-        s.mail[turn][3] = (second ? tokens2 : tokens) | kMark;
+      mark += 1ull << 32;
+      const u64 before = s.told[0] + s.ahead[0][warp] + end - value[0] - value[1];
+      if (before < target && before + value[0] + value[1] >= target) {
+        const bool second = before + value[0] < target;
+        s.mail[turn][0] = b0 + second;
+        s.mail[turn][1] = before + (second ? value[0] : 0);
+        s.mail[turn][2] = second ? value[1] : value[0];
+        s.mail[turn][3] = (second ? tokens[1] : tokens[0]) | mark;
       }
       barrier();
-      u64 bin = 0, from = 0, mass = 0, in = 0;
-      for (unsigned c = 0; c < size; ++c) {
-        const u64 m = remote(&s.mail[turn][3], c);
-        if (m & kMark) {
-          in = m & ~kMark;
-          bin = remote(&s.mail[turn][0], c);
-          from = remote(&s.mail[turn][1], c);
-          mass = remote(&s.mail[turn][2], c);
-        }
+      if (warp == 0) {
+        const u64 in = lane < size ? remote(&s.mail[turn][3], lane) : 0;
+        const int owner = __ffs(__ballot_sync(htr::kFullWarp, in >> 32 == mark >> 32)) - 1;
+        if (lane < 4) s.told[lane] = remote(&s.mail[turn][lane], owner);
       }
-      barrier();
-      if (tid == 0) s.mail[turn][3] = 0;
-      const uint32_t new_hi = hi - ((uint32_t)bin << shift), step = (1u << shift) - 1, new_lo = new_hi - lo > step ? new_hi - step : lo;
-      if (shift <= L::kGap || in == 1) {                   // one value
-        const u64 each = counts ? 1 : mass / in;
-        const u64 need = each ? (target - from + each - 1) / each : in;
-        low = new_lo;
-        high = new_hi;
-        ties = (unsigned)min(max(need, (u64)1), (u64)0xFFFFFFFFu);
+      turn ^= 1;
+      __syncthreads();
+      const uint32_t in = (uint32_t)s.told[3];
+      const u64 mass = s.told[2], so_far = s.told[1];
+      hi -= (uint32_t)s.told[0] << shift;
+      if (hi - lo >> shift) lo = hi - ((1u << shift) - 1);
+      if (shift <= L::kGap) {                              // one value
+        const u64 one = counts ? 1 : mass / in, need = one ? (target - so_far + one - 1) / one : in;
+        low = lo;
+        high = hi;
+        tied = in;
+        ties = (unsigned)min(max(need, (u64)1), (u64)in);
         return;
       }
-      above = from;
-      hi = new_hi;
-      lo = new_lo;
+      above = so_far;
     }
   };
-  if (tid == 0) s.mail[0][3] = s.mail[1][3] = 0;
-  __syncthreads();
-  if (by_k) find(true, (u64)k);
-  if (by_p) {
-    u64 all = 0, tied = 0, each = 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const uint32_t key = L::key(src, i);
-      if (key > high) {
-        all += weigh(key);
-      } else if (key >= low && key) {
-        ++tied;
-        each = weigh(key);
-      }
-    }
-    u64 none = 0;
-    if (by_k) {                                            // every tie weighs the same
-      each *= tied;
-      sum_all(each, tied);
-      if (tied) each = each / tied * min(tied, (u64)ties);
-    }
-    sum_all(all, none);
-    find(false, max(part_of(all + each, p, true), (u64)1));
+  if (by_k) find(true, (u64)k, 0.f);
+  if (by_p) find(false, 0, p);
+  // ---- the token: a warp takes consecutive tokens, a lane kVec at a time
+  const float from = low < 0x00800000u ? -3.402823466e38f : logit_of(low);
+  const int seg = ((vectors + kWarps - 1) / kWarps + 31) / 32 * 32, first = min(warp * seg, vectors), last = min(first + seg, vectors);
+  u64 each = 0;                                            // the weight of a tie
+  if (tied) {
+    each = weigh(L::only(low, high));
+    if (each < bound) each = 0;
   }
-  // ---- the token: a warp takes consecutive tokens
-  const int seg = (n + kWarps - 1) / kWarps, first = min(warp * seg, n), last = min(first + seg, n);
-  const auto kept = [&](uint32_t key, bool& tie) -> u64 {   // the weight of a token that is kept, or may be: a tie
-    tie = false;
-    if (key == 0 || key < low) return 0;
-    const u64 w = weigh(key);
-    if ((double)w < bound) return 0;
-    tie = key <= high;
-    return w;
-  };
-  u64 mine = 0, tied = 0, each = 0;
-  for (int i = first + lane; i < last; i += 32) {
-    bool tie;
-    const u64 w = kept(L::key(src, i), tie);
-    if (tie) {
-      ++tied;
-      each = w;
-    } else {
-      mine += w;
+  // of a lane's vector: the weight of what lies above the border, and how many ties there are
+  const auto weight_of = [&](const uint4& w, unsigned& here) {
+    u64 sum = 0;
+    here = 0;
+    if (!(L::largest(w) >= from)) return sum;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const uint32_t key = key_of(L::at(w, j));
+      if (key == 0 || key < low) continue;
+      if (key <= high) {
+        ++here;
+        continue;
+      }
+      const u64 v = weigh(key);
+      if (v >= bound) sum += v;
     }
+    return sum;
+  };
+  u64 mine = 0;
+  unsigned mine_tied = 0;
+  for (int x = first + lane; x < last; x += 32) {
+    unsigned here;
+    mine += weight_of(fetch(x), here);
+    mine_tied += here;
   }
   mine = warp_sum(mine);
-  tied = warp_sum(tied);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const u64 v = __shfl_xor_sync(htr::kFullWarp, each, o);
-    each = v > each ? v : each;
+  mine_tied = __reduce_add_sync(htr::kFullWarp, mine_tied);
+  // sums before this warp: over the thread block, then over the cluster
+  if (lane == 0) {
+    s.red[0][warp] = mine;
+    s.red[1][warp] = mine_tied;
   }
-  // ties before this warp: over the thread block, then over the cluster
   __syncthreads();
-  if (lane == 0) s.red[0][warp] = tied;
-  __syncthreads();
-  u64 tied_before = 0, tied_block = 0;
-  {
-    const u64 v = s.red[0][lane], e = warp_scan(v, lane);
-    tied_before = __shfl_sync(htr::kFullWarp, e - v, warp);
-    tied_block = __shfl_sync(htr::kFullWarp, e, 31);
+  if (warp == 0) {
+    const u64 x = s.red[0][lane], y = s.red[1][lane], ex = warp_scan(x, lane), ey = warp_scan(y, lane);
+    s.ahead[0][lane] = ex - x;
+    s.ahead[1][lane] = ey - y;
+    if (lane == 31) {
+      s.mail[turn][0] = ex;
+      s.mail[turn][1] = ey;
+    }
   }
-  if (tid == 0) s.mail[turn][0] = tied_block;
   barrier();
-  for (unsigned c = 0; c < rank; ++c) tied_before += remote(&s.mail[turn][0], c);
-  turn ^= 1;
-  const u64 room = ties > tied_before ? ties - tied_before : 0;
-  mine += each * min(tied, room);
-  __syncthreads();
-  if (lane == 0) s.red[0][warp] = mine;
-  __syncthreads();
-  u64 before = 0, total = 0;
-  {
-    const u64 v = s.red[0][lane], e = warp_scan(v, lane);
-    before = __shfl_sync(htr::kFullWarp, e - v, warp);
-    total = __shfl_sync(htr::kFullWarp, e, 31);
+  if (warp == 0) {
+    const u64 x = lane < size ? remote(&s.mail[turn][0], lane) : 0, y = lane < size ? remote(&s.mail[turn][1], lane) : 0;
+    const u64 bx = warp_sum(lane < rank ? x : 0), by = warp_sum(lane < rank ? y : 0), all = warp_sum(x);
+    if (lane == 0) {
+      s.told[0] = bx;
+      s.told[1] = by;
+      s.told[2] = all;
+    }
   }
-  if (tid == 0) s.mail[turn][0] = total;
-  barrier();
-  total = 0;
-  for (unsigned c = 0; c < size; ++c) {
-    const u64 v = remote(&s.mail[turn][0], c);
-    if (c < rank) before += v;
-    total += v;
-  }
-  barrier();                                               // nothing remote is read any more
-  const float u = fminf(fmaxf(a.u[r], 0.f), 0.99999994f);
-  const u64 target = part_of(total, u, false);
-  if (before > target || target >= before + mine) return;
-  // this warp holds the token
-  u64 tied_here = 0;
-  for (int base = first; base < last; base += 32) {
-    bool tie = false;
-    const int i = base + lane;
-    const uint32_t key = i < last ? L::key(src, i) : 0;
-    u64 w = kept(key, tie);
-    const unsigned mark = __ballot_sync(htr::kFullWarp, tie);
-    if (tie && tied_here + __popc(mark & ((1u << lane) - 1)) >= room) w = 0;
-    tied_here += __popc(mark);
-    const u64 end = before + warp_scan(w, lane);
+  __syncthreads();
+  if (size > 1) htr::cluster_arrive();                     // nothing remote is read any more; waited for before a thread block leaves
+  const u64 ahead = s.told[1] + s.ahead[1][warp], total = s.told[2] + each * min((u64)tied, (u64)ties), target = part_of(total, u, false);
+  u64 before = s.told[0] + s.ahead[0][warp] + each * min(ahead, (u64)ties);
+  u64 room = ties > ahead ? ties - ahead : 0;              // ties of this warp and of later ones that are kept
+  mine += each * min((u64)mine_tied, room);
+  // the warp that holds the token
+  for (int base = before <= target && target < before + mine ? first : last; base < last; base += 32) {
+    const int x = base + lane;
+    unsigned here = 0;
+    uint4 w = {};
+    u64 sum = 0;
+    if (x < last) {
+      w = fetch(x);
+      sum = weight_of(w, here);
+    }
+    const u64 passed = warp_scan(here, lane), mine_room = room > passed - here ? room - (passed - here) : 0;
+    sum += each * min((u64)here, mine_room);
+    const u64 end = before + warp_scan(sum, lane);
     const unsigned hit = __ballot_sync(htr::kFullWarp, end > target);
     if (hit) {
+      u64 run = end - sum, tie = 0;
       if (lane == __ffs(hit) - 1) {
-        a.tokens[r] = begin + i;
-        if (a.logprobs) {
-          const double x = (double)logit_of(key);
-          a.logprobs[r] = (float)((x == weigh.max ? 0.0 : (x - weigh.max) * weigh.inv) - log((double)total / kOne));
+#pragma unroll 1
+        for (int j = 0; j < kVec && run <= target; ++j) {
+          const uint32_t key = key_of(L::at(w, j));
+          if (key == 0 || key < low || (key <= high && tie++ >= mine_room)) continue;
+          const u64 v = weigh(key);
+          if (v < bound) continue;
+          run += v;
+          if (run <= target) continue;
+          a.tokens[r] = begin + x * kVec + j;
+          if (a.logprobs) {
+            const double d = (double)logit_of(key);
+            a.logprobs[r] = (float)((d == weigh.max ? 0.0 : (d - weigh.max) / (double)t) - log((double)total / kOne));
+          }
         }
       }
-      return;
+      break;
     }
     before = __shfl_sync(htr::kFullWarp, end, 31);
+    const u64 gone = __shfl_sync(htr::kFullWarp, passed, 31);
+    room = room > gone ? room - gone : 0;
   }
+  if (size > 1) htr::cluster_wait();
 }
 
 template <int DT>
@@ -464,13 +539,13 @@ int run(const SampleArgs& a, cudaStream_t st) {
   static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
   int dev = 0, e = (int)cudaGetDevice(&dev);
   if (!e && (dev < 0 || dev >= 64 || !allowed[dev])) {
-    e = (int)cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    e = (int)cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage + (int)sizeof(Shared<DT>));
     if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.rows * size);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = staged ? (size_t)per * Logit<DT>::kBytes : 0;
+  cfg.dynamicSmemBytes = sizeof(Shared<DT>) + (staged ? (size_t)per * Logit<DT>::kBytes : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
