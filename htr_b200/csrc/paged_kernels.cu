@@ -280,8 +280,7 @@ struct AppendArgs {
 template <typename T, int D>
 struct Row {
   static constexpr int kLanes = D / 8;
-  static __device__ __forceinline__ void load(const T* row, int lane, float (&v)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(row + lane * 8);
+  static __device__ __forceinline__ void widen(const uint4& raw, float (&v)[8]) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -301,37 +300,44 @@ struct Row {
   }
 };
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256, kQueryHeads = 4, kMaxPage = 128;
 
-// grid (windows of tokens, 2 * kv_heads + 1): y < 2 * kv_heads: the keys (even) or values (odd) of one head; the last: the queries.
+// grid (windows of tokens, 2 * kv_heads + groups of query heads): y < 2 * kv_heads: the keys (even) or values (odd) of one head; then the queries.
 // A run = the tokens of this step that lie in one page; the block of the window in which a run begins writes it whole, so that one
-// block alone reads and writes the page's scale.
+// block alone reads and writes the page's scale.  A prompt is bound by its bytes: a run stays in registers between the search for
+// its largest element and the rounding, and query rows are read four heads at a time, whose angles are the same.  A few tokens are
+// bound by latency: slots and positions, then rows, angles and the old scale at once, then the maximum.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const AppendArgs a) {
   using R = Row<T, D>;
-  constexpr int kRows = kAppendThreads / R::kLanes;        // rows of a pass
-  __shared__ float red[kAppendThreads / 32];
-  __shared__ int s_run;
+  constexpr int kRows = kAppendThreads / R::kLanes, kPasses = kMaxPage / kRows, kWarps = kAppendThreads / 32;   // rows of a pass; passes of a page
+  __shared__ float red[kWarps];
+  __shared__ int s_slot[1 + 2 * kMaxPage], s_pos[1 + 2 * kMaxPage], s_fail[kMaxPage / 32];
+  __shared__ unsigned s_begins[kMaxPage / 32];
   pdl_enter();
   const int tid = threadIdx.x, lane = tid % R::kLanes, row = tid / R::kLanes, page = 1 << a.shift;
   const T* qkv = static_cast<const T*>(a.qkv);
-  const auto slot_of = [&](int t) {                        // -1: the token is not written
-    const int slot = a.slots[t], pos = a.positions[t];
-    return slot >= 0 && slot < a.slots_total && pos >= 0 && pos < a.angle_rows ? slot : -1;
-  };
   const int t0 = blockIdx.x * a.window, t1 = min(t0 + a.window, a.tokens);
-  if (blockIdx.y == 2 * a.kv_heads) {                      // queries: the angles of a row serve all of its heads
+  const auto valid = [&](int slot, int pos) { return slot >= 0 && slot < a.slots_total && pos >= 0 && pos < a.angle_rows; };
+  if (blockIdx.y >= 2 * a.kv_heads) {                      // queries
+    const int h0 = (blockIdx.y - 2 * a.kv_heads) * kQueryHeads, heads = min(kQueryHeads, a.q_heads - h0);
     for (int t = t0 + row; t < t1; t += kRows) {
-      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (size_t)t * a.q_heads * D + lane * 8);
-      const T* in = qkv + (size_t)t * a.row_stride;
-      const bool ok = slot_of(t) >= 0;
-      if (!ok && a.status && lane == 0 && a.slots[t] != -1) atomicOr(a.status, 16);
-      const size_t at = ok ? (size_t)a.positions[t] * (D / 2) + lane * 4 : 0;
-      const float4 c = ok ? *reinterpret_cast<const float4*>(a.cosv + at) : make_float4(0, 0, 0, 0);
-      const float4 s = ok ? *reinterpret_cast<const float4*>(a.sinv + at) : make_float4(0, 0, 0, 0);
-      for (int h = 0; h < a.q_heads; ++h) {
+      const int slot = a.slots[t], pos = a.positions[t];
+      uint4 raw[kQueryHeads];
+      const T* in = qkv + (size_t)t * a.row_stride + (size_t)h0 * D + lane * 8;
+#pragma unroll
+      for (int h = 0; h < kQueryHeads; ++h)
+        if (h < heads) raw[h] = *reinterpret_cast<const uint4*>(in + h * D);
+      const bool ok = valid(slot, pos);
+      if (!ok && a.status && lane == 0 && h0 == 0 && slot != -1) atomicOr(a.status, 16);
+      const size_t at = ok ? (size_t)pos * (D / 2) + lane * 4 : 0;
+      const float4 c = *reinterpret_cast<const float4*>(a.cosv + at), s = *reinterpret_cast<const float4*>(a.sinv + at);
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + ((size_t)t * a.q_heads + h0) * D + lane * 8);
+#pragma unroll
+      for (int h = 0; h < kQueryHeads; ++h) {
+        if (h >= heads) continue;
         float v[8];
-        R::load(in + (size_t)h * D, lane, v);
+        R::widen(raw[h], v);
         R::rotate(v, c, s);
         uint4 r = {Half<T>::narrow(v[0], v[1]), Half<T>::narrow(v[2], v[3]), Half<T>::narrow(v[4], v[5]), Half<T>::narrow(v[6], v[7])};
         if (!ok) r = {0, 0, 0, 0};
@@ -345,43 +351,88 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
   uint8_t* cache = values ? a.v_cache : a.k_cache;
   float* scales = values ? a.v_scale : a.k_scale;
   const T* in = qkv + (size_t)(a.q_heads + (values ? a.kv_heads : 0) + head) * D;
-  for (int t = t0; t < t1; ++t) {
-    const int slot = slot_of(t), off = slot & (page - 1);
-    if (slot < 0 || (off != 0 && t > 0 && slot_of(t - 1) == slot - 1)) continue;     // (the whole block)
-    if (tid == 0) s_run = page - off;
+  // slots of the window, of the token before it and of a page behind it; negative: the token is not written
+  for (int i = tid; i < 1 + a.window + page; i += kAppendThreads) {
+    const int t = t0 - 1 + i;
+    int slot = -2, pos = 0;
+    if (t >= 0 && t < a.tokens) {
+      slot = a.slots[t];
+      pos = a.positions[t];
+      if (!valid(slot, pos)) slot = -2;
+    }
+    s_slot[i] = slot;
+    s_pos[i] = pos;
+  }
+  __syncthreads();
+  if (tid < kMaxPage) {                                    // where runs begin
+    const int slot = tid < t1 - t0 ? s_slot[1 + tid] : -2;
+    const unsigned begins = __ballot_sync(htr::kFullWarp, slot >= 0 && ((slot & (page - 1)) == 0 || s_slot[tid] != slot - 1));
+    if ((tid & 31) == 0) s_begins[tid >> 5] = begins;
+  }
+  __syncthreads();
+  unsigned begins = s_begins[0];
+  for (int word = 0;;) {
+    while (begins == 0 && ++word < kMaxPage / 32) begins = s_begins[word];
+    if (begins == 0) break;
+    const int t = t0 + 32 * word + __ffs(begins) - 1;
+    begins &= begins - 1;
+    const int slot = s_slot[1 + t - t0], off = slot & (page - 1);
+    const size_t unit = (size_t)(slot >> a.shift) * a.kv_heads + head;
+    const float old_scale = off ? scales[unit] : 0.f;
+    // its run: the first place that does not follow
+    if (tid < kMaxPage) {
+      const unsigned fail = __ballot_sync(htr::kFullWarp, tid >= page - off || s_slot[1 + t - t0 + tid] != slot + tid);
+      if ((tid & 31) == 0) s_fail[tid >> 5] = fail ? tid + __ffs(fail) - 1 : kMaxPage;
+    }
     __syncthreads();
-    for (int i = tid; i < page - off; i += kAppendThreads)
-      if (t + i >= a.tokens || slot_of(t + i) != slot + i) atomicMin(&s_run, i);
-    __syncthreads();
-    const int run = s_run;
-    const auto fetch = [&](int i, float (&v)[8]) {
-      R::load(in + (size_t)(t + i) * a.row_stride, lane, v);
-      if (!values) {
-        const size_t at = (size_t)a.positions[t + i] * (D / 2) + lane * 4;
-        R::rotate(v, *reinterpret_cast<const float4*>(a.cosv + at), *reinterpret_cast<const float4*>(a.sinv + at));
-      }
-    };
-    float most = 0.f;
-    for (int i = row; i < run; i += kRows) {
-      float v[8];
-      fetch(i, v);
+    int run = kMaxPage;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float m = fabsf(v[j]);
-        if (m <= 3.402823466e38f) most = fmaxf(most, m);   // infinities saturate and NaN stays: neither sets the scale
+    for (int w = 0; w < kMaxPage / 32; ++w) run = min(run, s_fail[w]);
+    float v[kPasses][8];
+    uint4 raw[kPasses];                                    // all loads before the first use
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) raw[x] = x * kRows + row < run ? *reinterpret_cast<const uint4*>(in + (size_t)(t + x * kRows + row) * a.row_stride + lane * 8) : uint4{0, 0, 0, 0};
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) R::widen(raw[x], v[x]);
+    if (!values) {
+#pragma unroll
+      for (int x0 = 0; x0 < kPasses; x0 += 4) {
+        float4 c[4], s[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const size_t from = (size_t)s_pos[1 + t - t0 + min((x0 + x) * kRows + row, run - 1)] * (D / 2) + lane * 4;
+          c[x] = *reinterpret_cast<const float4*>(a.cosv + from);
+          s[x] = *reinterpret_cast<const float4*>(a.sinv + from);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) R::rotate(v[x0 + x], c[x], s[x]);
+        if ((x0 + 4) * kRows >= run) break;
       }
     }
+    // the largest of the run, NaN left aside; infinities saturate and do not set the scale either: where there is one, once more without
+    const auto largest = [&](float limit) {
+      float most = 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, o));
-    if ((tid & 31) == 0) red[tid >> 5] = most;
-    __syncthreads();
+      for (int x = 0; x < kPasses; ++x)
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) most = fmaxf(most, red[w]);
-    const size_t unit = (size_t)(slot >> a.shift) * a.kv_heads + head;
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, limit > 0.f && fabsf(v[x][j]) > limit ? 0.f : fabsf(v[x][j]));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, o));
+      if ((tid & 31) == 0) red[tid >> 5] = most;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) most = fmaxf(most, red[w]);
+      return most;
+    };
+    float most = largest(0.f);
+    if (most > 3.402823466e38f) {
+      __syncthreads();
+      most = largest(3.402823466e38f);
+    }
     uint8_t* at = cache + (unit << a.shift) * D;
     int e = scale_exponent(most);
     if (off) {                                             // older tokens: their scale never shrinks, and they follow where it grows
-      const int old = max((int)((__float_as_uint(scales[unit]) >> 23) & 255) - 127, kScaleFloor);
+      const int old = max((int)((__float_as_uint(old_scale) >> 23) & 255) - 127, kScaleFloor);
       if (old >= e) {
         e = old;
       } else {
@@ -395,15 +446,16 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
       }
     }
     const float up = exp2i(-e);
-    for (int i = row; i < run; i += kRows) {
-      float v[8];
-      fetch(i, v);
-      const uint2 r = {to_e4m3(v[0] * up, v[1] * up) | to_e4m3(v[2] * up, v[3] * up) << 16,
-                       to_e4m3(v[4] * up, v[5] * up) | to_e4m3(v[6] * up, v[7] * up) << 16};
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) {
+      const int i = x * kRows + row;
+      if (i >= run) continue;
+      const uint2 r = {to_e4m3(v[x][0] * up, v[x][1] * up) | to_e4m3(v[x][2] * up, v[x][3] * up) << 16,
+                       to_e4m3(v[x][4] * up, v[x][5] * up) | to_e4m3(v[x][6] * up, v[x][7] * up) << 16};
       *reinterpret_cast<uint2*>(at + (size_t)(off + i) * D + lane * 8) = r;
     }
-    __syncthreads();                                       // the old scale has been read by all
-    if (tid == 0) scales[unit] = exp2i(e);
+    if (tid == 0) scales[unit] = exp2i(e);                 // (the old one was read by all before the last barrier)
+    __syncthreads();                                       // s_fail and red have been read
   }
 }
 
@@ -954,9 +1006,9 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
   if (tokens == 0) return HTR_OK;
   if (!qkv || !positions || !slots || !cosv || !sinv || !k_cache || !v_cache || !k_scale || !v_scale || !q_out) return HTR_ERR_NULL;
   if (!aligned16(qkv) || !aligned16(cosv) || !aligned16(sinv) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q_out)) return HTR_ERR_ALIGNMENT;
-  const int units = 2 * kv_heads + 1;
+  const int units = 2 * kv_heads + (q_heads + kQueryHeads - 1) / kQueryHeads;
   int window = 1;                                          // tokens of a thread block: few where there is little to share out
-  while (window < page_size && (int64_t)tokens * units > (int64_t)window * 148 * 16) window *= 2;
+  while (window < page_size && (int64_t)tokens * units > (int64_t)window * 148 * 8) window *= 2;
   const AppendArgs a = {qkv, row_stride, positions, slots, tokens, cosv, sinv, angle_rows, q_heads, kv_heads, static_cast<uint8_t*>(k_cache),
                         static_cast<uint8_t*>(v_cache), k_scale, v_scale, (int64_t)pages << shift, shift, window, q_out, status};
   const dim3 grid((unsigned)((tokens + window - 1) / window), units);
