@@ -583,8 +583,23 @@ PyObject* py_plan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   const int dev = lengths->get_device();
   OnDevice on(dev);
-  const auto ints = [&](int64_t size) { return at::detail::empty_cuda({size}, at::kInt, where, std::nullopt); };
-  at::Tensor out[6] = {ints(R + 1), ints(T), ints(T), ints(R), lengths_out ? at::Tensor() : ints(R), count_out ? at::Tensor() : ints(1)};
+  // one allocation, and the six tensors as parts of it
+  const at::Tensor all_ints = at::detail::empty_cuda({3 * R + 2 + 2 * (int64_t)T}, at::kInt, where, std::nullopt);
+  int64_t used = 0;
+  const auto ints = [&](int64_t size) {
+    at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all_ints.storage()), all_ints.key_set(), all_ints.dtype());
+    part.unsafeGetTensorImpl()->set_storage_offset(used);
+    part.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    used += size;
+    return part;
+  };
+  at::Tensor out[6];
+  out[0] = ints(R + 1);
+  out[1] = ints(T);
+  out[2] = ints(T);
+  out[3] = ints(R);
+  if (!lengths_out) out[4] = ints(R);
+  if (!count_out) out[5] = ints(1);
   if (!lengths_out) lengths_out = out[4].data_ptr();
   if (!count_out) count_out = out[5].data_ptr();
   if (g_lib.page_plan(lengths->const_data_ptr<int>(), added->const_data_ptr<int>(), (int)R, tables->data_ptr<int>(), stride, (int)tables->size(1),

@@ -57,7 +57,7 @@ int launch(Kern kern, dim3 grid, dim3 block, int cluster, size_t smem, cudaStrea
 // itself (at most 8192 of them, in shared memory) and then fills its share of the tokens by binary search: 20 times the additions of a
 // scan across thread blocks, and no waiting for one another.  The outputs may be the inputs' own buffers (lengths, count): the thread
 // blocks are one cluster, and nothing is written over before all of them have read.
-constexpr int kPlanThreads = 512, kPlanMaxRequests = 8192, kPlanMaxCluster = 8;
+constexpr int kPlanThreads = 1024, kPlanMaxRequests = 8192, kPlanMaxCluster = 8;
 
 struct PlanArgs {
   const int *lengths, *added;
@@ -75,27 +75,26 @@ struct PlanArgs {
 // inclusive scan of a pair over the block; totals come back in `total`
 __device__ __forceinline__ longlong2 block_scan(longlong2 v, longlong2* part, longlong2* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const auto scan = [lane](longlong2 v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(htr::kFullWarp, v.x, o), y = __shfl_up_sync(htr::kFullWarp, v.y, o);
-    if (lane >= o) {
-      v.x += x;
-      v.y += y;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(htr::kFullWarp, v.x, o), y = __shfl_up_sync(htr::kFullWarp, v.y, o);
+      if (lane >= o) {
+        v.x += x;
+        v.y += y;
+      }
     }
-  }
+    return v;
+  };
+  v = scan(v);
   __syncthreads();
   if (lane == 31) part[warp] = v;
   __syncthreads();
-  longlong2 sum = {0, 0};
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w == warp) {
-      v.x += sum.x;
-      v.y += sum.y;
-    }
-    sum.x += part[w].x;
-    sum.y += part[w].y;
-  }
-  *total = sum;
+  const longlong2 w = lane < kPlanThreads / 32 ? part[lane] : longlong2{0, 0}, e = scan(w);
+  v.x += __shfl_sync(htr::kFullWarp, e.x - w.x, warp);
+  v.y += __shfl_sync(htr::kFullWarp, e.y - w.y, warp);
+  total->x = __shfl_sync(htr::kFullWarp, e.x, 31);
+  total->y = __shfl_sync(htr::kFullWarp, e.y, 31);
   return v;
 }
 
@@ -114,6 +113,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
   extern __shared__ int plan_smem[];
   int *ends = plan_smem, *need_end = ends + a.requests, *back_end = need_end + a.requests, *held = back_end + a.requests;
   __shared__ longlong2 part[kPlanThreads / 32];
+  __shared__ int s_taken[kPlanThreads / 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, R = a.requests, page = 1 << a.shift;
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
   run = block_scan(mine, part, &total);
   run.x -= mine.x;
   const long long supply = (long long)count + back;
-  longlong2 granted = {0, 0};
+  int granted = 0;                                         // the requests that are served and need pages come first of all that need some
   for (int r = first; r < last; ++r) {
     const int need = need_end[r];
     run.x += max(need, 0);
@@ -167,13 +167,15 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
       held[r] = -1;
       bad |= 1;
     } else if (need > 0) {
-      granted.x += need;
+      granted = (int)run.x;
     }
   }
-  block_scan(granted, part, &total);
-  const int taken = (int)total.x;
-  if (bad && a.status && block == 0) atomicOr(a.status, bad);
+  granted = __reduce_max_sync(htr::kFullWarp, granted);
   __syncthreads();
+  if ((tid & 31) == 0) s_taken[tid >> 5] = granted;
+  __syncthreads();
+  const int taken = __reduce_max_sync(htr::kFullWarp, s_taken[tid & 31]);
+  if (bad && a.status && block == 0) atomicOr(a.status, bad);
   // page i of what this step takes: first those that came back, then the top of the free pages
   const auto returned = [&](int i) {
     const int r = above(back_end, R, i);
@@ -185,19 +187,30 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
     return at >= 0 ? a.free_pages[at] : -1;
   };
   const int stride = blocks * kPlanThreads, me = block * kPlanThreads + tid;
-  for (int t = me; t < a.max_tokens; t += stride) {
-    int pos = -1, slot = -1;
-    if (t < tokens) {
-      const int r = above(ends, R, t);
-      if (r < R && held[r] >= 0) {
-        pos = held[r] + t - (r ? ends[r - 1] : 0);
-        const int at = pos >> a.shift, have = (int)(((long long)held[r] + page - 1) >> a.shift);
-        const int id = at < have ? a.tables[r * a.table_stride + at] : supplied((r ? need_end[r - 1] : 0) + at - have);
-        slot = id >= 0 && id < a.pages ? (id << a.shift) + (pos & (page - 1)) : -1;
+  // a thread takes four tokens in a row where there are many: they mostly share their request and its page
+  const int row = a.max_tokens > stride ? 4 : 1;
+  for (int t0 = me * row; t0 < a.max_tokens; t0 += stride * row) {
+    int r = above(ends, R, t0), at = -1, id = -1;
+    for (int t = t0; t < min(t0 + row, a.max_tokens); ++t) {
+      int pos = -1, slot = -1;
+      if (t < tokens) {
+        while (r < R && ends[r] <= t) {
+          ++r;
+          at = -1;
+        }
+        if (r < R && held[r] >= 0) {
+          pos = held[r] + t - (r ? ends[r - 1] : 0);
+          if (at != pos >> a.shift) {
+            at = pos >> a.shift;
+            const int have = (int)(((long long)held[r] + page - 1) >> a.shift);
+            id = at < have ? a.tables[r * a.table_stride + at] : supplied((r ? need_end[r - 1] : 0) + at - have);
+          }
+          slot = id >= 0 && id < a.pages ? (id << a.shift) + (pos & (page - 1)) : -1;
+        }
       }
+      a.positions[t] = pos;
+      a.slots[t] = slot;
     }
-    a.positions[t] = pos;
-    a.slots[t] = slot;
   }
   for (int i = me; i < taken; i += stride) {                 // the new pages enter the tables
     const int r = above(need_end, R, i);
@@ -990,7 +1003,7 @@ int htr_page_plan(const int* lengths, const int* added, int requests, int* table
     }
   }
   const int work = max_tokens > requests ? max_tokens : requests;
-  const int blocks = work <= 2 * kPlanThreads ? 1 : kPlanMaxCluster;
+  const int blocks = work <= kPlanThreads ? 1 : kPlanMaxCluster;
   return launch(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), blocks, smem, static_cast<cudaStream_t>(stream), a);
 }
 
