@@ -1,0 +1,694 @@
+// Attention over the paged 8-bit cache for many rows a request (prompts, shared key/value heads): tcgen05.mma with accumulators in tensor
+// memory.
+//
+// A tile is up to 128 rows: the query heads of one key/value head for as many whole tokens as fit (row = token * group + head).  Per 128
+// cached tokens: S = Q K^T (128 x 128), P = 2^(S - m) in fp16, O += P V.  S, P and O are in tensor memory (P over S), Q, K and V in shared
+// memory as fp16 core matrices; keys and values are e4m3 in the cache and become fp16, exactly, on the way there.
+// Three roles per thread block, two thread blocks per SM, so that one's products run while the other's roles wait for one another:
+//   warps 0-3  a thread per row (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.
+//   warps 4-7  cache -> registers (the next 128 tokens are on their way) -> fp16 core matrices.  Values are transposed on the way (their
+//              operand wants eight tokens of a dimension side by side): byte permutes of eight rows in registers.
+//   warp 8     issues the products; barriers: K full -> S full (K free) -> P and V full -> product done (V, P free).
+// What bounds it: per 128 tokens and 128 rows 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM), and about 900 of
+// issue on each scheduler; the three overlap between the two thread blocks.
+// The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
+// the sum; see paged_kernels.cu, whose cut of the work into even runs over the thread blocks, parts and join this kernel shares, with
+// runs of units of 128 tokens of (request, tile, head), each as many as its last token sees.
+#include "paged_common.cuh"
+
+namespace {
+
+using namespace htr;
+
+constexpr int kThreads = 288, kRows = 128, kUnit = 128, kMaxRequests = 1024, kBlocksPerSm = 2;
+constexpr int kTmemColumns = 256;                          // S (P over it) at 0, O at 128
+constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
+
+template <int D>
+struct Layout {                                            // bytes of the operands: core matrices of 8 rows x 16 bytes
+  static constexpr int kGroup = 16 * D;                    // Q, K: between groups of 8 rows; 128 between neighbours in K
+  static constexpr int kTokens = 16 * D + 16;              // V: between groups of 8 tokens (16 more: stores of 8 groups meet 8 bank groups)
+  static constexpr int kQ = 0, kK = kQ + 16 * kGroup, kV = kK + 16 * kGroup, kBytes = kV + 16 * kTokens;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// start, distance of core matrices adjacent in K, distance of groups of 8 rows, in 16 bytes; version 1, no swizzle
+__device__ __forceinline__ uint64_t descriptor(uint32_t at, int next_k, int next_rows) {
+  return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)(next_k >> 4) << 16 | (uint64_t)(next_rows >> 4) << 32 | 1ull << 46;
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+  return done != 0;
+}
+// bounded: false when the limit ran out or another role has given up
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* fail) {
+  if (bar_try(bar, parity)) return true;
+  for (unsigned i = 0; i < kSpinLimit; ++i) {
+    if (bar_try(bar, parity)) return true;
+    if ((i & 255) == 255 && *fail) return false;
+  }
+  *fail = 1;
+  return false;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+               "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+               "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 16 or 32 columns of this thread's lane of tensor memory
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a request's tiles, and what one of them sees
+struct Request {
+  int start, n, seen, per, tiles;                          // per: tokens of a tile
+  __device__ __forceinline__ Request(const AttentionArgs& a, int r) {
+    start = max(a.starts[r], 0);
+    n = max(min(a.starts[r + 1], a.tokens) - start, 0);
+    seen = min(max(a.seen[r], 0), a.width << a.shift);
+    per = kRows / a.group;
+    tiles = (min(n, a.max_new) + per - 1) / per;
+  }
+  __device__ __forceinline__ int tokens(const AttentionArgs& a, int tile) const { return min(per, min(n, a.max_new) - tile * per); }
+  __device__ __forceinline__ int end(const AttentionArgs& a, int tile) const { return max(seen - n + tile * per + tokens(a, tile), 0); }
+  __device__ __forceinline__ int units(const AttentionArgs& a, int tile) const { return max((end(a, tile) + kUnit - 1) / kUnit, 1); }
+};
+
+struct Shared {
+  unsigned long long k_full, s_full, v_full, p_full, pv_done, q_full, drained;
+  long long sums[kMaxRequests];                            // units of each request
+  long long total, skip;
+  int r, tile, head, unit;                                 // where this thread block's run begins
+  uint32_t tmem;
+  int fail, nan;
+  float ks[2][8], lv[2][8], inv[2][8];                     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
+  unsigned real[2];                                        // groups that have a page
+};
+
+// the run of a thread block, piece by piece: every role walks it for itself
+struct Walk {
+  int r, tile, head, u0, u1, units;
+  long long left;
+  int start, n, seen, per, tiles, row_tokens, least, end;
+  __device__ __forceinline__ Walk(const Shared& s, long long count) : r(s.r), tile(s.tile), head(s.head), u0(s.unit), left(count) {}
+  __device__ __forceinline__ void look(const AttentionArgs& a) {
+    Request x(a, r);
+    while (x.tiles == 0) x = Request(a, ++r);              // (there is one: `left` counts its units)
+    start = x.start; n = x.n; seen = x.seen; per = x.per; tiles = x.tiles;
+    row_tokens = x.tokens(a, tile);
+    least = max(seen - n + tile * per + 1, 0);
+    end = x.end(a, tile);
+    units = x.units(a, tile);
+    u1 = (int)min((long long)units, u0 + left);
+  }
+  __device__ __forceinline__ void next(const AttentionArgs& a) {
+    left -= u1 - u0;
+    u0 = 0;
+    if (++head < a.kv_heads) return;
+    head = 0;
+    if (++tile < tiles) return;
+    tile = 0;
+    ++r;
+  }
+};
+
+template <int D>
+constexpr int kPartFloats = kRows * (D + 2);
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_kernel(const AttentionArgs a) {
+  using Y = Layout<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Shared s;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* fail = &s.fail;
+  // ---- this thread block's run: units of each request by its warps, then the place where the run begins
+  for (int r = warp; r < a.requests; r += kThreads / 32) {
+    const Request x(a, r);
+    long long sum = 0;
+    for (int t = lane; t < x.tiles; t += 32) sum += x.units(a, t);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullWarp, sum, o);
+    if (lane == 0) s.sums[r] = sum * a.kv_heads;
+  }
+  if (tid == 0) {
+    s.fail = s.nan = 0;
+    bar_init(smem_u32(&s.k_full), 128);
+    bar_init(smem_u32(&s.s_full), 1);
+    bar_init(smem_u32(&s.v_full), 128);
+    bar_init(smem_u32(&s.p_full), 128);
+    bar_init(smem_u32(&s.pv_done), 1);
+    bar_init(smem_u32(&s.q_full), 128);
+    bar_init(smem_u32(&s.drained), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    a.cuts[blockIdx.x] = {0, 0, 0, 0};
+  }
+  if (warp == 8) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"((uint32_t)kTmemColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  // (tensor memory is ours: a dependent launch that starts early cannot take it from thread blocks of this one)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  long long total = 0, share = 1, from = 0;
+  if (warp == 0) {
+    for (int r = lane; r < a.requests; r += 32) total += s.sums[r];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(kFullWarp, total, o);
+    share = max((total + gridDim.x - 1) / gridDim.x, 1LL);
+    from = blockIdx.x * share;
+    if (lane == 0) s.total = total;
+    if (from < total) {
+      int r = 0;
+      long long before = 0;                                // units before the request
+      for (int base = 0; base < a.requests; base += 32) {
+        const long long mine = base + lane < a.requests ? s.sums[base + lane] : 0;
+        long long end = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long x = __shfl_up_sync(kFullWarp, end, o);
+          if (lane >= o) end += x;
+        }
+        const unsigned hit = __ballot_sync(kFullWarp, before + end > from);
+        if (hit) {
+          r = base + __ffs(hit) - 1;
+          before += __shfl_sync(kFullWarp, end - mine, __ffs(hit) - 1);
+          break;
+        }
+        before += __shfl_sync(kFullWarp, end, 31);
+      }
+      const Request x(a, r);
+      for (int base = 0; base < x.tiles; base += 32) {
+        const long long mine = base + lane < x.tiles ? (long long)x.units(a, base + lane) * a.kv_heads : 0;
+        long long end = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(kFullWarp, end, o);
+          if (lane >= o) end += y;
+        }
+        const unsigned hit = __ballot_sync(kFullWarp, before + end > from);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            const long long rest = from - (before + end - mine);
+            const int units = x.units(a, base + lane);
+            s.r = r;
+            s.tile = base + lane;
+            s.head = (int)(rest / units);
+            s.unit = (int)(rest % units);
+          }
+          break;
+        }
+        before += __shfl_sync(kFullWarp, end, 31);
+      }
+    }
+  }
+  __syncthreads();
+  total = s.total;
+  share = max((total + gridDim.x - 1) / gridDim.x, 1LL);
+  from = blockIdx.x * share;
+  const long long count = min(share, total - from);
+  const uint32_t tmem = s.tmem;
+  const uint32_t k_full = smem_u32(&s.k_full), s_full = smem_u32(&s.s_full), v_full = smem_u32(&s.v_full), p_full = smem_u32(&s.p_full),
+                 pv_done = smem_u32(&s.pv_done), q_full = smem_u32(&s.q_full);
+  uint32_t phase = 0;                                      // of the barriers of a unit: units so far, modulo 2
+  if (count > 0 && warp < 4) {
+    // ================= softmax: a thread per row
+    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+    const int row = tid;
+    bool ok = true;
+    Walk w(s, count);
+    for (int segment = 0; w.left > 0 && ok; ++segment, w.next(a)) {
+      w.look(a);
+      const int i = row / a.group, head = w.head * a.group + row - i * a.group, rows = w.row_tokens * a.group;
+      const bool mine = row < rows;
+      const size_t place = ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
+      const int row_end = mine ? max(w.seen - w.n + w.tile * w.per + i + 1, 0) : 0;
+      // queries: fp16 under a power of two per row
+      float row_scale;
+      {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + place);
+        float most = 0.f;
+        if (mine)
+#pragma unroll 4
+          for (int j = 0; j < D / 8; ++j) {
+            const uint4 raw = src[j];
+            const float2 f[4] = {Half<T>::wide(raw.x), Half<T>::wide(raw.y), Half<T>::wide(raw.z), Half<T>::wide(raw.w)};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) most = fmaxf(most, fmaxf(fabsf(f[x].x), fabsf(f[x].y)));
+          }
+        const int e = query_exponent(most);
+        const float up = exp2i(e);
+        row_scale = exp2i(-e) * a.scale;
+        uint8_t* dst = smem + Y::kQ + (row >> 3) * Y::kGroup + (row & 7) * 16;
+#pragma unroll 4
+        for (int j = 0; j < D / 8; ++j) {
+          uint4 r = {0, 0, 0, 0};
+          if (mine) {
+            const uint4 raw = src[j];
+            const float2 f[4] = {Half<T>::wide(raw.x), Half<T>::wide(raw.y), Half<T>::wide(raw.z), Half<T>::wide(raw.w)};
+            r = {pack_half(f[0].x * up, f[0].y * up), pack_half(f[1].x * up, f[1].y * up), pack_half(f[2].x * up, f[2].y * up),
+                 pack_half(f[3].x * up, f[3].y * up)};
+          }
+          *reinterpret_cast<uint4*>(dst + j * 128) = r;
+        }
+        fence_async();
+        bar_arrive(q_full);
+      }
+      float m = kNone, l = 0.f;
+      for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1) {
+        ok = bar_wait(k_full, phase, fail) && bar_wait(s_full, phase, fail);
+        ok = __all_sync(kFullWarp, ok);
+        if (!ok) break;
+        fence_after();
+        const int at = u * kUnit;
+        const unsigned real = s.real[phase];
+        const bool edge = at + kUnit > w.least || real != 0xFFu;
+        if (32 * warp < rows) {
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {                    // 32 tokens: two groups of 16
+            uint32_t raw[32];
+            tmem_load(lanes + 32 * j, raw);
+            float v[32], base = m == kNone ? 0.f : m, most = kNone;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const float by = row_scale * s.ks[phase][2 * j + g], add = s.lv[phase][2 * j + g] - base;
+#pragma unroll
+              for (int c = 0; c < 16; ++c) v[16 * g + c] = fmaf(__uint_as_float(raw[16 * g + c]), by, add);
+            }
+            if (edge) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (at + 32 * j + c >= row_end || !(real >> (2 * j + (c >> 4)) & 1)) v[c] = kNone;
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) most = fmaxf(most, v[c]);
+            const bool grows = m == kNone ? most > kNone : most > 14.f;
+            if (__any_sync(kFullWarp, grows)) {            // a new reference, 2^6 above which the largest lies; what there is follows
+              const float now = grows ? base + most - 6.f : m, f = grows && m != kNone ? exp2_fast(m - now) : 1.f;
+              if (grows) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[c] += base - now;
+                m = now;
+                l *= f;
+              }
+              __syncwarp();
+              tmem_stored();
+              if (u > w.u0)
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                  uint32_t o[16];
+                  tmem_load16(lanes + 128 + c, o);
+#pragma unroll
+                  for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                  tmem_store(lanes + 128 + c, o);
+                }
+#pragma unroll 1
+              for (int c = 0; c < 16 * j; c += 16) {
+                uint32_t o[16];
+                tmem_load16(lanes + c, o);
+                const __half2 h = __float2half2_rn(f);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o[x]), h);
+                  o[x] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+                tmem_store(lanes + c, o);
+              }
+              tmem_stored();
+            }
+            uint32_t p[16];
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float x = exp2_fast(v[2 * c]), y = exp2_fast(v[2 * c + 1]);
+              sum[c >> 3] += x + y;
+              p[c] = pack_half(x, y);
+            }
+            __syncwarp();
+            l = fmaf(sum[0], s.inv[phase][2 * j], fmaf(sum[1], s.inv[phase][2 * j + 1], l));
+            tmem_store(lanes + 16 * j, p);
+          }
+          tmem_stored();
+        }
+        fence_before();
+        bar_arrive(p_full);
+      }
+      if (!ok) break;
+      ok = __all_sync(kFullWarp, bar_wait(pv_done, phase ^ 1, fail));
+      if (!ok) break;
+      fence_after();
+      // ---- the tile, or this run's part of it
+      const bool whole = w.u0 == 0 && w.u1 == w.units;
+      float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPartFloats<D>;
+      const float by = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;     // a row that sees nothing: zeros
+      const bool empty = l == 0.f;
+      const bool nan = *(volatile int*)&s.nan != 0;
+      if (32 * warp < rows) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          __syncwarp();
+          tmem_load16(lanes + 128 + c, o);
+          if (mine) {
+          float f[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) f[x] = empty ? 0.f : __uint_as_float(o[x]) * by;
+          if (nan)                                         // values that are NaN were left out of the last units: given to the rows that see them
+            for (int token = max(w.least, w.u0 * kUnit); token < min(row_end, w.u1 * kUnit); ++token) {
+              const int id = a.tables[w.r * a.table_stride + (token >> a.shift)];
+              if (id < 0 || id >= a.pages) continue;
+              const uint8_t* v = a.v_cache + ((((size_t)id * a.kv_heads + w.head) << a.shift) + (token & ((1 << a.shift) - 1))) * D + c;
+#pragma unroll
+              for (int x = 0; x < 16; ++x)
+                if ((v[x] & 0x7F) == 0x7F) f[x] = __int_as_float(0x7FC00000);
+            }
+          if (whole) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + place + c);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              dst[x] = {Half<T>::narrow(f[8 * x], f[8 * x + 1]), Half<T>::narrow(f[8 * x + 2], f[8 * x + 3]),
+                        Half<T>::narrow(f[8 * x + 4], f[8 * x + 5]), Half<T>::narrow(f[8 * x + 6], f[8 * x + 7])};
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              *reinterpret_cast<float4*>(part + ((c / 4 + x) * kRows + row) * 4) = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
+          }
+          }
+        }
+        if (!whole && mine) {
+          part[kRows * D + row] = m;
+          part[kRows * D + kRows + row] = l;
+        }
+      }
+      if (!whole && w.u0 == 0 && tid == 0)                 // it begins here and ends elsewhere: request, tile, parts, head and place of the first
+        a.cuts[blockIdx.x] = {w.r, w.tile, 1 + (int)((w.units - w.u1 + share - 1) / share), 2 * w.head + (segment != 0)};
+      fence_before();                                      // (the next tile's first product into O comes after this thread's next arrival)
+    }
+  } else if (count > 0 && warp < 8) {
+    // ================= cache -> fp16 core matrices
+    constexpr int kKeys = D / 16;                          // pieces of 16 bytes of keys of a thread
+    const int t = tid - 128, cw = warp - 4;
+    const int tg = (lane & 7) + 8 * (cw & 1), dc = (lane >> 3) + 4 * (cw >> 1);      // values: group of 8 tokens, piece of D / 8 dimensions
+    bool ok = true, bad = false;
+    uint4 kr[kKeys];
+    uint32_t vr[8][D / 32];
+    Walk w(s, count);
+    w.look(a);
+    // the unit that is fetched is one ahead of the one that is written
+    int fu = w.u0;
+    Walk f = w;
+    float ks = 0.f, vs = 0.f;
+    bool real = false;
+    const auto fetch = [&] {
+      const int at = fu * kUnit;
+      const int* table = a.tables + f.r * a.table_stride;
+      const auto page = [&](int token) {
+        if (token >= f.end) return -1;
+        const int id = table[token >> a.shift];
+        if (id >= 0 && id < a.pages) return id;
+        bad = true;
+        return -1;
+      };
+      const int place_mask = (1 << a.shift) - 1;
+      // keys: a warp's piece is 8 tokens x 64 bytes; a thread's are at tokens 32 cw + 8 (..) + lane % 8
+#pragma unroll
+      for (int b = 0; b < 4; b += 2) {
+        const int token16 = at + 32 * cw + 8 * b;
+        const int id = page(token16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int token = token16 + 8 * h + (lane & 7);
+          const uint8_t* src = a.k_cache + ((((size_t)id * a.kv_heads + f.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x)
+            kr[(b + h) * (D / 64) + x] = id >= 0 && token < f.end ? *reinterpret_cast<const uint4*>(src + 64 * x) : uint4{0, 0, 0, 0};
+        }
+      }
+      const int vtoken = at + 8 * tg, vid = page(vtoken);
+      const uint8_t* src = a.v_cache + ((((size_t)vid * a.kv_heads + f.head) << a.shift) + (vtoken & place_mask)) * D + dc * (D / 8);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const bool in = vid >= 0 && vtoken + x < f.end;    // behind the request's tokens lies what an earlier one left
+        if constexpr (D == 128) {
+          const uint4 raw = in ? *reinterpret_cast<const uint4*>(src + x * D) : uint4{0, 0, 0, 0};
+          vr[x][0] = raw.x; vr[x][1] = raw.y; vr[x][2] = raw.z; vr[x][3] = raw.w;
+        } else {
+          const uint2 raw = in ? *reinterpret_cast<const uint2*>(src + x * D) : uint2{0, 0};
+          vr[x][0] = raw.x; vr[x][1] = raw.y;
+        }
+      }
+      if (t < 8) {                                         // scales of the unit's groups
+        const int id = page(at + 16 * t);
+        real = id >= 0;
+        ks = real ? a.k_scale[(size_t)id * a.kv_heads + f.head] : 0.f;
+        vs = real ? a.v_scale[(size_t)id * a.kv_heads + f.head] : 1.f;
+      }
+      // the next one
+      if (++fu == f.u1) {
+        f.next(a);
+        if (f.left > 0) {
+          f.look(a);
+          fu = f.u0;
+        }
+      }
+    };
+    fetch();
+    bool first = true;
+    for (; w.left > 0 && ok;) {
+      for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1, first = false) {
+        // ---- keys
+        if (!first) ok = bar_wait(s_full, phase ^ 1, fail);
+        if (!(ok = __all_sync(kFullWarp, ok))) break;
+        if (cw == 0) {
+          const unsigned mask = __ballot_sync(kFullWarp, t < 8 && real);
+          if (t < 8) {
+            s.ks[phase][t] = ks;
+            s.lv[phase][t] = __log2f(vs);                  // of a power of two: exact
+            s.inv[phase][t] = __fdividef(1.f, vs);
+          }
+          // (a group behind the last token has no page either: the rows' ends mask it)
+          if (t == 0) s.real[phase] = mask;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            const uint4 raw = kr[b * (D / 64) + x];
+            uint8_t* dst = smem + Y::kK + (4 * cw + b) * Y::kGroup + (lane & 7) * 16 + (2 * ((lane >> 3) + 4 * x)) * 128;
+            *reinterpret_cast<uint4*>(dst) = {from_e4m3(raw.x & 0xFFFFu), from_e4m3(raw.x >> 16), from_e4m3(raw.y & 0xFFFFu), from_e4m3(raw.y >> 16)};
+            *reinterpret_cast<uint4*>(dst + 128) = {from_e4m3(raw.z & 0xFFFFu), from_e4m3(raw.z >> 16), from_e4m3(raw.w & 0xFFFFu), from_e4m3(raw.w >> 16)};
+          }
+        fence_async();
+        // (the product of these keys has to wait for P anyway; until then no one is a phase behind on this barrier)
+        if (!first) ok = bar_wait(p_full, phase ^ 1, fail);
+        if (!(ok = __all_sync(kFullWarp, ok))) break;
+        bar_arrive(k_full);
+        // ---- values
+        if (!first) ok = bar_wait(pv_done, phase ^ 1, fail);
+        if (!(ok = __all_sync(kFullWarp, ok))) break;
+        const int vtoken = u * kUnit + 8 * tg;
+        if (vtoken + 8 > w.least) {                        // tokens that not all rows see: a NaN there is not for the others
+          uint32_t any = 0;
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+              const uint32_t b = vtoken + x >= w.least ? nan_bytes(vr[x][j]) : 0;
+              vr[x][j] &= ~b;
+              any |= b;
+            }
+          if (any) s.nan = 1;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {                 // four dimensions of eight tokens
+          uint32_t lo[4], hi[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            lo[x] = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], 0x5140);
+            hi[x] = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], 0x7362);
+          }
+          const int d = dc * (D / 8) + 4 * j;
+          uint8_t* dst = smem + Y::kV + tg * Y::kTokens + (d >> 3) * 128 + (d & 7) * 16;
+          *reinterpret_cast<uint4*>(dst) = {from_e4m3(lo[0] & 0xFFFFu), from_e4m3(lo[1] & 0xFFFFu), from_e4m3(lo[2] & 0xFFFFu), from_e4m3(lo[3] & 0xFFFFu)};
+          *reinterpret_cast<uint4*>(dst + 16) = {from_e4m3(lo[0] >> 16), from_e4m3(lo[1] >> 16), from_e4m3(lo[2] >> 16), from_e4m3(lo[3] >> 16)};
+          *reinterpret_cast<uint4*>(dst + 32) = {from_e4m3(hi[0] & 0xFFFFu), from_e4m3(hi[1] & 0xFFFFu), from_e4m3(hi[2] & 0xFFFFu), from_e4m3(hi[3] & 0xFFFFu)};
+          *reinterpret_cast<uint4*>(dst + 48) = {from_e4m3(hi[0] >> 16), from_e4m3(hi[1] >> 16), from_e4m3(hi[2] >> 16), from_e4m3(hi[3] >> 16)};
+        }
+        fence_async();
+        bar_arrive(v_full);
+        if (f.left > 0) fetch();
+      }
+      if (!ok) break;
+      w.next(a);
+      if (w.left > 0) w.look(a);
+    }
+    if (bad && a.status) atomicOr(a.status, 32);
+  } else if (count > 0) {
+    // ================= products
+    const uint32_t idesc_s = 1u << 4 | (128u >> 3) << 17 | (128u >> 4) << 24, idesc_o = 1u << 4 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
+    const uint64_t dq = descriptor(smem_u32(smem + Y::kQ), 128, Y::kGroup), dk = descriptor(smem_u32(smem + Y::kK), 128, Y::kGroup),
+                   dv = descriptor(smem_u32(smem + Y::kV), Y::kTokens, 128);
+    bool ok = true;
+    uint32_t q_phase = 0;
+    Walk w(s, count);
+    for (; w.left > 0 && ok; w.next(a), q_phase ^= 1) {
+      w.look(a);
+      ok = __all_sync(kFullWarp, bar_wait(q_full, q_phase, fail));
+      for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1) {
+        ok = __all_sync(kFullWarp, bar_wait(k_full, phase, fail));
+        if (!ok) break;
+        fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) mma_ss(tmem, dq + 16 * k, dk + 16 * k, idesc_s, k != 0);
+          commit(s_full);
+        }
+        __syncwarp();
+        ok = __all_sync(kFullWarp, bar_wait(p_full, phase, fail) && bar_wait(v_full, phase, fail));
+        if (!ok) break;
+        fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mma_ts(tmem + 128, tmem + 8 * k, dv + (uint64_t)(k * (2 * Y::kTokens >> 4)), idesc_o, u != w.u0 || k != 0);
+          commit(pv_done);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {                                             // products in flight end before the tensor memory goes back
+      if (elect_one()) commit(smem_u32(&s.drained));
+      __syncwarp();
+      for (unsigned i = 0; i < kSpinLimit && !bar_try(smem_u32(&s.drained), 0); ++i) {}
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (tid == 0 && s.fail && a.status) atomicOr(a.status, 64);
+  if (warp == 8) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemColumns) : "memory");
+  }
+}
+
+// Joins the parts of the tiles that were cut: a thread block per run of the launch before, a thread per row and four dimensions.
+template <typename T, int D>
+__global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const AttentionArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 cut = a.cuts[blockIdx.x];
+  if (cut.z == 0) return;
+  const Request x(a, cut.x);
+  const int kvh = cut.w >> 1, rows = x.tokens(a, cut.y) * a.group;
+  const float *head = a.parts + ((size_t)blockIdx.x * 2 + (cut.w & 1)) * kPartFloats<D>, *tail = a.parts + (size_t)blockIdx.x * 2 * kPartFloats<D>;
+  for (int z = threadIdx.x; z < kRows * (D / 4); z += 512) {
+    const int row = z % kRows, d = z / kRows;
+    if (row >= rows) continue;
+    float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
+    float4 y = *reinterpret_cast<const float4*>(head + (d * kRows + row) * 4);
+#pragma unroll 2
+    for (int i = 1; i < cut.z; ++i) {
+      const float* part = tail + (size_t)i * 2 * kPartFloats<D>;
+      const float pm = part[kRows * D + row], pl = part[kRows * D + kRows + row];
+      const float4 v = *reinterpret_cast<const float4*>(part + (d * kRows + row) * 4);
+      const float now = fmaxf(m, pm), f = now == kNone ? 1.f : exp2_fast(m - now), h = now == kNone ? 1.f : exp2_fast(pm - now);
+      m = now;
+      l = l * f + pl * h;
+      y.x = y.x * f + v.x * h; y.y = y.y * f + v.y * h; y.z = y.z * f + v.z * h; y.w = y.w * f + v.w * h;
+    }
+    const float by = l == 0.f ? 0.f : 1.f / l;
+    const int i = row / a.group;
+    T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + cut.y * x.per + i) * a.q_heads + (size_t)kvh * a.group + row - i * a.group) * D + 4 * d;
+    *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};
+  }
+}
+
+int device_sms() {
+  static int cache[64] = {0};
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
+  if (dev >= 0 && dev < 64) cache[dev] = v;
+  return v;
+}
+
+template <typename T, int D>
+int run(const AttentionArgs& a, cudaStream_t st) {
+  static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
+  int dev = 0, e = (int)cudaGetDevice(&dev);
+  if (!e && (dev < 0 || dev >= 64 || !allowed[dev])) {
+    e = (int)cudaFuncSetAttribute(paged_attention_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
+    if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
+  }
+  if (e) return paged_fail(e);
+  const dim3 grid(device_sms() * kBlocksPerSm);
+  const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, Layout<D>::kBytes, st, a);
+  return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, grid, dim3(512), 1, 0, st, a);
+}
+
+}  // namespace
+
+namespace htr {
+
+// More than 16 rows a tile: the other kernel takes 16 of them per pass over the cache.
+bool attention_tc_serves(int requests, int group, int max_new) { return requests <= kMaxRequests && group <= kRows && (long long)group * max_new > 16; }
+
+size_t attention_tc_workspace(int head_dim) {
+  return (size_t)device_sms() * kBlocksPerSm * (sizeof(int4) + 2 * sizeof(float) * (head_dim == 128 ? kPartFloats<128> : kPartFloats<64>));
+}
+
+int attention_tc_run(const AttentionArgs& args, int dtype, int head_dim, void* workspace, cudaStream_t st) {
+  AttentionArgs a = args;
+  a.cuts = static_cast<int4*>(workspace);
+  a.parts = reinterpret_cast<float*>(a.cuts + device_sms() * kBlocksPerSm);
+  if (dtype == HTR_DTYPE_BF16) return head_dim == 128 ? run<__nv_bfloat16, 128>(a, st) : run<__nv_bfloat16, 64>(a, st);
+  return head_dim == 128 ? run<__half, 128>(a, st) : run<__half, 64>(a, st);
+}
+
+}  // namespace htr

@@ -1,0 +1,104 @@
+// What the kernels of the paged 8-bit cache share: element types, e4m3 conversions, the arguments of the attention, launches.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/htr_b200.h"
+#include "htr_common.cuh"
+
+namespace htr {
+
+int paged_fail(int cuda_error);                            // keeps the error for htr_paged_last_cuda_error, HTR_ERR_CUDA
+
+template <typename Kern, typename... Args>
+int paged_launch(Kern kern, dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const int e = (int)cudaLaunchKernelEx(&cfg, kern, args...);
+  if (!e) return HTR_OK;
+  (void)cudaGetLastError();                                // a refused launch leaves no error behind for the caller's next check
+  return paged_fail(e);
+}
+
+template <typename T> struct Half;
+template <> struct Half<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+  static __device__ __forceinline__ uint32_t narrow(float x, float y) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <> struct Half<__half> {
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t narrow(float x, float y) {
+    const __half2 r = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+
+// two floats as e4m3, the first in the low byte (beyond the range: the largest value; NaN stays NaN)
+__device__ __forceinline__ uint32_t to_e4m3(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t from_e4m3(uint32_t two) {   // two e4m3 in the low half -> two fp16
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  return r;
+}
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {     // 0xFF where a byte is one of e4m3's NaN
+  return __vcmpeq4(v & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+}
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 r = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+constexpr float kNone = -__builtin_huge_valf();
+
+struct AttentionArgs {
+  const void* q;
+  const int *starts, *seen, *tables;
+  long long table_stride;
+  int width, requests, tokens, q_heads, kv_heads, group, max_new;
+  const uint8_t *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  int pages, shift;
+  float scale;                                             // of the scores, times log2(e)
+  void* out;
+  int* status;
+  float* parts;                                            // two per thread block: results, maxima, sums of a tile's rows
+  int4* cuts;                                              // per thread block, of the tile that begins in its run and goes beyond it
+};
+
+// the exponent that brings a row of queries to the upper end of fp16: `most` is its largest magnitude
+__device__ __forceinline__ int query_exponent(float most) {
+  return most > 0.f && most <= 3.402823466e38f ? min(max(14 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100) : 0;
+}
+
+// attention for many rows a request, on the tensor cores (paged_attention_tc.cu)
+bool attention_tc_serves(int requests, int group, int max_new);
+size_t attention_tc_workspace(int head_dim);
+int attention_tc_run(const AttentionArgs& a, int dtype, int head_dim, void* workspace, cudaStream_t st);
+
+}  // namespace htr

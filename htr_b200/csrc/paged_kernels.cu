@@ -7,16 +7,11 @@
 // Why e4m3 under powers of two: a page fills token by token, and a later token may be larger than what its scale admits.  The scale
 // then grows and the older tokens are rescaled by a power of two, which keeps their three mantissa bits (only values that fall among
 // the subnormals, 2^-15 of the page's largest and less, are rounded again); 8-bit integers would be rounded anew every time.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include <cstdint>
-
-#include "../../include/htr_b200.h"
-#include "htr_common.cuh"
+#include "paged_common.cuh"
 
 namespace {
+
+using namespace htr;
 
 constexpr int kScaleFloor = -100;                          // smallest exponent of a scale: products of two scales stay normal floats
 
@@ -26,30 +21,6 @@ __device__ __forceinline__ void pdl_enter() {
 }
 
 thread_local int t_last_cuda = 0;
-
-template <typename Kern, typename... Args>
-int launch(Kern kern, dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const int e = (int)cudaLaunchKernelEx(&cfg, kern, args...);
-  if (e) {
-    t_last_cuda = e;
-    (void)cudaGetLastError();                              // a refused launch leaves no error behind for the caller's next check
-    return HTR_ERR_CUDA;
-  }
-  return HTR_OK;
-}
 
 // ---- the plan of a step -----------------------------------------------------------------------------------------------------------
 //
@@ -236,35 +207,6 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
 }
 
 // ---- the cache's writing side -----------------------------------------------------------------------------------------------------
-
-template <typename T> struct Half;
-template <> struct Half<__nv_bfloat16> {
-  static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
-  static __device__ __forceinline__ uint32_t narrow(float x, float y) {
-    const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-template <> struct Half<__half> {
-  static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-  static __device__ __forceinline__ uint32_t narrow(float x, float y) {
-    const __half2 r = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-
-// two floats as e4m3, the first in the low byte (beyond the range: the largest value; NaN stays NaN)
-__device__ __forceinline__ uint32_t to_e4m3(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t from_e4m3(uint32_t two) {   // two e4m3 in the low half -> two fp16
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
-  return r;
-}
-__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
 
 // the exponent of the smallest power of two under which `most` (finite, not negative) lies within e4m3
 __device__ __forceinline__ int scale_exponent(float most) {
@@ -491,21 +433,6 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
 // (P' = 2^(s + log2 scale - m)), and the sum of the probabilities takes it out again.  2^-11 each at most, averaged over the tokens: below
 // the rounding of the output.  m follows the largest exponent only when that grows by 2^14 (P' stays below 2^14, sums are float32).
 
-struct AttentionArgs {
-  const void* q;
-  const int *starts, *seen, *tables;
-  long long table_stride;
-  int width, requests, tokens, q_heads, kv_heads, group, max_new;
-  const uint8_t *k_cache, *v_cache;
-  const float *k_scale, *v_scale;
-  int pages, shift;
-  float scale;                                             // of the scores, times log2(e)
-  void* out;
-  int* status;
-  float* parts;                                            // two per thread block: rows x (D results, maximum, sum)
-  int4* cuts;                                              // per thread block, of the tile that begins in its run and goes beyond it: see below
-};
-
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -516,18 +443,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8x8 matrix 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-  const __half2 r = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 constexpr int kAttWarps = 4, kAttThreads = kAttWarps * 32, kUnit = kAttWarps * 16;   // tokens of a unit
-constexpr float kNone = -__builtin_huge_valf();
 // thread blocks per SM, by the registers that the tiles in flight and the results need
 template <int D, int NT>
 constexpr int kAttBlocks = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
@@ -557,8 +473,7 @@ struct Rows {
       }
       most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 1));
       most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 2));
-      int e = 0;
-      if (most > 0.f && most <= 3.402823466e38f) e = min(max(14 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
+      const int e = query_exponent(most);
       const float up = exp2i(e);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -611,10 +526,6 @@ struct Tile {
     vs = a.v_scale[unit];
   }
 };
-
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {   // 0xFF where a byte is one of e4m3's NaN
-  return __vcmpeq4(v & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-}
 
 // running softmax of a warp: results O^T (dimension D/8 g + 2 j + i / 2, rows 2 c + i % 2), maximum and sum of this lane's rows
 template <int D, int NT>
@@ -961,8 +872,8 @@ int attention_tiles(int group, int max_new) { return (long long)group * max_new 
 template <typename T, int D, int NT>
 int attention_run(const AttentionArgs& a, cudaStream_t st) {
   const dim3 grid(attention_blocks(D, NT)), block(kAttThreads);
-  const int rc = launch(paged_attention_kernel<T, D, NT>, grid, block, 1, 0, st, a);
-  return rc != HTR_OK ? rc : launch(paged_attention_join_kernel<T, D, NT>, grid, block, 1, 0, st, a);
+  const int rc = paged_launch(paged_attention_kernel<T, D, NT>, grid, block, 1, 0, st, a);
+  return rc != HTR_OK ? rc : paged_launch(paged_attention_join_kernel<T, D, NT>, grid, block, 1, 0, st, a);
 }
 
 template <typename T>
@@ -973,11 +884,20 @@ int attention_of(const AttentionArgs& a, int head_dim, int max_new, cudaStream_t
 
 template <typename T>
 int append_of(const AppendArgs& a, int head_dim, dim3 grid, cudaStream_t st) {
-  return head_dim == 128 ? launch(rope_append_kernel<T, 128>, grid, dim3(kAppendThreads), 1, 0, st, a)
-                         : launch(rope_append_kernel<T, 64>, grid, dim3(kAppendThreads), 1, 0, st, a);
+  return head_dim == 128 ? paged_launch(rope_append_kernel<T, 128>, grid, dim3(kAppendThreads), 1, 0, st, a)
+                         : paged_launch(rope_append_kernel<T, 64>, grid, dim3(kAppendThreads), 1, 0, st, a);
 }
 
 }  // namespace
+
+namespace htr {
+
+int paged_fail(int cuda_error) {
+  t_last_cuda = cuda_error;
+  return HTR_ERR_CUDA;
+}
+
+}  // namespace htr
 
 extern "C" {
 
@@ -997,14 +917,11 @@ int htr_page_plan(const int* lengths, const int* added, int requests, int* table
   const size_t smem = 4 * sizeof(int) * (size_t)requests;
   if (smem > 40960) {
     const int e = (int)cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * sizeof(int) * kPlanMaxRequests);
-    if (e) {
-      t_last_cuda = e;
-      return HTR_ERR_CUDA;
-    }
+    if (e) return paged_fail(e);
   }
   const int work = max_tokens > requests ? max_tokens : requests;
   const int blocks = work <= kPlanThreads ? 1 : kPlanMaxCluster;
-  return launch(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), blocks, smem, static_cast<cudaStream_t>(stream), a);
+  return paged_launch(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), blocks, smem, static_cast<cudaStream_t>(stream), a);
 }
 
 int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* positions, const int* slots, int tokens, const float* cosv,
@@ -1031,6 +948,7 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
 
 size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new) {
   if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_new < 1 || (head_dim != 64 && head_dim != 128)) return 0;
+  if (attention_tc_serves(requests, q_heads / kv_heads, max_new)) return attention_tc_workspace(head_dim);
   const int tiles = attention_tiles(q_heads / kv_heads, max_new);
   const size_t rows = 8 * tiles;
   return attention_blocks(head_dim, tiles) * (2 * rows * (head_dim + 2) * sizeof(float) + sizeof(int4));
@@ -1053,11 +971,13 @@ int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts,
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return HTR_ERR_ALIGNMENT;
   if (!workspace || workspace_bytes < htr_paged_attention_workspace_bytes(tokens, requests, q_heads, kv_heads, head_dim, max_new)) return HTR_ERR_WORKSPACE;
   if (!aligned16(workspace)) return HTR_ERR_ALIGNMENT;
+  const bool tc = attention_tc_serves(requests, q_heads / kv_heads, max_new);
   int4* cuts = static_cast<int4*>(workspace);
   const AttentionArgs a = {q, starts, seen, tables, table_stride, table_width, requests, tokens, q_heads, kv_heads, q_heads / kv_heads, max_new,
                            static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), k_scale, v_scale, pages, shift,
                            scale * 1.4426950408889634f, out, status, reinterpret_cast<float*>(cuts + attention_blocks(head_dim, attention_tiles(q_heads / kv_heads, max_new))), cuts};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (tc) return attention_tc_run(a, dtype, head_dim, workspace, st);
   return dtype == HTR_DTYPE_BF16 ? attention_of<__nv_bfloat16>(a, head_dim, max_new, st) : attention_of<__half>(a, head_dim, max_new, st);
 }
 
