@@ -4,11 +4,11 @@
 // A tile is up to 128 rows: the query heads of one key/value head for as many whole tokens as fit (row = token * group + head).  Per 128
 // cached tokens: S = Q K^T (128 x 128), P = 2^(S - m) in fp16, O += P V.  S, P and O are in tensor memory (P over S), Q, K and V in shared
 // memory as fp16 core matrices; keys and values are e4m3 in the cache and become fp16, exactly, on the way there.
-// Three roles per thread block, two thread blocks per SM, so that one's products run while the other's roles wait for one another:
+// Two roles per thread block, two thread blocks per SM, so that one's products run while the other's roles wait for one another:
 //   warps 0-3  a thread per row (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.
 //   warps 4-7  cache -> registers (the next 128 tokens are on their way) -> fp16 core matrices.  Values are transposed on the way (their
 //              operand wants eight tokens of a dimension side by side): byte permutes of eight rows in registers.
-//   warp 8     issues the products; barriers: K full -> S full (K free) -> P and V full -> product done (V, P free).
+// Barriers: K full -> S full (K free) -> P and V full -> product done (V, P free); warp 4 issues the products.
 // What bounds it: per 128 tokens and 128 rows 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM), and about 900 of
 // issue on each scheduler; the three overlap between the two thread blocks.
 // The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
@@ -20,7 +20,7 @@ namespace {
 
 using namespace htr;
 
-constexpr int kThreads = 288, kRows = 128, kUnit = 128, kMaxRequests = 1024, kBlocksPerSm = 2;
+constexpr int kThreads = 256, kRows = 128, kUnit = 128, kMaxRequests = 1024, kBlocksPerSm = 2;
 constexpr int kTmemColumns = 256;                          // S (P over it) at 0, O at 128
 constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
 
@@ -80,7 +80,7 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
         "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
         "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
@@ -98,6 +98,15 @@ __device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&r)[16]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                  "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(at) : "memory");
+}
+// (what was loaded goes through the wait, so that no use of it is moved before)
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :: "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -186,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     a.cuts[blockIdx.x] = {0, 0, 0, 0};
   }
-  if (warp == 8) {
+  if (warp == 0) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"((uint32_t)kTmemColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -262,6 +271,32 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
     const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
     const int row = tid;
     bool ok = true;
+    // results (where there are any) and the first `chunks` pieces of P, relative to a new reference
+    const auto follow = [&](float f, bool results, int chunks) {
+      tmem_stored();
+      if (results)
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          tmem_load16(lanes + 128 + c, o);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+          tmem_store(lanes + 128 + c, o);
+        }
+#pragma unroll 1
+      for (int c = 0; c < 16 * chunks; c += 16) {
+        uint32_t o[16];
+        tmem_load16(lanes + c, o);
+        const __half2 h = __float2half2_rn(f);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o[x]), h);
+          o[x] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        tmem_store(lanes + c, o);
+      }
+      tmem_stored();
+    };
     Walk w(s, count);
     for (int segment = 0; w.left > 0 && ok; ++segment, w.next(a)) {
       w.look(a);
@@ -298,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
           *reinterpret_cast<uint4*>(dst + j * 128) = r;
         }
         fence_async();
+        fence_before();
         bar_arrive(q_full);
       }
       float m = kNone, l = 0.f;
@@ -310,68 +346,53 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
         const unsigned real = s.real[phase];
         const bool edge = at + kUnit > w.least || real != 0xFFu;
         if (32 * warp < rows) {
-#pragma unroll 1
-          for (int j = 0; j < 4; ++j) {                    // 32 tokens: two groups of 16
-            uint32_t raw[32];
-            tmem_load(lanes + 32 * j, raw);
-            float v[32], base = m == kNone ? 0.f : m, most = kNone;
+          uint32_t raw[2][32];                             // 32 tokens (two groups of 16), and the next ones on their way
+          tmem_load(lanes, raw[0]);
+          tmem_loaded(raw[0]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float v[32], base = m == kNone ? 0.f : m, most[4];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const float by = row_scale * s.ks[phase][2 * j + g], add = s.lv[phase][2 * j + g] - base;
 #pragma unroll
-              for (int c = 0; c < 16; ++c) v[16 * g + c] = fmaf(__uint_as_float(raw[16 * g + c]), by, add);
+              for (int c = 0; c < 16; ++c) v[16 * g + c] = fmaf(__uint_as_float(raw[j & 1][16 * g + c]), by, add);
             }
+            if (j < 3) tmem_load(lanes + 32 * (j + 1), raw[(j + 1) & 1]);
             if (edge) {
 #pragma unroll
               for (int c = 0; c < 32; ++c)
                 if (at + 32 * j + c >= row_end || !(real >> (2 * j + (c >> 4)) & 1)) v[c] = kNone;
             }
 #pragma unroll
-            for (int c = 0; c < 32; ++c) most = fmaxf(most, v[c]);
-            const bool grows = m == kNone ? most > kNone : most > 14.f;
-            if (__any_sync(kFullWarp, grows)) {            // a new reference, 2^6 above which the largest lies; what there is follows
-              const float now = grows ? base + most - 6.f : m, f = grows && m != kNone ? exp2_fast(m - now) : 1.f;
-              if (grows) {
+            for (int x = 0; x < 4; ++x) {
+              most[x] = fmaxf(v[8 * x], v[8 * x + 1]);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] += base - now;
-                m = now;
-                l *= f;
-              }
-              __syncwarp();
-              tmem_stored();
-              if (u > w.u0)
-#pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                  uint32_t o[16];
-                  tmem_load16(lanes + 128 + c, o);
-#pragma unroll
-                  for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                  tmem_store(lanes + 128 + c, o);
-                }
-#pragma unroll 1
-              for (int c = 0; c < 16 * j; c += 16) {
-                uint32_t o[16];
-                tmem_load16(lanes + c, o);
-                const __half2 h = __float2half2_rn(f);
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o[x]), h);
-                  o[x] = *reinterpret_cast<const uint32_t*>(&y);
-                }
-                tmem_store(lanes + c, o);
-              }
-              tmem_stored();
+              for (int c = 2; c < 8; c += 2) most[x] = fmaxf(fmaxf(most[x], v[8 * x + c]), v[8 * x + c + 1]);
             }
+            most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+            const bool grows = m == kNone ? most[0] > kNone : most[0] > 14.f;
+            if (__any_sync(kFullWarp, grows)) {            // a new reference, 2^6 above which the largest lies; what there is follows
+              const float now = grows ? base + most[0] - 6.f : m, f = grows && m != kNone ? exp2_fast(m - now) : 1.f, down = grows ? base - now : 0.f;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) v[c] += down;
+              m = now;
+              l *= f;
+              __syncwarp();
+              if (j < 3) tmem_loaded(raw[(j + 1) & 1]);
+              follow(f, u > w.u0, j);
+            }
+            float sum[4];
             uint32_t p[16];
-            float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               const float x = exp2_fast(v[2 * c]), y = exp2_fast(v[2 * c + 1]);
-              sum[c >> 3] += x + y;
+              sum[c >> 2] = (c & 3) ? sum[c >> 2] + (x + y) : x + y;
               p[c] = pack_half(x, y);
             }
+            l = fmaf(sum[0] + sum[1], s.inv[phase][2 * j], fmaf(sum[2] + sum[3], s.inv[phase][2 * j + 1], l));
             __syncwarp();
-            l = fmaf(sum[0], s.inv[phase][2 * j], fmaf(sum[1], s.inv[phase][2 * j + 1], l));
+            if (j < 3) tmem_loaded(raw[(j + 1) & 1]);                      // (P goes over columns that have been read)
             tmem_store(lanes + 16 * j, p);
           }
           tmem_stored();
@@ -440,56 +461,23 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
     uint32_t vr[8][D / 32];
     Walk w(s, count);
     w.look(a);
-    // the unit that is fetched is one ahead of the one that is written
-    int fu = w.u0;
+    // three units are under way: one that is written, the next, whose rows are being fetched, and the one after it, whose pages are
     Walk f = w;
-    float ks = 0.f, vs = 0.f;
-    bool real = false;
-    const auto fetch = [&] {
-      const int at = fu * kUnit;
+    int fu = w.u0;                                         // of the pages that are fetched
+    struct Pages {
+      int k[2], v, scale, head, at;
+      bool all;                                            // every token of the unit lies in a page and before the end
+    };
+    const auto pages_of = [&](Pages& p) {
+      p.at = fu * kUnit;
+      p.head = f.head;
       const int* table = a.tables + f.r * a.table_stride;
-      const auto page = [&](int token) {
-        if (token >= f.end) return -1;
-        const int id = table[token >> a.shift];
-        if (id >= 0 && id < a.pages) return id;
-        bad = true;
-        return -1;
-      };
-      const int place_mask = (1 << a.shift) - 1;
-      // keys: a warp's piece is 8 tokens x 64 bytes; a thread's are at tokens 32 cw + 8 (..) + lane % 8
-#pragma unroll
-      for (int b = 0; b < 4; b += 2) {
-        const int token16 = at + 32 * cw + 8 * b;
-        const int id = page(token16);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int token = token16 + 8 * h + (lane & 7);
-          const uint8_t* src = a.k_cache + ((((size_t)id * a.kv_heads + f.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
-#pragma unroll
-          for (int x = 0; x < D / 64; ++x)
-            kr[(b + h) * (D / 64) + x] = id >= 0 && token < f.end ? *reinterpret_cast<const uint4*>(src + 64 * x) : uint4{0, 0, 0, 0};
-        }
-      }
-      const int vtoken = at + 8 * tg, vid = page(vtoken);
-      const uint8_t* src = a.v_cache + ((((size_t)vid * a.kv_heads + f.head) << a.shift) + (vtoken & place_mask)) * D + dc * (D / 8);
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const bool in = vid >= 0 && vtoken + x < f.end;    // behind the request's tokens lies what an earlier one left
-        if constexpr (D == 128) {
-          const uint4 raw = in ? *reinterpret_cast<const uint4*>(src + x * D) : uint4{0, 0, 0, 0};
-          vr[x][0] = raw.x; vr[x][1] = raw.y; vr[x][2] = raw.z; vr[x][3] = raw.w;
-        } else {
-          const uint2 raw = in ? *reinterpret_cast<const uint2*>(src + x * D) : uint2{0, 0};
-          vr[x][0] = raw.x; vr[x][1] = raw.y;
-        }
-      }
-      if (t < 8) {                                         // scales of the unit's groups
-        const int id = page(at + 16 * t);
-        real = id >= 0;
-        ks = real ? a.k_scale[(size_t)id * a.kv_heads + f.head] : 0.f;
-        vs = real ? a.v_scale[(size_t)id * a.kv_heads + f.head] : 1.f;
-      }
-      // the next one
+      const auto page = [&](int token) { return token < f.end ? table[token >> a.shift] : -1; };
+      p.k[0] = page(p.at + 32 * cw);
+      p.k[1] = page(p.at + 32 * cw + 16);
+      p.v = page(p.at + 8 * tg);
+      p.scale = page(p.at + 16 * (t & 7));
+      p.all = p.at + kUnit <= f.end;
       if (++fu == f.u1) {
         f.next(a);
         if (f.left > 0) {
@@ -498,15 +486,74 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
         }
       }
     };
-    fetch();
+    const int place_mask = (1 << a.shift) - 1;
+    const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
+    // (a page that is none is read as the first one and left aside later)
+    const auto keys_of = [&](const Pages& p) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int id = valid(p.k[b >> 1]) ? p.k[b >> 1] : 0, token = p.at + 32 * cw + 8 * b + (lane & 7);
+        const uint8_t* src = a.k_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) kr[b * (D / 64) + x] = *reinterpret_cast<const uint4*>(src + 64 * x);
+      }
+    };
+    const auto values_of = [&](const Pages& p) {
+      const int id = valid(p.v) ? p.v : 0, token = p.at + 8 * tg;
+      const uint8_t* src = a.v_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + dc * (D / 8);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        if constexpr (D == 128) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(src + x * D);
+          vr[x][0] = raw.x; vr[x][1] = raw.y; vr[x][2] = raw.z; vr[x][3] = raw.w;
+        } else {
+          const uint2 raw = *reinterpret_cast<const uint2*>(src + x * D);
+          vr[x][0] = raw.x; vr[x][1] = raw.y;
+        }
+      }
+    };
+    float ks = 0.f, vs = 1.f;
+    const auto scales_of = [&](const Pages& p) {
+      const size_t at = (size_t)(valid(p.scale) ? p.scale : 0) * a.kv_heads + p.head;
+      ks = a.k_scale[at];
+      vs = a.v_scale[at];
+    };
+    Pages now, next, later;                                // of the unit that is written, of the next, of the one after it
+    pages_of(now);
+    keys_of(now);
+    values_of(now);
+    scales_of(now);
+    next = now;
+    if (f.left > 0) pages_of(next);
+    long long owed = count - 1;                            // units whose rows have not been fetched
+    // the products, issued by the first of these warps, which wait for P and the keys anyway
+    const uint32_t idesc_s = 1u << 4 | (128u >> 3) << 17 | (128u >> 4) << 24, idesc_o = 1u << 4 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
+    const uint64_t dq = descriptor(smem_u32(smem + Y::kQ), 128, Y::kGroup), dk = descriptor(smem_u32(smem + Y::kK), 128, Y::kGroup),
+                   dv = descriptor(smem_u32(smem + Y::kV), Y::kTokens, 128);
+    uint32_t fresh = 0, q_phase = 0;                       // fresh: 0 where the unit before is the first of its tile
+    const auto results = [&](uint32_t of) {                // O of the unit of that phase, whose P is there
+      const bool ok = __all_sync(kFullWarp, bar_wait(v_full, of, fail));
+      if (!ok) return false;
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mma_ts(tmem + 128, tmem + 8 * k, dv + (uint64_t)(k * (2 * Y::kTokens >> 4)), idesc_o, k != 0 ? 1u : fresh);
+        commit(pv_done);
+      }
+      __syncwarp();
+      return true;
+    };
     bool first = true;
     for (; w.left > 0 && ok;) {
       for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1, first = false) {
         // ---- keys
         if (!first) ok = bar_wait(s_full, phase ^ 1, fail);
         if (!(ok = __all_sync(kFullWarp, ok))) break;
+        later = next;
+        if (f.left > 0) pages_of(later);
         if (cw == 0) {
-          const unsigned mask = __ballot_sync(kFullWarp, t < 8 && real);
+          const unsigned mask = __ballot_sync(kFullWarp, t < 8 && valid(now.scale));
+          bad |= now.scale != -1 && !valid(now.scale);     // (-1: behind the last token)
           if (t < 8) {
             s.ks[phase][t] = ks;
             s.lv[phase][t] = __log2f(vs);                  // of a power of two: exact
@@ -526,13 +573,38 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
           }
         fence_async();
         // (the product of these keys has to wait for P anyway; until then no one is a phase behind on this barrier)
+        if (owed > 0) {
+          keys_of(next);
+          scales_of(next);
+        }
         if (!first) ok = bar_wait(p_full, phase ^ 1, fail);
         if (!(ok = __all_sync(kFullWarp, ok))) break;
+        if (cw == 0 && !first && !(ok = results(phase ^ 1))) break;
         bar_arrive(k_full);
+        if (cw == 0) {
+          ok = __all_sync(kFullWarp, bar_wait(k_full, phase, fail) && (u != w.u0 || bar_wait(q_full, q_phase, fail)));
+          if (!ok) break;
+          fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) mma_ss(tmem, dq + 16 * k, dk + 16 * k, idesc_s, k != 0);
+            commit(s_full);
+          }
+          __syncwarp();
+          if (u == w.u0) q_phase ^= 1;
+          fresh = u != w.u0;
+        }
         // ---- values
         if (!first) ok = bar_wait(pv_done, phase ^ 1, fail);
         if (!(ok = __all_sync(kFullWarp, ok))) break;
         const int vtoken = u * kUnit + 8 * tg;
+        if (!now.all || !valid(now.v)) {                   // behind the request's tokens lies what an earlier one left
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+              if (vtoken + x >= w.end || !valid(now.v)) vr[x][j] = 0;
+        }
         if (vtoken + 8 > w.least) {                        // tokens that not all rows see: a NaN there is not for the others
           uint32_t any = 0;
 #pragma unroll
@@ -562,55 +634,29 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
         }
         fence_async();
         bar_arrive(v_full);
-        if (f.left > 0) fetch();
+        if (owed > 0) values_of(next);
+        --owed;
+        now = next;
+        next = later;
       }
       if (!ok) break;
       w.next(a);
       if (w.left > 0) w.look(a);
     }
-    if (bad && a.status) atomicOr(a.status, 32);
-  } else if (count > 0) {
-    // ================= products
-    const uint32_t idesc_s = 1u << 4 | (128u >> 3) << 17 | (128u >> 4) << 24, idesc_o = 1u << 4 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
-    const uint64_t dq = descriptor(smem_u32(smem + Y::kQ), 128, Y::kGroup), dk = descriptor(smem_u32(smem + Y::kK), 128, Y::kGroup),
-                   dv = descriptor(smem_u32(smem + Y::kV), Y::kTokens, 128);
-    bool ok = true;
-    uint32_t q_phase = 0;
-    Walk w(s, count);
-    for (; w.left > 0 && ok; w.next(a), q_phase ^= 1) {
-      w.look(a);
-      ok = __all_sync(kFullWarp, bar_wait(q_full, q_phase, fail));
-      for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1) {
-        ok = __all_sync(kFullWarp, bar_wait(k_full, phase, fail));
-        if (!ok) break;
-        fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) mma_ss(tmem, dq + 16 * k, dk + 16 * k, idesc_s, k != 0);
-          commit(s_full);
-        }
+    if (cw == 0) {
+      if (ok) ok = __all_sync(kFullWarp, bar_wait(p_full, phase ^ 1, fail)) && results(phase ^ 1);
+      if (!ok) {                                           // products in flight end before the tensor memory goes back
+        if (elect_one()) commit(smem_u32(&s.drained));
         __syncwarp();
-        ok = __all_sync(kFullWarp, bar_wait(p_full, phase, fail) && bar_wait(v_full, phase, fail));
-        if (!ok) break;
-        fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) mma_ts(tmem + 128, tmem + 8 * k, dv + (uint64_t)(k * (2 * Y::kTokens >> 4)), idesc_o, u != w.u0 || k != 0);
-          commit(pv_done);
-        }
-        __syncwarp();
+        for (unsigned i = 0; i < kSpinLimit && !bar_try(smem_u32(&s.drained), 0); ++i) {}
       }
     }
-    if (!ok) {                                             // products in flight end before the tensor memory goes back
-      if (elect_one()) commit(smem_u32(&s.drained));
-      __syncwarp();
-      for (unsigned i = 0; i < kSpinLimit && !bar_try(smem_u32(&s.drained), 0); ++i) {}
-    }
+    if (bad && a.status) atomicOr(a.status, 32);
   }
   fence_before();
   __syncthreads();
   if (tid == 0 && s.fail && a.status) atomicOr(a.status, 64);
-  if (warp == 8) {
+  if (warp == 0) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemColumns) : "memory");
   }
