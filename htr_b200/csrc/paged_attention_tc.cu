@@ -1,34 +1,41 @@
 // Attention over the paged 8-bit cache for many rows a request (prompts, shared key/value heads): tcgen05.mma with accumulators in tensor
 // memory.
 //
-// A tile is up to 128 rows: the query heads of one key/value head for as many whole tokens as fit (row = token * group + head).  Per 128
-// cached tokens: S = Q K^T (128 x 128), P = 2^(S - m) in fp16, O += P V.  S, P and O are in tensor memory (P over S), Q, K and V in shared
-// memory as fp16 core matrices; keys and values are e4m3 in the cache and become fp16, exactly, on the way there.
-// Two roles per thread block, two thread blocks per SM, so that one's products run while the other's roles wait for one another:
-//   warps 0-3  a thread per row (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.
-//   warps 4-7  cache -> registers (the next 128 tokens are on their way) -> fp16 core matrices.  Values are transposed on the way (their
-//              operand wants eight tokens of a dimension side by side): byte permutes of eight rows in registers.
-// Barriers: K full -> S full (K free) -> P and V full -> product done (V, P free); warp 4 issues the products.
-// What bounds it: per 128 tokens and 128 rows 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM), and about 900 of
-// issue on each scheduler; the three overlap between the two thread blocks.
+// A tile is up to 128 rows: the query heads of one key/value head for as many whole tokens as fit (row = token * group + head).  Per unit of 64
+// cached tokens: S = Q K^T (128 x 64), P = 2^(S - m) in fp16, O += P V.  S, P and O are in tensor memory (P over S, two of them in turns), Q, K and V
+// in shared memory as core matrices.
+//  * Keys are multiplied as they are, e4m3, and go from memory straight to their core matrices; a row of Q is a sum of e4m3 parts of four significant
+//    bits each under one power of two (two parts for bf16, three for fp16: exact down to 2^-18 of the row's largest element), which costs what
+//    one product of 16-bit operands would, without its conversions.
+//  * Values become fp16, exactly, on their way (P would need three e4m3 parts, at four conversions an element), transposed by byte permutes
+//    of eight rows in registers: their operand wants eight tokens of a dimension side by side.
+// Two roles per thread block, two thread blocks per SM:
+//   warps 0-3  a thread per row (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.  S of the next unit
+//              is there when one is done.
+//   warps 4-7  keys and values of the next unit; the first of them issues the products, Q K^T of the next unit before P V of this one.
+// What bounds it: per 128 rows and 64 tokens 512 cycles of tensor pipe, 512 of exponentials (16 a cycle and SM) and about 400 of issue on each
+// scheduler, which the two thread blocks overlap.
 // The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
 // the sum; see paged_kernels.cu, whose cut of the work into even runs over the thread blocks, parts and join this kernel shares, with
-// runs of units of 128 tokens of (request, tile, head), each as many as its last token sees.
+// runs of units of (request, tile, head), each as many as its last token sees.
 #include "paged_common.cuh"
 
 namespace {
 
 using namespace htr;
 
-constexpr int kThreads = 256, kRows = 128, kUnit = 128, kMaxRequests = 1024, kBlocksPerSm = 2;
-constexpr int kTmemColumns = 256;                          // S (P over it) at 0, O at 128
+constexpr int kThreads = 256, kRows = 128, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024, kBlocksPerSm = 2;
+constexpr int kTmemColumns = 256;                          // S (P over it) at 0 and 64, O at 128
 constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
 
-template <int D>
+template <typename T, int D>
 struct Layout {                                            // bytes of the operands: core matrices of 8 rows x 16 bytes
-  static constexpr int kGroup = 16 * D;                    // Q, K: between groups of 8 rows; 128 between neighbours in K
+  // Q as a sum of e4m3 of four significant bits each: two for the 8 bits of bf16, three for the 11 of fp16
+  static constexpr int kParts = Half<T>::kBits > 8 ? 3 : 2;
+  static constexpr int kGroup = 8 * D;                     // Q, K: between groups of 8 rows; 128 between neighbours in K
   static constexpr int kTokens = 16 * D + 16;              // V: between groups of 8 tokens (16 more: stores of 8 groups meet 8 bank groups)
-  static constexpr int kQ = 0, kK = kQ + 16 * kGroup, kV = kK + 16 * kGroup, kBytes = kV + 16 * kTokens;
+  static constexpr int kQ = 0, kPart = 16 * kGroup, kK = kQ + kParts * kPart, kKeys = 8 * kGroup, kV = kK + 2 * kKeys,
+                       kValues = 8 * kTokens, kBytes = kV + 2 * kValues;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -61,8 +68,8 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
   return is != 0;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {      // e4m3
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
                "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -110,6 +117,20 @@ __device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// two lanes of float32 arithmetic in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, uint32_t a, uint32_t b, float by, float add) {
+  asm("{\n\t.reg .b64 r, s, t;\n\tmov.b64 r, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 t, {%5, %5};\n\tfma.rn.f32x2 r, r, s, t;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(x), "=f"(y) : "r"(a), "r"(b), "f"(by), "f"(add));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 r, s;\n\tmov.b64 r, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 r, r, s;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // a request's tiles, and what one of them sees
 struct Request {
   int start, n, seen, per, tiles;                          // per: tokens of a tile
@@ -126,13 +147,13 @@ struct Request {
 };
 
 struct Shared {
-  unsigned long long k_full, s_full, v_full, p_full, pv_done, q_full, drained;
+  unsigned long long k_full[2], s_full[2], v_full[2], p_full[2], pv_done[2], q_full, drained;    // of the units in turns
   long long sums[kMaxRequests];                            // units of each request
   long long total, skip;
   int r, tile, head, unit;                                 // where this thread block's run begins
   uint32_t tmem;
   int fail, nan;
-  float ks[2][8], lv[2][8], inv[2][8];                     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
+  float ks[2][kGroups], lv[2][kGroups], inv[2][kGroups];                     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
   unsigned real[2];                                        // groups that have a page
 };
 
@@ -168,7 +189,7 @@ constexpr int kPartFloats = kRows * (D + 2);
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_kernel(const AttentionArgs a) {
-  using Y = Layout<D>;
+  using Y = Layout<T, D>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared s;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -185,11 +206,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
   }
   if (tid == 0) {
     s.fail = s.nan = 0;
-    bar_init(smem_u32(&s.k_full), 128);
-    bar_init(smem_u32(&s.s_full), 1);
-    bar_init(smem_u32(&s.v_full), 128);
-    bar_init(smem_u32(&s.p_full), 128);
-    bar_init(smem_u32(&s.pv_done), 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(smem_u32(&s.k_full[i]), 128);
+      bar_init(smem_u32(&s.s_full[i]), 1);
+      bar_init(smem_u32(&s.v_full[i]), 128);
+      bar_init(smem_u32(&s.p_full[i]), 128);
+      bar_init(smem_u32(&s.pv_done[i]), 1);
+    }
     bar_init(smem_u32(&s.q_full), 128);
     bar_init(smem_u32(&s.drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -263,37 +286,24 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
   from = blockIdx.x * share;
   const long long count = min(share, total - from);
   const uint32_t tmem = s.tmem;
-  const uint32_t k_full = smem_u32(&s.k_full), s_full = smem_u32(&s.s_full), v_full = smem_u32(&s.v_full), p_full = smem_u32(&s.p_full),
-                 pv_done = smem_u32(&s.pv_done), q_full = smem_u32(&s.q_full);
-  uint32_t phase = 0;                                      // of the barriers of a unit: units so far, modulo 2
+  const uint32_t k_full = smem_u32(s.k_full), s_full = smem_u32(s.s_full), v_full = smem_u32(s.v_full), p_full = smem_u32(s.p_full),
+                 pv_done = smem_u32(s.pv_done), q_full = smem_u32(&s.q_full);
+  // barrier and phase of unit n of this thread block
+  const auto reached = [&](uint32_t bars, uint32_t n) { return bar_wait(bars + 8 * (n & 1), n >> 1 & 1, fail); };
+  uint32_t n = 0;                                          // units so far
   if (count > 0 && warp < 4) {
     // ================= softmax: a thread per row
     const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
     const int row = tid;
     bool ok = true;
-    // results (where there are any) and the first `chunks` pieces of P, relative to a new reference
-    const auto follow = [&](float f, bool results, int chunks) {
-      tmem_stored();
-      if (results)
+    const auto follow = [&](float f) {                     // results relative to a new reference
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16];
-          tmem_load16(lanes + 128 + c, o);
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-          tmem_store(lanes + 128 + c, o);
-        }
-#pragma unroll 1
-      for (int c = 0; c < 16 * chunks; c += 16) {
+      for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
-        tmem_load16(lanes + c, o);
-        const __half2 h = __float2half2_rn(f);
+        tmem_load16(lanes + 128 + c, o);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o[x]), h);
-          o[x] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-        tmem_store(lanes + c, o);
+        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+        tmem_store(lanes + 128 + c, o);
       }
       tmem_stored();
     };
@@ -304,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
       const bool mine = row < rows;
       const size_t place = ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
       const int row_end = mine ? max(w.seen - w.n + w.tile * w.per + i + 1, 0) : 0;
-      // queries: fp16 under a power of two per row
+      // queries: e4m3 parts under a power of two per row
       float row_scale;
       {
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + place);
@@ -317,91 +327,119 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
 #pragma unroll
             for (int x = 0; x < 4; ++x) most = fmaxf(most, fmaxf(fabsf(f[x].x), fabsf(f[x].y)));
           }
-        const int e = query_exponent(most);
-        const float up = exp2i(e);
+        const int e = query_exponent(most) - 7;            // the largest between 2^7 and 2^8
+        const float up = most > 3.402823466e38f ? __int_as_float(0x7FC00000) : exp2i(e);       // (an infinite element: all scores are NaN or infinite)
         row_scale = exp2i(-e) * a.scale;
         uint8_t* dst = smem + Y::kQ + (row >> 3) * Y::kGroup + (row & 7) * 16;
-#pragma unroll 4
-        for (int j = 0; j < D / 8; ++j) {
-          uint4 r = {0, 0, 0, 0};
-          if (mine) {
-            const uint4 raw = src[j];
-            const float2 f[4] = {Half<T>::wide(raw.x), Half<T>::wide(raw.y), Half<T>::wide(raw.z), Half<T>::wide(raw.w)};
-            r = {pack_half(f[0].x * up, f[0].y * up), pack_half(f[1].x * up, f[1].y * up), pack_half(f[2].x * up, f[2].y * up),
-                 pack_half(f[3].x * up, f[3].y * up)};
+#pragma unroll 1
+        for (int j = 0; j < D / 16; ++j) {                 // 16 dimensions: 16 bytes of each part
+          float f[16];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint4 raw = mine ? src[2 * j + x] : uint4{0, 0, 0, 0};
+            const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float2 v = Half<T>::wide(w4[y]);
+              f[8 * x + 2 * y] = v.x * up;
+              f[8 * x + 2 * y + 1] = v.y * up;
+            }
           }
-          *reinterpret_cast<uint4*>(dst + j * 128) = r;
+#pragma unroll
+          for (int part = 0; part < Y::kParts; ++part) {
+            uint32_t r[4];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const uint32_t two = to_e4m3(f[2 * x], f[2 * x + 1]);
+              const float2 held = Half<__half>::wide(from_e4m3(two));
+              f[2 * x] -= held.x;                          // what is left for the next part, exactly
+              f[2 * x + 1] -= held.y;
+              r[x >> 1] = x & 1 ? r[x >> 1] | two << 16 : two;
+            }
+            *reinterpret_cast<uint4*>(dst + part * Y::kPart + j * 128) = make_uint4(r[0], r[1], r[2], r[3]);
+          }
         }
         fence_async();
         fence_before();
         bar_arrive(q_full);
       }
       float m = kNone, l = 0.f;
-      for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1) {
-        ok = bar_wait(k_full, phase, fail) && bar_wait(s_full, phase, fail);
-        ok = __all_sync(kFullWarp, ok);
+      for (int u = w.u0; u < w.u1 && ok; ++u, ++n) {
+        ok = __all_sync(kFullWarp, reached(k_full, n) && reached(s_full, n));
         if (!ok) break;
         fence_after();
-        const int at = u * kUnit;
-        const unsigned real = s.real[phase];
-        const bool edge = at + kUnit > w.least || real != 0xFFu;
+        const int at = u * kUnit, turn = n & 1;
+        const unsigned real = s.real[turn];
+        const uint32_t scores = lanes + 64 * turn;
         if (32 * warp < rows) {
-          uint32_t raw[2][32];                             // 32 tokens (two groups of 16), and the next ones on their way
-          tmem_load(lanes, raw[0]);
+          uint32_t raw[2][32];
+          tmem_load(scores, raw[0]);
+          tmem_load(scores + 32, raw[1]);
           tmem_loaded(raw[0]);
+          tmem_loaded(raw[1]);
+          float v[kUnit], base = m == kNone ? 0.f : m;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float v[32], base = m == kNone ? 0.f : m, most[4];
+          for (int g = 0; g < kGroups; ++g) {
+            const float by = row_scale * s.ks[turn][g], add = s.lv[turn][g] - base;
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const float by = row_scale * s.ks[phase][2 * j + g], add = s.lv[phase][2 * j + g] - base;
+            for (int c = 16 * g; c < 16 * g + 16; c += 2) fma2(v[c], v[c + 1], raw[c >> 5][c & 31], raw[c >> 5][(c & 31) + 1], by, add);
+          }
+          if (at + kUnit > w.least || real != (1u << kGroups) - 1) {
 #pragma unroll
-              for (int c = 0; c < 16; ++c) v[16 * g + c] = fmaf(__uint_as_float(raw[j & 1][16 * g + c]), by, add);
-            }
-            if (j < 3) tmem_load(lanes + 32 * (j + 1), raw[(j + 1) & 1]);
-            if (edge) {
+            for (int c = 0; c < kUnit; ++c)
+              if (at + c >= row_end || !(real >> (c >> 4) & 1)) v[c] = kNone;
+          }
+          float sum[kGroups][2];
+          uint32_t p[kUnit / 2];
+          const auto exponentials = [&] {
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (at + 32 * j + c >= row_end || !(real >> (2 * j + (c >> 4)) & 1)) v[c] = kNone;
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              most[x] = fmaxf(v[8 * x], v[8 * x + 1]);
-#pragma unroll
-              for (int c = 2; c < 8; c += 2) most[x] = fmaxf(fmaxf(most[x], v[8 * x + c]), v[8 * x + c + 1]);
-            }
-            most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-            const bool grows = m == kNone ? most[0] > kNone : most[0] > 14.f;
-            if (__any_sync(kFullWarp, grows)) {            // a new reference, 2^6 above which the largest lies; what there is follows
-              const float now = grows ? base + most[0] - 6.f : m, f = grows && m != kNone ? exp2_fast(m - now) : 1.f, down = grows ? base - now : 0.f;
-#pragma unroll
-              for (int c = 0; c < 32; ++c) v[c] += down;
-              m = now;
-              l *= f;
-              __syncwarp();
-              if (j < 3) tmem_loaded(raw[(j + 1) & 1]);
-              follow(f, u > w.u0, j);
-            }
-            float sum[4];
-            uint32_t p[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
+            for (int c = 0; c < kUnit / 2; ++c) {
               const float x = exp2_fast(v[2 * c]), y = exp2_fast(v[2 * c + 1]);
-              sum[c >> 2] = (c & 3) ? sum[c >> 2] + (x + y) : x + y;
+              if (c & 7) add2(sum[c >> 3][0], sum[c >> 3][1], x, y);
+              else sum[c >> 3][0] = x, sum[c >> 3][1] = y;
               p[c] = pack_half(x, y);
             }
-            l = fmaf(sum[0] + sum[1], s.inv[phase][2 * j], fmaf(sum[2] + sum[3], s.inv[phase][2 * j + 1], l));
-            __syncwarp();
-            if (j < 3) tmem_loaded(raw[(j + 1) & 1]);                      // (P goes over columns that have been read)
-            tmem_store(lanes + 16 * j, p);
+          };
+          exponentials();
+          // whether P stays below 2^14: of its halves, whose overflow is infinite
+          uint32_t most[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) most[c] = max_half2(max_half2(p[c], p[c + 8]), max_half2(p[c + 16], p[c + 24]));
+#pragma unroll
+          for (int c = 4; c; c >>= 1)
+#pragma unroll
+            for (int x = 0; x < c; ++x) most[x] = max_half2(most[x], most[x + c]);
+          const float2 pair = Half<__half>::wide(most[0]);
+          const bool grows = m == kNone || fmaxf(pair.x, pair.y) > 16384.f;
+          if (__any_sync(kFullWarp, grows)) {              // a new reference, 2^6 above which the largest lies; what there is follows
+            float top = kNone;
+#pragma unroll
+            for (int c = 0; c < kUnit; ++c) top = fmaxf(top, v[c]);
+            const bool moves = grows && top > kNone;
+            const float now = moves ? base + top - 6.f : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
+#pragma unroll
+            for (int c = 0; c < kUnit; ++c) v[c] += down;
+            m = now;
+            l *= f;
+            if (u > w.u0) {
+              ok = __all_sync(kFullWarp, reached(pv_done, n - 1));   // (S of this unit came before the results of the last one)
+              fence_after();
+              if (ok) follow(f);
+            }
+            exponentials();
           }
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) l = fmaf(sum[g][0] + sum[g][1], s.inv[turn][g], l);
+          __syncwarp();
+          tmem_store(scores, reinterpret_cast<const uint32_t (&)[16]>(p[0]));
+          tmem_store(scores + 16, reinterpret_cast<const uint32_t (&)[16]>(p[16]));
           tmem_stored();
         }
         fence_before();
-        bar_arrive(p_full);
+        bar_arrive(p_full + 8 * turn);
       }
       if (!ok) break;
-      ok = __all_sync(kFullWarp, bar_wait(pv_done, phase ^ 1, fail));
+      ok = __all_sync(kFullWarp, reached(pv_done, n - 1));
       if (!ok) break;
       fence_after();
       // ---- the tile, or this run's part of it
@@ -453,19 +491,17 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
     }
   } else if (count > 0 && warp < 8) {
     // ================= cache -> fp16 core matrices
-    constexpr int kKeys = D / 16;                          // pieces of 16 bytes of keys of a thread
     const int t = tid - 128, cw = warp - 4;
-    const int tg = (lane & 7) + 8 * (cw & 1), dc = (lane >> 3) + 4 * (cw >> 1);      // values: group of 8 tokens, piece of D / 8 dimensions
+    const int tg = lane & 7, dc = (lane >> 3) + 4 * cw;    // values: group of 8 tokens, piece of D / 16 dimensions
     bool ok = true, bad = false;
-    uint4 kr[kKeys];
-    uint32_t vr[8][D / 32];
+    uint32_t vr[8][D / 64];
     Walk w(s, count);
     w.look(a);
     // three units are under way: one that is written, the next, whose rows are being fetched, and the one after it, whose pages are
     Walk f = w;
     int fu = w.u0;                                         // of the pages that are fetched
     struct Pages {
-      int k[2], v, scale, head, at;
+      int k, v, scale, head, at;
       bool all;                                            // every token of the unit lies in a page and before the end
     };
     const auto pages_of = [&](Pages& p) {
@@ -473,10 +509,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
       p.head = f.head;
       const int* table = a.tables + f.r * a.table_stride;
       const auto page = [&](int token) { return token < f.end ? table[token >> a.shift] : -1; };
-      p.k[0] = page(p.at + 32 * cw);
-      p.k[1] = page(p.at + 32 * cw + 16);
+      p.k = page(p.at + 16 * cw);
       p.v = page(p.at + 8 * tg);
-      p.scale = page(p.at + 16 * (t & 7));
+      p.scale = page(p.at + 16 * (t & (kGroups - 1)));
       p.all = p.at + kUnit <= f.end;
       if (++fu == f.u1) {
         f.next(a);
@@ -489,26 +524,28 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
     const int place_mask = (1 << a.shift) - 1;
     const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
     // (a page that is none is read as the first one and left aside later)
-    const auto keys_of = [&](const Pages& p) {
+    const auto keys_of = [&](const Pages& p, uint32_t n) { // straight to their core matrices
+      const int id = valid(p.k) ? p.k : 0;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int id = valid(p.k[b >> 1]) ? p.k[b >> 1] : 0, token = p.at + 32 * cw + 8 * b + (lane & 7);
+      for (int b = 0; b < 2; ++b) {
+        const int token = p.at + 16 * cw + 8 * b + (lane & 7);
         const uint8_t* src = a.k_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
+        const uint32_t dst = smem_u32(smem + Y::kK + (n & 1) * Y::kKeys + (2 * cw + b) * Y::kGroup + (lane & 7) * 16 + (lane >> 3) * 128);
 #pragma unroll
-        for (int x = 0; x < D / 64; ++x) kr[b * (D / 64) + x] = *reinterpret_cast<const uint4*>(src + 64 * x);
+        for (int x = 0; x < D / 64; ++x)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * 512), "l"(src + 64 * x) : "memory");
       }
     };
     const auto values_of = [&](const Pages& p) {
       const int id = valid(p.v) ? p.v : 0, token = p.at + 8 * tg;
-      const uint8_t* src = a.v_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + dc * (D / 8);
+      const uint8_t* src = a.v_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + dc * (D / 16);
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
         if constexpr (D == 128) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(src + x * D);
-          vr[x][0] = raw.x; vr[x][1] = raw.y; vr[x][2] = raw.z; vr[x][3] = raw.w;
-        } else {
           const uint2 raw = *reinterpret_cast<const uint2*>(src + x * D);
           vr[x][0] = raw.x; vr[x][1] = raw.y;
+        } else {
+          vr[x][0] = *reinterpret_cast<const uint32_t*>(src + x * D);
         }
       }
     };
@@ -520,89 +557,75 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
     };
     Pages now, next, later;                                // of the unit that is written, of the next, of the one after it
     pages_of(now);
-    keys_of(now);
+    keys_of(now, 0);
     values_of(now);
     scales_of(now);
     next = now;
     if (f.left > 0) pages_of(next);
-    long long owed = count - 1;                            // units whose rows have not been fetched
-    // the products, issued by the first of these warps, which wait for P and the keys anyway
-    const uint32_t idesc_s = 1u << 4 | (128u >> 3) << 17 | (128u >> 4) << 24, idesc_o = 1u << 4 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
+    long long owed = count - 1;                            // units that come after this one
+    // the products, issued by the first of these warps
+    const uint32_t idesc_s = 1u << 4 | (uint32_t)(kUnit >> 3) << 17 | (128u >> 4) << 24, idesc_o = 1u << 4 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
     const uint64_t dq = descriptor(smem_u32(smem + Y::kQ), 128, Y::kGroup), dk = descriptor(smem_u32(smem + Y::kK), 128, Y::kGroup),
                    dv = descriptor(smem_u32(smem + Y::kV), Y::kTokens, 128);
     uint32_t fresh = 0, q_phase = 0;                       // fresh: 0 where the unit before is the first of its tile
-    const auto results = [&](uint32_t of) {                // O of the unit of that phase, whose P is there
-      const bool ok = __all_sync(kFullWarp, bar_wait(v_full, of, fail));
-      if (!ok) return false;
+    const auto scores = [&](uint32_t n, bool first) {
+      if (!__all_sync(kFullWarp, reached(k_full, n) && (!first || bar_wait(q_full, q_phase, fail)))) return false;
       fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mma_ts(tmem + 128, tmem + 8 * k, dv + (uint64_t)(k * (2 * Y::kTokens >> 4)), idesc_o, k != 0 ? 1u : fresh);
-        commit(pv_done);
+        for (int part = 0; part < Y::kParts; ++part)
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k)
+            mma_ss(tmem + 64 * (n & 1), dq + part * (Y::kPart >> 4) + 16 * k, dk + (n & 1) * (Y::kKeys >> 4) + 16 * k, idesc_s, (part | k) != 0);
+        commit(s_full + 8 * (n & 1));
+      }
+      __syncwarp();
+      if (first) q_phase ^= 1;
+      return true;
+    };
+    const auto results = [&](uint32_t n) {                 // (P of the unit is there)
+      if (!__all_sync(kFullWarp, reached(v_full, n))) return false;
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kUnit / 16; ++k)
+          mma_ts(tmem + 128, tmem + 64 * (n & 1) + 8 * k, dv + (n & 1) * (Y::kValues >> 4) + (uint64_t)(k * (2 * Y::kTokens >> 4)), idesc_o, k != 0 ? 1u : fresh);
+        commit(pv_done + 8 * (n & 1));
       }
       __syncwarp();
       return true;
     };
-    bool first = true;
     for (; w.left > 0 && ok;) {
-      for (int u = w.u0; u < w.u1 && ok; ++u, phase ^= 1, first = false) {
-        // ---- keys
-        if (!first) ok = bar_wait(s_full, phase ^ 1, fail);
-        if (!(ok = __all_sync(kFullWarp, ok))) break;
-        later = next;
-        if (f.left > 0) pages_of(later);
+      for (int u = w.u0; u < w.u1 && ok; ++u, ++n) {
+        const bool first = u == w.u0;                      // of its tile: its queries come after the results of the last tile
+        const int turn = n & 1;
+        // ---- keys, which are on their way, and scales
         if (cw == 0) {
-          const unsigned mask = __ballot_sync(kFullWarp, t < 8 && valid(now.scale));
+          const unsigned mask = __ballot_sync(kFullWarp, t < kGroups && valid(now.scale));
           bad |= now.scale != -1 && !valid(now.scale);     // (-1: behind the last token)
-          if (t < 8) {
-            s.ks[phase][t] = ks;
-            s.lv[phase][t] = __log2f(vs);                  // of a power of two: exact
-            s.inv[phase][t] = __fdividef(1.f, vs);
+          if (t < kGroups) {
+            s.ks[turn][t] = ks;
+            s.lv[turn][t] = __log2f(vs);                   // of a power of two: exact
+            s.inv[turn][t] = __fdividef(1.f, vs);
           }
           // (a group behind the last token has no page either: the rows' ends mask it)
-          if (t == 0) s.real[phase] = mask;
+          if (t == 0) s.real[turn] = mask;
         }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int x = 0; x < D / 64; ++x) {
-            const uint4 raw = kr[b * (D / 64) + x];
-            uint8_t* dst = smem + Y::kK + (4 * cw + b) * Y::kGroup + (lane & 7) * 16 + (2 * ((lane >> 3) + 4 * x)) * 128;
-            *reinterpret_cast<uint4*>(dst) = {from_e4m3(raw.x & 0xFFFFu), from_e4m3(raw.x >> 16), from_e4m3(raw.y & 0xFFFFu), from_e4m3(raw.y >> 16)};
-            *reinterpret_cast<uint4*>(dst + 128) = {from_e4m3(raw.z & 0xFFFFu), from_e4m3(raw.z >> 16), from_e4m3(raw.w & 0xFFFFu), from_e4m3(raw.w >> 16)};
-          }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         fence_async();
-        // (the product of these keys has to wait for P anyway; until then no one is a phase behind on this barrier)
-        if (owed > 0) {
-          keys_of(next);
-          scales_of(next);
-        }
-        if (!first) ok = bar_wait(p_full, phase ^ 1, fail);
-        if (!(ok = __all_sync(kFullWarp, ok))) break;
-        if (cw == 0 && !first && !(ok = results(phase ^ 1))) break;
-        bar_arrive(k_full);
-        if (cw == 0) {
-          ok = __all_sync(kFullWarp, bar_wait(k_full, phase, fail) && (u != w.u0 || bar_wait(q_full, q_phase, fail)));
-          if (!ok) break;
-          fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) mma_ss(tmem, dq + 16 * k, dk + 16 * k, idesc_s, k != 0);
-            commit(s_full);
-          }
-          __syncwarp();
-          if (u == w.u0) q_phase ^= 1;
-          fresh = u != w.u0;
-        }
-        // ---- values
-        if (!first) ok = bar_wait(pv_done, phase ^ 1, fail);
-        if (!(ok = __all_sync(kFullWarp, ok))) break;
+        bar_arrive(k_full + 8 * turn);
+        if (cw == 0 && !first && !(ok = scores(n, false))) break;
+        later = next;
+        if (f.left > 0) pages_of(later);
+        // ---- values, once the results of the unit before the last are done
+        if (n >= 2) ok = __all_sync(kFullWarp, reached(pv_done, n - 2));
+        if (!ok) break;
         const int vtoken = u * kUnit + 8 * tg;
         if (!now.all || !valid(now.v)) {                   // behind the request's tokens lies what an earlier one left
 #pragma unroll
           for (int x = 0; x < 8; ++x)
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j)
+            for (int j = 0; j < D / 64; ++j)
               if (vtoken + x >= w.end || !valid(now.v)) vr[x][j] = 0;
         }
         if (vtoken + 8 > w.least) {                        // tokens that not all rows see: a NaN there is not for the others
@@ -610,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
 #pragma unroll
           for (int x = 0; x < 8; ++x)
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
+            for (int j = 0; j < D / 64; ++j) {
               const uint32_t b = vtoken + x >= w.least ? nan_bytes(vr[x][j]) : 0;
               vr[x][j] &= ~b;
               any |= b;
@@ -618,33 +641,48 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
           if (any) s.nan = 1;
         }
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {                 // four dimensions of eight tokens
+        for (int j = 0; j < D / 64; ++j) {                 // four dimensions of eight tokens
           uint32_t lo[4], hi[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             lo[x] = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], 0x5140);
             hi[x] = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], 0x7362);
           }
-          const int d = dc * (D / 8) + 4 * j;
-          uint8_t* dst = smem + Y::kV + tg * Y::kTokens + (d >> 3) * 128 + (d & 7) * 16;
+          const int d = dc * (D / 16) + 4 * j;
+          uint8_t* dst = smem + Y::kV + turn * Y::kValues + tg * Y::kTokens + (d >> 3) * 128 + (d & 7) * 16;
           *reinterpret_cast<uint4*>(dst) = {from_e4m3(lo[0] & 0xFFFFu), from_e4m3(lo[1] & 0xFFFFu), from_e4m3(lo[2] & 0xFFFFu), from_e4m3(lo[3] & 0xFFFFu)};
           *reinterpret_cast<uint4*>(dst + 16) = {from_e4m3(lo[0] >> 16), from_e4m3(lo[1] >> 16), from_e4m3(lo[2] >> 16), from_e4m3(lo[3] >> 16)};
           *reinterpret_cast<uint4*>(dst + 32) = {from_e4m3(hi[0] & 0xFFFFu), from_e4m3(hi[1] & 0xFFFFu), from_e4m3(hi[2] & 0xFFFFu), from_e4m3(hi[3] & 0xFFFFu)};
           *reinterpret_cast<uint4*>(dst + 48) = {from_e4m3(hi[0] >> 16), from_e4m3(hi[1] >> 16), from_e4m3(hi[2] >> 16), from_e4m3(hi[3] >> 16)};
         }
         fence_async();
-        bar_arrive(v_full);
-        if (owed > 0) values_of(next);
+        bar_arrive(v_full + 8 * turn);
+        // ---- the next unit's rows; its keys go where those of the last unit were
+        if (owed > 0) {
+          values_of(next);
+          scales_of(next);
+          if (n >= 1) ok = __all_sync(kFullWarp, reached(s_full, n - 1));
+          if (!ok) break;
+          keys_of(next, n + 1);
+        }
         --owed;
         now = next;
         next = later;
+        // ---- results of the last unit.  (All of these warps wait for its P: none is then two phases ahead of a thread that still waits for keys.)
+        if (n >= 1) {
+          ok = __all_sync(kFullWarp, reached(p_full, n - 1));
+          if (!ok || (cw == 0 && !(ok = results(n - 1)))) break;
+        }
+        if (cw == 0 && first && !(ok = scores(n, true))) break;
+        fresh = !first;
       }
       if (!ok) break;
       w.next(a);
       if (w.left > 0) w.look(a);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (cw == 0) {
-      if (ok) ok = __all_sync(kFullWarp, bar_wait(p_full, phase ^ 1, fail)) && results(phase ^ 1);
+      if (ok) ok = __all_sync(kFullWarp, reached(p_full, n - 1)) && results(n - 1);
       if (!ok) {                                           // products in flight end before the tensor memory goes back
         if (elect_one()) commit(smem_u32(&s.drained));
         __syncwarp();
@@ -709,12 +747,12 @@ int run(const AttentionArgs& a, cudaStream_t st) {
   static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
   int dev = 0, e = (int)cudaGetDevice(&dev);
   if (!e && (dev < 0 || dev >= 64 || !allowed[dev])) {
-    e = (int)cudaFuncSetAttribute(paged_attention_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
+    e = (int)cudaFuncSetAttribute(paged_attention_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (Layout<T, D>::kBytes));
     if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
   }
   if (e) return paged_fail(e);
   const dim3 grid(device_sms() * kBlocksPerSm);
-  const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, Layout<D>::kBytes, st, a);
+  const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, (Layout<T, D>::kBytes), st, a);
   return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, grid, dim3(512), 1, 0, st, a);
 }
 

@@ -36,6 +36,7 @@ int paged_launch(Kern kern, dim3 grid, dim3 block, int cluster, size_t smem, cud
 
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
+  static constexpr int kBits = 8;                          // significant
   static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
   static __device__ __forceinline__ uint32_t narrow(float x, float y) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
@@ -43,6 +44,7 @@ template <> struct Half<__nv_bfloat16> {
   }
 };
 template <> struct Half<__half> {
+  static constexpr int kBits = 11;
   static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   static __device__ __forceinline__ uint32_t narrow(float x, float y) {
     const __half2 r = __floats2half2_rn(x, y);
