@@ -1,47 +1,54 @@
 // Attention over the paged 8-bit cache for many rows a request (prompts, shared key/value heads): tcgen05.mma with accumulators in tensor
 // memory.
 //
-// A tile is up to 128 rows: the query heads of one key/value head for as many whole tokens as fit (row = token * group + head).  Per unit of 64
-// cached tokens: S = Q K^T (128 x 64), P = 2^(S - m) in fp16, O += P V.  S, P and O are in tensor memory (P over S, two of them in turns), Q, K and V
-// in shared memory as core matrices.
+// An item is up to 256 rows, two tiles of 128: the query heads of one key/value head for as many whole tokens as fit (row = token * group +
+// head).  Per unit of 64 cached tokens and tile: S = Q K^T (128 x 64), P = 2^(S - m) in fp16, O += P V.  S, P and O are in tensor memory (P over S, two
+// of them in turns), Q, K and V in shared memory.  An item of at most 128 rows is a twin: its units go to the two tiles in
+// turns, and their results are joined at the end.
 //  * Keys are multiplied as they are, e4m3, and go from memory straight to their core matrices; a row of Q is a sum of e4m3 parts of four significant
 //    bits each under one power of two (two parts for bf16, three for fp16: exact down to 2^-18 of the row's largest element), which costs what
 //    one product of 16-bit operands would, without its conversions.
-//  * Values become fp16, exactly, on their way (P would need three e4m3 parts, at four conversions an element), transposed by byte permutes
-//    of eight rows in registers: their operand wants eight tokens of a dimension side by side.
-// Two roles per thread block, two thread blocks per SM:
-//   warps 0-3  a thread per row (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.  S of the next unit
-//              is there when one is done.
-//   warps 4-7  keys and values of the next unit; the first of them issues the products, Q K^T of the next unit before P V of this one.
-// What bounds it: per 128 rows and 64 tokens 512 cycles of tensor pipe, 512 of exponentials (16 a cycle and SM) and about 400 of issue on each
-// scheduler, which the two thread blocks overlap.
+//  * Values become fp16, exactly, on their way (P would need three e4m3 parts, at four conversions an element).
+//  * All operands lie in the swizzled layouts (rows of 128 bytes; values with the dimensions inside): from core matrices without a swizzle the
+//    products were fetched at a quarter of the rate, 288 us for a prompt of 2048 tokens behind 2048.
+// Roles of the one thread block of an SM:
+//   warps 0-7    a thread per row and tile (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.
+//   warps 8-11   values of the units, two of them on their way in registers, into a ring of four
+//   warps 12-13  keys (copies that pass no register) and scales, into a ring of four
+//   warp 14      the products: Q K^T up to two units (a twin: four) before the P V that follow
+// What bounds it: per 256 rows and 64 tokens 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM).
 // The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
 // the sum; see paged_kernels.cu, whose cut of the work into even runs over the thread blocks, parts and join this kernel shares, with
-// runs of units of (request, tile, head), each as many as its last token sees.
+// runs of units of (request, item, head), each as many as its last token sees.
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace {
 
 using namespace htr;
 
-constexpr int kThreads = 256, kRows = 128, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024, kBlocksPerSm = 2;
-constexpr int kTmemColumns = 256;                          // S (P over it) at 0 and 64, O at 128
+constexpr int kThreads = 480, kTile = 128, kRows = 256, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024;
+constexpr int kTmemColumns = 512;                          // of a tile: S (P over it) at 0 and 64, O at 128
+constexpr int kRing = 4, kScales = 8;                      // units of keys and of values in shared memory; of their scales, read by all rows
 constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
 
 template <typename T, int D>
-struct Layout {                                            // bytes of the operands: core matrices of 8 rows x 16 bytes
+struct Layout {                                            // bytes of the operands
   // Q as a sum of e4m3 of four significant bits each: two for the 8 bits of bf16, three for the 11 of fp16
   static constexpr int kParts = Half<T>::kBits > 8 ? 3 : 2;
-  static constexpr int kGroup = 8 * D;                     // Q, K: between groups of 8 rows; 128 between neighbours in K
-  static constexpr int kTokens = 16 * D + 16;              // V: between groups of 8 tokens (16 more: stores of 8 groups meet 8 bank groups)
-  static constexpr int kQ = 0, kPart = 16 * kGroup, kK = kQ + kParts * kPart, kKeys = 8 * kGroup, kV = kK + 2 * kKeys,
-                       kValues = 8 * kTokens, kBytes = kV + 2 * kValues;
+  static constexpr int kQ = 0, kPart = kTile * D, kQTile = kParts * kPart, kK = kQ + 2 * kQTile, kKeys = kUnit * D, kV = kK + kRing * kKeys,
+                       kValues = kUnit * 2 * D, kBytes = kV + kRing * kValues + 1024;      // (1024: to align the first)
+  // 16-byte piece of a row of D bytes, swizzled (128 or 64 bytes)
+  static __device__ __forceinline__ int piece(int row, int chunk) { return row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ (row >> 1 & 3)) << 4); }
+  // 8 dimensions of a token's values in fp16: rows of 64 dimensions
+  static __device__ __forceinline__ int value(int token, int chunk) { return (chunk >> 3) * (kUnit * 128) + token * 128 + (((chunk & 7) ^ (token & 7)) << 4); }
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// start, distance of core matrices adjacent in K, distance of groups of 8 rows, in 16 bytes; version 1, no swizzle
-__device__ __forceinline__ uint64_t descriptor(uint32_t at, int next_k, int next_rows) {
-  return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)(next_k >> 4) << 16 | (uint64_t)(next_rows >> 4) << 32 | 1ull << 46;
+// start; distances of 128-byte columns (where rows are longer) and of groups of 8 rows, in 16 bytes; version 1; swizzle of 128 bytes (2) or 64 (4)
+__device__ __forceinline__ uint64_t descriptor(uint32_t at, int next_column, int next_rows, uint64_t swizzle) {
+  return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)(next_column >> 4) << 16 | (uint64_t)(next_rows >> 4) << 32 | 1ull << 46 | swizzle << 61;
 }
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -147,27 +154,32 @@ struct Request {
 };
 
 struct Shared {
-  unsigned long long k_full[2], s_full[2], v_full[2], p_full[2], pv_done[2], q_full, drained;    // of the units in turns
+  unsigned long long k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], scales[kScales];      // of the units in turns
+  unsigned long long s_full[4], p_full[4], pv_done[4];     // of a tile's units in turns: 2 * tile + turn
+  unsigned long long q_full, twin_full, twin_done, drained;
   long long sums[kMaxRequests];                            // units of each request
-  long long total, skip;
+  long long total;
   int r, tile, head, unit;                                 // where this thread block's run begins
   uint32_t tmem;
   int fail, nan;
-  float ks[2][kGroups], lv[2][kGroups], inv[2][kGroups];                     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
-  unsigned real[2];                                        // groups that have a page
+  float ks[kScales][kGroups], lv[kScales][kGroups], inv[kScales][kGroups];     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
+  unsigned char real[kScales][kGroups];                    // groups that have a page
+  float twin_m[kTile], twin_l[kTile];
 };
 
 // the run of a thread block, piece by piece: every role walks it for itself
 struct Walk {
   int r, tile, head, u0, u1, units;
   long long left;
-  int start, n, seen, per, tiles, row_tokens, least, end;
+  int start, n, seen, per, tiles, rows, least, end;
+  bool twin;
   __device__ __forceinline__ Walk(const Shared& s, long long count) : r(s.r), tile(s.tile), head(s.head), u0(s.unit), left(count) {}
   __device__ __forceinline__ void look(const AttentionArgs& a) {
     Request x(a, r);
     while (x.tiles == 0) x = Request(a, ++r);              // (there is one: `left` counts its units)
     start = x.start; n = x.n; seen = x.seen; per = x.per; tiles = x.tiles;
-    row_tokens = x.tokens(a, tile);
+    rows = x.tokens(a, tile) * a.group;
+    twin = rows <= kTile;
     least = max(seen - n + tile * per + 1, 0);
     end = x.end(a, tile);
     units = x.units(a, tile);
@@ -188,9 +200,10 @@ template <int D>
 constexpr int kPartFloats = kRows * (D + 2);
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const AttentionArgs a) {
   using Y = Layout<T, D>;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t raw_smem[];
+  uint8_t* smem = raw_smem + (-smem_u32(raw_smem) & 1023);
   __shared__ Shared s;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -206,14 +219,21 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
   }
   if (tid == 0) {
     s.fail = s.nan = 0;
-    for (int i = 0; i < 2; ++i) {
-      bar_init(smem_u32(&s.k_full[i]), 128);
-      bar_init(smem_u32(&s.s_full[i]), 1);
+    for (int i = 0; i < kRing; ++i) {
+      bar_init(smem_u32(&s.k_full[i]), 64);
+      bar_init(smem_u32(&s.k_free[i]), 1);
       bar_init(smem_u32(&s.v_full[i]), 128);
+      bar_init(smem_u32(&s.v_free[i]), 1);
+    }
+    for (int i = 0; i < kScales; ++i) bar_init(smem_u32(&s.scales[i]), 64);
+    for (int i = 0; i < 4; ++i) {
+      bar_init(smem_u32(&s.s_full[i]), 1);
       bar_init(smem_u32(&s.p_full[i]), 128);
       bar_init(smem_u32(&s.pv_done[i]), 1);
     }
-    bar_init(smem_u32(&s.q_full), 128);
+    bar_init(smem_u32(&s.q_full), 256);
+    bar_init(smem_u32(&s.twin_full), 128);
+    bar_init(smem_u32(&s.twin_done), 128);
     bar_init(smem_u32(&s.drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     a.cuts[blockIdx.x] = {0, 0, 0, 0};
@@ -286,35 +306,34 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
   from = blockIdx.x * share;
   const long long count = min(share, total - from);
   const uint32_t tmem = s.tmem;
-  const uint32_t k_full = smem_u32(s.k_full), s_full = smem_u32(s.s_full), v_full = smem_u32(s.v_full), p_full = smem_u32(s.p_full),
-                 pv_done = smem_u32(s.pv_done), q_full = smem_u32(&s.q_full);
-  // barrier and phase of unit n of this thread block
-  const auto reached = [&](uint32_t bars, uint32_t n) { return bar_wait(bars + 8 * (n & 1), n >> 1 & 1, fail); };
-  uint32_t n = 0;                                          // units so far
-  if (count > 0 && warp < 4) {
-    // ================= softmax: a thread per row
-    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
-    const int row = tid;
+  // unit n of the thread block in a ring of bars, and unit c of a tile in its two
+  const auto ring = [&](unsigned long long* bars, uint32_t size, uint32_t n) { return bar_wait(smem_u32(bars + n % size), n / size & 1, fail); };
+  const auto turn = [&](unsigned long long* bars, int x, uint32_t c) { return bar_wait(smem_u32(bars + 2 * x + (c & 1)), c >> 1 & 1, fail); };
+  if (count > 0 && warp < 8) {
+    // ================= softmax: a thread per row of tile x
+    const int x = warp >> 2, row = tid & (kTile - 1);
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), mine_at = lanes + 256 * x;
     bool ok = true;
     const auto follow = [&](float f) {                     // results relative to a new reference
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
-        tmem_load16(lanes + 128 + c, o);
+        tmem_load16(mine_at + 128 + c, o);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-        tmem_store(lanes + 128 + c, o);
+        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+        tmem_store(mine_at + 128 + c, o);
       }
       tmem_stored();
     };
     Walk w(s, count);
+    uint32_t n = 0, done = 0, twins = 0;                   // units of the thread block, of this tile; twins so far
     for (int segment = 0; w.left > 0 && ok; ++segment, w.next(a)) {
       w.look(a);
-      const int i = row / a.group, head = w.head * a.group + row - i * a.group, rows = w.row_tokens * a.group;
-      const bool mine = row < rows;
+      const int place_row = w.twin ? row : x * kTile + row, i = place_row / a.group, head = w.head * a.group + place_row - i * a.group;
+      const bool mine = place_row < w.rows, warp_has_rows = (w.twin ? 0 : x * kTile) + 32 * (warp & 3) < w.rows;
       const size_t place = ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
       const int row_end = mine ? max(w.seen - w.n + w.tile * w.per + i + 1, 0) : 0;
-      // queries: e4m3 parts under a power of two per row
+      // queries: e4m3 parts under a power of two per row (of a twin: both tiles hold them)
       float row_scale;
       {
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + place);
@@ -325,53 +344,55 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
             const uint4 raw = src[j];
             const float2 f[4] = {Half<T>::wide(raw.x), Half<T>::wide(raw.y), Half<T>::wide(raw.z), Half<T>::wide(raw.w)};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) most = fmaxf(most, fmaxf(fabsf(f[x].x), fabsf(f[x].y)));
+            for (int y = 0; y < 4; ++y) most = fmaxf(most, fmaxf(fabsf(f[y].x), fabsf(f[y].y)));
           }
         const int e = query_exponent(most) - 7;            // the largest between 2^7 and 2^8
         const float up = most > 3.402823466e38f ? __int_as_float(0x7FC00000) : exp2i(e);       // (an infinite element: all scores are NaN or infinite)
         row_scale = exp2i(-e) * a.scale;
-        uint8_t* dst = smem + Y::kQ + (row >> 3) * Y::kGroup + (row & 7) * 16;
+        uint8_t* dst = smem + Y::kQ + x * Y::kQTile;
 #pragma unroll 1
         for (int j = 0; j < D / 16; ++j) {                 // 16 dimensions: 16 bytes of each part
           float f[16];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint4 raw = mine ? src[2 * j + x] : uint4{0, 0, 0, 0};
+          for (int y = 0; y < 2; ++y) {
+            const uint4 raw = mine ? src[2 * j + y] : uint4{0, 0, 0, 0};
             const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const float2 v = Half<T>::wide(w4[y]);
-              f[8 * x + 2 * y] = v.x * up;
-              f[8 * x + 2 * y + 1] = v.y * up;
+            for (int z = 0; z < 4; ++z) {
+              const float2 v = Half<T>::wide(w4[z]);
+              f[8 * y + 2 * z] = v.x * up;
+              f[8 * y + 2 * z + 1] = v.y * up;
             }
           }
 #pragma unroll
           for (int part = 0; part < Y::kParts; ++part) {
             uint32_t r[4];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const uint32_t two = to_e4m3(f[2 * x], f[2 * x + 1]);
+            for (int z = 0; z < 8; ++z) {
+              const uint32_t two = to_e4m3(f[2 * z], f[2 * z + 1]);
               const float2 held = Half<__half>::wide(from_e4m3(two));
-              f[2 * x] -= held.x;                          // what is left for the next part, exactly
-              f[2 * x + 1] -= held.y;
-              r[x >> 1] = x & 1 ? r[x >> 1] | two << 16 : two;
+              f[2 * z] -= held.x;                          // what is left for the next part, exactly
+              f[2 * z + 1] -= held.y;
+              r[z >> 1] = z & 1 ? r[z >> 1] | two << 16 : two;
             }
-            *reinterpret_cast<uint4*>(dst + part * Y::kPart + j * 128) = make_uint4(r[0], r[1], r[2], r[3]);
+            *reinterpret_cast<uint4*>(dst + part * Y::kPart + Y::piece(row, j)) = make_uint4(r[0], r[1], r[2], r[3]);
           }
         }
         fence_async();
         fence_before();
-        bar_arrive(q_full);
+        bar_arrive(smem_u32(&s.q_full));
       }
       float m = kNone, l = 0.f;
+      bool results = false;                                // of an earlier unit of this tile
       for (int u = w.u0; u < w.u1 && ok; ++u, ++n) {
-        ok = __all_sync(kFullWarp, reached(k_full, n) && reached(s_full, n));
+        if (w.twin && ((u - w.u0) & 1) != x) continue;
+        ok = __all_sync(kFullWarp, ring(s.scales, kScales, n) && turn(s.s_full, x, done));
         if (!ok) break;
         fence_after();
-        const int at = u * kUnit, turn = n & 1;
-        const unsigned real = s.real[turn];
-        const uint32_t scores = lanes + 64 * turn;
-        if (32 * warp < rows) {
+        const int at = u * kUnit, slot = n % kScales;
+        const unsigned real = *reinterpret_cast<const unsigned*>(s.real[slot]);
+        const uint32_t scores = mine_at + 64 * (done & 1);
+        if (warp_has_rows) {
           uint32_t raw[2][32];
           tmem_load(scores, raw[0]);
           tmem_load(scores + 32, raw[1]);
@@ -380,36 +401,36 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
           float v[kUnit], base = m == kNone ? 0.f : m;
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) {
-            const float by = row_scale * s.ks[turn][g], add = s.lv[turn][g] - base;
+            const float by = row_scale * s.ks[slot][g], add = s.lv[slot][g] - base;
 #pragma unroll
             for (int c = 16 * g; c < 16 * g + 16; c += 2) fma2(v[c], v[c + 1], raw[c >> 5][c & 31], raw[c >> 5][(c & 31) + 1], by, add);
           }
-          if (at + kUnit > w.least || real != (1u << kGroups) - 1) {
+          if (at + kUnit > w.least || real != 0x01010101u) {
 #pragma unroll
             for (int c = 0; c < kUnit; ++c)
-              if (at + c >= row_end || !(real >> (c >> 4) & 1)) v[c] = kNone;
+              if (at + c >= row_end || !(real >> (8 * (c >> 4)) & 1)) v[c] = kNone;
           }
           float sum[kGroups][2];
           uint32_t p[kUnit / 2];
           const auto exponentials = [&] {
 #pragma unroll
             for (int c = 0; c < kUnit / 2; ++c) {
-              const float x = exp2_fast(v[2 * c]), y = exp2_fast(v[2 * c + 1]);
-              if (c & 7) add2(sum[c >> 3][0], sum[c >> 3][1], x, y);
-              else sum[c >> 3][0] = x, sum[c >> 3][1] = y;
-              p[c] = pack_half(x, y);
+              const float y = exp2_fast(v[2 * c]), z = exp2_fast(v[2 * c + 1]);
+              if (c & 7) add2(sum[c >> 3][0], sum[c >> 3][1], y, z);
+              else sum[c >> 3][0] = y, sum[c >> 3][1] = z;
+              p[c] = pack_half(y, z);
             }
           };
           exponentials();
           // whether P stays below 2^14: of its halves, whose overflow is infinite
-          uint32_t most[8];
+          uint32_t big[8];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) most[c] = max_half2(max_half2(p[c], p[c + 8]), max_half2(p[c + 16], p[c + 24]));
+          for (int c = 0; c < 8; ++c) big[c] = max_half2(max_half2(p[c], p[c + 8]), max_half2(p[c + 16], p[c + 24]));
 #pragma unroll
           for (int c = 4; c; c >>= 1)
 #pragma unroll
-            for (int x = 0; x < c; ++x) most[x] = max_half2(most[x], most[x + c]);
-          const float2 pair = Half<__half>::wide(most[0]);
+            for (int y = 0; y < c; ++y) big[y] = max_half2(big[y], big[y + c]);
+          const float2 pair = Half<__half>::wide(big[0]);
           const bool grows = m == kNone || fmaxf(pair.x, pair.y) > 16384.f;
           if (__any_sync(kFullWarp, grows)) {              // a new reference, 2^6 above which the largest lies; what there is follows
             float top = kNone;
@@ -421,276 +442,332 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_attention_tc_ker
             for (int c = 0; c < kUnit; ++c) v[c] += down;
             m = now;
             l *= f;
-            if (u > w.u0) {
-              ok = __all_sync(kFullWarp, reached(pv_done, n - 1));   // (S of this unit came before the results of the last one)
+            if (results) {
+              ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));        // (S of this unit came before the results of the last one)
               fence_after();
               if (ok) follow(f);
             }
             exponentials();
           }
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) l = fmaf(sum[g][0] + sum[g][1], s.inv[turn][g], l);
+          for (int g = 0; g < kGroups; ++g) l = fmaf(sum[g][0] + sum[g][1], s.inv[slot][g], l);
           __syncwarp();
           tmem_store(scores, reinterpret_cast<const uint32_t (&)[16]>(p[0]));
           tmem_store(scores + 16, reinterpret_cast<const uint32_t (&)[16]>(p[16]));
           tmem_stored();
         }
         fence_before();
-        bar_arrive(p_full + 8 * turn);
+        bar_arrive(smem_u32(&s.p_full[2 * x + (done & 1)]));
+        results = true;
+        ++done;
       }
       if (!ok) break;
-      ok = __all_sync(kFullWarp, reached(pv_done, n - 1));
+      if (results) ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));
       if (!ok) break;
       fence_after();
-      // ---- the tile, or this run's part of it
+      // ---- a twin's results are joined by the threads of the first tile, which can read both
+      float here = 1.f, there = 0.f;                       // factors of this tile's results and of the other's
+      bool other = false;
+      if (w.twin) {
+        if (x == 1) {
+          s.twin_m[row] = m;
+          s.twin_l[row] = l;
+          fence_before();
+          bar_arrive(smem_u32(&s.twin_full));
+          ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s.twin_done), twins & 1, fail));
+          ++twins;
+          fence_after();
+          continue;
+        }
+        ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s.twin_full), twins & 1, fail));
+        ++twins;
+        if (!ok) break;
+        fence_after();
+        const float tm = s.twin_m[row], tl = s.twin_l[row], now = fmaxf(m, tm);
+        other = w.u1 - w.u0 > 1;
+        if (now != kNone) {
+          here = exp2_fast(m - now);
+          there = exp2_fast(tm - now);
+        }
+        l = l * here + tl * there;
+        m = now;
+      }
+      // ---- the item, or this run's part of it
       const bool whole = w.u0 == 0 && w.u1 == w.units;
       float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPartFloats<D>;
-      const float by = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;     // a row that sees nothing: zeros
-      const bool empty = l == 0.f;
+      const bool empty = l == 0.f;                         // a row that sees nothing: zeros
+      const float by = whole && !empty ? 1.f / l : 1.f;
       const bool nan = *(volatile int*)&s.nan != 0;
-      if (32 * warp < rows) {
+      if (warp_has_rows) {
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
           uint32_t o[16];
           __syncwarp();
-          tmem_load16(lanes + 128 + c, o);
-          if (mine) {
+          tmem_load16(mine_at + 128 + c, o);
           float f[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) f[x] = empty ? 0.f : __uint_as_float(o[x]) * by;
-          if (nan)                                         // values that are NaN were left out of the last units: given to the rows that see them
-            for (int token = max(w.least, w.u0 * kUnit); token < min(row_end, w.u1 * kUnit); ++token) {
-              const int id = a.tables[w.r * a.table_stride + (token >> a.shift)];
-              if (id < 0 || id >= a.pages) continue;
-              const uint8_t* v = a.v_cache + ((((size_t)id * a.kv_heads + w.head) << a.shift) + (token & ((1 << a.shift) - 1))) * D + c;
+          for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : __uint_as_float(o[y]) * here * by;
+          if (other) {
+            __syncwarp();
+            tmem_load16(mine_at + 256 + 128 + c, o);
 #pragma unroll
-              for (int x = 0; x < 16; ++x)
-                if ((v[x] & 0x7F) == 0x7F) f[x] = __int_as_float(0x7FC00000);
-            }
-          if (whole) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + place + c);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              dst[x] = {Half<T>::narrow(f[8 * x], f[8 * x + 1]), Half<T>::narrow(f[8 * x + 2], f[8 * x + 3]),
-                        Half<T>::narrow(f[8 * x + 4], f[8 * x + 5]), Half<T>::narrow(f[8 * x + 6], f[8 * x + 7])};
-          } else {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              *reinterpret_cast<float4*>(part + ((c / 4 + x) * kRows + row) * 4) = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
+            for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : fmaf(__uint_as_float(o[y]) * there, by, f[y]);
           }
+          if (mine) {
+            if (nan)                                       // values that are NaN were left out of the last units: given to the rows that see them
+              for (int token = max(w.least, w.u0 * kUnit); token < min(row_end, w.u1 * kUnit); ++token) {
+                const int id = a.tables[w.r * a.table_stride + (token >> a.shift)];
+                if (id < 0 || id >= a.pages) continue;
+                const uint8_t* v = a.v_cache + ((((size_t)id * a.kv_heads + w.head) << a.shift) + (token & ((1 << a.shift) - 1))) * D + c;
+#pragma unroll
+                for (int y = 0; y < 16; ++y)
+                  if ((v[y] & 0x7F) == 0x7F) f[y] = __int_as_float(0x7FC00000);
+              }
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + place + c);
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                dst[y] = {Half<T>::narrow(f[8 * y], f[8 * y + 1]), Half<T>::narrow(f[8 * y + 2], f[8 * y + 3]),
+                          Half<T>::narrow(f[8 * y + 4], f[8 * y + 5]), Half<T>::narrow(f[8 * y + 6], f[8 * y + 7])};
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                *reinterpret_cast<float4*>(part + ((c / 4 + y) * kRows + place_row) * 4) = make_float4(f[4 * y], f[4 * y + 1], f[4 * y + 2], f[4 * y + 3]);
+            }
           }
         }
         if (!whole && mine) {
-          part[kRows * D + row] = m;
-          part[kRows * D + kRows + row] = l;
+          part[kRows * D + place_row] = m;
+          part[kRows * D + kRows + place_row] = l;
         }
       }
-      if (!whole && w.u0 == 0 && tid == 0)                 // it begins here and ends elsewhere: request, tile, parts, head and place of the first
+      __syncwarp();
+      fence_before();
+      if (w.twin) bar_arrive(smem_u32(&s.twin_done));
+      if (!whole && w.u0 == 0 && tid == 0)                 // it begins here and ends elsewhere: request, item, parts, head and place of the first
         a.cuts[blockIdx.x] = {w.r, w.tile, 1 + (int)((w.units - w.u1 + share - 1) / share), 2 * w.head + (segment != 0)};
-      fence_before();                                      // (the next tile's first product into O comes after this thread's next arrival)
     }
-  } else if (count > 0 && warp < 8) {
-    // ================= cache -> fp16 core matrices
-    const int t = tid - 128, cw = warp - 4;
-    const int tg = lane & 7, dc = (lane >> 3) + 4 * cw;    // values: group of 8 tokens, piece of D / 16 dimensions
-    bool ok = true, bad = false;
-    uint32_t vr[8][D / 64];
-    Walk w(s, count);
-    w.look(a);
-    // three units are under way: one that is written, the next, whose rows are being fetched, and the one after it, whose pages are
-    Walk f = w;
-    int fu = w.u0;                                         // of the pages that are fetched
-    struct Pages {
-      int k, v, scale, head, at;
-      bool all;                                            // every token of the unit lies in a page and before the end
-    };
-    const auto pages_of = [&](Pages& p) {
-      p.at = fu * kUnit;
-      p.head = f.head;
-      const int* table = a.tables + f.r * a.table_stride;
-      const auto page = [&](int token) { return token < f.end ? table[token >> a.shift] : -1; };
-      p.k = page(p.at + 16 * cw);
-      p.v = page(p.at + 8 * tg);
-      p.scale = page(p.at + 16 * (t & (kGroups - 1)));
-      p.all = p.at + kUnit <= f.end;
-      if (++fu == f.u1) {
-        f.next(a);
-        if (f.left > 0) {
-          f.look(a);
-          fu = f.u0;
-        }
-      }
-    };
+  } else if (count > 0 && warp < 14) {
+    // ================= values (warps 8-11) and keys (12-13)
+    const bool keys = warp >= 12;
+    const int kw = warp - 12, vw = warp - 8;
     const int place_mask = (1 << a.shift) - 1;
     const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
-    // (a page that is none is read as the first one and left aside later)
-    const auto keys_of = [&](const Pages& p, uint32_t n) { // straight to their core matrices
-      const int id = valid(p.k) ? p.k : 0;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int token = p.at + 16 * cw + 8 * b + (lane & 7);
-        const uint8_t* src = a.k_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
-        const uint32_t dst = smem_u32(smem + Y::kK + (n & 1) * Y::kKeys + (2 * cw + b) * Y::kGroup + (lane & 7) * 16 + (lane >> 3) * 128);
-#pragma unroll
-        for (int x = 0; x < D / 64; ++x)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * 512), "l"(src + 64 * x) : "memory");
-      }
+    bool ok = true, bad = false;
+    // units one after the other; the pages of the next are fetched while the rows of one are
+    struct Unit {
+      int id[2], head, at, end, least;
     };
-    const auto values_of = [&](const Pages& p) {
-      const int id = valid(p.v) ? p.v : 0, token = p.at + 8 * tg;
-      const uint8_t* src = a.v_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + dc * (D / 16);
+    Walk f(s, count);
+    f.look(a);
+    int fu = f.u0;
+    const auto pages_of = [&](Unit& p) {
+      p.at = fu * kUnit;
+      p.head = f.head;
+      p.end = f.end;
+      p.least = f.least;
+      const int* table = a.tables + f.r * a.table_stride;
+      const int token = p.at + (keys ? 32 * kw : 16 * vw);
+      p.id[0] = token < f.end ? table[token >> a.shift] : -1;
+      if (keys) p.id[1] = token + 16 < f.end ? table[(token + 16) >> a.shift] : -1;
+      if (++fu < f.u1) return;
+      f.next(a);
+      if (f.left <= 0) return;
+      f.look(a);
+      fu = f.u0;
+    };
+    Unit next;
+    pages_of(next);
+    if (keys) {
+      // ---- straight to their place; a unit is announced when the copies of the two after it are under way
+      float ks = 0.f, vs = 1.f;
+      bool real = false;
+      const auto announce_scales = [&](uint32_t n) {       // of the unit before: lane g holds those of group 2 kw + g
+        const int slot = n % kScales;
+        if (lane < 2) {
+          s.ks[slot][2 * kw + lane] = ks;
+          s.lv[slot][2 * kw + lane] = __log2f(vs);         // of a power of two: exact
+          s.inv[slot][2 * kw + lane] = __fdividef(1.f, vs);
+          s.real[slot][2 * kw + lane] = real;
+        }
+        __syncwarp();
+        bar_arrive(smem_u32(&s.scales[slot]));
+      };
+      const auto announce_keys = [&](uint32_t n) {
+        fence_async();
+        bar_arrive(smem_u32(&s.k_full[n % kRing]));
+      };
+      uint32_t n = 0;
+      for (; n < count && ok; ++n) {
+        const Unit now = next;
+        if (n + 1 < count) pages_of(next);
+        if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.k_free, kRing, n - kRing));
+        if (!ok) break;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        if constexpr (D == 128) {
-          const uint2 raw = *reinterpret_cast<const uint2*>(src + x * D);
-          vr[x][0] = raw.x; vr[x][1] = raw.y;
-        } else {
-          vr[x][0] = *reinterpret_cast<const uint32_t*>(src + x * D);
+        for (int b = 0; b < 4; ++b) {
+          const int id = valid(now.id[b >> 1]) ? now.id[b >> 1] : 0, token = now.at + 32 * kw + 8 * b + (lane & 7);
+          const uint8_t* src = a.k_cache + ((((size_t)id * a.kv_heads + now.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
+          const uint32_t dst = smem_u32(smem + Y::kK + (n % kRing) * Y::kKeys);
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + Y::piece(32 * kw + 8 * b + (lane & 7), (lane >> 3) + 4 * y)), "l"(src + 64 * y)
+                         : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (n >= 1) announce_scales(n - 1);
+        {
+          const int id = now.id[lane & 1];
+          real = valid(id);
+          bad |= id != -1 && !real;                        // (-1: behind the last token)
+          const size_t at = (size_t)(real ? id : 0) * a.kv_heads + now.head;
+          ks = a.k_scale[at];
+          vs = a.v_scale[at];
+        }
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        if (n >= 2) announce_keys(n - 2);
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (ok) {
+        announce_scales(n - 1);
+        if (n >= 2) announce_keys(n - 2);
+        announce_keys(n - 1);
+      }
+      if (bad && a.status) atomicOr(a.status, 32);
+    } else {
+      // ---- through registers, widened: a warp takes 16 tokens, a lane two of them (8 apart), 16 dimensions of each 64
+      uint4 v[2][2][D / 64];
+      Unit unit[2];
+      const auto rows_of = [&](const Unit& p, uint4 (&v)[2][D / 64]) {         // (a page that is none is read as the first one and left aside later)
+        const int id = valid(p.id[0]) ? p.id[0] : 0, token = p.at + 16 * vw + (lane & 7);
+        const uint8_t* src = a.v_cache + ((((size_t)id * a.kv_heads + p.head) << a.shift) + (token & place_mask)) * D + (lane >> 3) * 16;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) v[b][y] = *reinterpret_cast<const uint4*>(src + 8 * b * D + 64 * y);
+      };
+      const auto write = [&](const Unit& p, uint4 (&v)[2][D / 64], uint32_t n) {
+        if (p.at + 16 * vw + 16 > p.least || !valid(p.id[0])) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            // behind the request's tokens lies what an earlier one left; a NaN of a token that not all rows see is not for the others
+            const int token = p.at + 16 * vw + 8 * b + (lane & 7);
+            const bool gone = token >= p.end || !valid(p.id[0]), some = token >= p.least;
+            const auto clean = [&](uint32_t& w) {
+              if (gone) w = 0;
+              const uint32_t nan = some ? nan_bytes(w) : 0;
+              w &= ~nan;
+              any |= nan;
+            };
+#pragma unroll
+            for (int y = 0; y < D / 64; ++y) {
+              clean(v[b][y].x);
+              clean(v[b][y].y);
+              clean(v[b][y].z);
+              clean(v[b][y].w);
+            }
+          }
+          if (any) s.nan = 1;
+        }
+        uint8_t* dst = smem + Y::kV + (n % kRing) * Y::kValues;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) {
+            const uint4 w = v[b][y];
+            const int token = 16 * vw + 8 * b + (lane & 7), chunk = 2 * ((lane >> 3) + 4 * y);
+            *reinterpret_cast<uint4*>(dst + Y::value(token, chunk)) = {from_e4m3(w.x & 0xFFFFu), from_e4m3(w.x >> 16), from_e4m3(w.y & 0xFFFFu), from_e4m3(w.y >> 16)};
+            *reinterpret_cast<uint4*>(dst + Y::value(token, chunk + 1)) = {from_e4m3(w.z & 0xFFFFu), from_e4m3(w.z >> 16), from_e4m3(w.w & 0xFFFFu), from_e4m3(w.w >> 16)};
+          }
+        fence_async();
+        bar_arrive(smem_u32(&s.v_full[n % kRing]));
+      };
+      // the rows of unit n + 1 are fetched before those of unit n are written, the pages of unit n + 2 before that
+      unit[0] = next;
+      if (count > 1) pages_of(next);
+      rows_of(unit[0], v[0]);
+      for (uint32_t n = 0; n < count && ok; n += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (n + h >= count || !ok) break;
+          if (n + h + 1 < count) {
+            unit[h ^ 1] = next;
+            rows_of(unit[h ^ 1], v[h ^ 1]);
+            if (n + h + 2 < count) pages_of(next);
+          }
+          if (n + h >= kRing) ok = __all_sync(kFullWarp, ring(s.v_free, kRing, n + h - kRing));
+          if (ok) write(unit[h], v[h], n + h);
         }
       }
-    };
-    float ks = 0.f, vs = 1.f;
-    const auto scales_of = [&](const Pages& p) {
-      const size_t at = (size_t)(valid(p.scale) ? p.scale : 0) * a.kv_heads + p.head;
-      ks = a.k_scale[at];
-      vs = a.v_scale[at];
-    };
-    Pages now, next, later;                                // of the unit that is written, of the next, of the one after it
-    pages_of(now);
-    keys_of(now, 0);
-    values_of(now);
-    scales_of(now);
-    next = now;
-    if (f.left > 0) pages_of(next);
-    long long owed = count - 1;                            // units that come after this one
-    // the products, issued by the first of these warps
-    const uint32_t idesc_s = 1u << 4 | (uint32_t)(kUnit >> 3) << 17 | (128u >> 4) << 24, idesc_o = 1u << 4 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
-    const uint64_t dq = descriptor(smem_u32(smem + Y::kQ), 128, Y::kGroup), dk = descriptor(smem_u32(smem + Y::kK), 128, Y::kGroup),
-                   dv = descriptor(smem_u32(smem + Y::kV), Y::kTokens, 128);
-    uint32_t fresh = 0, q_phase = 0;                       // fresh: 0 where the unit before is the first of its tile
-    const auto scores = [&](uint32_t n, bool first) {
-      if (!__all_sync(kFullWarp, reached(k_full, n) && (!first || bar_wait(q_full, q_phase, fail)))) return false;
-      fence_after();
-      if (elect_one()) {
+    }
+  } else if (count > 0) {
+    // ================= products: one thread, and as few instructions between two of them as can be (24 a unit, 50 to 60 cycles each to issue)
+    if (elect_one()) {
+      const uint32_t idesc_s = 1u << 4 | (uint32_t)(kUnit >> 3) << 17 | (128u >> 4) << 24,
+                     idesc_o = 1u << 4 | 1u << 16 | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;      // (1 << 16: values with the dimensions inside)
+      constexpr uint64_t kSwizzle = D == 128 ? 2 : 4;
+      const uint64_t dq = descriptor(smem_u32(smem + Y::kQ), 16, 8 * D, kSwizzle), dk = descriptor(smem_u32(smem + Y::kK), 16, 8 * D, kSwizzle),
+                     dv = descriptor(smem_u32(smem + Y::kV), kUnit * 128, 1024, 2);
+      const uint32_t k_full = smem_u32(s.k_full), k_free = smem_u32(s.k_free), v_full = smem_u32(s.v_full), v_free = smem_u32(s.v_free),
+                     s_full = smem_u32(s.s_full), p_full = smem_u32(s.p_full), pv_done = smem_u32(s.pv_done), q_full = smem_u32(&s.q_full);
+      bool ok = true;
+      uint32_t items = 0, qn = 0, pn = 0;                  // items, units of the thread block whose scores and whose results have been issued
+      uint32_t qc[2] = {0, 0}, pc[2] = {0, 0};             // the same of the tiles
+      const auto scores_of = [&](auto tile) {
+        constexpr int x = decltype(tile)::value;
+        const uint64_t k = dk + (qn % kRing) * (Y::kKeys >> 4);
+        const uint32_t to = tmem + 256 * x + 64 * (qc[x] & 1);
 #pragma unroll
         for (int part = 0; part < Y::kParts; ++part)
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k)
-            mma_ss(tmem + 64 * (n & 1), dq + part * (Y::kPart >> 4) + 16 * k, dk + (n & 1) * (Y::kKeys >> 4) + 16 * k, idesc_s, (part | k) != 0);
-        commit(s_full + 8 * (n & 1));
-      }
-      __syncwarp();
-      if (first) q_phase ^= 1;
-      return true;
-    };
-    const auto results = [&](uint32_t n) {                 // (P of the unit is there)
-      if (!__all_sync(kFullWarp, reached(v_full, n))) return false;
-      fence_after();
-      if (elect_one()) {
+          for (int y = 0; y < D / 32; ++y)
+            mma_ss(to, dq + (x * Y::kQTile + part * Y::kPart >> 4) + 2 * y, k + 2 * y, idesc_s, (part | y) != 0);
+        commit(s_full + 16 * x + 8 * (qc[x] & 1));
+        ++qc[x];
+      };
+      const auto results_of = [&](auto tile, uint32_t fresh) {
+        constexpr int x = decltype(tile)::value;
+        if (!bar_wait(p_full + 16 * x + 8 * (pc[x] & 1), pc[x] >> 1 & 1, fail)) return false;
+        fence_after();
+        const uint64_t v = dv + (pn % kRing) * (Y::kValues >> 4);
+        const uint32_t from = tmem + 256 * x + 64 * (pc[x] & 1);
 #pragma unroll
-        for (int k = 0; k < kUnit / 16; ++k)
-          mma_ts(tmem + 128, tmem + 64 * (n & 1) + 8 * k, dv + (n & 1) * (Y::kValues >> 4) + (uint64_t)(k * (2 * Y::kTokens >> 4)), idesc_o, k != 0 ? 1u : fresh);
-        commit(pv_done + 8 * (n & 1));
-      }
-      __syncwarp();
-      return true;
-    };
-    for (; w.left > 0 && ok;) {
-      for (int u = w.u0; u < w.u1 && ok; ++u, ++n) {
-        const bool first = u == w.u0;                      // of its tile: its queries come after the results of the last tile
-        const int turn = n & 1;
-        // ---- keys, which are on their way, and scales
-        if (cw == 0) {
-          const unsigned mask = __ballot_sync(kFullWarp, t < kGroups && valid(now.scale));
-          bad |= now.scale != -1 && !valid(now.scale);     // (-1: behind the last token)
-          if (t < kGroups) {
-            s.ks[turn][t] = ks;
-            s.lv[turn][t] = __log2f(vs);                   // of a power of two: exact
-            s.inv[turn][t] = __fdividef(1.f, vs);
+        for (int y = 0; y < kUnit / 16; ++y) mma_ts(tmem + 256 * x + 128, from + 8 * y, v + y * (2048 >> 4), idesc_o, y != 0 ? 1u : fresh);
+        commit(pv_done + 16 * x + 8 * (pc[x] & 1));
+        ++pc[x];
+        return true;
+      };
+      Walk w(s, count);
+      for (; w.left > 0 && ok; w.next(a)) {
+        w.look(a);
+        ok = bar_wait(q_full, items++ & 1, fail);
+        const int units = w.u1 - w.u0, ahead = w.twin ? 4 : 2;
+        // scores of unit i of the item come `ahead` places before the results of the unit that is that far behind
+        for (int i = 1 - ahead; i < units && ok; ++i) {
+          const int j = i + ahead - 1;
+          if (j < units) {
+            if (!(ok = bar_wait(k_full + 8 * (qn % kRing), qn / kRing & 1, fail))) break;
+            fence_after();
+            if (!w.twin || !(j & 1)) scores_of(std::integral_constant<int, 0>{});
+            if (!w.twin || (j & 1)) scores_of(std::integral_constant<int, 1>{});
+            commit(k_free + 8 * (qn % kRing));
+            ++qn;
           }
-          // (a group behind the last token has no page either: the rows' ends mask it)
-          if (t == 0) s.real[turn] = mask;
+          if (i < 0) continue;
+          if (!(ok = bar_wait(v_full + 8 * (pn % kRing), pn / kRing & 1, fail))) break;
+          const uint32_t fresh = i >= (w.twin ? 2 : 1);    // 0: the tile's first unit of this item
+          if (!w.twin || !(i & 1)) ok = results_of(std::integral_constant<int, 0>{}, fresh);
+          if (ok && (!w.twin || (i & 1))) ok = results_of(std::integral_constant<int, 1>{}, fresh);
+          commit(v_free + 8 * (pn % kRing));
+          ++pn;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_async();
-        bar_arrive(k_full + 8 * turn);
-        if (cw == 0 && !first && !(ok = scores(n, false))) break;
-        later = next;
-        if (f.left > 0) pages_of(later);
-        // ---- values, once the results of the unit before the last are done
-        if (n >= 2) ok = __all_sync(kFullWarp, reached(pv_done, n - 2));
-        if (!ok) break;
-        const int vtoken = u * kUnit + 8 * tg;
-        if (!now.all || !valid(now.v)) {                   // behind the request's tokens lies what an earlier one left
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j)
-              if (vtoken + x >= w.end || !valid(now.v)) vr[x][j] = 0;
-        }
-        if (vtoken + 8 > w.least) {                        // tokens that not all rows see: a NaN there is not for the others
-          uint32_t any = 0;
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-              const uint32_t b = vtoken + x >= w.least ? nan_bytes(vr[x][j]) : 0;
-              vr[x][j] &= ~b;
-              any |= b;
-            }
-          if (any) s.nan = 1;
-        }
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {                 // four dimensions of eight tokens
-          uint32_t lo[4], hi[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            lo[x] = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], 0x5140);
-            hi[x] = __byte_perm(vr[2 * x][j], vr[2 * x + 1][j], 0x7362);
-          }
-          const int d = dc * (D / 16) + 4 * j;
-          uint8_t* dst = smem + Y::kV + turn * Y::kValues + tg * Y::kTokens + (d >> 3) * 128 + (d & 7) * 16;
-          *reinterpret_cast<uint4*>(dst) = {from_e4m3(lo[0] & 0xFFFFu), from_e4m3(lo[1] & 0xFFFFu), from_e4m3(lo[2] & 0xFFFFu), from_e4m3(lo[3] & 0xFFFFu)};
-          *reinterpret_cast<uint4*>(dst + 16) = {from_e4m3(lo[0] >> 16), from_e4m3(lo[1] >> 16), from_e4m3(lo[2] >> 16), from_e4m3(lo[3] >> 16)};
-          *reinterpret_cast<uint4*>(dst + 32) = {from_e4m3(hi[0] & 0xFFFFu), from_e4m3(hi[1] & 0xFFFFu), from_e4m3(hi[2] & 0xFFFFu), from_e4m3(hi[3] & 0xFFFFu)};
-          *reinterpret_cast<uint4*>(dst + 48) = {from_e4m3(hi[0] >> 16), from_e4m3(hi[1] >> 16), from_e4m3(hi[2] >> 16), from_e4m3(hi[3] >> 16)};
-        }
-        fence_async();
-        bar_arrive(v_full + 8 * turn);
-        // ---- the next unit's rows; its keys go where those of the last unit were
-        if (owed > 0) {
-          values_of(next);
-          scales_of(next);
-          if (n >= 1) ok = __all_sync(kFullWarp, reached(s_full, n - 1));
-          if (!ok) break;
-          keys_of(next, n + 1);
-        }
-        --owed;
-        now = next;
-        next = later;
-        // ---- results of the last unit.  (All of these warps wait for its P: none is then two phases ahead of a thread that still waits for keys.)
-        if (n >= 1) {
-          ok = __all_sync(kFullWarp, reached(p_full, n - 1));
-          if (!ok || (cw == 0 && !(ok = results(n - 1)))) break;
-        }
-        if (cw == 0 && first && !(ok = scores(n, true))) break;
-        fresh = !first;
       }
-      if (!ok) break;
-      w.next(a);
-      if (w.left > 0) w.look(a);
+      // products in flight end before the tensor memory goes back
+      commit(smem_u32(&s.drained));
+      for (unsigned i = 0; i < kSpinLimit && !bar_try(smem_u32(&s.drained), 0); ++i) {}
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (cw == 0) {
-      if (ok) ok = __all_sync(kFullWarp, reached(p_full, n - 1)) && results(n - 1);
-      if (!ok) {                                           // products in flight end before the tensor memory goes back
-        if (elect_one()) commit(smem_u32(&s.drained));
-        __syncwarp();
-        for (unsigned i = 0; i < kSpinLimit && !bar_try(smem_u32(&s.drained), 0); ++i) {}
-      }
-    }
-    if (bad && a.status) atomicOr(a.status, 32);
   }
+  __syncwarp();
   fence_before();
   __syncthreads();
   if (tid == 0 && s.fail && a.status) atomicOr(a.status, 64);
@@ -751,7 +828,7 @@ int run(const AttentionArgs& a, cudaStream_t st) {
     if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
   }
   if (e) return paged_fail(e);
-  const dim3 grid(device_sms() * kBlocksPerSm);
+  const dim3 grid(device_sms());
   const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, (Layout<T, D>::kBytes), st, a);
   return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, grid, dim3(512), 1, 0, st, a);
 }
@@ -764,13 +841,13 @@ namespace htr {
 bool attention_tc_serves(int requests, int group, int max_new) { return requests <= kMaxRequests && group <= kRows && (long long)group * max_new > 16; }
 
 size_t attention_tc_workspace(int head_dim) {
-  return (size_t)device_sms() * kBlocksPerSm * (sizeof(int4) + 2 * sizeof(float) * (head_dim == 128 ? kPartFloats<128> : kPartFloats<64>));
+  return (size_t)device_sms() * (sizeof(int4) + 2 * sizeof(float) * (head_dim == 128 ? kPartFloats<128> : kPartFloats<64>));
 }
 
 int attention_tc_run(const AttentionArgs& args, int dtype, int head_dim, void* workspace, cudaStream_t st) {
   AttentionArgs a = args;
   a.cuts = static_cast<int4*>(workspace);
-  a.parts = reinterpret_cast<float*>(a.cuts + device_sms() * kBlocksPerSm);
+  a.parts = reinterpret_cast<float*>(a.cuts + device_sms());
   if (dtype == HTR_DTYPE_BF16) return head_dim == 128 ? run<__nv_bfloat16, 128>(a, st) : run<__nv_bfloat16, 64>(a, st);
   return head_dim == 128 ? run<__half, 128>(a, st) : run<__half, 64>(a, st);
 }
