@@ -28,7 +28,7 @@ namespace {
 
 using namespace htr;
 
-constexpr int kThreads = 480, kTile = 128, kRows = 256, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024;
+constexpr int kThreads = 512, kTile = 128, kRows = 256, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024;
 constexpr int kTmemColumns = 512;                          // of a tile: S (P over it) at 0 and 64, O at 128
 constexpr int kRing = 4, kScales = 8;                      // units of keys and of values in shared memory; of their scales, read by all rows
 constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
@@ -133,11 +133,6 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
   asm("{\n\t.reg .b64 r, s;\n\tmov.b64 r, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 r, r, s;\n\tmov.b64 {%0, %1}, r;\n\t}"
       : "+f"(x), "+f"(y) : "f"(a), "f"(b));
 }
-__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // a request's tiles, and what one of them sees
 struct Request {
   int start, n, seen, per, tiles;                          // per: tokens of a tile
@@ -154,7 +149,7 @@ struct Request {
 };
 
 struct Shared {
-  unsigned long long k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], scales[kScales];      // of the units in turns
+  unsigned long long k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing];      // of the units in turns
   unsigned long long s_full[4], p_full[4], pv_done[4];     // of a tile's units in turns: 2 * tile + turn
   unsigned long long q_full, twin_full, twin_done, drained;
   long long sums[kMaxRequests];                            // units of each request
@@ -162,7 +157,7 @@ struct Shared {
   int r, tile, head, unit;                                 // where this thread block's run begins
   uint32_t tmem;
   int fail, nan;
-  float ks[kScales][kGroups], lv[kScales][kGroups], inv[kScales][kGroups];     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
+  alignas(16) float ks[kScales][kGroups], lv[kScales][kGroups], inv[kScales][kGroups];     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
   unsigned char real[kScales][kGroups];                    // groups that have a page
   float twin_m[kTile], twin_l[kTile];
 };
@@ -196,6 +191,7 @@ struct Walk {
   }
 };
 
+constexpr int kJoins = 8;
 template <int D>
 constexpr int kPartFloats = kRows * (D + 2);
 
@@ -225,7 +221,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       bar_init(smem_u32(&s.v_full[i]), 128);
       bar_init(smem_u32(&s.v_free[i]), 1);
     }
-    for (int i = 0; i < kScales; ++i) bar_init(smem_u32(&s.scales[i]), 64);
     for (int i = 0; i < 4; ++i) {
       bar_init(smem_u32(&s.s_full[i]), 1);
       bar_init(smem_u32(&s.p_full[i]), 128);
@@ -309,247 +304,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   // unit n of the thread block in a ring of bars, and unit c of a tile in its two
   const auto ring = [&](unsigned long long* bars, uint32_t size, uint32_t n) { return bar_wait(smem_u32(bars + n % size), n / size & 1, fail); };
   const auto turn = [&](unsigned long long* bars, int x, uint32_t c) { return bar_wait(smem_u32(bars + 2 * x + (c & 1)), c >> 1 & 1, fail); };
-  if (count > 0 && warp < 8) {
-    // ================= softmax: a thread per row of tile x
-    const int x = warp >> 2, row = tid & (kTile - 1);
-    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), mine_at = lanes + 256 * x;
-    bool ok = true;
-    const auto follow = [&](float f) {                     // results relative to a new reference
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        uint32_t o[16];
-        tmem_load16(mine_at + 128 + c, o);
-#pragma unroll
-        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-        tmem_store(mine_at + 128 + c, o);
-      }
-      tmem_stored();
-    };
-    Walk w(s, count);
-    uint32_t n = 0, done = 0, twins = 0;                   // units of the thread block, of this tile; twins so far
-    for (int segment = 0; w.left > 0 && ok; ++segment, w.next(a)) {
-      w.look(a);
-      const int place_row = w.twin ? row : x * kTile + row, i = place_row / a.group, head = w.head * a.group + place_row - i * a.group;
-      const bool mine = place_row < w.rows, warp_has_rows = (w.twin ? 0 : x * kTile) + 32 * (warp & 3) < w.rows;
-      const size_t place = ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
-      const int row_end = mine ? max(w.seen - w.n + w.tile * w.per + i + 1, 0) : 0;
-      // queries: e4m3 parts under a power of two per row (of a twin: both tiles hold them)
-      float row_scale;
-      {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + place);
-        float most = 0.f;
-        if (mine)
-#pragma unroll 4
-          for (int j = 0; j < D / 8; ++j) {
-            const uint4 raw = src[j];
-            const float2 f[4] = {Half<T>::wide(raw.x), Half<T>::wide(raw.y), Half<T>::wide(raw.z), Half<T>::wide(raw.w)};
-#pragma unroll
-            for (int y = 0; y < 4; ++y) most = fmaxf(most, fmaxf(fabsf(f[y].x), fabsf(f[y].y)));
-          }
-        const int e = query_exponent(most) - 7;            // the largest between 2^7 and 2^8
-        const float up = most > 3.402823466e38f ? __int_as_float(0x7FC00000) : exp2i(e);       // (an infinite element: all scores are NaN or infinite)
-        row_scale = exp2i(-e) * a.scale;
-        uint8_t* dst = smem + Y::kQ + x * Y::kQTile;
-#pragma unroll 1
-        for (int j = 0; j < D / 16; ++j) {                 // 16 dimensions: 16 bytes of each part
-          float f[16];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint4 raw = mine ? src[2 * j + y] : uint4{0, 0, 0, 0};
-            const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const float2 v = Half<T>::wide(w4[z]);
-              f[8 * y + 2 * z] = v.x * up;
-              f[8 * y + 2 * z + 1] = v.y * up;
-            }
-          }
-#pragma unroll
-          for (int part = 0; part < Y::kParts; ++part) {
-            uint32_t r[4];
-#pragma unroll
-            for (int z = 0; z < 8; ++z) {
-              const uint32_t two = to_e4m3(f[2 * z], f[2 * z + 1]);
-              const float2 held = Half<__half>::wide(from_e4m3(two));
-              f[2 * z] -= held.x;                          // what is left for the next part, exactly
-              f[2 * z + 1] -= held.y;
-              r[z >> 1] = z & 1 ? r[z >> 1] | two << 16 : two;
-            }
-            *reinterpret_cast<uint4*>(dst + part * Y::kPart + Y::piece(row, j)) = make_uint4(r[0], r[1], r[2], r[3]);
-          }
-        }
-        fence_async();
-        fence_before();
-        bar_arrive(smem_u32(&s.q_full));
-      }
-      float m = kNone, l = 0.f;
-      bool results = false;                                // of an earlier unit of this tile
-      for (int u = w.u0; u < w.u1 && ok; ++u, ++n) {
-        if (w.twin && ((u - w.u0) & 1) != x) continue;
-        ok = __all_sync(kFullWarp, ring(s.scales, kScales, n) && turn(s.s_full, x, done));
-        if (!ok) break;
-        fence_after();
-        const int at = u * kUnit, slot = n % kScales;
-        const unsigned real = *reinterpret_cast<const unsigned*>(s.real[slot]);
-        const uint32_t scores = mine_at + 64 * (done & 1);
-        if (warp_has_rows) {
-          uint32_t raw[2][32];
-          tmem_load(scores, raw[0]);
-          tmem_load(scores + 32, raw[1]);
-          tmem_loaded(raw[0]);
-          tmem_loaded(raw[1]);
-          float v[kUnit], base = m == kNone ? 0.f : m;
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            const float by = row_scale * s.ks[slot][g], add = s.lv[slot][g] - base;
-#pragma unroll
-            for (int c = 16 * g; c < 16 * g + 16; c += 2) fma2(v[c], v[c + 1], raw[c >> 5][c & 31], raw[c >> 5][(c & 31) + 1], by, add);
-          }
-          if (at + kUnit > w.least || real != 0x01010101u) {
-#pragma unroll
-            for (int c = 0; c < kUnit; ++c)
-              if (at + c >= row_end || !(real >> (8 * (c >> 4)) & 1)) v[c] = kNone;
-          }
-          float sum[kGroups][2];
-          uint32_t p[kUnit / 2];
-          const auto exponentials = [&] {
-#pragma unroll
-            for (int c = 0; c < kUnit / 2; ++c) {
-              const float y = exp2_fast(v[2 * c]), z = exp2_fast(v[2 * c + 1]);
-              if (c & 7) add2(sum[c >> 3][0], sum[c >> 3][1], y, z);
-              else sum[c >> 3][0] = y, sum[c >> 3][1] = z;
-              p[c] = pack_half(y, z);
-            }
-          };
-          exponentials();
-          // whether P stays below 2^14: of its halves, whose overflow is infinite
-          uint32_t big[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) big[c] = max_half2(max_half2(p[c], p[c + 8]), max_half2(p[c + 16], p[c + 24]));
-#pragma unroll
-          for (int c = 4; c; c >>= 1)
-#pragma unroll
-            for (int y = 0; y < c; ++y) big[y] = max_half2(big[y], big[y + c]);
-          const float2 pair = Half<__half>::wide(big[0]);
-          const bool grows = m == kNone || fmaxf(pair.x, pair.y) > 16384.f;
-          if (__any_sync(kFullWarp, grows)) {              // a new reference, 2^6 above which the largest lies; what there is follows
-            float top = kNone;
-#pragma unroll
-            for (int c = 0; c < kUnit; ++c) top = fmaxf(top, v[c]);
-            const bool moves = grows && top > kNone;
-            const float now = moves ? base + top - 6.f : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
-#pragma unroll
-            for (int c = 0; c < kUnit; ++c) v[c] += down;
-            m = now;
-            l *= f;
-            if (results) {
-              ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));        // (S of this unit came before the results of the last one)
-              fence_after();
-              if (ok) follow(f);
-            }
-            exponentials();
-          }
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g) l = fmaf(sum[g][0] + sum[g][1], s.inv[slot][g], l);
-          __syncwarp();
-          tmem_store(scores, reinterpret_cast<const uint32_t (&)[16]>(p[0]));
-          tmem_store(scores + 16, reinterpret_cast<const uint32_t (&)[16]>(p[16]));
-          tmem_stored();
-        }
-        fence_before();
-        bar_arrive(smem_u32(&s.p_full[2 * x + (done & 1)]));
-        results = true;
-        ++done;
-      }
-      if (!ok) break;
-      if (results) ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));
-      if (!ok) break;
-      fence_after();
-      // ---- a twin's results are joined by the threads of the first tile, which can read both
-      float here = 1.f, there = 0.f;                       // factors of this tile's results and of the other's
-      bool other = false;
-      if (w.twin) {
-        if (x == 1) {
-          s.twin_m[row] = m;
-          s.twin_l[row] = l;
-          fence_before();
-          bar_arrive(smem_u32(&s.twin_full));
-          ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s.twin_done), twins & 1, fail));
-          ++twins;
-          fence_after();
-          continue;
-        }
-        ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s.twin_full), twins & 1, fail));
-        ++twins;
-        if (!ok) break;
-        fence_after();
-        const float tm = s.twin_m[row], tl = s.twin_l[row], now = fmaxf(m, tm);
-        other = w.u1 - w.u0 > 1;
-        if (now != kNone) {
-          here = exp2_fast(m - now);
-          there = exp2_fast(tm - now);
-        }
-        l = l * here + tl * there;
-        m = now;
-      }
-      // ---- the item, or this run's part of it
-      const bool whole = w.u0 == 0 && w.u1 == w.units;
-      float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPartFloats<D>;
-      const bool empty = l == 0.f;                         // a row that sees nothing: zeros
-      const float by = whole && !empty ? 1.f / l : 1.f;
-      const bool nan = *(volatile int*)&s.nan != 0;
-      if (warp_has_rows) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16];
-          __syncwarp();
-          tmem_load16(mine_at + 128 + c, o);
-          float f[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : __uint_as_float(o[y]) * here * by;
-          if (other) {
-            __syncwarp();
-            tmem_load16(mine_at + 256 + 128 + c, o);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : fmaf(__uint_as_float(o[y]) * there, by, f[y]);
-          }
-          if (mine) {
-            if (nan)                                       // values that are NaN were left out of the last units: given to the rows that see them
-              for (int token = max(w.least, w.u0 * kUnit); token < min(row_end, w.u1 * kUnit); ++token) {
-                const int id = a.tables[w.r * a.table_stride + (token >> a.shift)];
-                if (id < 0 || id >= a.pages) continue;
-                const uint8_t* v = a.v_cache + ((((size_t)id * a.kv_heads + w.head) << a.shift) + (token & ((1 << a.shift) - 1))) * D + c;
-#pragma unroll
-                for (int y = 0; y < 16; ++y)
-                  if ((v[y] & 0x7F) == 0x7F) f[y] = __int_as_float(0x7FC00000);
-              }
-            if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + place + c);
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-                dst[y] = {Half<T>::narrow(f[8 * y], f[8 * y + 1]), Half<T>::narrow(f[8 * y + 2], f[8 * y + 3]),
-                          Half<T>::narrow(f[8 * y + 4], f[8 * y + 5]), Half<T>::narrow(f[8 * y + 6], f[8 * y + 7])};
-            } else {
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                *reinterpret_cast<float4*>(part + ((c / 4 + y) * kRows + place_row) * 4) = make_float4(f[4 * y], f[4 * y + 1], f[4 * y + 2], f[4 * y + 3]);
-            }
-          }
-        }
-        if (!whole && mine) {
-          part[kRows * D + place_row] = m;
-          part[kRows * D + kRows + place_row] = l;
-        }
-      }
-      __syncwarp();
-      fence_before();
-      if (w.twin) bar_arrive(smem_u32(&s.twin_done));
-      if (!whole && w.u0 == 0 && tid == 0)                 // it begins here and ends elsewhere: request, item, parts, head and place of the first
-        a.cuts[blockIdx.x] = {w.r, w.tile, 1 + (int)((w.units - w.u1 + share - 1) / share), 2 * w.head + (segment != 0)};
-    }
-  } else if (count > 0 && warp < 14) {
-    // ================= values (warps 8-11) and keys (12-13)
-    const bool keys = warp >= 12;
+  // ================= values (warps 8-11) and keys (12-13)
+  const auto feed = [&](auto which) {
+    constexpr bool keys = decltype(which)::value;
     const int kw = warp - 12, vw = warp - 8;
     const int place_mask = (1 << a.shift) - 1;
     const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
@@ -578,11 +335,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
     };
     Unit next;
     pages_of(next);
-    if (keys) {
+    if constexpr (keys) {
       // ---- straight to their place; a unit is announced when the copies of the two after it are under way
       float ks = 0.f, vs = 1.f;
       bool real = false;
-      const auto announce_scales = [&](uint32_t n) {       // of the unit before: lane g holds those of group 2 kw + g
+      const auto write_scales = [&](uint32_t n) {          // lane g holds those of group 2 kw + g
         const int slot = n % kScales;
         if (lane < 2) {
           s.ks[slot][2 * kw + lane] = ks;
@@ -590,8 +347,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
           s.inv[slot][2 * kw + lane] = __fdividef(1.f, vs);
           s.real[slot][2 * kw + lane] = real;
         }
-        __syncwarp();
-        bar_arrive(smem_u32(&s.scales[slot]));
       };
       const auto announce_keys = [&](uint32_t n) {
         fence_async();
@@ -614,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
                          : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (n >= 1) announce_scales(n - 1);
+        if (n >= 1) write_scales(n - 1);
         {
           const int id = now.id[lane & 1];
           real = valid(id);
@@ -628,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       if (ok) {
-        announce_scales(n - 1);
+        write_scales(n - 1);
         if (n >= 2) announce_keys(n - 2);
         announce_keys(n - 1);
       }
@@ -700,7 +455,280 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         }
       }
     }
-  } else if (count > 0) {
+  };
+  // registers of the four warpgroups: 2 * 160 + 2 * 96 = 4 * 128, what the launch has
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    if (count > 0) {
+    // ================= softmax: a thread per row of tile x
+    const int x = warp >> 2, row = tid & (kTile - 1);
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), mine_at = lanes + 256 * x;
+    bool ok = true;
+    const auto follow = [&](float f) {                     // results relative to a new reference
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_load(mine_at + 128 + c, o);
+        tmem_loaded(o);
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+        tmem_store(mine_at + 128 + c, reinterpret_cast<const uint32_t (&)[16]>(o[0]));
+        tmem_store(mine_at + 128 + c + 16, reinterpret_cast<const uint32_t (&)[16]>(o[16]));
+      }
+      tmem_stored();
+    };
+    Walk w(s, count);
+    uint32_t n = 0, done = 0, twins = 0;                   // units of the thread block, of this tile; twins so far
+    for (int segment = 0; w.left > 0 && ok; ++segment, w.next(a)) {
+      w.look(a);
+      const int place_row = w.twin ? row : x * kTile + row, i = place_row / a.group, head = w.head * a.group + place_row - i * a.group;
+      const bool mine = place_row < w.rows, warp_has_rows = (w.twin ? 0 : x * kTile) + 32 * (warp & 3) < w.rows;
+      const size_t place = ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
+      const int row_end = mine ? max(w.seen - w.n + w.tile * w.per + i + 1, 0) : 0;
+      // queries: e4m3 parts under a power of two per row (of a twin: both tiles hold them)
+      float row_scale;
+      {
+        // 8 lanes a row, 4 rows at once: whole lines are read; a lane holds dimensions 8 * (lane & 7) to + 7 of each 64
+        uint8_t* dst = smem + Y::kQ + x * Y::kQTile;
+        const int first = row & ~31;                       // of this warp
+        const auto row_of = [&](int t) { return 4 * t + (lane >> 3); };
+        const long long at = mine ? (long long)place : -1;
+        uint4 raw[8][D / 64];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const long long from = __shfl_sync(kFullWarp, at, row_of(t));
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + max(from, 0LL)) + (lane & 7);
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) raw[t][y] = from >= 0 ? src[8 * y] : uint4{0, 0, 0, 0};
+        }
+        row_scale = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          float f[D / 64][8], most = 0.f;
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) {
+            const uint32_t w4[4] = {raw[t][y].x, raw[t][y].y, raw[t][y].z, raw[t][y].w};
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const float2 v = Half<T>::wide(w4[z]);
+              f[y][2 * z] = v.x;
+              f[y][2 * z + 1] = v.y;
+              most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
+            }
+          }
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(kFullWarp, most, o));
+          const int e = query_exponent(most) - 7;          // the largest between 2^7 and 2^8
+          const float up = most > 3.402823466e38f ? __int_as_float(0x7FC00000) : exp2i(e);     // (an infinite element: all scores are NaN or infinite)
+          const int owner = __shfl_sync(kFullWarp, e, (lane & 3) * 8);
+          if (lane >> 2 == t) row_scale = exp2i(-owner) * a.scale;
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) {
+#pragma unroll
+            for (int z = 0; z < 8; ++z) f[y][z] *= up;
+#pragma unroll
+            for (int part = 0; part < Y::kParts; ++part) {
+              uint32_t r[2];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                const uint32_t two = to_e4m3(f[y][2 * z], f[y][2 * z + 1]);
+                const float2 held = Half<__half>::wide(from_e4m3(two));
+                f[y][2 * z] -= held.x;                     // what is left for the next part, exactly
+                f[y][2 * z + 1] -= held.y;
+                r[z >> 1] = z & 1 ? r[z >> 1] | two << 16 : two;
+              }
+              *reinterpret_cast<uint2*>(dst + part * Y::kPart + Y::piece(first + row_of(t), 4 * y + ((lane & 7) >> 1)) + 8 * (lane & 1)) = make_uint2(r[0], r[1]);
+            }
+          }
+        }
+        fence_async();
+        fence_before();
+        bar_arrive(smem_u32(&s.q_full));
+      }
+      float m = kNone, l = 0.f;
+      bool results = false;                                // of an earlier unit of this tile
+      const uint32_t step = w.twin ? 2 : 1;                // of this tile's units
+      n += w.twin ? x : 0;
+      int u = w.u0 + (w.twin ? x : 0);
+      for (; u < w.u1 && ok; u += step, n += step) {
+        // (the scales were there before the keys, the keys before the scores)
+        ok = __all_sync(kFullWarp, turn(s.s_full, x, done));
+        if (!ok) break;
+        fence_after();
+        const int at = u * kUnit, slot = n % kScales;
+        const uint32_t scores = mine_at + 64 * (done & 1);
+        if (warp_has_rows) {
+          uint32_t raw[2][32];
+          tmem_load(scores, raw[0]);
+          tmem_load(scores + 32, raw[1]);
+          const float4 ks = *reinterpret_cast<const float4*>(s.ks[slot]), lv = *reinterpret_cast<const float4*>(s.lv[slot]),
+                       inv = *reinterpret_cast<const float4*>(s.inv[slot]);
+          const unsigned real = *reinterpret_cast<const unsigned*>(s.real[slot]);
+          const float base = m == kNone ? 0.f : m;
+          const float by[kGroups] = {row_scale * ks.x, row_scale * ks.y, row_scale * ks.z, row_scale * ks.w};
+          const float add[kGroups] = {lv.x - base, lv.y - base, lv.z - base, lv.w - base};
+          tmem_loaded(raw[0]);
+          tmem_loaded(raw[1]);
+          float v[kUnit];
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int c = 16 * g; c < 16 * g + 16; c += 2) fma2(v[c], v[c + 1], raw[c >> 5][c & 31], raw[c >> 5][(c & 31) + 1], by[g], add[g]);
+          if (at + kUnit > w.least || real != 0x01010101u) {
+#pragma unroll
+            for (int c = 0; c < kUnit; ++c)
+              if (at + c >= row_end || !(real >> (8 * (c >> 4)) & 1)) v[c] = kNone;
+          }
+          float sum[kGroups][2];
+          uint32_t p[kUnit / 2];
+          const auto exponentials = [&] {
+#pragma unroll
+            for (int c = 0; c < kUnit / 2; ++c) {
+              const float y = exp2_fast(v[2 * c]), z = exp2_fast(v[2 * c + 1]);
+              if (c & 7) add2(sum[c >> 3][0], sum[c >> 3][1], y, z);
+              else sum[c >> 3][0] = y, sum[c >> 3][1] = z;
+              p[c] = pack_half(y, z);
+            }
+          };
+          exponentials();
+          // a sum within the range of fp16: so is each of its terms
+          const float most = fmaxf(fmaxf(sum[0][0] + sum[0][1], sum[1][0] + sum[1][1]), fmaxf(sum[2][0] + sum[2][1], sum[3][0] + sum[3][1]));
+          const bool grows = m == kNone || most > 60000.f;
+          if (__any_sync(kFullWarp, grows)) {              // a new reference, 2^2 above which the largest lies; what there is follows
+            float top = kNone;
+#pragma unroll
+            for (int c = 0; c < kUnit; ++c) top = fmaxf(top, v[c]);
+            const bool moves = grows && top > kNone;
+            const float now = moves ? base + top - 2.f : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
+#pragma unroll
+            for (int c = 0; c < kUnit; ++c) v[c] += down;
+            m = now;
+            l *= f;
+            if (results) {
+              ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));        // (S of this unit came before the results of the last one)
+              fence_after();
+              if (ok) follow(f);
+            }
+            exponentials();
+          }
+          l = fmaf(sum[0][0] + sum[0][1], inv.x, fmaf(sum[1][0] + sum[1][1], inv.y, fmaf(sum[2][0] + sum[2][1], inv.z, fmaf(sum[3][0] + sum[3][1], inv.w, l))));
+          __syncwarp();
+          tmem_store(scores, reinterpret_cast<const uint32_t (&)[16]>(p[0]));
+          tmem_store(scores + 16, reinterpret_cast<const uint32_t (&)[16]>(p[16]));
+          tmem_stored();
+        }
+        fence_before();
+        bar_arrive(smem_u32(&s.p_full[2 * x + (done & 1)]));
+        results = true;
+        ++done;
+      }
+      n += w.u1 - u;                                       // (a twin's tiles end one apart)
+      if (!ok) break;
+      if (results) ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));
+      if (!ok) break;
+      fence_after();
+      // ---- a twin's results are joined by the threads of the first tile, which can read both
+      float here = 1.f, there = 0.f;                       // factors of this tile's results and of the other's
+      bool other = false;
+      if (w.twin) {
+        if (x == 1) {
+          s.twin_m[row] = m;
+          s.twin_l[row] = l;
+          fence_before();
+          bar_arrive(smem_u32(&s.twin_full));
+          ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s.twin_done), twins & 1, fail));
+          ++twins;
+          fence_after();
+          continue;
+        }
+        ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s.twin_full), twins & 1, fail));
+        ++twins;
+        if (!ok) break;
+        fence_after();
+        const float tm = s.twin_m[row], tl = s.twin_l[row], now = fmaxf(m, tm);
+        other = w.u1 - w.u0 > 1;
+        if (now != kNone) {
+          here = exp2_fast(m - now);
+          there = exp2_fast(tm - now);
+        }
+        l = l * here + tl * there;
+        m = now;
+      }
+      // ---- the item, or this run's part of it
+      const bool whole = w.u0 == 0 && w.u1 == w.units;
+      float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPartFloats<D>;
+      const bool empty = l == 0.f;                         // a row that sees nothing: zeros
+      const float by = whole && !empty ? 1.f / l : 1.f;
+      const bool nan = *(volatile int*)&s.nan != 0;
+      // results wait where the queries of the same rows were, whose products are done
+      const auto staged = [&](int row, int chunk) { return smem + Y::kQ + x * Y::kQTile + chunk / (D / 16) * Y::kPart + Y::piece(row, chunk % (D / 16)); };
+      if (warp_has_rows) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          __syncwarp();
+          tmem_load16(mine_at + 128 + c, o);
+          float f[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : __uint_as_float(o[y]) * here * by;
+          if (other) {
+            __syncwarp();
+            tmem_load16(mine_at + 256 + 128 + c, o);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : fmaf(__uint_as_float(o[y]) * there, by, f[y]);
+          }
+          if (mine) {
+            if (nan)                                       // values that are NaN were left out of the last units: given to the rows that see them
+              for (int token = max(w.least, w.u0 * kUnit); token < min(row_end, w.u1 * kUnit); ++token) {
+                const int id = a.tables[w.r * a.table_stride + (token >> a.shift)];
+                if (id < 0 || id >= a.pages) continue;
+                const uint8_t* v = a.v_cache + ((((size_t)id * a.kv_heads + w.head) << a.shift) + (token & ((1 << a.shift) - 1))) * D + c;
+#pragma unroll
+                for (int y = 0; y < 16; ++y)
+                  if ((v[y] & 0x7F) == 0x7F) f[y] = __int_as_float(0x7FC00000);
+              }
+            if (whole) {
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                *reinterpret_cast<uint4*>(staged(row, c / 8 + y)) = {Half<T>::narrow(f[8 * y], f[8 * y + 1]), Half<T>::narrow(f[8 * y + 2], f[8 * y + 3]),
+                                                                     Half<T>::narrow(f[8 * y + 4], f[8 * y + 5]), Half<T>::narrow(f[8 * y + 6], f[8 * y + 7])};
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                *reinterpret_cast<float4*>(part + ((c / 4 + y) * kRows + place_row) * 4) = make_float4(f[4 * y], f[4 * y + 1], f[4 * y + 2], f[4 * y + 3]);
+            }
+          }
+        }
+        if (whole) {                                       // whole lines are written: D / 8 lanes a row
+          __syncwarp();
+          const long long at = mine ? (long long)place : -1;
+#pragma unroll 4
+          for (int t = 0; t < D / 8; ++t) {
+            const int from = t * (256 / D) + lane / (D / 8), chunk = lane % (D / 8);
+            const long long to = __shfl_sync(kFullWarp, at, from);
+            const uint4 v = *reinterpret_cast<const uint4*>(staged((row & ~31) + from, chunk));
+            if (to >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + 8 * chunk) = v;
+          }
+        }
+        if (!whole && mine) {
+          part[kRows * D + place_row] = m;
+          part[kRows * D + kRows + place_row] = l;
+        }
+      }
+      __syncwarp();
+      fence_before();
+      if (w.twin) bar_arrive(smem_u32(&s.twin_done));
+      if (!whole && w.u0 == 0 && tid == 0)                 // it begins here and ends elsewhere: request, item, parts, head and place of the first
+        a.cuts[blockIdx.x] = {w.r, w.tile, 1 + (int)((w.units - w.u1 + share - 1) / share), 2 * w.head + (segment != 0)};
+    }
+    }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (count > 0) feed(std::false_type{});
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (count > 0 && warp < 14) feed(std::true_type{});
+    if (count > 0 && warp == 14) {
     // ================= products: one thread, and as few instructions between two of them as can be (24 a unit, 50 to 60 cycles each to issue)
     if (elect_one()) {
       const uint32_t idesc_s = 1u << 4 | (uint32_t)(kUnit >> 3) << 17 | (128u >> 4) << 24,
@@ -766,6 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       commit(smem_u32(&s.drained));
       for (unsigned i = 0; i < kSpinLimit && !bar_try(smem_u32(&s.drained), 0); ++i) {}
     }
+    }
   }
   __syncwarp();
   fence_before();
@@ -777,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   }
 }
 
-// Joins the parts of the tiles that were cut: a thread block per run of the launch before, a thread per row and four dimensions.
+// Joins the parts of the tiles that were cut: kJoins thread blocks per run of the launch before, a thread per row and four dimensions.
 template <typename T, int D>
 __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const AttentionArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -787,7 +816,7 @@ __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const Atte
   const Request x(a, cut.x);
   const int kvh = cut.w >> 1, rows = x.tokens(a, cut.y) * a.group;
   const float *head = a.parts + ((size_t)blockIdx.x * 2 + (cut.w & 1)) * kPartFloats<D>, *tail = a.parts + (size_t)blockIdx.x * 2 * kPartFloats<D>;
-  for (int z = threadIdx.x; z < kRows * (D / 4); z += 512) {
+  for (int z = blockIdx.y * 512 + threadIdx.x; z < kRows * (D / 4); z += kJoins * 512) {
     const int row = z % kRows, d = z / kRows;
     if (row >= rows) continue;
     float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
@@ -830,7 +859,7 @@ int run(const AttentionArgs& a, cudaStream_t st) {
   if (e) return paged_fail(e);
   const dim3 grid(device_sms());
   const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, (Layout<T, D>::kBytes), st, a);
-  return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, grid, dim3(512), 1, 0, st, a);
+  return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, dim3(grid.x, kJoins), dim3(512), 1, 0, st, a);
 }
 
 }  // namespace
