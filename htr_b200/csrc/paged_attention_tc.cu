@@ -485,6 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const bool mine = place_row < w.rows, warp_has_rows = (w.twin ? 0 : x * kTile) + 32 * (warp & 3) < w.rows;
       const size_t place = ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
       const int row_end = mine ? max(w.seen - w.n + w.tile * w.per + i + 1, 0) : 0;
+      // 16 bytes of a row as it is in memory: of queries before they are taken apart, of results where the queries were, whose products are done
+      const auto staged = [&](int row, int chunk) { return smem + Y::kQ + x * Y::kQTile + chunk / (D / 16) * Y::kPart + Y::piece(row, chunk % (D / 16)); };
       // queries: e4m3 parts under a power of two per row (of a twin: both tiles hold them)
       float row_scale;
       {
@@ -493,21 +495,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         const int first = row & ~31;                       // of this warp
         const auto row_of = [&](int t) { return 4 * t + (lane >> 3); };
         const long long at = mine ? (long long)place : -1;
-        uint4 raw[8][D / 64];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
+#pragma unroll 4
+        for (int t = 0; t < 8; ++t) {                      // all rows on their way, to where the parts will lie
           const long long from = __shfl_sync(kFullWarp, at, row_of(t));
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + max(from, 0LL)) + (lane & 7);
+          const T* src = static_cast<const T*>(a.q) + max(from, 0LL) + 8 * (lane & 7);
 #pragma unroll
-          for (int y = 0; y < D / 64; ++y) raw[t][y] = from >= 0 ? src[8 * y] : uint4{0, 0, 0, 0};
+          for (int y = 0; y < D / 64; ++y)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(staged(first + row_of(t), 8 * y + (lane & 7)))), "l"(src + 64 * y),
+                         "r"(from >= 0 ? 16 : 0) : "memory");
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         row_scale = 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 8; ++t) {
+          uint4 raw[D / 64];                               // (read by the lane that fetched it; the parts of a row go where its lanes' pieces were)
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) raw[y] = *reinterpret_cast<const uint4*>(staged(first + row_of(t), 8 * y + (lane & 7)));
+          __syncwarp();
           float f[D / 64][8], most = 0.f;
 #pragma unroll
           for (int y = 0; y < D / 64; ++y) {
-            const uint32_t w4[4] = {raw[t][y].x, raw[t][y].y, raw[t][y].z, raw[t][y].w};
+            const uint32_t w4[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
               const float2 v = Half<T>::wide(w4[z]);
@@ -660,8 +668,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const bool empty = l == 0.f;                         // a row that sees nothing: zeros
       const float by = whole && !empty ? 1.f / l : 1.f;
       const bool nan = *(volatile int*)&s.nan != 0;
-      // results wait where the queries of the same rows were, whose products are done
-      const auto staged = [&](int row, int chunk) { return smem + Y::kQ + x * Y::kQTile + chunk / (D / 16) * Y::kPart + Y::piece(row, chunk % (D / 16)); };
       if (warp_has_rows) {
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
