@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         row_scale = 0.f;
-#pragma unroll 1
+#pragma unroll 2
         for (int t = 0; t < 8; ++t) {
           uint4 raw[D / 64];                               // (read by the lane that fetched it; the parts of a row go where its lanes' pieces were)
 #pragma unroll
@@ -670,18 +670,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const bool nan = *(volatile int*)&s.nan != 0;
       if (warp_has_rows) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16];
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
           __syncwarp();
-          tmem_load16(mine_at + 128 + c, o);
-          float f[16];
+          tmem_load(mine_at + 128 + c, o);
+          tmem_loaded(o);
+          float f[32];
 #pragma unroll
-          for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : __uint_as_float(o[y]) * here * by;
+          for (int y = 0; y < 32; ++y) f[y] = empty ? 0.f : __uint_as_float(o[y]) * here * by;
           if (other) {
             __syncwarp();
-            tmem_load16(mine_at + 256 + 128 + c, o);
+            tmem_load(mine_at + 256 + 128 + c, o);
+            tmem_loaded(o);
 #pragma unroll
-            for (int y = 0; y < 16; ++y) f[y] = empty ? 0.f : fmaf(__uint_as_float(o[y]) * there, by, f[y]);
+            for (int y = 0; y < 32; ++y) f[y] = empty ? 0.f : fmaf(__uint_as_float(o[y]) * there, by, f[y]);
           }
           if (mine) {
             if (nan)                                       // values that are NaN were left out of the last units: given to the rows that see them
@@ -690,17 +692,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
                 if (id < 0 || id >= a.pages) continue;
                 const uint8_t* v = a.v_cache + ((((size_t)id * a.kv_heads + w.head) << a.shift) + (token & ((1 << a.shift) - 1))) * D + c;
 #pragma unroll
-                for (int y = 0; y < 16; ++y)
+                for (int y = 0; y < 32; ++y)
                   if ((v[y] & 0x7F) == 0x7F) f[y] = __int_as_float(0x7FC00000);
               }
             if (whole) {
 #pragma unroll
-              for (int y = 0; y < 2; ++y)
+              for (int y = 0; y < 4; ++y)
                 *reinterpret_cast<uint4*>(staged(row, c / 8 + y)) = {Half<T>::narrow(f[8 * y], f[8 * y + 1]), Half<T>::narrow(f[8 * y + 2], f[8 * y + 3]),
                                                                      Half<T>::narrow(f[8 * y + 4], f[8 * y + 5]), Half<T>::narrow(f[8 * y + 6], f[8 * y + 7])};
             } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
+              for (int y = 0; y < 8; ++y)
                 *reinterpret_cast<float4*>(part + ((c / 4 + y) * kRows + place_row) * 4) = make_float4(f[4 * y], f[4 * y + 1], f[4 * y + 2], f[4 * y + 3]);
             }
           }
