@@ -82,7 +82,7 @@ def _load():
     lib.htr_page_plan.argtypes = [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.htr_paged_append.argtypes = [vp, i32, i64, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp]
     lib.htr_paged_attention_workspace_bytes.restype = sz
-    lib.htr_paged_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
+    lib.htr_paged_attention_workspace_bytes.argtypes = [i32] * 8
     lib.htr_paged_attention.argtypes = [vp, i32, i32, vp, vp, i32, vp, i64, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, ctypes.c_float, vp, vp, vp,
                                         sz, vp]
     lib.htr_sample.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]

@@ -668,7 +668,7 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!o || !plain(*o, where, q->scalar_type()) || o->sizes() != q->sizes()) return none();
     y = *o;
   }
-  const size_t need = g_lib.paged_attention_workspace_bytes((int)T, (int)R, (int)hq, c.heads, c.dim, most);
+  const size_t need = g_lib.paged_attention_workspace_bytes((int)T, (int)R, (int)hq, c.heads, c.dim, most, (int)tables->size(1), c.page);
   if (need) work = at::detail::empty_cuda({(int64_t)need}, at::kByte, where, std::nullopt);
   if (g_lib.paged_attention(q->const_data_ptr(), dt, (int)T, starts->const_data_ptr<int>(), seen->const_data_ptr<int>(), (int)R, tables->const_data_ptr<int>(),
                             stride, (int)tables->size(1), c.k, c.v, c.ks, c.vs, c.pages, c.page, (int)hq, c.heads, c.dim, most, (float)scale, y.data_ptr(),

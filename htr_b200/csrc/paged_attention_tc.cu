@@ -90,7 +90,7 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 16 or 32 columns of this thread's lane of tensor memory
+// 32 columns of this thread's lane of tensor memory (stores: 16)
 __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
@@ -105,13 +105,6 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16])
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
                "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
-}
-__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&r)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-               "tcgen05.wait::ld.sync.aligned;"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-               : "r"(at) : "memory");
 }
 // (what was loaded goes through the wait, so that no use of it is moved before)
 __device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
@@ -874,8 +867,15 @@ int run(const AttentionArgs& a, cudaStream_t st) {
 
 namespace htr {
 
-// More than 16 rows a tile: the other kernel takes 16 of them per pass over the cache.
-bool attention_tc_serves(int requests, int group, int max_new) { return requests <= kMaxRequests && group <= kRows && (long long)group * max_new > 16; }
+// The other kernel passes over the cache once per 16 rows; this one takes up to 128 of them for the same time, but begins and joins more slowly.
+// In the long run they are level at about 48 rows of 128 dimensions and 96 of 64; and below some 1.5e9 elements of scores times dimensions (of the
+// tables' whole width: lengths are not known here) the other is ahead.  Measured, us, the other / this one: 64 requests over 2000, 2 heads of 128:
+// 32 rows 50 / 64, 64 rows 75 / 64, 128 rows 124 / 67, 256 rows 216 / 79; of 64 dimensions: 64 rows 48 / 62, 128 rows 77 / 62, 256 rows 135 / 71;
+// one request over 8000, 256 rows: 34 / 68; 9 over 5000, 1 head of 64, 72 rows: 26 / 27, 2 heads of 128, 128 rows: 52 / 46.
+bool attention_tc_serves(int tokens, int requests, int q_heads, int group, int max_new, long long width, int head_dim) {
+  return requests <= kMaxRequests && group <= kRows && (long long)group * max_new * head_dim > 6144 &&
+         (double)tokens * q_heads * (double)width * head_dim > 1.5e9;
+}
 
 size_t attention_tc_workspace(int head_dim) {
   return (size_t)device_sms() * (sizeof(int4) + 2 * sizeof(float) * (head_dim == 128 ? kPartFloats<128> : kPartFloats<64>));

@@ -99,7 +99,7 @@ __device__ __forceinline__ int query_exponent(float most) {
 }
 
 // attention for many rows a request, on the tensor cores (paged_attention_tc.cu)
-bool attention_tc_serves(int requests, int group, int max_new);
+bool attention_tc_serves(int tokens, int requests, int q_heads, int group, int max_new, long long width, int head_dim);
 size_t attention_tc_workspace(int head_dim);
 int attention_tc_run(const AttentionArgs& a, int dtype, int head_dim, void* workspace, cudaStream_t st);
 

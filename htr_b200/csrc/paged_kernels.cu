@@ -946,9 +946,9 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
   return dtype == HTR_DTYPE_BF16 ? append_of<__nv_bfloat16>(a, head_dim, grid, st) : append_of<__half>(a, head_dim, grid, st);
 }
 
-size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new) {
-  if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_new < 1 || (head_dim != 64 && head_dim != 128)) return 0;
-  if (attention_tc_serves(requests, q_heads / kv_heads, max_new)) return attention_tc_workspace(head_dim);
+size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new, int table_width, int page_size) {
+  if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_new < 1 || table_width < 1 || page_shift(page_size) < 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  if (attention_tc_serves(tokens, requests, q_heads, q_heads / kv_heads, max_new, (long long)table_width * page_size, head_dim)) return attention_tc_workspace(head_dim);
   const int tiles = attention_tiles(q_heads / kv_heads, max_new);
   const size_t rows = 8 * tiles;
   return attention_blocks(head_dim, tiles) * (2 * rows * (head_dim + 2) * sizeof(float) + sizeof(int4));
@@ -969,9 +969,10 @@ int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts,
   if (tokens == 0) return HTR_OK;
   if (!q || !starts || !seen || !tables || !k_cache || !v_cache || !k_scale || !v_scale || !out) return HTR_ERR_NULL;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return HTR_ERR_ALIGNMENT;
-  if (!workspace || workspace_bytes < htr_paged_attention_workspace_bytes(tokens, requests, q_heads, kv_heads, head_dim, max_new)) return HTR_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < htr_paged_attention_workspace_bytes(tokens, requests, q_heads, kv_heads, head_dim, max_new, table_width, page_size))
+    return HTR_ERR_WORKSPACE;
   if (!aligned16(workspace)) return HTR_ERR_ALIGNMENT;
-  const bool tc = attention_tc_serves(requests, q_heads / kv_heads, max_new);
+  const bool tc = attention_tc_serves(tokens, requests, q_heads, q_heads / kv_heads, max_new, (long long)table_width * page_size, head_dim);
   int4* cuts = static_cast<int4*>(workspace);
   const AttentionArgs a = {q, starts, seen, tables, table_stride, table_width, requests, tokens, q_heads, kv_heads, q_heads / kv_heads, max_new,
                            static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), k_scale, v_scale, pages, shift,

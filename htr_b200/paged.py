@@ -162,7 +162,7 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     [starts[r], starts[r + 1]) of request r the i-th stands at position seen[r] - n + i and sees the cached positions up to its own; one that
     sees nothing gets zeros.  max_new: at least the largest n (tokens of a request beyond it are not computed).  scale: of the scores, 1 / sqrt(head_dim) by default.
     Returns `out`, or a new tensor like q; its rows behind starts[-1] are left as they are.  A table entry that is no page hides its
-    tokens (status 32)."""
+    tokens (status 32).  Status 64: a wait inside the kernel ran out (about two seconds), and the results are not to be used."""
     what = "attention"
     y = _host.attention(q, starts, seen, tables, cache, max_new, scale, out, status)
     if y is not None:
@@ -188,7 +188,7 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     if T == 0:
         return out
     most = min(int(max_new), T)
-    need = _lib.lib.htr_paged_attention_workspace_bytes(T, R, q_heads, kv_heads, dim, most)
+    need = _lib.lib.htr_paged_attention_workspace_bytes(T, R, q_heads, kv_heads, dim, most, tables.shape[1], page)
     with torch.cuda.device(dev):
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         rc = _lib.lib.htr_paged_attention(q.data_ptr(), _HALF[q.dtype], T, starts.data_ptr(), seen.data_ptr(), R, tables.data_ptr(), stride,

@@ -325,7 +325,21 @@ def attend_exactly(q, starts, seen, tables, cache, scale):
     return out, spread
 
 
+def widened(q, tables, cache):
+    """The tables with so many more (unused) columns that many rows a request are taken to be much work: by their width, for lengths are not known on the host."""
+    page, width = cache.k.shape[2], tables.shape[1]
+    more = int(1.6e9 / (max(q.shape[0], 1) * q.shape[1] * q.shape[2] * page)) + 1 - width
+    return tables if more <= 0 else torch.cat([tables, torch.full((tables.shape[0], more), -1, dtype=torch.int32, device=tables.device)], 1)
+
+
 def check_attention(q, starts, seen, tables, cache, max_new, scale=None, **kw):
+    """By both kernels where there are many rows a request."""
+    if q.shape[1] // cache.k.shape[1] * min(max_new, q.shape[0]) * q.shape[2] > 6144:
+        check_one_attention(q, starts, seen, widened(q, tables, cache), cache, max_new, scale, **kw)
+    return check_one_attention(q, starts, seen, tables, cache, max_new, scale, **kw)
+
+
+def check_one_attention(q, starts, seen, tables, cache, max_new, scale, **kw):
     from htr_b200 import paged
 
     got = paged.attention(q, starts, seen, tables, cache, max_new, scale=scale, **kw)
@@ -380,12 +394,14 @@ def test_rows_that_see_nothing_and_rows_behind_the_last():
 
 
 @gpu
-@pytest.mark.parametrize("adds", ((3, 1), (9, 2), (100, 1)))
-def test_a_nan_reaches_only_those_that_see_it(adds):
+@pytest.mark.parametrize("adds,wide", (((3, 1), False), ((9, 2), False), ((100, 1), False), ((20, 1), True), ((100, 1), True)))
+def test_a_nan_reaches_only_those_that_see_it(adds, wide):
     """Keys and values of a step's later tokens, and all behind the last, may be NaN: earlier tokens do not see them."""
     q, starts, seen, tables, cache = filled(torch.bfloat16, 128, 16, 8, 2, (40, 17), adds)
     from htr_b200 import paged
 
+    if wide:
+        tables = widened(q, tables, cache)
     want = paged.attention(q, starts, seen, tables, cache, max(adds))
     at, n = 40 + adds[0] - 2, adds[0]                            # the last token but one of request 0
     page = int(tables[0, at // 16])
@@ -399,17 +415,52 @@ def test_a_nan_reaches_only_those_that_see_it(adds):
 
 
 @gpu
-@pytest.mark.parametrize("adds", ((1, 1), (40, 1)))
-def test_table_entries_that_are_no_page_hide_their_tokens(adds):
+@pytest.mark.parametrize("adds,wide", (((1, 1), False), ((60, 1), False), ((60, 1), True)))
+def test_table_entries_that_are_no_page_hide_their_tokens(adds, wide):
     from htr_b200 import paged
 
     q, starts, seen, tables, cache = filled(torch.bfloat16, 64, 16, 2, 1, (100, 64), adds)
+    if wide:
+        tables = widened(q, tables, cache)
     status = ints([0])
     want = paged.attention(q, starts, seen, tables, cache, max(adds), status=status).clone()
     assert int(status) == 0
     tables[0, 2], tables[1, :] = 1 << 30, -1
     got = paged.attention(q, starts, seen, tables, cache, max(adds), status=status)
     assert int(status) == 32 and torch.isfinite(got).all() and (got[int(starts[1]):] == 0).all() and not torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,hq,hkv,adds", ((128, 1, 1, (127, 128, 129)), (64, 1, 1, (255, 256, 257)), (128, 3, 1, (42, 43, 85)), (64, 6, 2, (86, 85, 1)), (128, 7, 1, (73, 19)),
+                                           (64, 256, 1, (1, 3)), (128, 200, 1, (2, 1)), (64, 300, 1, (2,)), (128, 34, 2, (4, 1))))
+def test_attention_at_the_ends_of_tiles(dtype, D, hq, hkv, adds):
+    check_attention(*filled(dtype, D, 32, hq, hkv, (70, 0, 300)[:len(adds)], adds), max_new=max(adds))
+
+
+@gpu
+@pytest.mark.parametrize("bad", (float("nan"), float("inf"), float("-inf")))
+@pytest.mark.parametrize("D,adds,wide", ((128, (2, 1), False), (64, (40, 1), False), (64, (40, 1), True), (128, (40, 1), True)))
+def test_queries_that_are_not_finite(bad, D, adds, wide):
+    """Their own rows become NaN, and no others change."""
+    from htr_b200 import paged
+
+    q, starts, seen, tables, cache = filled(torch.bfloat16, D, 16, 8, 2, (40, 17), adds)
+    if wide:
+        tables = widened(q, tables, cache)
+    want = paged.attention(q, starts, seen, tables, cache, max(adds))
+    q[1, 5, 3] = bad
+    got = paged.attention(q, starts, seen, tables, cache, max(adds))
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[1, 5] = True
+    assert torch.equal(got.isnan(), hit) and torch.equal(got[~hit], want[~hit])
+
+
+@gpu
+def test_attention_of_many_requests():
+    adds = [1] * 1100
+    adds[700], adds[3] = 90, 0
+    check_attention(*filled(torch.bfloat16, 128, 16, 1, 1, [r % 5 for r in range(1100)], adds), max_new=90)
 
 
 @gpu
@@ -436,12 +487,14 @@ def test_pages_beyond_four_gigabytes():
 
 
 @gpu
-@pytest.mark.parametrize("adds", ((1, 1, 1), (90, 1, 200)))
-def test_two_graphs_and_another_stream(adds):
+@pytest.mark.parametrize("adds,wide", (((1, 1, 1), False), ((90, 1, 200), False), ((90, 1, 200), True)))
+def test_two_graphs_and_another_stream(adds, wide):
     """Captured calls keep no buffers in common with one another or with eager ones: replayed at the same time they give what each gives alone."""
     from htr_b200 import paged
 
     sets = [filled(torch.bfloat16, 128, 16, 8, 2, have, adds, seed=s) for s, have in enumerate(((3000, 1, 50), (40, 2500, 700)))]
+    if wide:
+        sets = [(q, starts, seen, widened(q, tables, cache), cache) for q, starts, seen, tables, cache in sets]
     want = [paged.attention(*x, max(adds)).clone() for x in sets]
     graphs, outs = [], []
     for x in sets:
@@ -508,6 +561,10 @@ def test_status_codes_without_a_gpu():
     assert [attend(T=-1), attend(R=0), attend(stride=2), attend(page=17), attend(hq=5), attend(hkv=0), attend(D=32), attend(most=0)] == [-2] * 8
     assert [attend(R=8193), attend(pages=1 << 28), attend(most=1 << 30)] == [-8] * 3
     assert attend(T=0, at=None) == 0 and attend(at=None) == -5 and attend(at=24) == -6
+    assert [attend(work=None), attend(size=0), attend(work=None, T=900, most=900, stride=1 << 20, width=1 << 20),
+            attend(size=1 << 16, T=900, most=900, stride=1 << 20, width=1 << 20)] == [-4] * 4
+    need = L.htr_paged_attention_workspace_bytes
+    assert need(3, 2, 4, 2, 64, 1, 3, 16) > 0 and [need(3, 2, 4, 2, 96, 1, 3, 16), need(3, 2, 4, 2, 64, 1, 0, 16), need(3, 2, 4, 2, 64, 1, 3, 24), need(0, 2, 4, 2, 64, 1, 3, 16)] == [0] * 4
 
 
 @gpu
