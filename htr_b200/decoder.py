@@ -13,13 +13,17 @@ they run); `fused=False` evaluates the same glue with plain torch ops, which is 
 most 8 rows (decoding) fold the norms, the SwiGLU and the residual adds into the packed GEMVs themselves
 (`ops.linear_fused`) and, for a single token, the rotary embedding and cache write into the attention kernel: five launches
 per layer.  A decode step reads its position from a device tensor, so one CUDA graph captured once serves every step.
+
+Many sequences at once are served from a paged 8-bit cache (`paged.PagedCache`): `forward_paged` is one step of all of them, prompts and single
+tokens together, and `generate_batch` runs prompts of different lengths to the end, its decoding steps a CUDA graph that plans the
+pages, appends, attends and samples (`sampling.sample`) without the host.
 """
 import dataclasses
 import math
 
 import torch
 
-from . import _lib, ops, wire
+from . import _lib, ops, paged, sampling, wire
 
 
 @dataclasses.dataclass
@@ -54,9 +58,7 @@ class PackedDecoder:
         if weights is None:
             weights = self.random_weights(cfg, device, seed, dtype)
         self.layers, self.head, self.ln_f, self.embed = weights["layers"], weights["head"], weights["ln_f"], weights["embed"]
-        inv = 1.0 / (c.rope_theta ** (torch.arange(0, c.head_dim, 2).float() / c.head_dim))
-        ang = torch.arange(c.max_len).float()[:, None] * inv[None, :]
-        self.cos, self.sin = ang.cos().to(device), ang.sin().to(device)
+        self.cos, self.sin = self._angles(c.max_len)
         self.k_cache = torch.zeros(c.layers, c.max_len, c.kv_heads, c.head_dim, dtype=dtype, device=device)
         self.v_cache = torch.zeros_like(self.k_cache)
         self.arange = torch.arange(c.max_len, device=device)
@@ -184,6 +186,11 @@ class PackedDecoder:
         per_layer = (wire.payload_bytes(qkv_out, c.hidden, c.K) + wire.payload_bytes(c.hidden, c.q_heads * c.head_dim, c.K) +
                      wire.payload_bytes(2 * c.intermediate, c.hidden, c.K) + wire.payload_bytes(c.hidden, c.intermediate, c.K))
         return c.layers * per_layer + wire.payload_bytes(c.vocab, c.hidden, c.K_head)
+
+    def _angles(self, positions):
+        inv = 1.0 / (self.cfg.rope_theta ** (torch.arange(0, self.cfg.head_dim, 2).float() / self.cfg.head_dim))
+        ang = torch.arange(positions).float()[:, None] * inv[None, :]
+        return ang.cos().to(self.device), ang.sin().to(self.device)
 
     def _rope(self, t, pos):
         cos, sin = self.cos.index_select(0, pos)[:, None, :], self.sin.index_select(0, pos)[:, None, :]
@@ -344,3 +351,149 @@ class PackedDecoder:
         if int(self.status.item()):
             raise _lib.HTRError(f"a decode step used a position outside the {self.cfg.max_len}-row caches (status {int(self.status.item())})")
         return out, ev[0].elapsed_time(ev[1]) * 1e-3, ev[1].elapsed_time(ev[2]) * 1e-3
+
+    def paged_cache(self, requests, pages, page_size=64, max_len=None):
+        """A paged cache for this model: `pages` pages of `page_size` tokens shared by `requests` sequences of at most max_len tokens (as many as the
+        pages hold by default; not bound by cfg.max_len)."""
+        max_len = pages * page_size if max_len is None else max_len
+        cache = paged.PagedCache(self.cfg.layers, self.cfg.kv_heads, self.cfg.head_dim, pages, page_size, requests, max_len, self.device)
+        cache.cos, cache.sin = self._angles(cache.tables.shape[1] * page_size)
+        return cache
+
+    def forward_paged(self, ids, plan, cache, max_new):
+        """One step of many sequences: ids [tokens] in the order of `plan` (what cache.plan(new, tokens) returned; entries behind the last token are any
+        ids), max_new: at least the most tokens that a request adds.  Appends keys and values to `cache` (of `paged_cache`) and returns logits
+        [requests, vocab] of each request's last token; the row of a request that adds none holds no result.  No host synchronisation: a step of
+        fixed sizes can be captured into a CUDA graph.  Errors of the requests set bits of cache.status."""
+        c, L_ = self.cfg, _lib.lib
+        T = ids.shape[0]
+        if T < 1 or cache.cos is None:
+            raise _lib.HTRError("forward_paged: wants at least one token and a cache of paged_cache")
+        kernels = self.fused and self.dtype == torch.bfloat16
+        fold = kernels and self.fold and T <= ops.GEMV_MAX_M
+        x = self.embed.index_select(0, ids)                     # residual stream
+        att = torch.zeros(T, c.q_heads, c.head_dim, dtype=self.dtype, device=self.device)      # rows behind the last token stay zero
+        flat = att.view(T, c.q_heads * c.head_dim)
+        st = torch.cuda.current_stream(self.device).cuda_stream
+        delta = None                                            # what the residual stream has still to get
+
+        def normed(x, delta, weight):                           # of x + delta; x gets it in place
+            if not kernels:
+                if delta is not None:
+                    x += delta
+                return _rms_norm(x, weight, c.eps)
+            h = torch.empty_like(x)
+            _lib.check(L_.htr_dec_add_rmsnorm(x.data_ptr(), None if delta is None else delta.data_ptr(), weight.data_ptr(), h.data_ptr(), x.shape[0], c.hidden,
+                                              c.eps, st), "htr_dec_add_rmsnorm")
+            return h
+
+        for li, L in enumerate(self.layers):
+            if fold:
+                qkv = ops.linear_fused(x, *L["qkv"], prologue=ops.PROLOGUE_RMSNORM, norm_weight=L["ln1"], eps=c.eps)
+            else:
+                qkv = ops.linear(normed(x, delta, L["ln1"]), *L["qkv"])
+            layer = cache.layer(li)
+            q = paged.rope_append(qkv, plan.positions, plan.slots, cache.cos, cache.sin, layer, c.q_heads, status=cache.status)
+            paged.attention(q, plan.starts, plan.seen, cache.tables, layer, max_new, out=att, status=cache.status)
+            if fold:
+                ops.linear_fused(flat, *L["o"], out=x, residual=True)
+                gu = ops.linear_fused(x, *L["gate_up"], prologue=ops.PROLOGUE_RMSNORM, norm_weight=L["ln2"], eps=c.eps)
+                ops.linear_fused(gu, *L["down"], out=x, prologue=ops.PROLOGUE_SWIGLU, residual=True)
+                continue
+            gu = ops.linear(normed(x, ops.linear(flat, *L["o"]), L["ln2"]), *L["gate_up"])
+            if kernels:
+                act = torch.empty(T, c.intermediate, dtype=self.dtype, device=self.device)
+                _lib.check(L_.htr_dec_swiglu(gu.data_ptr(), act.data_ptr(), T, c.intermediate, st), "htr_dec_swiglu")
+            else:
+                act = torch.nn.functional.silu(gu[:, :c.intermediate]) * gu[:, c.intermediate:]
+            delta = ops.linear(act, *L["down"])
+        last = (plan.starts[1:] - 1).clamp_(0, T - 1)
+        x = x.index_select(0, last)
+        if fold and last.numel() <= ops.GEMV_MAX_M:
+            return ops.linear_fused(x, *self.head, prologue=ops.PROLOGUE_RMSNORM, norm_weight=self.ln_f, eps=c.eps)
+        return ops.linear(normed(x, None if delta is None else delta.index_select(0, last), self.ln_f), *self.head)
+
+    @torch.no_grad()
+    def generate_batch(self, prompts, new_tokens, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0, eos=None, chunk=4096, page_size=64, cache=None,
+                       use_graph=True):
+        """Continues all `prompts` (1-D tensors of ids, each at least one) by new_tokens tokens, or up to and with `eos`.
+
+        The settings of `sampling.sample` are one for all or one per prompt (temperature 0: greedy).  Prompts go through in steps of at most `chunk`
+        tokens, and then one token of each sequence a step (one CUDA graph).  `cache`: one of `paged_cache` with no sequence in it, and room for as
+        many as there are prompts; its pages come back at the end.  Returns (tokens [prompts, new_tokens], -1 behind an eos; their log-probabilities)."""
+        dev, R = self.device, len(prompts)
+        lens = [int(p.numel()) for p in prompts]
+        if min(lens, default=0) < 1 or new_tokens < 1 or chunk < 1:
+            raise _lib.HTRError("generate_batch: wants at least one prompt of at least one token, new_tokens >= 1 and chunk >= 1")
+        if cache is None:
+            cache = self.paged_cache(R, sum(-(-(n + new_tokens) // page_size) for n in lens), page_size, max(lens) + new_tokens)
+        elif cache.lengths.numel() != R or cache.cos is None or int(cache.lengths.max()) > 0:
+            raise _lib.HTRError(f"generate_batch: the cache must be one of paged_cache for {R} requests, with none in it")
+        flat = [torch.as_tensor(p, dtype=torch.long).reshape(-1).to(dev) for p in prompts]
+        every = torch.cat(flat)
+        if int(every.min()) < 0 or int(every.max()) >= self.embed.shape[0]:
+            raise _lib.HTRError(f"generate_batch: token ids must lie in [0, {self.embed.shape[0]})")
+
+        def setting(v, dtype):
+            v = torch.as_tensor(v, dtype=dtype).to(dev)
+            if v.dim() and tuple(v.shape) != (R,):
+                raise _lib.HTRError(f"generate_batch: settings are one number, or one for each of the {R} prompts")
+            return v.expand(R).contiguous()
+
+        how = dict(temperature=setting(temperature, torch.float32), top_k=setting(top_k, torch.int32), top_p=setting(top_p, torch.float32),
+                   min_p=setting(min_p, torch.float32))
+        u = torch.rand(new_tokens, R, generator=torch.Generator().manual_seed(seed)).to(dev)
+        tokens = torch.full((new_tokens, R), -1, dtype=torch.long, device=dev)
+        logprobs = torch.zeros(new_tokens, R, dtype=torch.float32, device=dev)
+        cur = torch.zeros(R, dtype=torch.long, device=dev)      # what each sequence adds next
+        over = torch.zeros(R, dtype=torch.bool, device=dev)
+        at = torch.zeros(1, dtype=torch.long, device=dev)       # step of the decoding
+
+        def choose(logits, which):
+            """The next token of the requests `which`."""
+            token, logprob = sampling.sample(logits, u.index_select(0, at)[0], **how)
+            chosen = which & ~over
+            for rows, value, none in ((tokens, token, -1), (logprobs, logprob, 0.0)):
+                rows.index_copy_(0, at, torch.where(chosen, value, torch.where(which, none, rows.index_select(0, at)[0]))[None])
+            cur.copy_(torch.where(chosen & (token >= 0), token, cur))
+            over.logical_or_(chosen & ((token < 0) if eos is None else ((token == eos) | (token < 0))))
+
+        done = [0] * R
+        while done != lens:
+            new, room = [0] * R, chunk
+            for r in range(R):
+                new[r] = min(lens[r] - done[r], room)
+                room -= new[r]
+            plan = cache.plan(torch.tensor(new, dtype=torch.int32, device=dev), sum(new))
+            ids = torch.cat([p[d:d + n] for p, d, n in zip(flat, done, new)])
+            logits = self.forward_paged(ids, plan, cache, max(new))
+            done = [d + n for d, n in zip(done, new)]
+            choose(logits, torch.tensor([n > 0 and d == l for n, d, l in zip(new, done, lens)], device=dev))
+        everyone = torch.ones(R, dtype=torch.bool, device=dev)
+        rows = torch.arange(R, dtype=torch.int32, device=dev)
+
+        def step():
+            plan = cache.plan(torch.where(over, -1, 1).int(), R)
+            request = torch.searchsorted(plan.starts[1:], rows, right=True).clamp_(max=R - 1)       # whose token a row is
+            logits = self.forward_paged(cur.index_select(0, request), plan, cache, 1)
+            at.add_(1)
+            choose(logits, everyone)
+
+        left = new_tokens - 1
+        if use_graph and left > 2:
+            step()                                              # (also makes what a capture may not)
+            torch.cuda.synchronize(dev)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+            for _ in range(left - 1):
+                graph.replay()
+        else:
+            for _ in range(left):
+                step()
+        cache.plan(torch.full((R,), -1, dtype=torch.int32, device=dev), 0)
+        status = int(cache.status.item())
+        if status:
+            cache.status.zero_()
+            raise _lib.HTRError(f"generate_batch: a request could not be served (status {status}; 1: no pages left, 2: its table is full)")
+        return tokens.t().contiguous(), logprobs.t().contiguous()

@@ -219,6 +219,7 @@ class PagedCache:
         self.free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device)       # page 0 is taken first
         self.count = torch.full((1,), pages, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.cos = self.sin = None                            # angles of the positions, where a model lays them out (PackedDecoder.paged_cache)
 
     def layer(self, i):
         return LayerCache(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i])
