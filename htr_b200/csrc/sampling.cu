@@ -60,6 +60,8 @@ struct Logit {
     const __half2 h = *reinterpret_cast<const __half2*>(&w);
     return j & 1 ? __high2float(h) : __low2float(h);
   }
+  // bf16: upper halves of the keys of two logits (of -0: 32767)
+  static __device__ __forceinline__ uint32_t two_keys(uint32_t w) { return w ^ ((w >> 15 & 0x00010001u) * 0xFFFFu | 0x80008000u); }
   // the largest of a vector, NaN left aside
   static __device__ __forceinline__ float largest(const uint4& v) {
     if constexpr (DT == HTR_DTYPE_F32) {
@@ -141,8 +143,8 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
 
 template <int DT>
 struct Shared {
-  u64 known[DT == HTR_DTYPE_BF16 ? 2 * kBins : 2];
-  unsigned count[kBins], lo[kBins], hi[kBins];             // of a range of keys: tokens, and their weight in two words
+  u64 known[DT == HTR_DTYPE_BF16 ? 2 * kBins + 2 : 2];
+  unsigned count[2 * kBins], lo[kBins];                    // of a range of keys: tokens, and their weight in two words (the upper from kBins on)
   u64 red[2][kWarps], ahead[2][kWarps];                    // of the warps: what each has, and what those before it have
   double table[64];
   u64 mail[2][4];                                          // what the thread blocks of a cluster tell one another, in turns
@@ -263,10 +265,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
         const uint32_t from = b < kBins ? top_key : kNegative, step = (uint32_t)(b & (kBins - 1)) << 16;
         s.known[b] = from > step ? weigh.computed(from - step) : 0;
       }
+      if (tid == 0) s.known[2 * kBins] = 0;
       weigh.known = s.known;
       __syncthreads();
     }
   }
+  // bf16 whose values have a place in s.known by a subtraction (zero lies below the first 2048, and nothing is infinite): without a branch per logit
+  const bool quick = weigh.known && !weigh.infinite && (top_key >> 16) - 0x8000u >= (uint32_t)kBins;
+  const auto place_of = [&](uint32_t half) {               // 2 * kBins: none
+    const uint32_t d = (top_key >> 16) - half, e = (kNegative >> 16) - half;
+    return d < (uint32_t)kBins ? d : (uint32_t)kBins + min(e, (uint32_t)kBins);
+  };
+  const auto half_of = [&](const uint4& w, int j) {
+    const uint32_t y = L::two_keys(j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w);
+    return j & 1 ? y >> 16 : y & 0xFFFFu;
+  };
+  const auto real_half = [](uint32_t half) { return half - 0x80u <= 0xFF80u - 0x80u; };       // neither NaN nor -infinity
   // ---- the border: keys above `high` are kept, and of the `tied` tokens in [low, high], which are all equal, the first `ties`
   uint32_t low = 0, high = 0;
   unsigned ties = 0xFFFFFFFFu, tied = 0;
@@ -277,16 +291,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     uint32_t hi = top_key, lo = 0;
     for (bool first = true;; first = false) {
       if (first) {                                         // 16-bit logits: as many values as there are bins
-        lo = L::kGap ? (hi > (uint32_t)(kBins - 1) << L::kGap ? hi - ((uint32_t)(kBins - 1) << L::kGap) : 0)
+        // (what is counted is few, and lies within two binades as a rule: the more values, the more tokens to count)
+        const uint32_t values = counts && L::kGap == 16 ? 255 : kBins - 1;
+        lo = L::kGap ? (hi > values << L::kGap ? hi - (values << L::kGap) : 0)
                      : key_of((float)(weigh.max - 12.0 * (double)t));
         lo = max(weigh.infinite ? hi : lo, low);
       }
       const int shift = max(21 - __clz(hi - lo), 0);       // at most kBins bins
       const bool single = L::kGap && shift <= L::kGap;     // bins are single values
       const bool sums = first && !counts;                  // the weight of all is needed
-      const bool below = sums && L::kGap == 16;            // the negative values from -2^-8 to -2^8 have bins too, in s.hi
+      const bool below = sums && L::kGap == 16;            // the negative values from -2^-8 to -2^8 have bins too, behind the others
       for (int b = tid; b < kBins; b += kThreads) {
-        s.count[b] = s.hi[b] = 0;
+        s.count[b] = s.count[kBins + b] = 0;
         if (!single) s.lo[b] = 0;
       }
       __syncthreads();
@@ -296,6 +312,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       for (int x = tid; x < vectors; x += kThreads) {
         const uint4 w = fetch(x);
         if (!(L::largest(w) >= from)) continue;
+        if (below && single && quick) {
+          unsigned odd = 0;                                // logits without a place
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const uint32_t half = half_of(w, j), at = place_of(half);
+            if (at < 2u * kBins) atomicAdd(&s.count[at], 1u);
+            else if (real_half(half)) odd |= 1u << j;
+          }
+          for (; odd; odd &= odd - 1) rest += weigh.computed(key_of(L::at(w, __ffs(odd) - 1)));
+          continue;
+        }
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
           const uint32_t key = key_of(L::at(w, j));
@@ -306,9 +333,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
             if (counts || single) continue;
             const u64 v = weigh(key);
             const unsigned y = (unsigned)v, was = atomicAdd(&s.lo[b], y), z = (unsigned)(v >> 32) + (was + y < y);
-            if (z) atomicAdd(&s.hi[b], z);
+            if (z) atomicAdd(&s.count[kBins + b], z);
           } else if (below && single && kNegative - key < (uint32_t)kBins << 16) {
-            atomicAdd(&s.hi[(kNegative - key) >> 16], 1u);
+            atomicAdd(&s.count[kBins + ((kNegative - key) >> 16)], 1u);
           } else {
             rest += weigh(key);
           }
@@ -332,9 +359,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
               tokens[j] += remote(&s.count[b], c);
               if (counts) continue;
               if (single) {
-                if (below) more += remote(&s.hi[b], c);
+                if (below) more += remote(&s.count[kBins + b], c);
               } else {
-                mass += ((u64)remote(&s.hi[b], c) << 32) + remote(&s.lo[b], c);
+                mass += ((u64)remote(&s.count[kBins + b], c) << 32) + remote(&s.lo[b], c);
               }
             }
           if (single && !counts) {
@@ -428,11 +455,38 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     each = weigh(L::only(low, high));
     if (each < bound) each = 0;
   }
+  if (quick && bound) {                                    // (min-p: from here on what lies below it weighs nothing)
+    for (int b = tid; b < 2 * kBins; b += kThreads)
+      if (s.known[b] < bound) s.known[b] = 0;
+    __syncthreads();
+  }
+  const uint32_t tie = tied ? L::only(low, high) >> 16 : 0, tie_placed = quick && place_of(tie) < 2u * kBins ? tie : 0x10000u;
   // of a lane's vector: the weight of what lies above the border, and how many ties there are
   const auto weight_of = [&](const uint4& w, unsigned& here) {
     u64 sum = 0;
     here = 0;
     if (!(L::largest(w) >= from)) return sum;
+    if (quick) {
+      unsigned odd = 0;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const uint32_t half = half_of(w, j), at = place_of(half);
+        sum += s.known[half > tie ? at : 2 * kBins];
+        here += half == tie_placed;
+        if (at == 2u * kBins && real_half(half)) odd |= 1u << j;
+      }
+      for (; odd; odd &= odd - 1) {
+        const uint32_t key = key_of(L::at(w, __ffs(odd) - 1));
+        if (key < low) continue;
+        if (key <= high) {
+          ++here;
+          continue;
+        }
+        const u64 v = weigh.computed(key);
+        if (v >= bound) sum += v;
+      }
+      return sum;
+    }
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const uint32_t key = key_of(L::at(w, j));
