@@ -272,15 +272,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
   }
   // bf16 whose values have a place in s.known by a subtraction (zero lies below the first 2048, and nothing is infinite): without a branch per logit
   const bool quick = weigh.known && !weigh.infinite && (top_key >> 16) - 0x8000u >= (uint32_t)kBins;
-  const auto place_of = [&](uint32_t half) {               // 2 * kBins: none
-    const uint32_t d = (top_key >> 16) - half, e = (kNegative >> 16) - half;
-    return d < (uint32_t)kBins ? d : (uint32_t)kBins + min(e, (uint32_t)kBins);
+  const uint32_t top_half = top_key >> 16, real = top_half - 0x7Fu;       // (0x7F: of -infinity)
+  const auto place_of = [&](uint32_t half, bool& odd) {    // 2 * kBins: none; odd: and it is neither NaN nor -infinity
+    const uint32_t d = top_half - half, e = (kNegative >> 16) - half, at = d < (uint32_t)kBins ? d : (uint32_t)kBins + min(e, (uint32_t)kBins);
+    odd = d < real && at == 2u * kBins;
+    return at;
   };
   const auto half_of = [&](const uint4& w, int j) {
     const uint32_t y = L::two_keys(j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w);
     return j & 1 ? y >> 16 : y & 0xFFFFu;
   };
-  const auto real_half = [](uint32_t half) { return half - 0x80u <= 0xFF80u - 0x80u; };       // neither NaN nor -infinity
   // ---- the border: keys above `high` are kept, and of the `tied` tokens in [low, high], which are all equal, the first `ties`
   uint32_t low = 0, high = 0;
   unsigned ties = 0xFFFFFFFFu, tied = 0;
@@ -316,9 +317,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
           unsigned odd = 0;                                // logits without a place
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
-            const uint32_t half = half_of(w, j), at = place_of(half);
+            bool is;
+            const uint32_t at = place_of(half_of(w, j), is);
             if (at < 2u * kBins) atomicAdd(&s.count[at], 1u);
-            else if (real_half(half)) odd |= 1u << j;
+            if (is) odd |= 1u << j;
           }
           for (; odd; odd &= odd - 1) rest += weigh.computed(key_of(L::at(w, __ffs(odd) - 1)));
           continue;
@@ -455,12 +457,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     each = weigh(L::only(low, high));
     if (each < bound) each = 0;
   }
-  if (quick && bound) {                                    // (min-p: from here on what lies below it weighs nothing)
-    for (int b = tid; b < 2 * kBins; b += kThreads)
-      if (s.known[b] < bound) s.known[b] = 0;
+  // from here on what is not kept weighs nothing, and ties are counted
+  const uint32_t tie = tied ? L::only(low, high) >> 16 : 0;
+  if (quick && (tied || bound)) {
+    __syncthreads();
+    for (int b = tid; b < 2 * kBins; b += kThreads) {
+      const uint32_t half = (b < kBins ? top_half : kNegative >> 16) - (b & (kBins - 1));
+      if (half <= tie || s.known[b] < bound) s.known[b] = 0;
+    }
     __syncthreads();
   }
-  const uint32_t tie = tied ? L::only(low, high) >> 16 : 0, tie_placed = quick && place_of(tie) < 2u * kBins ? tie : 0x10000u;
   // of a lane's vector: the weight of what lies above the border, and how many ties there are
   const auto weight_of = [&](const uint4& w, unsigned& here) {
     u64 sum = 0;
@@ -470,10 +476,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       unsigned odd = 0;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const uint32_t half = half_of(w, j), at = place_of(half);
-        sum += s.known[half > tie ? at : 2 * kBins];
-        here += half == tie_placed;
-        if (at == 2u * kBins && real_half(half)) odd |= 1u << j;
+        bool is;
+        sum += s.known[place_of(half_of(w, j), is)];
+        if (is) odd |= 1u << j;
+      }
+      if (tied) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) here += half_of(w, j) == tie && !(odd >> j & 1);
       }
       for (; odd; odd &= odd - 1) {
         const uint32_t key = key_of(L::at(w, __ffs(odd) - 1));
@@ -561,8 +570,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
         for (int j = 0; j < kVec && run <= target; ++j) {
           const uint32_t key = key_of(L::at(w, j));
           if (key == 0 || key < low || (key <= high && tie++ >= mine_room)) continue;
-          const u64 v = weigh(key);
-          if (v < bound) continue;
+          const u64 v = key <= high ? each : weigh(key);
+          if (v < bound || v == 0) continue;
           run += v;
           if (run <= target) continue;
           a.tokens[r] = begin + x * kVec + j;
