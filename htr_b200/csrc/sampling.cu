@@ -76,6 +76,16 @@ struct Logit {
       return fmaxf(f.x, f.y);
     }
   }
+  // bf16: which of a vector's logits are at least `from` (bit i: the lower of word i, 16 + i: the upper), and the logit of a bit
+  static __device__ __forceinline__ unsigned at_least(const uint4& v, float from) {
+    const uint32_t half = __float_as_uint(from) >> 16, pair = half << 16 | half;              // (what is cut off lies between two logits)
+    const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&pair), *w = reinterpret_cast<const __nv_bfloat162*>(&v);
+    return (__hge2_mask(w[0], f) & 0x00010001u) | (__hge2_mask(w[1], f) & 0x00020002u) | (__hge2_mask(w[2], f) & 0x00040004u) | (__hge2_mask(w[3], f) & 0x00080008u);
+  }
+  static __device__ __forceinline__ float of_bit(const uint4& v, int bit) {
+    const uint32_t w = bit & 2 ? (bit & 1 ? v.w : v.z) : (bit & 1 ? v.y : v.x);
+    return __uint_as_float(bit & 16 ? w & 0xFFFF0000u : w << 16);
+  }
   // the key in [low, high], of which there is one: logits of 16 bits end in zeros, keys of negative ones in ones
   static __device__ __forceinline__ uint32_t only(uint32_t low, uint32_t high) {
     const uint32_t rest = (1u << kGap) - 1, positive = high & ~rest;
@@ -149,6 +159,7 @@ struct Shared {
   double table[64];
   u64 mail[2][4];                                          // what the thread blocks of a cluster tell one another, in turns
   u64 told[4];                                             // what its first warp tells a thread block
+  u64 won[4];                                              // what lies before the warp that holds the token, the ties left there, and its part
 };
 
 template <typename V>
@@ -223,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     most = fmaxf(most, L::largest(w));
   }
   if (tid < 64) s.table[tid] = exp2(tid / 64.0);
-  if (tid == 64) s.mail[0][3] = s.mail[1][3] = 0;
+  if (tid == 64) s.mail[0][3] = s.mail[1][3] = s.won[2] = 0;
   // of all threads of the cluster: the largest of a 32-bit value
   const auto largest_of = [&](uint32_t v) {
     v = __reduce_max_sync(htr::kFullWarp, v);
@@ -325,14 +336,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
           for (; odd; odd &= odd - 1) rest += weigh.computed(key_of(L::at(w, __ffs(odd) - 1)));
           continue;
         }
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const uint32_t key = key_of(L::at(w, j));
-          if (key > hi || key < from_key || key == 0) continue;
+        const auto take = [&](uint32_t key) {
+          if (key > hi || key < from_key || key == 0) return;
           if (key >= lo) {
             const int b = (hi - key) >> shift;
             atomicAdd(&s.count[b], 1u);
-            if (counts || single) continue;
+            if (counts || single) return;
             const u64 v = weigh(key);
             const unsigned y = (unsigned)v, was = atomicAdd(&s.lo[b], y), z = (unsigned)(v >> 32) + (was + y < y);
             if (z) atomicAdd(&s.count[kBins + b], z);
@@ -341,6 +350,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
           } else {
             rest += weigh(key);
           }
+        };
+        if constexpr (L::kGap == 16) {                     // few, as a rule
+          for (unsigned some = L::at_least(w, from); some; some &= some - 1) take(key_of(L::of_bit(w, __ffs(some) - 1)));
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) take(key_of(L::at(w, j)));
         }
       }
       barrier();
@@ -496,16 +511,20 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       }
       return sum;
     }
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const uint32_t key = key_of(L::at(w, j));
-      if (key == 0 || key < low) continue;
+    const auto take = [&](uint32_t key) {
+      if (key == 0 || key < low) return;
       if (key <= high) {
         ++here;
-        continue;
+        return;
       }
       const u64 v = weigh(key);
       if (v >= bound) sum += v;
+    };
+    if constexpr (L::kGap == 16) {
+      for (unsigned some = L::at_least(w, from); some; some &= some - 1) take(key_of(L::of_bit(w, __ffs(some) - 1)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) take(key_of(L::at(w, j)));
     }
     return sum;
   };
@@ -549,43 +568,50 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
   u64 before = s.told[0] + s.ahead[0][warp] + each * min(ahead, (u64)ties);
   u64 room = ties > ahead ? ties - ahead : 0;              // ties of this warp and of later ones that are kept
   mine += each * min((u64)mine_tied, room);
-  // the warp that holds the token
-  for (int base = before <= target && target < before + mine ? first : last; base < last; base += 32) {
-    const int x = base + lane;
+  // the warp that holds the token: its part, 32 vectors at a time, by all warps (32 times at most: a thread block has 2^17 logits at most)
+  if (lane == 0 && before <= target && target < before + mine) {
+    s.won[0] = before;
+    s.won[1] = room;
+    s.won[2] = (u64)first << 32 | (unsigned)last;
+  }
+  __syncthreads();
+  if (s.won[2]) {
+    const int x = (int)(s.won[2] >> 32) + tid, end_of = (int)(unsigned)s.won[2];
     unsigned here = 0;
     uint4 w = {};
     u64 sum = 0;
-    if (x < last) {
+    if (x < end_of) {
       w = fetch(x);
       sum = weight_of(w, here);
     }
-    const u64 passed = warp_scan(here, lane), mine_room = room > passed - here ? room - (passed - here) : 0;
-    sum += each * min((u64)here, mine_room);
-    const u64 end = before + warp_scan(sum, lane);
-    const unsigned hit = __ballot_sync(htr::kFullWarp, end > target);
-    if (hit) {
-      u64 run = end - sum, tie = 0;
-      if (lane == __ffs(hit) - 1) {
+    const unsigned passed = (unsigned)warp_scan(here, lane);
+    const u64 run_of = warp_scan(sum, lane);               // (without ties)
+    if (lane == 31) {
+      s.red[0][warp] = run_of;
+      s.red[1][warp] = passed;
+    }
+    __syncthreads();
+    const u64 earlier = warp_sum(lane < warp ? s.red[0][lane] : 0), ties_before = warp_sum(lane < warp ? s.red[1][lane] : 0) + passed - here;
+    room = s.won[1];
+    const u64 mine_room = room > ties_before ? room - ties_before : 0;
+    u64 run = s.won[0] + earlier + run_of - sum + each * min(ties_before, room);
+    if (run <= target && target < run + sum + each * min((u64)here, mine_room)) {
+      u64 tie_at = 0;
 #pragma unroll 1
-        for (int j = 0; j < kVec && run <= target; ++j) {
-          const uint32_t key = key_of(L::at(w, j));
-          if (key == 0 || key < low || (key <= high && tie++ >= mine_room)) continue;
-          const u64 v = key <= high ? each : weigh(key);
-          if (v < bound || v == 0) continue;
-          run += v;
-          if (run <= target) continue;
-          a.tokens[r] = begin + x * kVec + j;
-          if (a.logprobs) {
-            const double d = (double)logit_of(key);
-            a.logprobs[r] = (float)((d == weigh.max ? 0.0 : (d - weigh.max) / (double)t) - log((double)total / kOne));
-          }
+      for (int j = 0; j < kVec && run <= target; ++j) {
+        const uint32_t key = key_of(L::at(w, j));
+        if (key == 0 || key < low || (key <= high && tie_at++ >= mine_room)) continue;
+        const u64 v = key <= high ? each : weigh(key);
+        if (v < bound || v == 0) continue;
+        run += v;
+        if (run <= target) continue;
+        a.tokens[r] = begin + x * kVec + j;
+        if (a.logprobs) {
+          const double d = (double)logit_of(key);
+          a.logprobs[r] = (float)((d == weigh.max ? 0.0 : (d - weigh.max) / (double)t) - log((double)total / kOne));
         }
       }
-      break;
     }
-    before = __shfl_sync(htr::kFullWarp, end, 31);
-    const u64 gone = __shfl_sync(htr::kFullWarp, passed, 31);
-    room = room > gone ? room - gone : 0;
   }
   if (size > 1) htr::cluster_wait();
 }
