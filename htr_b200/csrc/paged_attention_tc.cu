@@ -31,7 +31,6 @@ using namespace htr;
 constexpr int kThreads = 512, kTile = 128, kRows = 256, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024;
 constexpr int kTmemColumns = 512;                          // of a tile: S (P over it) at 0 and 64, O at 128
 constexpr int kRing = 4, kScales = 8;                      // units of keys and of values in shared memory; of their scales, read by all rows
-constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
 
 template <typename T, int D>
 struct Layout {                                            // bytes of the operands
@@ -45,30 +44,9 @@ struct Layout {                                            // bytes of the opera
   static __device__ __forceinline__ int value(int token, int chunk) { return (chunk >> 3) * (kUnit * 128) + token * 128 + (((chunk & 7) ^ (token & 7)) << 4); }
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // start; distances of 128-byte columns (where rows are longer) and of groups of 8 rows, in 16 bytes; version 1; swizzle of 128 bytes (2) or 64 (4)
 __device__ __forceinline__ uint64_t descriptor(uint32_t at, int next_column, int next_rows, uint64_t swizzle) {
   return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)(next_column >> 4) << 16 | (uint64_t)(next_rows >> 4) << 32 | 1ull << 46 | swizzle << 61;
-}
-__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
-               : "=r"(done) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
-  return done != 0;
-}
-// bounded: false when the limit ran out or another role has given up
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* fail) {
-  if (bar_try(bar, parity)) return true;
-  for (unsigned i = 0; i < kSpinLimit; ++i) {
-    if (bar_try(bar, parity)) return true;
-    if ((i & 255) == 255 && *fail) return false;
-  }
-  *fail = 1;
-  return false;
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t is;
@@ -810,8 +788,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
 // Joins the parts of the tiles that were cut: kJoins thread blocks per run of the launch before, a thread per row and four dimensions.
 template <typename T, int D>
 __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const AttentionArgs a) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int4 cut = a.cuts[blockIdx.x];
   if (cut.z == 0) return;
   const Request x(a, cut.x);

@@ -78,6 +78,36 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 constexpr float kNone = -__builtin_huge_valf();
 
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+  return done != 0;
+}
+constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
+// bounded: false when the limit ran out or another has given up
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* fail) {
+  if (bar_try(bar, parity)) return true;
+  for (unsigned i = 0; i < kSpinLimit; ++i) {
+    if (bar_try(bar, parity)) return true;
+    if ((i & 255) == 255 && fail && *fail) return false;
+  }
+  if (fail) *fail = 1;
+  return false;
+}
+// contiguous bytes (both addresses and the size multiples of 16) to shared memory
+__device__ __forceinline__ void bulk_load(uint32_t to, const void* from, int bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+
 struct AttentionArgs {
   const void* q;
   const int *starts, *seen, *tables;

@@ -418,15 +418,19 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
 //
 // What bounds it for single tokens: the cache's bytes.  The query heads of one key/value head and a request's tokens of this step are the
 // rows of one product, 8 or 16 at a time (row = token * group + head), on warp-level matrix instructions m16n8k16 with the cache as the
-// 16-row operand (S^T = K Q^T, O^T = V^T P^T), so that 8 rows fill a tile.  A warp takes 16 cached tokens at a time for itself alone, with
-// the next 16 in flight in its registers.  The dimensions that a product sums over and the rows of a result may be taken in any order, so
-// every lane (g = lane / 4, c = lane % 4) loads whole 16-byte pieces of the cache's rows straight into fragments: of K those of the tokens g
+// 16-row operand (S^T = K Q^T, O^T = V^T P^T), so that 8 rows fill a tile.  A warp takes 16 cached tokens at a time for itself alone.  The dimensions that a product sums over and the rows of a result may be taken in any order, so
+// every lane (g = lane / 4, c = lane % 4) reads whole 16-byte pieces of the cache's rows straight into fragments: of K those of the tokens g
 // and g + 8 at dimensions 16 c ..., of V those of the tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 at dimensions 16 g ...; e4m3 becomes fp16, which
-// holds it exactly, on the way.  No shared memory, no barrier until a warp's tokens are through.
+// holds it exactly, on the way.  The tiles come through a ring of four per warp in shared memory, two bulk copies each, so that up to 190 KB
+// are on their way to an SM; no barrier until a warp's tokens are through.
 //
 // The work is cut evenly, whatever the requests' lengths: a flat list of units of 64 tokens (of every request, row tile and key/value
-// head) in equal runs over the thread blocks.  A tile that lies in one run is finished there; of a tile that is cut every thread
-// block leaves its part (maximum, sum, result) in the workspace, and a second launch joins them in the order of the tokens.
+// head, each with kBegin units more for what its beginning and end cost) in equal runs over the thread blocks.  A tile that lies in one run is finished
+// there; of a tile that is cut every thread block leaves its part (maximum, sum, result) in the workspace, and a second launch joins them in the
+// order of the tokens.
+//
+// 64 requests of 10 to 16384 tokens, 32 heads of 128 on 8 (759 MB): 128 us, 5.9 TB/s.  With tiles in registers 172; with bank conflicts among the pieces of V 162;
+// in runs that count units alone 171; rows of V apart, by a copy for every two, 165.
 //
 // Queries are fp16 under a power of two per row (bf16 keeps all its bits: 29 binades of normal fp16 below the row's largest element).
 // Probabilities are rounded to fp16, relative to the contribution that they make: the scale of the values' page is part of the exponent
@@ -444,9 +448,13 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8x8 matrix 
   return r;
 }
 constexpr int kAttWarps = 4, kAttThreads = kAttWarps * 32, kUnit = kAttWarps * 16;   // tokens of a unit
-// thread blocks per SM, by the registers that the tiles in flight and the results need
+// thread blocks per SM, by the registers that results and a tile need without spills (128 dimensions, 8 rows: four blocks instead of three 161 us, not 150,
+// at decode_64's sizes below)
 template <int D, int NT>
 constexpr int kAttBlocks = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
+constexpr int kDepth = 4;                                  // stages of a warp's ring
+template <int D>
+constexpr int kRingBytes = kDepth * 32 * D;                // of a warp
 
 // a row of queries as the right operand: fragments of rows g + 8 * tile, their scale (times that of the scores), for this lane's rows 2 c, 2 c + 1
 template <typename T, int D, int NT>
@@ -491,39 +499,38 @@ struct Rows {
   }
 };
 
-// what a warp has in flight: 16 tokens of keys and values of one page
+// 16 tokens of keys and values of one page
 template <int D>
 struct Tile {
   uint4 k[2][D / 64];
   uint32_t v[4][D / 32];
   float ks, vs;
-  bool real;
-  __device__ __forceinline__ void load(const AttentionArgs& a, int id, int at, int kvh, int lane, bool& bad) {
-    real = id >= 0 && id < a.pages;
-    if (!real) {                                           // no such page: its tokens are not seen
-      bad = true;
-      return;
-    }
+  __device__ __forceinline__ void read(const uint8_t* stage, int lane) {
     const int g = lane >> 2, c = lane & 3;
-    const size_t unit = (size_t)id * a.kv_heads + kvh, base = ((unit << a.shift) + (at & ((1 << a.shift) - 1))) * D;
-    const uint8_t *kp = a.k_cache + base + (size_t)g * D + 16 * c, *vp = a.v_cache + base + (size_t)(2 * c) * D + D / 8 * g;
+    const uint8_t *kp = stage + g * D + 16 * c, *vp = stage + 16 * D + 2 * c * D + D / 8 * g;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) k[t][i] = *reinterpret_cast<const uint4*>(kp + 8 * t * D + 64 * i);
+      for (int i = 0; i < D / 64; ++i) k[t][i] = *reinterpret_cast<const uint4*>(kp + 8 * t * D + 64 * (D == 128 ? i ^ (g & 1) : i));
+    // (rows of 128 bytes lie in the same banks: odd ones begin with their other half, and lanes with odd c with the other half of a piece of V)
+    if (D == 128 && (g & 1))
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint4 y = k[t][0];
+        k[t][0] = k[t][D / 64 - 1];
+        k[t][D / 64 - 1] = y;
+      }
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const uint8_t* src = vp + ((x & 1) + 8 * (x >> 1)) * D;
       if constexpr (D == 128) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(src);
-        v[x][0] = raw.x; v[x][1] = raw.y; v[x][2] = raw.z; v[x][3] = raw.w;
+        const uint2 one = *reinterpret_cast<const uint2*>(src + 8 * (c & 1)), two = *reinterpret_cast<const uint2*>(src + 8 * (~c & 1));
+        v[x][0] = c & 1 ? two.x : one.x; v[x][1] = c & 1 ? two.y : one.y; v[x][2] = c & 1 ? one.x : two.x; v[x][3] = c & 1 ? one.y : two.y;
       } else {
         const uint2 raw = *reinterpret_cast<const uint2*>(src);
         v[x][0] = raw.x; v[x][1] = raw.y;
       }
     }
-    ks = a.k_scale[unit];
-    vs = a.v_scale[unit];
   }
 };
 
@@ -543,7 +550,6 @@ struct Running {
   // 16 tokens from `at` on; `least`: tokens that every row sees, `end`: that some row sees
   template <typename R>
   __device__ __forceinline__ void add(Tile<D>& x, const R& rows, int at, int least, int end, int lane) {
-    if (!x.real) return;
     const int g = lane >> 2, c = lane & 3;
     float s[NT][4];
 #pragma unroll
@@ -656,6 +662,8 @@ struct Running {
   }
 };
 
+// what an item costs besides its units (0: 171 us, 2: 133, 3: 128, 4: 128 at the sizes above)
+constexpr int kBegin = 3;
 // units of a request: every row tile and key/value head has as many as its tokens fill, at least one (which writes the zeros)
 struct Span {
   int start, n, seen, rows, units;
@@ -666,20 +674,30 @@ struct Span {
     seen = min(max(a.seen[r], 0), a.width << a.shift);
     rows = min(n, a.max_new) * a.group;
     units = max((seen + kUnit - 1) / kUnit, 1);
-    total = (long long)((rows + tile_rows - 1) / tile_rows) * units * a.kv_heads;
+    total = (long long)((rows + tile_rows - 1) / tile_rows) * (units + kBegin) * a.kv_heads;
   }
 };
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attention_kernel(const AttentionArgs a) {
   constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
-  __shared__ float s_o[kAttWarps][kRows][D + 4];
+  constexpr int kRing = kRingBytes<D>;
+  static_assert(kRing >= kRows * (D + 4) * 4, "a warp's results lie where its tiles were");
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ unsigned long long s_full[kAttWarps][kDepth];
+  __shared__ int s_fail;
   __shared__ float s_m[kAttWarps][kRows], s_l[kAttWarps][kRows];
   __shared__ long long s_sum[kAttWarps], s_at;
   __shared__ int s_r;
   pdl_enter();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  if (tid == 0) a.cuts[blockIdx.x] = {0, 0, 0, 0};
+  if (tid == 0) {
+    a.cuts[blockIdx.x] = {0, 0, 0, 0};
+    s_fail = 0;
+    for (int i = 0; i < kAttWarps * kDepth; ++i) bar_init(smem_u32(&s_full[0][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const auto results = [&](int w, int row) { return reinterpret_cast<float*>(ring + w * kRing) + row * (D + 4); };
   // ---- this thread block's run of units
   const int each = (a.requests + kAttThreads - 1) / kAttThreads, first = min(tid * each, a.requests), last = min(first + each, a.requests);
   long long mine = 0;
@@ -714,7 +732,9 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
   __syncthreads();
   int r = s_r;
   long long skip = s_at, left = to - from;
-  bool bad = false;
+  bool bad = false, ok = true;
+  int put = 0, get = 0, ahead = 0;                         // stages of this warp's ring, and how many tiles are on their way
+  uint32_t phase = 0;
   for (int segment = 0; left > 0; ++segment) {
     const Span x(a, r, kRows);
     if (skip >= x.total) {
@@ -723,40 +743,88 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       --segment;
       continue;
     }
-    const int item = (int)(skip / x.units), u0 = (int)(skip % x.units), u1 = (int)min((long long)x.units, u0 + left);
+    const int item = (int)(skip / (x.units + kBegin)), w0 = (int)(skip % (x.units + kBegin)), w1 = (int)min((long long)x.units + kBegin, w0 + left);
+    const int u0 = max(w0 - kBegin, 0), u1 = max(w1 - kBegin, 0);
+    skip += w1 - w0;
+    left -= w1 - w0;
+    if (u1 <= u0) {                                        // (only of what an item costs besides its units)
+      --segment;
+      continue;
+    }
     const int kvh = item % a.kv_heads, row0 = item / a.kv_heads * kRows, rows = min(x.rows - row0, kRows);
     const int last_token = (row0 + rows - 1) / a.group;
     const int least = max(x.seen - x.n + row0 / a.group + 1, 0), end = max(x.seen - x.n + last_token + 1, 0);
+    // ---- the tokens of this warp, 16 at a time: kDepth tiles are on their way.  Lane i holds page and scales of tile i of 32, and of the 32 after
+    // them, which are fetched in time.
+    if (segment) {                                         // the results of the last tile have been read
+      __syncthreads();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    const int* table = a.tables + r * a.table_stride;
+    const int stop = min(u1 * kUnit, end), first_at = u0 * kUnit + warp * 16;
+    const int tiles = first_at < stop && ok ? (stop - first_at + kUnit - 1) / kUnit : 0;
+    struct Pages {
+      int id;
+      float ks, vs;
+    };
+    Pages some, then;
+    const auto ids_of = [&](Pages& p, int tile) {          // (of a tile that is none: 0, not used)
+      p.id = tile + lane < tiles ? table[(first_at + (tile + lane) * kUnit) >> a.shift] : 0;
+    };
+    const auto scales_of = [&](Pages& p) {
+      const bool real = p.id >= 0 && p.id < a.pages;       // no such page: its tokens are not seen
+      bad |= !real;
+      const size_t unit = (size_t)(real ? p.id : 0) * a.kv_heads + kvh;
+      if (!real) p.id = -1;
+      p.ks = a.k_scale[unit];
+      p.vs = a.v_scale[unit];
+    };
+    const auto request = [&](int tile, int id) {           // by all lanes, of a stage that they have read
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&s_full[warp][put]), to_stage = smem_u32(ring + warp * kRing + put * 32 * D);
+        if (id >= 0 && id < a.pages) {
+          const size_t base = ((((size_t)id * a.kv_heads + kvh) << a.shift) + ((first_at + tile * kUnit) & ((1 << a.shift) - 1))) * D;
+          bar_expect(bar, 32 * D);
+          bulk_load(to_stage, a.k_cache + base, 16 * D, bar);
+          bulk_load(to_stage + 16 * D, a.v_cache + base, 16 * D, bar);
+        } else {
+          bar_arrive(bar);
+        }
+      }
+      if (++put == kDepth) put = 0;
+      ++ahead;
+    };
+    ids_of(some, 0);
+    for (int i = 0; i < min(kDepth, tiles); ++i) request(i, __shfl_sync(htr::kFullWarp, some.id, i));
+    scales_of(some);
+    then = some;
     Rows<T, D, NT> q;
     q.load(a, x.start, x.n, x.seen, row0, kvh, lane);
     Running<D, NT> run;
     run.clear();
-    // ---- the tokens of this warp: the next 16 and the page after them are on their way while 16 are worked on
-    const int* table = a.tables + r * a.table_stride;
-    const int stop = min(u1 * kUnit, end);
-    int at = u0 * kUnit + warp * 16;
-    int id = at < stop ? table[at >> a.shift] : 0, next_id = at + kUnit < stop ? table[(at + kUnit) >> a.shift] : 0;
-    Tile<D> now, next;
-    if (at < stop) now.load(a, id, at, kvh, lane, bad);
-    while (at < stop) {
-      if (at + kUnit < stop) {
-        id = next_id;
-        if (at + 2 * kUnit < stop) next_id = table[(at + 2 * kUnit) >> a.shift];
-        next.load(a, id, at + kUnit, kvh, lane, bad);
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+      const int j = i & 31;
+      if (j == 0 && i) some = then;
+      if (j == 0 && i + 32 < tiles) ids_of(then, i + 32);
+      if (j == 8 && i + 24 < tiles) scales_of(then);
+      ok = __all_sync(htr::kFullWarp, bar_wait(smem_u32(&s_full[warp][get]), phase, &s_fail));
+      if (!ok) break;
+      const int id = __shfl_sync(htr::kFullWarp, some.id, j);
+      Tile<D> tile;
+      tile.ks = __shfl_sync(htr::kFullWarp, some.ks, j);
+      tile.vs = __shfl_sync(htr::kFullWarp, some.vs, j);
+      tile.read(ring + warp * kRing + get * 32 * D, lane);
+      __syncwarp();
+      --ahead;
+      if (++get == kDepth) {
+        get = 0;
+        phase ^= 1;
       }
-      run.add(now, q, at, least, end, lane);
-      at += kUnit;
-      if (at >= stop) break;
-      if (at + kUnit < stop) {
-        id = next_id;
-        if (at + 2 * kUnit < stop) next_id = table[(at + 2 * kUnit) >> a.shift];
-        now.load(a, id, at + kUnit, kvh, lane, bad);
-      }
-      run.add(next, q, at, least, end, lane);
-      at += kUnit;
+      if (i + kDepth < tiles) request(i + kDepth, __shfl_sync(htr::kFullWarp, j + kDepth < 32 ? some.id : then.id, (j + kDepth) & 31));
+      if (id >= 0) run.add(tile, q, first_at + i * kUnit, least, end, lane);
     }
     // ---- the warps' parts
-    if (segment) __syncthreads();                          // those of the last tile have been read
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -771,7 +839,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
-          *reinterpret_cast<float2*>(&s_o[warp][row][D / 8 * g + 2 * j]) = make_float2(run.o[j][t][y], run.o[j][t][2 + y]);
+          *reinterpret_cast<float2*>(results(warp, row) + D / 8 * g + 2 * j) = make_float2(run.o[j][t][y], run.o[j][t][2 + y]);
       }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == x.units;
@@ -787,7 +855,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
 #pragma unroll
       for (int w = 0; w < kAttWarps; ++w) {
         const float f = most == kNone ? 1.f : exp2_fast(s_m[w][row] - most);
-        const float4 v = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
+        const float4 v = *reinterpret_cast<const float4*>(results(w, row) + d);
         l = fmaf(f, s_l[w][row], l);
         y.x = fmaf(f, v.x, y.x); y.y = fmaf(f, v.y, y.y); y.z = fmaf(f, v.z, y.z); y.w = fmaf(f, v.w, y.w);
       }
@@ -808,17 +876,27 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       const long long beyond = x.units - u1;
       a.cuts[blockIdx.x] = {r, item, 1 + (int)((beyond + share - 1) / share), segment != 0};
     }
-    skip += u1 - u0;
-    left -= u1 - u0;
   }
-  if (bad && a.status && lane == 0) atomicOr(a.status, 32);
+  if (!ok) {                                               // a wait ran out: what is on its way arrives before the memory goes back
+    for (; ahead > 0; --ahead) {
+      bar_wait(smem_u32(&s_full[warp][get]), phase, nullptr);
+      if (++get == kDepth) {
+        get = 0;
+        phase ^= 1;
+      }
+    }
+    if (a.status && lane == 0) atomicOr(a.status, 64);
+  }
+  if (__any_sync(htr::kFullWarp, bad) && a.status && lane == 0) atomicOr(a.status, 32);
 }
 
 // Joins the parts of the tiles that were cut: a thread block per run of the launch before.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const AttentionArgs a) {
   constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
-  pdl_enter();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (not before the wait: thread blocks of a next step's attention that found a place while this one's still ran cost it 35 us of 128)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int4 cut = a.cuts[blockIdx.x];
   if (cut.z == 0) return;
   const Span x(a, cut.x, kRows);
@@ -872,7 +950,15 @@ int attention_tiles(int group, int max_new) { return (long long)group * max_new 
 template <typename T, int D, int NT>
 int attention_run(const AttentionArgs& a, cudaStream_t st) {
   const dim3 grid(attention_blocks(D, NT)), block(kAttThreads);
-  const int rc = paged_launch(paged_attention_kernel<T, D, NT>, grid, block, 1, 0, st, a);
+  constexpr int kBytes = kAttWarps * kRingBytes<D>;
+  static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
+  int dev = 0, e = (int)cudaGetDevice(&dev);
+  if (!e && (dev < 0 || dev >= 64 || !allowed[dev])) {
+    e = (int)cudaFuncSetAttribute(paged_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
+  }
+  if (e) return htr::paged_fail(e);
+  const int rc = paged_launch(paged_attention_kernel<T, D, NT>, grid, block, 1, kBytes, st, a);
   return rc != HTR_OK ? rc : paged_launch(paged_attention_join_kernel<T, D, NT>, grid, block, 1, 0, st, a);
 }
 
