@@ -722,6 +722,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       uint32_t qc[2] = {0, 0}, pc[2] = {0, 0};             // the same of the tiles
       const auto scores_of = [&](auto tile) {
         constexpr int x = decltype(tile)::value;
+        // over the P of two units before: products of another kind are not kept in order by themselves
+        if (qc[x] >= 2 && !bar_wait(pv_done + 16 * x + 8 * (qc[x] & 1), (qc[x] - 2) >> 1 & 1, fail)) return false;
+        fence_after();
         const uint64_t k = dk + (qn % kRing) * (Y::kKeys >> 4);
         const uint32_t to = tmem + 256 * x + 64 * (qc[x] & 1);
 #pragma unroll
@@ -731,6 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
             mma_ss(to, dq + (x * Y::kQTile + part * Y::kPart >> 4) + 2 * y, k + 2 * y, idesc_s, (part | y) != 0);
         commit(s_full + 16 * x + 8 * (qc[x] & 1));
         ++qc[x];
+        return true;
       };
       const auto results_of = [&](auto tile, uint32_t fresh) {
         constexpr int x = decltype(tile)::value;
@@ -755,8 +759,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
           if (j < units) {
             if (!(ok = bar_wait(k_full + 8 * (qn % kRing), qn / kRing & 1, fail))) break;
             fence_after();
-            if (!w.twin || !(j & 1)) scores_of(std::integral_constant<int, 0>{});
-            if (!w.twin || (j & 1)) scores_of(std::integral_constant<int, 1>{});
+            if (!w.twin || !(j & 1)) ok = scores_of(std::integral_constant<int, 0>{});
+            if (ok && (!w.twin || (j & 1))) ok = scores_of(std::integral_constant<int, 1>{});
+            if (!ok) break;
             commit(k_free + 8 * (qn % kRing));
             ++qn;
           }
