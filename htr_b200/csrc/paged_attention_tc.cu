@@ -11,12 +11,17 @@
 //  * Values become fp16, exactly, on their way (P would need three e4m3 parts, at four conversions an element).
 //  * All operands lie in the swizzled layouts (rows of 128 bytes; values with the dimensions inside): from core matrices without a swizzle the
 //    products were fetched at a quarter of the rate, 288 us for a prompt of 2048 tokens behind 2048.
-// Roles of the one thread block of an SM:
+// Roles of the one thread block of an SM, whose registers are shared out among them (160 for the softmax, 96 for the others):
 //   warps 0-7    a thread per row and tile (its lane of tensor memory): scale, mask, running maximum and sum, exponentials, P.  No shuffles.
 //   warps 8-11   values of the units, two of them on their way in registers, into a ring of four
 //   warps 12-13  keys (copies that pass no register) and scales, into a ring of four
-//   warp 14      the products: Q K^T up to two units (a twin: four) before the P V that follow
-// What bounds it: per 256 rows and 64 tokens 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM).
+//   warp 14      (of 16) the products: Q K^T up to two units (a twin: four) before the P V that follow
+// What bounds it: per 256 rows and 64 tokens 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM).  Measured, a prompt's second
+// 2048 tokens over 4096 (32 heads of 128 on 8, 103 GFLOP): 168 us, 613 TFLOP/s; 2650 cycles a unit, of which the exponentials of the two tiles
+// side by side take 1350, tensor memory to registers and back 600, the hand-over between roles 500; 12000 to begin and end an item (a unit
+// of 128 tokens with one hand-over, but the products of a tile in line with its softmax: 179 us).
+// Reference of a row's softmax: 2^2 under the largest term when it moves, and it moves when the sum of 16 terms leaves the range of fp16: terms
+// down to 2^-16 of the largest keep all bits of fp16 (its step below that is 2^-24, of which P V sees at most a half each).
 // The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
 // the sum; see paged_kernels.cu, whose cut of the work into even runs over the thread blocks, parts and join this kernel shares, with
 // runs of units of (request, item, head), each as many as its last token sees.
