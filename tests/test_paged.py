@@ -457,6 +457,19 @@ def test_queries_that_are_not_finite(bad, D, adds, wide):
 
 
 @gpu
+@pytest.mark.parametrize("D,page,hq,hkv,most", ((128, 64, 8, 2, 1), (64, 16, 4, 4, 1), (128, 16, 4, 1, 9), (64, 32, 24, 2, 30)))
+@pytest.mark.parametrize("seed", (1, 2, 3))
+def test_lengths_of_all_kinds_in_one_step(D, page, hq, hkv, most, seed):
+    """The cut of the work falls everywhere: inside long requests, between short ones, at ones that add nothing."""
+    g = torch.Generator().manual_seed(seed)
+    R = 60
+    have = [int(2 ** float(x)) - 1 for x in torch.rand(R, generator=g) * 11.5]
+    adds = [int(x) for x in torch.randint(0, most + 1, (R,), generator=g)]
+    adds[seed] = most
+    check_attention(*filled(torch.bfloat16, D, page, hq, hkv, have, adds, seed=seed), max_new=most)
+
+
+@gpu
 def test_attention_of_many_requests():
     adds = [1] * 1100
     adds[700], adds[3] = 90, 0
