@@ -256,7 +256,7 @@ struct Row {
   }
 };
 
-constexpr int kAppendThreads = 256, kQueryHeads = 4, kMaxPage = 128;
+constexpr int kAppendThreads = 256, kQueryHeads = 4;
 
 // grid (windows of tokens, 2 * kv_heads + groups of query heads): y < 2 * kv_heads: the keys (even) or values (odd) of one head; then the queries.
 // A run = the tokens of this step that lie in one page; the block of the window in which a run begins writes it whole, so that one
@@ -265,10 +265,10 @@ constexpr int kAppendThreads = 256, kQueryHeads = 4, kMaxPage = 128;
 // bound by latency: slots and positions, then rows, angles and the old scale at once, then the maximum.
 // 4096 tokens of 32 heads of 128 on 8 (94 MB): 24.4 us, 3.9 TB/s (queries a token at a time 25.4; their blocks first 24.0, but 13 tokens 5.6 us
 // instead of 5.3).  8 tokens: 3.5 us.  The registers of a run leave two thread blocks on an SM, which is what keeps a prompt from its 14.6.
-template <typename T, int D>
+template <typename T, int D, int kMaxPage>
 __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const AppendArgs a) {
   using R = Row<T, D>;
-  constexpr int kRows = kAppendThreads / R::kLanes, kPasses = kMaxPage / kRows, kWarps = kAppendThreads / 32;   // rows of a pass; passes of a page
+  constexpr int kRows = kAppendThreads / R::kLanes, kPasses = kMaxPage / kRows, kAtOnce = kPasses < 4 ? kPasses : 4, kWarps = kAppendThreads / 32;   // rows of a pass; passes of a page
   __shared__ float red[kWarps];
   __shared__ int s_slot[1 + 2 * kMaxPage], s_pos[1 + 2 * kMaxPage], s_fail[kMaxPage / 32];
   __shared__ unsigned s_begins[kMaxPage / 32];
@@ -367,17 +367,17 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
     for (int x = 0; x < kPasses; ++x) R::widen(raw[x], v[x]);
     if (!values) {
 #pragma unroll
-      for (int x0 = 0; x0 < kPasses; x0 += 4) {
-        float4 c[4], s[4];
+      for (int x0 = 0; x0 < kPasses; x0 += kAtOnce) {
+        float4 c[kAtOnce], s[kAtOnce];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < kAtOnce; ++x) {
           const size_t from = (size_t)s_pos[1 + t - t0 + min((x0 + x) * kRows + row, run - 1)] * (D / 2) + lane * 4;
           c[x] = *reinterpret_cast<const float4*>(a.cosv + from);
           s[x] = *reinterpret_cast<const float4*>(a.sinv + from);
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) R::rotate(v[x0 + x], c[x], s[x]);
-        if ((x0 + 4) * kRows >= run) break;
+        for (int x = 0; x < kAtOnce; ++x) R::rotate(v[x0 + x], c[x], s[x]);
+        if ((x0 + kAtOnce) * kRows >= run) break;
       }
     }
     // the largest of the run, NaN left aside; infinities saturate and do not set the scale either: where there is one, once more without
@@ -984,10 +984,14 @@ int attention_of(const AttentionArgs& a, int head_dim, int max_new, cudaStream_t
   return head_dim == 128 ? attention_run<T, 128, 2>(a, st) : attention_run<T, 64, 2>(a, st);
 }
 
+template <typename T, int D>
+int append_run(const AppendArgs& a, dim3 grid, cudaStream_t st) {
+  return a.shift <= 6 ? paged_launch(rope_append_kernel<T, D, 64>, grid, dim3(kAppendThreads), 1, 0, st, a)
+                      : paged_launch(rope_append_kernel<T, D, 128>, grid, dim3(kAppendThreads), 1, 0, st, a);
+}
 template <typename T>
 int append_of(const AppendArgs& a, int head_dim, dim3 grid, cudaStream_t st) {
-  return head_dim == 128 ? paged_launch(rope_append_kernel<T, 128>, grid, dim3(kAppendThreads), 1, 0, st, a)
-                         : paged_launch(rope_append_kernel<T, 64>, grid, dim3(kAppendThreads), 1, 0, st, a);
+  return head_dim == 128 ? append_run<T, 128>(a, grid, st) : append_run<T, 64>(a, grid, st);
 }
 
 }  // namespace
