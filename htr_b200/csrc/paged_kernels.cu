@@ -263,10 +263,10 @@ constexpr int kAppendThreads = 256, kQueryHeads = 4;
 // block alone reads and writes the page's scale.  A prompt is bound by its bytes: a run stays in registers between the search for
 // its largest element and the rounding, and query rows are read four heads at a time, whose angles are the same.  A few tokens are
 // bound by latency: slots and positions, then rows, angles and the old scale at once, then the maximum.
-// 4096 tokens of 32 heads of 128 on 8 (94 MB): 24.4 us, 3.9 TB/s (queries a token at a time 25.4; their blocks first 24.0, but 13 tokens 5.6 us
-// instead of 5.3).  8 tokens: 3.5 us.  The registers of a run leave two thread blocks on an SM, which is what keeps a prompt from its 14.6.
+// What held a prompt back was the registers of a run, which for pages of 128 leave two thread blocks on an SM; for up to 64, half of them, four.
+// 4096 tokens of 32 heads of 128 on 8, pages of 64 (94 MB): 17.7 us, 5.3 TB/s (by the form for 128: 24.4).  8 tokens: 3.2 us (3.5).
 template <typename T, int D, int kMaxPage>
-__global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_append_kernel(const AppendArgs a) {
   using R = Row<T, D>;
   constexpr int kRows = kAppendThreads / R::kLanes, kPasses = kMaxPage / kRows, kAtOnce = kPasses < 4 ? kPasses : 4, kWarps = kAppendThreads / 32;   // rows of a pass; passes of a page
   __shared__ float red[kWarps];
