@@ -137,10 +137,10 @@ __device__ __forceinline__ u64 part_of(u64 w, float f, bool up) {
   return (hi << (64 - down) | lo >> down) + (up && (lo & (((u64)1 << down) - 1)) != 0);
 }
 
-__device__ __forceinline__ u64 warp_sum(u64 v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(htr::kFullWarp, v, o);
-  return v;
+__device__ __forceinline__ u64 warp_sum(u64 v) {            // in parts whose sums fit a reduction of 32 bits
+  const unsigned a = __reduce_add_sync(htr::kFullWarp, (unsigned)v & 0xFFFFFFu), b = __reduce_add_sync(htr::kFullWarp, (unsigned)(v >> 24) & 0xFFFFFFu),
+                 c = __reduce_add_sync(htr::kFullWarp, (unsigned)(v >> 48));
+  return a + ((u64)b << 24) + ((u64)c << 48);
 }
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
 #pragma unroll
@@ -157,7 +157,8 @@ struct Shared {
   unsigned count[2 * kBins], lo[kBins];                    // of a range of keys: tokens, and their weight in two words (the upper from kBins on)
   u64 red[2][kWarps], ahead[2][kWarps];                    // of the warps: what each has, and what those before it have
   double table[64];
-  u64 mail[2][4];                                          // what the thread blocks of a cluster tell one another, in turns
+  u64 mail[2][2][kMaxCluster];                             // what the thread blocks of a cluster tell one another, in turns
+  u64 border[4];                                           // what the one that holds a border tells all
   u64 told[4];                                             // what its first warp tells a thread block
   u64 won[4];                                              // what lies before the warp that holds the token, the ties left there, and its part
 };
@@ -170,6 +171,12 @@ __device__ __forceinline__ V remote(const V* mine, unsigned rank) {
   if constexpr (sizeof(V) == 8) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
   else asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
+}
+
+__device__ __forceinline__ void remote_store(const u64* mine, unsigned rank, u64 v) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
 
 // A cluster of thread blocks per row, each with a contiguous slice of it, which it reads from memory once, into shared memory (rows too
@@ -206,6 +213,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     if (size > 1) htr::cluster_sync();
     else __syncthreads();
   };
+  if (size > 1) htr::cluster_arrive();                     // (waited for before anything is written to another thread block)
+  // by the first warp, all lanes of which have v: to every thread block of the cluster
+  int turn = 0;                                            // of s.mail: a message is written over two exchanges later, when all have read it
+  const auto tell = [&](int what, u64 v) {
+    if (lane < size) remote_store(&s.mail[turn][what][rank], lane, v);
+  };
   // kVec logits; -infinity behind the last
   const auto from_memory = [&](int x) {
     if (aligned && (x + 1) * kVec <= n) return reinterpret_cast<const uint4*>(src)[x];
@@ -224,7 +237,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
   const auto fetch = [&](int x) { return staged ? reinterpret_cast<const uint4*>(stage)[x] : from_memory(x); };
-  int turn = 0;                                            // of s.mail: a message is written over two exchanges later, when all have read it
   // ---- the largest
   float most = -__builtin_huge_valf();
 #pragma unroll 2
@@ -234,7 +246,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     most = fmaxf(most, L::largest(w));
   }
   if (tid < 64) s.table[tid] = exp2(tid / 64.0);
-  if (tid == 64) s.mail[0][3] = s.mail[1][3] = s.won[2] = 0;
+  if (tid == 64) s.won[2] = 0;
+  if (size > 1) htr::cluster_wait();
   // of all threads of the cluster: the largest of a 32-bit value
   const auto largest_of = [&](uint32_t v) {
     v = __reduce_max_sync(htr::kFullWarp, v);
@@ -242,10 +255,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     __syncthreads();
     if (warp == 0) {
       v = __reduce_max_sync(htr::kFullWarp, (uint32_t)s.red[0][lane]);
-      if (lane == 0) s.mail[turn][0] = v;
+      tell(0, v);
     }
     barrier();
-    v = __reduce_max_sync(htr::kFullWarp, lane < size ? (uint32_t)remote(&s.mail[turn][0], lane) : 0u);
+    v = __reduce_max_sync(htr::kFullWarp, lane < size ? (uint32_t)s.mail[turn][0][lane] : 0u);
     turn ^= 1;
     return v;
   };
@@ -264,7 +277,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       a.tokens[r] = top_key == 0 ? -1 : (long long)at;
       if (a.logprobs) a.logprobs[r] = top_key == 0 ? __int_as_float(0x7FC00000) : 0.f;
     }
-    barrier();                                             // no thread block leaves while another reads its memory
     return;
   }
   Weigh weigh = {(double)logit_of(top_key), 64 * 1.4426950408889634 / (double)t, isinf(logit_of(top_key)) != 0, s.table, top_key, nullptr};
@@ -296,7 +308,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
   // ---- the border: keys above `high` are kept, and of the `tied` tokens in [low, high], which are all equal, the first `ties`
   uint32_t low = 0, high = 0;
   unsigned ties = 0xFFFFFFFFu, tied = 0;
-  u64 mark = 0;                                            // of the message, one of the cluster's, that tells a border: counts them
   // finds the border at which the tokens reach `count`, or their weight `part` of that of all that have been kept so far
   const auto find = [&](bool counts, u64 count, float part) {
     u64 above = 0, target = count;
@@ -400,15 +411,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
         const u64 v = s.red[0][lane], e = warp_scan(v, lane);
         s.ahead[0][lane] = e - v;
         rest = sums ? warp_sum(s.red[1][lane]) : 0;
-        if (lane == 31) {
-          s.mail[turn][0] = e;
-          s.mail[turn][1] = rest;
-        }
+        tell(0, __shfl_sync(htr::kFullWarp, e, 31));
+        if (sums) tell(1, rest);
       }
       barrier();
       if (warp == 0) {
-        const u64 v = lane < size ? remote(&s.mail[turn][0], lane) : 0, before = warp_sum(lane < rank ? v : 0), all = warp_sum(v);
-        rest = sums ? warp_sum(lane < size ? remote(&s.mail[turn][1], lane) : 0) : 0;
+        const u64 v = lane < size ? s.mail[turn][0][lane] : 0, before = warp_sum(lane < rank ? v : 0), all = warp_sum(v);
+        rest = sums ? warp_sum(lane < size ? s.mail[turn][1][lane] : 0) : 0;
         if (lane == 0) {
           s.told[0] = above + before;
           s.told[1] = above + all;
@@ -430,26 +439,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
         lo = low;
         continue;
       }
-      mark += 1ull << 32;
       const u64 before = s.told[0] + s.ahead[0][warp] + end - value[0] - value[1];
       if (before < target && before + value[0] + value[1] >= target) {
         const bool second = before + value[0] < target;
-        s.mail[turn][0] = b0 + second;
-        s.mail[turn][1] = before + (second ? value[0] : 0);
-        s.mail[turn][2] = second ? value[1] : value[0];
-        s.mail[turn][3] = (second ? tokens[1] : tokens[0]) | mark;
+        const u64 message[4] = {(u64)(b0 + second), before + (second ? value[0] : 0), second ? value[1] : value[0], second ? tokens[1] : tokens[0]};
+        for (unsigned c = 0; c < size; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) remote_store(&s.border[j], c, message[j]);
       }
       barrier();
-      if (warp == 0) {
-        const u64 in = lane < size ? remote(&s.mail[turn][3], lane) : 0;
-        const int owner = __ffs(__ballot_sync(htr::kFullWarp, in >> 32 == mark >> 32)) - 1;
-        if (lane < 4) s.told[lane] = remote(&s.mail[turn][lane], owner);
-      }
-      turn ^= 1;
-      __syncthreads();
-      const uint32_t in = (uint32_t)s.told[3];
-      const u64 mass = s.told[2], so_far = s.told[1];
-      hi -= (uint32_t)s.told[0] << shift;
+      const uint32_t in = (uint32_t)s.border[3];
+      const u64 mass = s.border[2], so_far = s.border[1];
+      hi -= (uint32_t)s.border[0] << shift;
       if (hi - lo >> shift) lo = hi - ((1u << shift) - 1);
       if (shift <= L::kGap) {                              // one value
         const u64 one = counts ? 1 : mass / in, need = one ? (target - so_far + one - 1) / one : in;
@@ -547,14 +548,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     const u64 x = s.red[0][lane], y = s.red[1][lane], ex = warp_scan(x, lane), ey = warp_scan(y, lane);
     s.ahead[0][lane] = ex - x;
     s.ahead[1][lane] = ey - y;
-    if (lane == 31) {
-      s.mail[turn][0] = ex;
-      s.mail[turn][1] = ey;
-    }
+    tell(0, __shfl_sync(htr::kFullWarp, ex, 31));
+    tell(1, __shfl_sync(htr::kFullWarp, ey, 31));
   }
   barrier();
   if (warp == 0) {
-    const u64 x = lane < size ? remote(&s.mail[turn][0], lane) : 0, y = lane < size ? remote(&s.mail[turn][1], lane) : 0;
+    const u64 x = lane < size ? s.mail[turn][0][lane] : 0, y = lane < size ? s.mail[turn][1][lane] : 0;
     const u64 bx = warp_sum(lane < rank ? x : 0), by = warp_sum(lane < rank ? y : 0), all = warp_sum(x);
     if (lane == 0) {
       s.told[0] = bx;
@@ -563,7 +562,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
     }
   }
   __syncthreads();
-  if (size > 1) htr::cluster_arrive();                     // nothing remote is read any more; waited for before a thread block leaves
   const u64 ahead = s.told[1] + s.ahead[1][warp], total = s.told[2] + each * min((u64)tied, (u64)ties), target = part_of(total, u, false);
   u64 before = s.told[0] + s.ahead[0][warp] + each * min(ahead, (u64)ties);
   u64 room = ties > ahead ? ties - ahead : 0;              // ties of this warp and of later ones that are kept
@@ -613,7 +611,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       }
     }
   }
-  if (size > 1) htr::cluster_wait();
 }
 
 template <int DT>
