@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/htr_b200.h"
 #include "htr_common.cuh"
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       const int shift = max(21 - __clz(hi - lo), 0);       // at most kBins bins
       const bool single = L::kGap && shift <= L::kGap;     // bins are single values
       const bool sums = first && !counts;                  // the weight of all is needed
-      const bool below = sums && L::kGap == 16;            // the negative values from -2^-8 to -2^8 have bins too, behind the others
+      const bool below = sums && single && L::kGap == 16;           // the negative values from -2^-8 to -2^8 have bins too, behind the others
       for (int b = tid; b < kBins; b += kThreads) {
         s.count[b] = s.count[kBins + b] = 0;
         if (!single) s.lo[b] = 0;
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       for (int x = tid; x < vectors; x += kThreads) {
         const uint4 w = fetch(x);
         if (!(L::largest(w) >= from)) continue;
-        if (below && single && quick) {
+        if (below && quick) {
           unsigned odd = 0;                                // logits without a place
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
             const u64 v = weigh(key);
             const unsigned y = (unsigned)v, was = atomicAdd(&s.lo[b], y), z = (unsigned)(v >> 32) + (was + y < y);
             if (z) atomicAdd(&s.count[kBins + b], z);
-          } else if (below && single && kNegative - key < (uint32_t)kBins << 16) {
+          } else if (below && kNegative - key < (uint32_t)kBins << 16) {
             atomicAdd(&s.count[kBins + ((kNegative - key) >> 16)], 1u);
           } else {
             rest += weigh(key);
@@ -381,17 +382,30 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
           const int b = b0 + j;
           unsigned more = 0;
           u64 mass = 0;
+          // (as many as may be at once: a load under a condition waits for the one before)
+          const auto gathered = [&](const unsigned* of, unsigned (&got)[kMaxCluster]) {
+            const auto some = [&](auto from, auto to) {
 #pragma unroll
-          for (int c = 0; c < kMaxCluster; ++c)
-            if (c < (int)size) {
-              tokens[j] += remote(&s.count[b], c);
-              if (counts) continue;
-              if (single) {
-                if (below) more += remote(&s.count[kBins + b], c);
-              } else {
-                mass += ((u64)remote(&s.count[kBins + b], c) << 32) + remote(&s.lo[b], c);
-              }
-            }
+              for (unsigned c = decltype(from)::value; c < decltype(to)::value; ++c) got[c] = remote(of, c < size ? c : rank);
+            };
+            some(std::integral_constant<unsigned, 0>{}, std::integral_constant<unsigned, 2>{});
+            if (size > 2) some(std::integral_constant<unsigned, 2>{}, std::integral_constant<unsigned, kMaxCluster>{});
+#pragma unroll
+            for (unsigned c = 0; c < kMaxCluster; ++c) got[c] = c < size ? got[c] : 0;
+          };
+          unsigned got[kMaxCluster], low_word[kMaxCluster];
+          gathered(&s.count[b], got);
+#pragma unroll
+          for (int c = 0; c < kMaxCluster; ++c) tokens[j] += got[c];
+          if (below || !(counts || single)) gathered(&s.count[kBins + b], got);
+          if (below) {
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; ++c) more += got[c];
+          } else if (!(counts || single)) {
+            gathered(&s.lo[b], low_word);
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; ++c) mass += ((u64)got[c] << 32) + low_word[c];
+          }
           if (single && !counts) {
             const uint32_t top_of = hi - ((uint32_t)b << shift);
             if (tokens[j]) mass = tokens[j] * weigh(L::only(top_of - min((1u << shift) - 1, top_of), top_of));
@@ -442,18 +456,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a, in
       const u64 before = s.told[0] + s.ahead[0][warp] + end - value[0] - value[1];
       if (before < target && before + value[0] + value[1] >= target) {
         const bool second = before + value[0] < target;
-        const u64 message[4] = {(u64)(b0 + second), before + (second ? value[0] : 0), second ? value[1] : value[0], second ? tokens[1] : tokens[0]};
+        const u64 message[3] = {(u64)(b0 + second), before + (second ? value[0] : 0), second ? tokens[1] : tokens[0]};
         for (unsigned c = 0; c < size; ++c)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) remote_store(&s.border[j], c, message[j]);
+          for (int j = 0; j < 3; ++j) remote_store(&s.border[j], c, message[j]);
       }
       barrier();
-      const uint32_t in = (uint32_t)s.border[3];
-      const u64 mass = s.border[2], so_far = s.border[1];
+      const uint32_t in = (uint32_t)s.border[2];
+      const u64 so_far = s.border[1];
       hi -= (uint32_t)s.border[0] << shift;
       if (hi - lo >> shift) lo = hi - ((1u << shift) - 1);
       if (shift <= L::kGap) {                              // one value
-        const u64 one = counts ? 1 : mass / in, need = one ? (target - so_far + one - 1) / one : in;
+        const u64 one = counts ? 1 : weigh(L::only(lo, hi)), need = one ? (target - so_far + one - 1) / one : in;
         low = lo;
         high = hi;
         tied = in;
