@@ -906,7 +906,9 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
   if (__any_sync(htr::kFullWarp, bad) && a.status && lane == 0) atomicOr(a.status, 32);
 }
 
-// Joins the parts of the tiles that were cut: a thread block per run of the launch before.
+// Joins the parts of the tiles that were cut: kJoins thread blocks per run of the launch before, a thread per row and four dimensions, eight parts on their way.
+template <int D, int NT>
+constexpr int kJoins = 8 * NT * (D / 4) / kAttThreads;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const AttentionArgs a) {
   constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
@@ -918,11 +920,11 @@ __global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const
   const Span x(a, cut.x, kRows);
   const int kvh = cut.y % a.kv_heads, row0 = cut.y / a.kv_heads * kRows, rows = min(x.rows - row0, kRows);
   const float *head = a.parts + ((size_t)blockIdx.x * 2 + cut.w) * kPart, *tail = a.parts + (size_t)blockIdx.x * 2 * kPart;
-  for (int z = threadIdx.x; z < rows * (D / 4); z += kAttThreads) {
+  for (int z = blockIdx.y * kAttThreads + threadIdx.x; z < rows * (D / 4); z += kJoins<D, NT> * kAttThreads) {
     const int row = z / (D / 4), d = z % (D / 4) * 4;
     float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
     float4 y = *reinterpret_cast<const float4*>(head + row * D + d);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 1; i < cut.z; ++i) {
       const float* part = tail + (size_t)i * 2 * kPart;
       const float pm = part[kRows * D + row], pl = part[kRows * D + kRows + row];
@@ -975,7 +977,7 @@ int attention_run(const AttentionArgs& a, cudaStream_t st) {
   }
   if (e) return htr::paged_fail(e);
   const int rc = paged_launch(paged_attention_kernel<T, D, NT>, grid, block, 1, kBytes, st, a);
-  return rc != HTR_OK ? rc : paged_launch(paged_attention_join_kernel<T, D, NT>, grid, block, 1, 0, st, a);
+  return rc != HTR_OK ? rc : paged_launch(paged_attention_join_kernel<T, D, NT>, dim3(grid.x, kJoins<D, NT>), block, 1, 0, st, a);
 }
 
 template <typename T>
