@@ -167,7 +167,8 @@ struct Walk {
   }
 };
 
-constexpr int kJoins = 8;
+template <int D>
+constexpr int kJoins = kRows * (D / 4) / 512;
 template <int D>
 constexpr int kPartFloats = kRows * (D + 2);
 
@@ -805,12 +806,12 @@ __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const Atte
   const Request x(a, cut.x);
   const int kvh = cut.w >> 1, rows = x.tokens(a, cut.y) * a.group;
   const float *head = a.parts + ((size_t)blockIdx.x * 2 + (cut.w & 1)) * kPartFloats<D>, *tail = a.parts + (size_t)blockIdx.x * 2 * kPartFloats<D>;
-  for (int z = blockIdx.y * 512 + threadIdx.x; z < kRows * (D / 4); z += kJoins * 512) {
+  for (int z = blockIdx.y * 512 + threadIdx.x; z < kRows * (D / 4); z += kJoins<D> * 512) {
     const int row = z % kRows, d = z / kRows;
     if (row >= rows) continue;
     float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
     float4 y = *reinterpret_cast<const float4*>(head + (d * kRows + row) * 4);
-#pragma unroll 2
+#pragma unroll 8
     for (int i = 1; i < cut.z; ++i) {
       const float* part = tail + (size_t)i * 2 * kPartFloats<D>;
       const float pm = part[kRows * D + row], pl = part[kRows * D + kRows + row];
@@ -848,7 +849,7 @@ int run(const AttentionArgs& a, cudaStream_t st) {
   if (e) return paged_fail(e);
   const dim3 grid(device_sms());
   const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, (Layout<T, D>::kBytes), st, a);
-  return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, dim3(grid.x, kJoins), dim3(512), 1, 0, st, a);
+  return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, dim3(grid.x, kJoins<D>), dim3(512), 1, 0, st, a);
 }
 
 }  // namespace
@@ -856,13 +857,13 @@ int run(const AttentionArgs& a, cudaStream_t st) {
 namespace htr {
 
 // The other kernel passes over the cache once per 16 rows; this one takes up to 128 of them for the same time, but begins and joins more slowly.
-// In the long run they are level at about 48 rows of 128 dimensions and 96 of 64; and below some 1.5e9 elements of scores times dimensions (of the
-// tables' whole width: lengths are not known here) the other is ahead.  Measured, us, the other / this one: 64 requests over 2000, 2 heads of 128:
-// 32 rows 50 / 64, 64 rows 75 / 64, 128 rows 124 / 67, 256 rows 216 / 79; of 64 dimensions: 64 rows 48 / 62, 128 rows 77 / 62, 256 rows 135 / 71;
-// one request over 8000, 256 rows: 34 / 68; 9 over 5000, 1 head of 64, 72 rows: 26 / 27, 2 heads of 128, 128 rows: 52 / 46.
+// In the long run they are level at about 50 rows of 128 dimensions and 90 of 64; and below some 0.9e9 elements of scores times dimensions (of the
+// tables' whole width: lengths are not known here) the other is ahead.  Measured behind a flush of L2, us, the other / this one: 64 requests over
+// 2000, 2 heads of 128: 32 rows 48 / 67, 64 rows 79 / 67, 128 rows 140 / 69, 256 rows 261 / 81; of 64 dimensions: 64 rows 54 / 67, 128 rows 91 / 67,
+// 256 rows 167 / 77; one request over 8000, 2 heads of 128, 256 rows: 30 / 44; 9 over 5000: 64 rows 38 / 42, 128 rows 56 / 44.
 bool attention_tc_serves(int tokens, int requests, int q_heads, int group, int max_new, long long width, int head_dim) {
   return requests <= kMaxRequests && group <= kRows && (long long)group * max_new * head_dim > 6144 &&
-         (double)tokens * q_heads * (double)width * head_dim > 1.5e9;
+         (double)tokens * q_heads * (double)width * head_dim > 0.9e9;
 }
 
 size_t attention_tc_workspace(int head_dim) {
