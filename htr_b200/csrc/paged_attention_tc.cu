@@ -811,16 +811,9 @@ __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const Atte
     if (row >= rows) continue;
     float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
     float4 y = *reinterpret_cast<const float4*>(head + (d * kRows + row) * 4);
-#pragma unroll 8
-    for (int i = 1; i < cut.z; ++i) {
-      const float* part = tail + (size_t)i * 2 * kPartFloats<D>;
-      const float pm = part[kRows * D + row], pl = part[kRows * D + kRows + row];
-      const float4 v = *reinterpret_cast<const float4*>(part + (d * kRows + row) * 4);
-      const float now = fmaxf(m, pm), f = now == kNone ? 1.f : exp2_fast(m - now), h = now == kNone ? 1.f : exp2_fast(pm - now);
-      m = now;
-      l = l * f + pl * h;
-      y.x = y.x * f + v.x * h; y.y = y.y * f + v.y * h; y.z = y.z * f + v.z * h; y.w = y.w * f + v.w * h;
-    }
+    const auto part = [&](int i) { return tail + (size_t)i * 2 * kPartFloats<D>; };
+    join_parts(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
+               [&](int i) { return reinterpret_cast<const float4*>(part(i) + (d * kRows + row) * 4); });
     const float by = l == 0.f ? 0.f : 1.f / l;
     const int i = row / a.group;
     T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + cut.y * x.per + i) * a.q_heads + (size_t)kvh * a.group + row - i * a.group) * D + 4 * d;
