@@ -17,7 +17,7 @@
 //   warps 12-13  keys (copies that pass no register) and scales, into a ring of four
 //   warp 14      (of 16) the products: Q K^T up to two units (a twin: four) before the P V that follow
 // What bounds it: per 256 rows and 64 tokens 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM).  Measured, a prompt's second
-// 2048 tokens over 4096 (32 heads of 128 on 8, 103 GFLOP): 168 us, 613 TFLOP/s; 2650 cycles a unit, of which the exponentials of the two tiles
+// 2048 tokens over 4096 (32 heads of 128 on 8, 103 GFLOP): 169 us, 610 TFLOP/s; 2650 cycles a unit, of which the exponentials of the two tiles
 // side by side take 1350, tensor memory to registers and back 600, the hand-over between roles 500; 12000 to begin and end an item (a unit
 // of 128 tokens with one hand-over, but the products of a tile in line with its softmax: 179 us).
 // Reference of a row's softmax: 2^2 under the largest term when it moves, and it moves when the sum of 16 terms leaves the range of fp16: terms
@@ -796,7 +796,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   }
 }
 
-// Joins the parts of the tiles that were cut: kJoins thread blocks per run of the launch before, a thread per row and four dimensions.
+// Joins the parts of the tiles that were cut: kJoins thread blocks per run of the launch before, a thread per row and four dimensions (a prompt's items have
+// two parts as a rule: batches of eight cost it 3 us, and of four 1).
 template <typename T, int D>
 __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const AttentionArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const Atte
     float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
     float4 y = *reinterpret_cast<const float4*>(head + (d * kRows + row) * 4);
     const auto part = [&](int i) { return tail + (size_t)i * 2 * kPartFloats<D>; };
-    join_parts(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
+    join_parts<4>(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
                [&](int i) { return reinterpret_cast<const float4*>(part(i) + (d * kRows + row) * 4); });
     const float by = l == 0.f ? 0.f : 1.f / l;
     const int i = row / a.group;

@@ -108,15 +108,15 @@ __device__ __forceinline__ void bulk_load(uint32_t to, const void* from, int byt
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
 }
 
-// Parts of a row's results (maximum m, sum l, four dimensions y), joined in their order: part i of `count` is at m_at(i) and so on; eight are fetched
-// at once, and a batch's factors do not wait for one another.
-template <typename M, typename L, typename Y>
+// Parts of a row's results (maximum m, sum l, four dimensions y), joined in their order: part i of `count` is at m_at(i) and so on; kBatch are
+// fetched at once, and their factors do not wait for one another.
+template <int kBatch, typename M, typename L, typename Y>
 __device__ __forceinline__ void join_parts(int count, float& m, float& l, float4& y, M m_at, L l_at, Y y_at) {
-  for (int first = 1; first < count; first += 8) {
-    float pm[8], pl[8];
-    float4 v[8];
+  for (int first = 1; first < count; first += kBatch) {
+    float pm[kBatch], pl[kBatch];
+    float4 v[kBatch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       pm[i] = kNone;
       pl[i] = 0.f;
       v[i] = {0.f, 0.f, 0.f, 0.f};
@@ -127,13 +127,13 @@ __device__ __forceinline__ void join_parts(int count, float& m, float& l, float4
     }
     float now = m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) now = fmaxf(now, pm[i]);
+    for (int i = 0; i < kBatch; ++i) now = fmaxf(now, pm[i]);
     const float base = now == kNone ? 0.f : now, f = now == kNone ? 1.f : exp2_fast(m - now);
     m = now;
     l *= f;
     y.x *= f; y.y *= f; y.z *= f; y.w *= f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const float by = exp2_fast(pm[i] - base);            // (0 where nothing was seen: a NaN there stays one)
       l = fmaf(pl[i], by, l);
       y.x = fmaf(v[i].x, by, y.x); y.y = fmaf(v[i].y, by, y.y); y.z = fmaf(v[i].z, by, y.z); y.w = fmaf(v[i].w, by, y.w);

@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const
     float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
     float4 y = *reinterpret_cast<const float4*>(head + row * D + d);
     const auto part = [&](int i) { return tail + (size_t)i * 2 * kPart; };
-    join_parts(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
+    join_parts<8>(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
                [&](int i) { return reinterpret_cast<const float4*>(part(i) + row * D + d); });
     const float by = l == 0.f ? 0.f : 1.f / l;
     const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
