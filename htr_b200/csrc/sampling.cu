@@ -133,9 +133,10 @@ __device__ __forceinline__ u64 part_of(u64 w, float f, bool up) {
   int e;
   const u64 bits = (u64)ldexpf(frexpf(f, &e), 24);         // f = bits * 2^(e - 24), e <= 0
   const u64 hi = __umul64hi(w, bits), lo = w * bits;       // below 2^86
-  const int down = 24 - e;
-  if (down >= 64) return up && w ? 1 : down < 128 && hi >> (down - 64);
-  return (hi << (64 - down) | lo >> down) + (up && (lo & (((u64)1 << down) - 1)) != 0);
+  const int down = 24 - e;                                 // at least 24
+  if (down < 64) return (hi << (64 - down) | lo >> down) + (up && (lo & (((u64)1 << down) - 1)) != 0);
+  const u64 whole = down < 128 ? hi >> (down - 64) : 0;    // (f below 2^-40)
+  return whole + (up && (lo != 0 || (down < 128 ? whole << (down - 64) : 0) != hi));
 }
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {            // in parts whose sums fit a reduction of 32 bits

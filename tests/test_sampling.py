@@ -130,6 +130,21 @@ def test_random_numbers_at_their_ends():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
+@pytest.mark.parametrize("power", (25, 39, 40, 41, 43, 47, 52, 56))
+def test_random_numbers_far_below_one(dtype, power):
+    """u times the sum of the weights at a fourth of the first token's weight, and at four times that: the first token, and the second."""
+    from htr_b200 import sampling
+
+    V, u = 131073, 2.0 ** -power                                 # fp16: 4 * 2^17 * 2^-25 is a weight of 2^-6 and 2^-10, a logit of -4 and -7
+    x = torch.zeros(2, V, device=DEV)
+    # weights are kept to 2^-43 of the largest: 2^-41 at the least, an eighth of it; a logit of -28 rounded to bf16 is off by 2^-4, a sixteenth
+    x[0, 0], x[1, 0] = math.log(4 * V * u), math.log(V * u / 4)
+    tokens, _ = sampling.sample(x.to(dtype), torch.full((2,), u, device=DEV))
+    assert tokens.tolist() == [0, 1]
+
+
+@gpu
 def test_frequencies_follow_the_weights():
     from htr_b200 import sampling
 
