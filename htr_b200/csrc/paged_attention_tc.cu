@@ -20,8 +20,8 @@
 // 2048 tokens over 4096 (32 heads of 128 on 8, 103 GFLOP): 169 us, 610 TFLOP/s; 2650 cycles a unit, of which the exponentials of the two tiles
 // side by side take 1350, tensor memory to registers and back 600, the hand-over between roles 500; 12000 to begin and end an item (a unit
 // of 128 tokens with one hand-over, but the products of a tile in line with its softmax: 179 us).
-// Reference of a row's softmax: 2^2 under the largest term when it moves, and it moves when the sum of 16 terms leaves the range of fp16: terms
-// down to 2^-16 of the largest keep all bits of fp16 (its step below that is 2^-24, of which P V sees at most a half each).
+// Reference of a row's softmax: 2^12 under the largest term when it moves, and it moves when the sum of eight terms leaves the range of fp16 (eight
+// that are equal do not): terms down to 2^-26 of the largest keep all bits of fp16 (its step below that is 2^-24, of which P V sees at most a half each).
 // The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
 // the sum; see paged_kernels.cu, whose cut of the work into even runs over the thread blocks, parts and join this kernel shares, with
 // runs of units of (request, item, head), each as many as its last token sees.
@@ -577,14 +577,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
           };
           exponentials();
           // a sum within the range of fp16: so is each of its terms
-          const float most = fmaxf(fmaxf(sum[0][0] + sum[0][1], sum[1][0] + sum[1][1]), fmaxf(sum[2][0] + sum[2][1], sum[3][0] + sum[3][1]));
+          const float most = fmaxf(fmaxf(fmaxf(sum[0][0], sum[0][1]), fmaxf(sum[1][0], sum[1][1])), fmaxf(fmaxf(sum[2][0], sum[2][1]), fmaxf(sum[3][0], sum[3][1])));
           const bool grows = m == kNone || most > 60000.f;
-          if (__any_sync(kFullWarp, grows)) {              // a new reference, 2^2 above which the largest lies; what there is follows
+          if (__any_sync(kFullWarp, grows)) {              // a new reference, 2^12 above which the largest lies; what there is follows
             float top = kNone;
 #pragma unroll
             for (int c = 0; c < kUnit; ++c) top = fmaxf(top, v[c]);
             const bool moves = grows && top > kNone;
-            const float now = moves ? base + top - 2.f : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
+            const float now = moves ? base + top - 12.f : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
 #pragma unroll
             for (int c = 0; c < kUnit; ++c) v[c] += down;
             m = now;

@@ -450,8 +450,10 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
 //
 // Queries are fp16 under a power of two per row (bf16 keeps all its bits: 29 binades of normal fp16 below the row's largest element).
 // Probabilities are rounded to fp16, relative to the contribution that they make: the scale of the values' page is part of the exponent
-// (P' = 2^(s + log2 scale - m)), and the sum of the probabilities takes it out again.  2^-11 each at most, averaged over the tokens: below
-// the rounding of the output.  m follows the largest exponent only when that grows by 2^14 (P' stays below 2^14, sums are float32).
+// (P' = 2^(s + log2 scale - m)), and the sum of the probabilities, in float32 and of what they were before, takes it out again.  m lies 2^12
+// below the largest P' when it moves, and it moves when one grows beyond 2^15.5, so that P' of 2^-26 of the largest and more are normal
+// numbers: 2^-11 each at most, half of bf16's rounding of the output and a quarter of it, but as much as fp16's; smaller ones are off by up to 2^-37 of the largest.
+// (A token that takes nearly everything and whose values are zero leaves the result to terms that small: 2^-26 is 18 nats.)
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -589,7 +591,7 @@ struct Running {
       for (int i = 0; i < 4; ++i) {                        // token g + 8 (i / 2), row 2 c + i % 2
         const float v = fmaf(s[t][i], rows.scale[t][i & 1] * x.ks, lv);
         s[t][i] = edge && at + g + 8 * (i >> 1) >= rows.end[t][i & 1] ? kNone : v;
-        grows |= s[t][i] > m[t][i & 1] + 14.f;
+        grows |= s[t][i] > m[t][i & 1] + 15.5f;
       }
     if (__any_sync(htr::kFullWarp, grows)) {
 #pragma unroll
@@ -599,7 +601,7 @@ struct Running {
           float most = fmaxf(s[t][y], s[t][2 + y]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, d));
-          const float now = fmaxf(m[t][y], most - 6.f);
+          const float now = fmaxf(m[t][y], most - 12.f);
           const float keep = now == kNone ? 1.f : exp2_fast(m[t][y] - now);
           m[t][y] = now;
           l[t][y] *= keep;

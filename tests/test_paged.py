@@ -457,6 +457,36 @@ def test_queries_that_are_not_finite(bad, D, adds, wide):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,adds,R", ((128, 1, 64), (64, 3, 64), (128, 40, 20), (64, 70, 20), (128, 20, 20)))
+@pytest.mark.parametrize("nats", (12, 15, 18))
+@pytest.mark.parametrize("spread", (0.0, 1.0))
+def test_a_token_that_takes_nearly_all_and_has_no_values(dtype, D, adds, R, nats, spread):
+    """The first token's score lies `nats` above those of 16500 others, which are equal or differ by `spread`, and its values are zero: the result is made of
+    the others' probabilities, which have all their bits.  So many requests and heads (of the same pages) that one thread block goes over most of them."""
+    from htr_b200 import paged
+
+    hkv, group = 8, 4
+    q, starts, seen, tables, cache = filled(dtype, D, 64, hkv * group, hkv, (16500,), (adds,))
+    q.zero_()
+    q[..., 0] = 1
+    g = torch.Generator(device=DEV).manual_seed(8)
+    cache.k_scale.fill_(1)
+    cache.v_scale.fill_(2.0 ** -7)
+    cache.k[..., 0] = (torch.randn(cache.k.shape[:3], device=DEV, generator=g) * (16 * spread)).clamp(-448, 448).to(E4M3)       # the only dimension that counts
+    cache.v.copy_((torch.randn(cache.v.shape, device=DEV, generator=g) * 60 + 100).clamp(-448, 448).to(E4M3))
+    id = int(tables[0, 0])
+    cache.k[id, :, 0, 0] = 16 * nats                             # (12, 15 and 18 times 16 are e4m3's)
+    cache.v[id, :, 0] = 0
+    want, spread = attend_exactly(q, starts, seen, tables, cache, 1 / 16)
+    got = paged.attention(q.repeat(R, 1, 1), ints([adds * r for r in range(R + 1)]), seen.repeat(R), widened(q, tables, cache).repeat(R, 1), cache, adds, scale=1 / 16)
+    # the bound of check_one_attention
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -10 * spread + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    off = (got.double().view(R, *q.shape) - want).abs()
+    assert (off <= bound).all(), float((off / bound).max())
+
+
+@gpu
 @pytest.mark.parametrize("D,page,hq,hkv,most", ((128, 64, 8, 2, 1), (64, 16, 4, 4, 1), (128, 16, 4, 1, 9), (64, 32, 24, 2, 30)))
 @pytest.mark.parametrize("seed", (1, 2, 3))
 def test_lengths_of_all_kinds_in_one_step(D, page, hq, hkv, most, seed):
