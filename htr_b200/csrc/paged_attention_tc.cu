@@ -6,8 +6,9 @@
 // of them in turns), Q, K and V in shared memory.  An item of at most 128 rows is a twin: its units go to the two tiles in
 // turns, and their results are joined at the end.
 //  * Keys are multiplied as they are, e4m3, and go from memory straight to their core matrices; a row of Q is a sum of e4m3 parts of four significant
-//    bits each under one power of two (two parts for bf16, three for fp16: exact down to 2^-18 of the row's largest element), which costs what
-//    one product of 16-bit operands would, without its conversions.
+//    bits each under one power of two, which costs what one product of 16-bit operands would, without its conversions.  Two parts for the 8 bits of
+//    bf16, three for the 11 of fp16; e4m3 ends at 2^-9 and the row's largest element lies at 2^7 to 2^8, so elements down to 2^-9 of it (fp16: 2^-6) are
+//    exact, and smaller ones are off by up to 2^-17 of the largest (the other kernel holds 28 binades).
 //  * Values become fp16, exactly, on their way (P would need three e4m3 parts, at four conversions an element).
 //  * All operands lie in the swizzled layouts (rows of 128 bytes; values with the dimensions inside): from core matrices without a swizzle the
 //    products were fetched at a quarter of the rate, 288 us for a prompt of 2048 tokens behind 2048.
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
           }
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(kFullWarp, most, o));
-          const int e = query_exponent(most) - 7;          // the largest between 2^7 and 2^8
+          const int e = query_exponent(most, 7);           // the largest between 2^7 and 2^8
           const float up = most > 3.402823466e38f ? __int_as_float(0x7FC00000) : exp2i(e);     // (an infinite element: all scores are NaN or infinite)
           const int owner = __shfl_sync(kFullWarp, e, (lane & 3) * 8);
           if (lane >> 2 == t) row_scale = exp2i(-owner) * a.scale;

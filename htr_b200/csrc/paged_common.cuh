@@ -156,9 +156,10 @@ struct AttentionArgs {
   int4* cuts;                                              // per thread block, of the tile that begins in its run and goes beyond it
 };
 
-// the exponent that brings a row of queries to the upper end of fp16: `most` is its largest magnitude
-__device__ __forceinline__ int query_exponent(float most) {
-  return most > 0.f && most <= 3.402823466e38f ? min(max(14 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100) : 0;
+// the exponent that brings a row of queries, whose largest magnitude is `most`, to [2^top, 2^(top + 1)): any finite one for 7 <= top <= 14, but for rows
+// below 2^(top - 126), which stay that much smaller (so that the power of two and its inverse are normal numbers)
+__device__ __forceinline__ int query_exponent(float most, int top) {
+  return most > 0.f && most <= 3.402823466e38f ? min(top - ((int)(__float_as_uint(most) >> 23) - 127), 126) : 0;
 }
 
 // attention for many rows a request, on the tensor cores (paged_attention_tc.cu)

@@ -13,7 +13,7 @@ namespace {
 
 using namespace htr;
 
-constexpr int kScaleFloor = -100;                          // smallest exponent of a scale: products of two scales stay normal floats
+constexpr int kScaleFloor = -100;                          // smallest exponent of a scale, which a page of zeros has: it and its inverse are normal floats
 
 __device__ __forceinline__ void pdl_enter() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -499,7 +499,7 @@ struct Rows {
       }
       most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 1));
       most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 2));
-      const int e = query_exponent(most);
+      const int e = query_exponent(most, 14);
       const float up = exp2i(e);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {

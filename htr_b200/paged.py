@@ -165,7 +165,8 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     tokens (status 32).  Status 64: a wait inside the kernel ran out (about two seconds), and the results are not to be used.
 
     Sums are float32.  A probability times the scale of its values' page is rounded to fp16: by 2^-11 of itself down to 2^-26 of the row's largest
-    (18 nats), below by up to 2^-37 of that.  For bf16 that is less than the rounding of the output, for fp16 as much."""
+    (18 nats), below by up to 2^-37 of that.  For bf16 that is less than the rounding of the output, for fp16 as much.  Where a request adds many
+    rows, elements of a query below 2^-9 (fp16: 2^-6) of its largest are held to 2^-17 of the largest."""
     what = "attention"
     y = _host.attention(q, starts, seen, tables, cache, max_new, scale, out, status)
     if y is not None:

@@ -487,6 +487,16 @@ def test_a_token_that_takes_nearly_all_and_has_no_values(dtype, D, adds, R, nats
 
 
 @gpu
+@pytest.mark.parametrize("D,adds", ((128, 2), (64, 40), (128, 60)))
+@pytest.mark.parametrize("of_q,of_k", ((120, 0), (116, -20), (100, 0), (-90, 0), (-120, 110)))
+def test_queries_at_the_ends_of_the_range(D, adds, of_q, of_k):
+    """Finite queries of any magnitude under a scale that brings the scores back."""
+    q, starts, seen, tables, cache = filled(torch.bfloat16, D, 16, 4, 2, (100, 33), (adds, 1))
+    cache.k_scale.mul_(2.0 ** of_k)
+    check_attention(q * 2.0 ** of_q, starts, seen, tables, cache, adds, scale=2.0 ** -(of_q + of_k) * D ** -0.5)
+
+
+@gpu
 @pytest.mark.parametrize("D,page,hq,hkv,most", ((128, 64, 8, 2, 1), (64, 16, 4, 4, 1), (128, 16, 4, 1, 9), (64, 32, 24, 2, 30)))
 @pytest.mark.parametrize("seed", (1, 2, 3))
 def test_lengths_of_all_kinds_in_one_step(D, page, hq, hkv, most, seed):
@@ -558,6 +568,27 @@ def test_two_graphs_and_another_stream(adds, wide):
         eager = paged.attention(*sets[0], max(adds))
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want)) and torch.equal(eager, want[0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,adds", ((128, 2), (64, 40), (128, 60)))
+@pytest.mark.parametrize("size", (8, 256, 4096))
+def test_queries_with_an_element_that_stands_out(dtype, D, adds, size):
+    """One dimension of the queries is larger than the others, and of the keys as much smaller.  The tcgen05 kernel holds queries to 2^-17 of the largest of their row."""
+    q, starts, seen, tables, cache = filled(dtype, D, 16, 4, 2, (300, 33), (adds, 1))
+    q[..., 5] *= size
+    cache.k[..., 5] = (cache.k[..., 5].float() / size).to(E4M3)
+    from htr_b200 import paged
+
+    for t in (tables, widened(q, tables, cache)):
+        got = paged.attention(q, starts, seen, t, cache, adds).double()
+        want, spread = attend_exactly(q, starts, seen, tables, cache, D ** -0.5)
+        # as in check_one_attention, and a score that is off by 2^-17 of the row's largest for all dimensions: so are the probability and, at most, the sum
+        keys = (cache.k.double().nan_to_num(0).abs().sum(-1) * cache.k_scale.double()[..., None]).max()
+        most = q.double().abs().amax(-1, keepdim=True)
+        bound = torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -10 + 2 * 2.0 ** -17 * most * keys * D ** -0.5) * spread + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
 
 
 # ---- refusals -------------------------------------------------------------------------------------------------------
