@@ -192,8 +192,8 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     if T == 0:
         return out
     most = min(int(max_new), T)
-    need = _lib.lib.htr_paged_attention_workspace_bytes(T, R, q_heads, kv_heads, dim, most, tables.shape[1], page)
     with torch.cuda.device(dev):
+        need = _lib.lib.htr_paged_attention_workspace_bytes(T, R, q_heads, kv_heads, dim, most, tables.shape[1], page)      # (by the device's SMs)
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         rc = _lib.lib.htr_paged_attention(q.data_ptr(), _HALF[q.dtype], T, starts.data_ptr(), seen.data_ptr(), R, tables.data_ptr(), stride,
                                           tables.shape[1], cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(), pages,

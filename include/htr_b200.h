@@ -320,7 +320,7 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
  * request r the i-th stands at position seen[r] - n + i (n of them) and sees the positions up to its own; a token that sees nothing gets
  * zeros.  q and out [tokens][q_heads][head_dim], bf16 or fp16; rows behind starts[requests] are left as they are.  max_new: the largest
  * n.  A table entry that is no page hides its tokens (status 32).  Status 64: a wait inside the kernel ran out,
- * and the results are not to be used.  The workspace needs no preparation. */
+ * and the results are not to be used.  The workspace needs no preparation; its size is that for the current device. */
 size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new,
                                            int table_width, int page_size);
 int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts, const int* seen, int requests, const int* tables,

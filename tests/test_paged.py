@@ -591,6 +591,38 @@ def test_queries_with_an_element_that_stands_out(dtype, D, adds, size):
         assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
 
 
+@gpu
+def test_the_workspace_is_sized_for_the_device_of_the_tensors(monkeypatch):
+    """It depends on the device's number of SMs: asked for, as the launch is, with that device as the current one."""
+    from htr_b200 import _lib, paged
+
+    inside, seen_by = [], []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            inside.append(1)
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            inside.pop()
+            return super().__exit__(*a)
+
+    class Library:
+        def __getattr__(self, name):
+            if name.startswith("htr_paged_attention"):
+                seen_by.append((name, bool(inside)))
+            return getattr(real, name)
+
+    real = _lib.lib
+    q, starts, seen, tables, cache = filled(torch.bfloat16, 64, 16, 4, 2, (20, 3), (1, 1))
+    want = paged.attention(q, starts, seen, tables, cache, 1)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "lib", Library())
+    strided = torch.stack([q, q], 2)[:, :, 0]                    # not contiguous: not for the native front
+    assert torch.equal(paged.attention(strided, starts, seen, tables, cache, 1), want)
+    assert [n for n, _ in seen_by] == ["htr_paged_attention_workspace_bytes", "htr_paged_attention"] and all(i for _, i in seen_by)
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------
 
 
