@@ -5,12 +5,24 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/htr_b200.h"
 #include "run_arith.cuh"
 
 namespace htr {
+
+// SMs of the current device (a B200's where there is none: a launch that follows fails by itself)
+inline int current_device_sms() {
+  static std::atomic<int> cache[64];
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64 && (v = cache[dev].load(std::memory_order_relaxed)) > 0) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
+  if (dev >= 0 && dev < 64) cache[dev].store(v, std::memory_order_relaxed);
+  return v;
+}
 
 constexpr float kInvSqrt128 = 0.08838834764831845f;  // 1/sqrt(128)
 constexpr unsigned kFullWarp = 0xFFFFFFFFu;

@@ -823,16 +823,6 @@ __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const Atte
   }
 }
 
-int device_sms() {
-  static int cache[64] = {0};
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
-  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
-  if (dev >= 0 && dev < 64) cache[dev] = v;
-  return v;
-}
-
 template <typename T, int D>
 int run(const AttentionArgs& a, cudaStream_t st) {
   static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
@@ -842,7 +832,7 @@ int run(const AttentionArgs& a, cudaStream_t st) {
     if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
   }
   if (e) return paged_fail(e);
-  const dim3 grid(device_sms());
+  const dim3 grid(current_device_sms());
   const int rc = paged_launch(paged_attention_tc_kernel<T, D>, grid, dim3(kThreads), 1, (Layout<T, D>::kBytes), st, a);
   return rc != HTR_OK ? rc : paged_launch(paged_attention_tc_join_kernel<T, D>, dim3(grid.x, kJoins<D>), dim3(512), 1, 0, st, a);
 }
@@ -862,13 +852,13 @@ bool attention_tc_serves(int tokens, int requests, int q_heads, int group, int m
 }
 
 size_t attention_tc_workspace(int head_dim) {
-  return (size_t)device_sms() * (sizeof(int4) + 2 * sizeof(float) * (head_dim == 128 ? kPartFloats<128> : kPartFloats<64>));
+  return (size_t)current_device_sms() * (sizeof(int4) + 2 * sizeof(float) * (head_dim == 128 ? kPartFloats<128> : kPartFloats<64>));
 }
 
 int attention_tc_run(const AttentionArgs& args, int dtype, int head_dim, void* workspace, cudaStream_t st) {
   AttentionArgs a = args;
   a.cuts = static_cast<int4*>(workspace);
-  a.parts = reinterpret_cast<float*>(a.cuts + device_sms());
+  a.parts = reinterpret_cast<float*>(a.cuts + current_device_sms());
   if (dtype == HTR_DTYPE_BF16) return head_dim == 128 ? run<__nv_bfloat16, 128>(a, st) : run<__nv_bfloat16, 64>(a, st);
   return head_dim == 128 ? run<__half, 128>(a, st) : run<__half, 64>(a, st);
 }

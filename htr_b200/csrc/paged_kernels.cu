@@ -945,18 +945,8 @@ int page_shift(int page_size) {
   return -1;
 }
 
-int device_sms() {
-  static int cache[64] = {0};
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev >= 0 && dev < 64 && cache[dev]) return cache[dev];
-  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
-  if (dev >= 0 && dev < 64) cache[dev] = v;
-  return v;
-}
-
 int attention_blocks(int head_dim, int tiles) {            // what the GPU holds at a time
-  return device_sms() * (head_dim == 128 ? (tiles == 1 ? kAttBlocks<128, 1> : kAttBlocks<128, 2>) : tiles == 1 ? kAttBlocks<64, 1> : kAttBlocks<64, 2>);
+  return current_device_sms() * (head_dim == 128 ? (tiles == 1 ? kAttBlocks<128, 1> : kAttBlocks<128, 2>) : tiles == 1 ? kAttBlocks<64, 1> : kAttBlocks<64, 2>);
 }
 int attention_tiles(int group, int max_new) { return (long long)group * max_new <= 8 ? 1 : 2; }
 
@@ -1041,7 +1031,7 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
   if (!aligned16(qkv) || !aligned16(cosv) || !aligned16(sinv) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q_out)) return HTR_ERR_ALIGNMENT;
   const int units = 2 * kv_heads + (q_heads + kQueryHeads - 1) / kQueryHeads;
   int window = 1;                                          // tokens of a thread block: few where there is little to share out
-  while (window < page_size && (int64_t)tokens * units > (int64_t)window * 148 * 8) window *= 2;
+  while (window < page_size && (int64_t)tokens * units > (int64_t)window * htr::current_device_sms() * 8) window *= 2;
   const AppendArgs a = {qkv, row_stride, positions, slots, tokens, cosv, sinv, angle_rows, q_heads, kv_heads, static_cast<uint8_t*>(k_cache),
                         static_cast<uint8_t*>(v_cache), k_scale, v_scale, (int64_t)pages << shift, shift, window, q_out, status};
   const dim3 grid((unsigned)((tokens + window - 1) / window), units);

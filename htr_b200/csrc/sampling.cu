@@ -632,8 +632,9 @@ template <int DT>
 int run(const SampleArgs& a, cudaStream_t st) {
   constexpr int kStage = 160 * 1024;
   // thread blocks per row: as many as the GPU has room for at one per SM; a row in fewer is one with fewer exchanges
+  const int sms = htr::current_device_sms();
   int size = 1;
-  while (size < kMaxCluster && (long long)a.rows * size * 2 <= 148 && a.vocab > size * 2048) size *= 2;
+  while (size < kMaxCluster && (long long)a.rows * size * 2 <= sms && a.vocab > size * 2048) size *= 2;
   while (size < kMaxCluster && (long long)a.vocab * Logit<DT>::kBytes > (long long)size * kStage) size *= 2;
   const int per = ((a.vocab + size - 1) / size + 15) / 16 * 16;
   const bool staged = (long long)per * Logit<DT>::kBytes <= kStage;
