@@ -192,6 +192,17 @@ class PackedDecoder:
         ang = torch.arange(positions).float()[:, None] * inv[None, :]
         return ang.cos().to(self.device), ang.sin().to(self.device)
 
+    def _far_angles(self, positions):
+        """The same for positions where a float32 angle has no bits left behind the point: 64 bits, rounded once, laid out on the device piece by piece."""
+        d = self.cfg.head_dim
+        inv = float(self.cfg.rope_theta) ** -(torch.arange(0, d, 2, dtype=torch.double, device=self.device) / d)
+        cos = torch.empty(positions, d // 2, dtype=torch.float32, device=self.device)
+        sin = torch.empty_like(cos)
+        for at in range(0, positions, 65536):
+            ang = torch.arange(at, min(at + 65536, positions), dtype=torch.double, device=self.device)[:, None] * inv
+            cos[at:at + 65536], sin[at:at + 65536] = ang.cos(), ang.sin()
+        return cos, sin
+
     def _rope(self, t, pos):
         cos, sin = self.cos.index_select(0, pos)[:, None, :], self.sin.index_select(0, pos)[:, None, :]
         t1, t2 = t[..., ::2].float(), t[..., 1::2].float()
@@ -354,10 +365,10 @@ class PackedDecoder:
 
     def paged_cache(self, requests, pages, page_size=64, max_len=None):
         """A paged cache for this model: `pages` pages of `page_size` tokens shared by `requests` sequences of at most max_len tokens (as many as the
-        pages hold by default; not bound by cfg.max_len)."""
+        pages hold by default; not bound by cfg.max_len).  Beside the pages it holds the angles of max_len positions, 4 * head_dim bytes each."""
         max_len = pages * page_size if max_len is None else max_len
         cache = paged.PagedCache(self.cfg.layers, self.cfg.kv_heads, self.cfg.head_dim, pages, page_size, requests, max_len, self.device)
-        cache.cos, cache.sin = self._angles(cache.tables.shape[1] * page_size)
+        cache.cos, cache.sin = self._far_angles(cache.tables.shape[1] * page_size)
         return cache
 
     def forward_paged(self, ids, plan, cache, max_new):
