@@ -260,7 +260,8 @@ constexpr int kAppendThreads = 256, kQueryHeads = 4;
 
 // grid (windows of tokens, 2 * kv_heads + groups of query heads): y < 2 * kv_heads: the keys (even) or values (odd) of one head; then the queries.
 // A run = the tokens of this step that lie in one page; the block of the window in which a run begins writes it whole, so that one
-// block alone reads and writes the page's scale.  A prompt is bound by its bytes: a run stays in registers between the search for
+// block alone reads and writes the page's scale.  Tokens that are not written do not end a run (the block of the next one would be another): a token
+// begins one where the written token before it, up to a page back, is not of its page, and a slot that does not rise closes its page.  A prompt is bound by its bytes: a run stays in registers between the search for
 // its largest element and the rounding, and query rows are read four heads at a time, whose angles are the same.  A few tokens are
 // bound by latency: slots and positions, then rows, angles and the old scale at once, then the maximum.
 // What held a prompt back was the registers of a run, which for pages of 128 leave two thread blocks on an SM; for up to 64, half of them, four.
@@ -270,8 +271,9 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
   using R = Row<T, D>;
   constexpr int kRows = kAppendThreads / R::kLanes, kPasses = kMaxPage / kRows, kAtOnce = kPasses < 4 ? kPasses : 4, kWarps = kAppendThreads / 32;   // rows of a pass; passes of a page
   __shared__ float red[kWarps];
-  __shared__ int s_slot[1 + 2 * kMaxPage], s_pos[1 + 2 * kMaxPage], s_fail[kMaxPage / 32];
-  __shared__ unsigned s_begins[kMaxPage / 32];
+  __shared__ int s_slot[3 * kMaxPage], s_pos[3 * kMaxPage];
+  __shared__ unsigned s_begins[kMaxPage / 32], s_ends[kMaxPage / 32], s_real[3 * kMaxPage / 32];
+  static_assert(3 * kMaxPage % 32 == 0 && kAppendThreads % 32 == 0, "a warp has the 32 places of a word");
   pdl_enter();
   const int tid = threadIdx.x, lane = tid % R::kLanes, row = tid / R::kLanes, page = 1 << a.shift;
   const T* qkv = static_cast<const T*>(a.qkv);
@@ -322,22 +324,38 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
   uint8_t* cache = values ? a.v_cache : a.k_cache;
   float* scales = values ? a.v_scale : a.k_scale;
   const T* in = qkv + (size_t)(a.q_heads + (values ? a.kv_heads : 0) + head) * D;
-  // slots of the window, of the token before it and of a page behind it; negative: the token is not written
-  for (int i = tid; i < 1 + a.window + page; i += kAppendThreads) {
-    const int t = t0 - 1 + i;
+  // slots of the window (from place `page` on) and of a page before and behind it; negative: the token is not written
+  for (int i = tid; i < 3 * kMaxPage; i += kAppendThreads) {
+    const int t = t0 - page + i;
     int slot = -2, pos = 0;
-    if (t >= 0 && t < a.tokens) {
+    if (t >= 0 && t < a.tokens && i < a.window + 2 * page) {
       slot = a.slots[t];
       pos = a.positions[t];
-      if (!valid(slot, pos)) slot = -2;
+      if (!valid(slot, pos)) slot = -2, pos = 0;
     }
     s_slot[i] = slot;
     s_pos[i] = pos;
+    const unsigned real = __ballot_sync(htr::kFullWarp, slot >= 0);
+    if ((tid & 31) == 0) s_real[i >> 5] = real;
   }
   __syncthreads();
+  const auto last_of = [&](int i, int n) {                 // the last written token's place among the n before place i; -1: none
+    int w = (i - 1) >> 5;
+    unsigned m = s_real[w] & 0xFFFFFFFFu >> (31 - ((i - 1) & 31));
+    while (m == 0 && 32 * w > i - n) m = s_real[--w];
+    const int j = 32 * w + 31 - __clz(m);
+    return m && j >= i - n ? j : -1;
+  };
+  const auto before = [&](int i) {                         // the slot of the written token before place i, fewer than `page` tokens back; negative: none
+    const int slot = s_slot[i - 1];
+    if (slot >= 0) return slot;
+    const int j = last_of(i, page - 1);
+    return j < 0 ? -2 : s_slot[j];
+  };
   if (tid < kMaxPage) {                                    // where runs begin
-    const int slot = tid < t1 - t0 ? s_slot[1 + tid] : -2;
-    const unsigned begins = __ballot_sync(htr::kFullWarp, slot >= 0 && ((slot & (page - 1)) == 0 || s_slot[tid] != slot - 1));
+    const int slot = tid < t1 - t0 ? s_slot[page + tid] : -2;
+    const bool is = slot >= 0 && before(page + tid) >> a.shift != slot >> a.shift;
+    const unsigned begins = __ballot_sync(htr::kFullWarp, is);
     if ((tid & 31) == 0) s_begins[tid >> 5] = begins;
   }
   __syncthreads();
@@ -347,22 +365,30 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
     if (begins == 0) break;
     const int t = t0 + 32 * word + __ffs(begins) - 1;
     begins &= begins - 1;
-    const int slot = s_slot[1 + t - t0], off = slot & (page - 1);
+    const int at_run = page + t - t0, slot = s_slot[at_run], off = slot & (page - 1);
     const size_t unit = (size_t)(slot >> a.shift) * a.kv_heads + head;
     const float old_scale = off ? scales[unit] : 0.f;
-    // its run: the first place that does not follow
+    // its run: up to the first token of another page or whose slot does not rise, without what is not written at the end
     if (tid < kMaxPage) {
-      const unsigned fail = __ballot_sync(htr::kFullWarp, tid >= page - off || s_slot[1 + t - t0 + tid] != slot + tid);
-      if ((tid & 31) == 0) s_fail[tid >> 5] = fail ? tid + __ffs(fail) - 1 : kMaxPage;
+      const int mine = tid < page ? s_slot[at_run + tid] : 0;
+      const bool is = tid >= page || (tid && mine >= 0 && (mine >> a.shift != slot >> a.shift || mine <= before(at_run + tid)));
+      const unsigned ends = __ballot_sync(htr::kFullWarp, is);
+      if ((tid & 31) == 0) s_ends[tid >> 5] = ends;
     }
     __syncthreads();
-    int run = kMaxPage;
+    int end = page;
 #pragma unroll
-    for (int w = 0; w < kMaxPage / 32; ++w) run = min(run, s_fail[w]);
+    for (int w = kMaxPage / 32 - 1; w >= 0; --w)
+      if (s_ends[w]) end = 32 * w + __ffs(s_ends[w]) - 1;
+    const int run = s_slot[at_run + end - 1] >= 0 ? end : last_of(at_run + end, end) + 1 - at_run;     // (the first is written)
+    if (tid == 0 && end < page && s_slot[at_run + end] >> a.shift == slot >> a.shift && blockIdx.y == 0 && a.status) atomicOr(a.status, 16);
+    int place[kPasses];                                    // of this thread's rows; negative: not written
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) place[x] = x * kRows + row < run ? s_slot[at_run + x * kRows + row] : -1;
     float v[kPasses][8];
     uint4 raw[kPasses];                                    // all loads before the first use
 #pragma unroll
-    for (int x = 0; x < kPasses; ++x) raw[x] = x * kRows + row < run ? *reinterpret_cast<const uint4*>(in + (size_t)(t + x * kRows + row) * a.row_stride + lane * 8) : uint4{0, 0, 0, 0};
+    for (int x = 0; x < kPasses; ++x) raw[x] = place[x] >= 0 ? *reinterpret_cast<const uint4*>(in + (size_t)(t + x * kRows + row) * a.row_stride + lane * 8) : uint4{0, 0, 0, 0};
 #pragma unroll
     for (int x = 0; x < kPasses; ++x) R::widen(raw[x], v[x]);
     if (!values) {
@@ -371,7 +397,7 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
         float4 c[kAtOnce], s[kAtOnce];
 #pragma unroll
         for (int x = 0; x < kAtOnce; ++x) {
-          const size_t from = (size_t)s_pos[1 + t - t0 + min((x0 + x) * kRows + row, run - 1)] * (D / 2) + lane * 4;
+          const size_t from = (size_t)s_pos[at_run + min((x0 + x) * kRows + row, run - 1)] * (D / 2) + lane * 4;
           c[x] = *reinterpret_cast<const float4*>(a.cosv + from);
           s[x] = *reinterpret_cast<const float4*>(a.sinv + from);
         }
@@ -419,14 +445,13 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
     const float up = exp2i(-e);
 #pragma unroll
     for (int x = 0; x < kPasses; ++x) {
-      const int i = x * kRows + row;
-      if (i >= run) continue;
+      if (place[x] < 0) continue;
       const uint2 r = {to_e4m3(v[x][0] * up, v[x][1] * up) | to_e4m3(v[x][2] * up, v[x][3] * up) << 16,
                        to_e4m3(v[x][4] * up, v[x][5] * up) | to_e4m3(v[x][6] * up, v[x][7] * up) << 16};
-      *reinterpret_cast<uint2*>(at + (size_t)(off + i) * D + lane * 8) = r;
+      *reinterpret_cast<uint2*>(at + (size_t)(place[x] & (page - 1)) * D + lane * 8) = r;
     }
     if (tid == 0) scales[unit] = exp2i(e);                 // (the old one was read by all before the last barrier)
-    __syncthreads();                                       // s_fail and red have been read
+    __syncthreads();                                       // s_ends and red have been read
   }
 }
 

@@ -123,7 +123,9 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None):
 
     A page's scale is the smallest power of two (at least 2^-100) under which all of its tokens lie within e4m3 (448); it begins anew with the
     page's first place, and where a later token makes it grow the older ones are rescaled.  Infinities are held as the largest value, NaN as NaN.
-    A token with slot -1 is not written and its query is zero; so is one whose slot or position lies outside the buffers (status 16)."""
+    A token with slot -1 is not written and its query is zero; so is one whose slot or position lies outside the buffers (status 16).
+    The tokens of one page stand one after the other in rising slots, as `plan_step` lays them out, within page_size tokens of the step (tokens that are not
+    written may lie between them); from a slot that does not rise on, that page's are not written (status 16)."""
     what = "rope_append"
     q = _host.rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status)
     if q is not None:

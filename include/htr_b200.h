@@ -311,8 +311,9 @@ int htr_page_plan(const int* lengths, const int* added, int requests, int* table
  * head_dim] (bf16 or fp16, rows row_stride elements apart, a multiple of 8); q -> q_out[tokens][q_heads][head_dim], k and v -> the cache at slots[token].
  * A page's scale is the smallest power of two (2^-100 at least) under which all of its tokens lie within e4m3; it begins anew with the
  * page's first place and grows with later ones, and then the older tokens are rescaled.  Infinities become the largest value, NaN
- * stays.  Tokens of one page are neighbours and in order, as htr_page_plan lays them out.  A token with slot -1 is not written and its
- * q row is zero; so is one whose slot or position lies outside (status 16). */
+ * stays.  Tokens of one page are neighbours in rising slots, as htr_page_plan lays them out, within page_size tokens (those that are not
+ * written may lie between them); from a slot that does not rise on, that page's are not written (status 16).  A token with slot -1 is not
+ * written and its q row is zero; so is one whose slot or position lies outside (status 16). */
 int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* positions, const int* slots, int tokens, const float* cosv,
                      const float* sinv, int angle_rows, int q_heads, int kv_heads, int head_dim, void* k_cache, void* v_cache,
                      float* k_scale, float* v_scale, int pages, int page_size, void* q_out, int* status, htr_stream_t stream);

@@ -277,6 +277,89 @@ def test_special_values_and_tokens_outside():
     assert int(status) == 16 and (cache.k.view(torch.uint8)[0] == 0).all()
 
 
+def runs_by_hand(slots, positions, page, total, rows):
+    """[(page, [tokens that are written])] and the status: a page's tokens follow one another, others that are not written between them, in rising slots."""
+    ok = [0 <= s < total and 0 <= p < rows for s, p in zip(slots, positions)]
+    status = 16 if any(not o and s != -1 for o, s in zip(ok, slots)) else 0
+    runs, closed, last = [], False, None
+    for t, o in enumerate(ok):
+        if not o:
+            continue
+        if last is None or t - last >= page or slots[last] // page != slots[t] // page:
+            runs.append((slots[t] // page, []))
+            closed = False
+        elif slots[t] <= slots[last]:
+            closed, status = True, 16
+        if not closed:
+            runs[-1][1].append(t)
+        last = t
+    return runs, ok, status
+
+
+def check_runs(dtype, D, page, hkv, slots, positions, pages, rows, seed=0):
+    from htr_b200 import paged
+
+    hq, T = 2, len(slots)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = (torch.randn(T, (hq + 2 * hkv) * D, device=DEV, generator=g) * torch.exp(2 * torch.randn(T, 1, device=DEV, generator=g))).to(dtype)
+    cos, sin = angles(rows, D)
+    cache, status = empty_cache(pages, hkv, page, D, fill=0x38), ints([0])       # 1.0 everywhere
+    for s in cache[2:]:
+        s.fill_(2.0 ** -12)
+    before = [t.clone() for t in cache]
+    q = paged.rope_append(x, ints(positions), ints(slots), cos, sin, cache, hq, status=status)
+    runs, ok, want = runs_by_hand(slots, positions, page, pages * page, rows)
+    assert int(status) == want and len({p for p, _ in runs}) == len(runs)        # (no page twice: that is not for the operator to put right)
+    assert (q[[not o for o in ok]] == 0).all() and all(bool((q[t] != 0).any()) for t in range(T) if ok[t])
+    y = x.double().view(T, hq + 2 * hkv, D)
+    at = torch.tensor([p if o else 0 for p, o in zip(positions, ok)], device=DEV)
+    exact = [rotated(y[:, hq:hq + hkv], cos.double()[at][:, None], sin.double()[at][:, None]), y[:, hq + hkv:]]
+    for data, scale, old, old_scale, new in ((cache.k, cache.k_scale, before[0], before[2], exact[0]), (cache.v, cache.v_scale, before[1], before[3], exact[1])):
+        touched = torch.zeros(pages, dtype=torch.bool, device=DEV)
+        for id, tokens in runs:
+            touched[id] = True
+            places = [slots[t] % page for t in tokens]
+            for h in range(hkv):
+                e = wanted_exponent(float(new[tokens, h].abs().max().float()))
+                s = float(scale[id, h])
+                assert s == 2.0 ** (max(e, -12) if places[0] else e)
+                got = data[id, h].double() * s
+                bound = torch.maximum(2.0 ** -4 * new[tokens, h].abs(), torch.tensor(2.0 ** -10 * s, device=DEV)) * (1 + 2.0 ** -12)
+                assert ((got[places] - new[tokens, h]).abs() <= bound).all()
+                rest = [p for p in range(page) if p not in places]
+                early, late = [p for p in rest if p < places[0]], [p for p in rest if p > places[0]]
+                # the older ones keep their value, but for half a step of e4m3's subnormals; what lies behind the first place and is not written keeps its bytes
+                assert ((got[early] - 2.0 ** -12).abs() <= 2.0 ** -10 * s).all() and (data[id, h].view(torch.uint8)[late] == 0x38).all()
+        assert torch.equal(data[~touched].view(torch.uint8), old[~touched].view(torch.uint8)) and torch.equal(scale[~touched], old_scale[~touched])
+
+
+@gpu
+@pytest.mark.parametrize("dtype,D,page,hkv", ((torch.bfloat16, 128, 64, 2), (torch.float16, 64, 16, 3), (torch.bfloat16, 64, 128, 1), (torch.bfloat16, 128, 32, 8)))
+@pytest.mark.parametrize("hole", ("positions", "slots", "order", "twice", "all"))
+@pytest.mark.parametrize("pieces", (3, 40))
+def test_pages_whose_tokens_are_not_all_written(dtype, D, page, hkv, hole, pieces):
+    """Positions without angles, slots of -1 and slots that do not rise in the middle of a page: one thread block writes it all the same."""
+    g = torch.Generator().manual_seed(page + pieces)
+    rows, slots, positions = 4 * page, [], []
+    for id in torch.randperm(pieces, generator=g).tolist():
+        off = int(torch.randint(0, page - 3, (1,), generator=g)) if id % 3 else 0
+        n = int(torch.randint(3, page - off + 1, (1,), generator=g))
+        mine, at = [id * page + off + i for i in range(n)], list(range(n))
+        for i in torch.randint(1, n, (max(1, n // 6),), generator=g).tolist():
+            how = hole if hole != "all" else ("positions", "slots", "order", "twice")[i % 4]
+            if how == "positions":
+                at[i] = (-5, rows, 1 << 30)[i % 3]
+            elif how == "slots":
+                mine[i] = -1
+            elif how == "order" and id % 2:
+                mine[i - 1], mine[i] = mine[i], mine[i - 1]
+            elif how == "twice" and id % 2:
+                mine[i] = mine[i - 1]
+        slots += mine
+        positions += at
+    check_runs(dtype, D, page, hkv, slots, positions, pieces + 1, rows, seed=page)
+
+
 # ---- attention ------------------------------------------------------------------------------------------------------
 
 
