@@ -137,6 +137,7 @@ struct Shared {
   alignas(16) float ks[kScales][kGroups], lv[kScales][kGroups], inv[kScales][kGroups];     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
   unsigned char real[kScales][kGroups];                    // groups that have a page
   float twin_m[kTile], twin_l[kTile];
+  int finished[8];                                         // items of the run that the rows of a warp are through with
 };
 
 // the run of a thread block, piece by piece: every role walks it for itself
@@ -327,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         }
       };
       const auto announce_keys = [&](uint32_t n) {
+        if (n == 0 && kw == 0 && a.withhold == (int)blockIdx.x + 1) return;
         fence_async();
         bar_arrive(smem_u32(&s.k_full[n % kRing]));
       };
@@ -457,7 +459,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
     };
     Walk w(s, count);
     uint32_t n = 0, done = 0, twins = 0;                   // units of the thread block, of this tile; twins so far
-    for (int segment = 0; w.left > 0 && ok; ++segment, w.next(a)) {
+    int segment = 0;
+    for (; w.left > 0 && ok; ++segment, w.next(a)) {
       w.look(a);
       const int place_row = w.twin ? row : x * kTile + row, i = place_row / a.group, head = w.head * a.group + place_row - i * a.group;
       const bool mine = place_row < w.rows, warp_has_rows = (w.twin ? 0 : x * kTile) + 32 * (warp & 3) < w.rows;
@@ -707,6 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       if (!whole && w.u0 == 0 && tid == 0)                 // it begins here and ends elsewhere: request, item, parts, head and place of the first
         a.cuts[blockIdx.x] = {w.r, w.tile, 1 + (int)((w.units - w.u1 + share - 1) / share), 2 * w.head + (segment != 0)};
     }
+    if (lane == 0) s.finished[warp] = segment;
     }
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -790,7 +794,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (tid == 0 && s.fail && a.status) atomicOr(a.status, 64);
+  if (s.fail && warp < 8) {                                // a wait ran out: rows that are not finished become NaN (of parts: by way of the sum)
+    // (the run once more, after all else: inside the loop over its items this costs the softmax registers, 197 us in place of 176 at the sizes above)
+    const int x = warp >> 2, row = tid & (kTile - 1);
+    const long long all = *(volatile long long*)&s.total, share = max((all + gridDim.x - 1) / gridDim.x, 1LL);
+    Walk w(s, min(share, all - blockIdx.x * share));
+    for (int segment = 0; w.left > 0; ++segment, w.next(a)) {
+      w.look(a);
+      if (segment < s.finished[warp]) continue;
+      const int place_row = w.twin ? row : x * kTile + row;
+      const bool whole = w.u0 == 0 && w.u1 == w.units;
+      if (!(w.twin && x) && place_row < w.rows) {
+        if (whole) {
+          const int i = place_row / a.group, head = w.head * a.group + place_row - i * a.group;
+          T* dst = static_cast<T*>(a.out) + ((size_t)(w.start + w.tile * w.per + i) * a.q_heads + head) * D;
+          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(dst + c) = {0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu};
+        } else {
+          float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPartFloats<D>;
+          part[kRows * D + place_row] = 0.f;
+          part[kRows * D + kRows + place_row] = __int_as_float(0x7FC00000);
+        }
+      }
+      if (!whole && w.u0 == 0 && tid == 0)
+        a.cuts[blockIdx.x] = {w.r, w.tile, 1 + (int)((w.units - w.u1 + share - 1) / share), 2 * w.head + (segment != 0)};
+    }
+    if (tid == 0 && a.status) atomicOr(a.status, 64);
+  }
   if (warp == 0) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemColumns) : "memory");

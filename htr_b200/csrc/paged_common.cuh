@@ -92,11 +92,13 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                : "=r"(done) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
   return done != 0;
 }
-constexpr unsigned kSpinLimit = 2000000u;                  // polls of a wait before it gives up (about two seconds)
+// polls of a wait before it gives up: about two seconds of one thread (1 us each) and of a warp whose lanes all poll (4 us); and half a second
+// of such a warp for what is still on its way then
+constexpr unsigned kSpinLimit = 2000000u, kWarpSpinLimit = 500000u, kDrainLimit = 125000u;
 // bounded: false when the limit ran out or another has given up
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* fail) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* fail, unsigned limit = kSpinLimit) {
   if (bar_try(bar, parity)) return true;
-  for (unsigned i = 0; i < kSpinLimit; ++i) {
+  for (unsigned i = 0; i < limit; ++i) {
     if (bar_try(bar, parity)) return true;
     if ((i & 255) == 255 && fail && *fail) return false;
   }
@@ -154,6 +156,7 @@ struct AttentionArgs {
   int* status;
   float* parts;                                            // two per thread block: results, maxima, sums of a tile's rows
   int4* cuts;                                              // per thread block, of the tile that begins in its run and goes beyond it
+  int withhold;                                            // test hook: the first keys of thread block withhold - 1 never arrive (0: none)
 };
 
 // the exponent that brings a row of queries, whose largest magnitude is `most`, to [2^top, 2^(top + 1)): any finite one for 7 <= top <= 14, but for rows

@@ -21,6 +21,7 @@ __device__ __forceinline__ void pdl_enter() {
 }
 
 thread_local int t_last_cuda = 0;
+thread_local int t_withhold = 0;                           // (htr_paged_attention_withhold)
 
 // ---- the plan of a step -----------------------------------------------------------------------------------------------------------
 //
@@ -822,8 +823,8 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       p.ks = a.k_scale[unit];
       p.vs = a.v_scale[unit];
     };
-    const auto request = [&](int tile, int id) {           // by all lanes, of a stage that they have read
-      if (lane == 0) {
+    const auto request = [&](int tile, int id, bool held) {            // by all lanes, of a stage that they have read
+      if (lane == 0 && !held) {
         const uint32_t bar = smem_u32(&s_full[warp][put]), to_stage = smem_u32(ring + warp * kRing + put * 32 * D);
         if (id >= 0 && id < a.pages) {
           const size_t base = ((((size_t)id * a.kv_heads + kvh) << a.shift) + ((first_at + tile * kUnit) & ((1 << a.shift) - 1))) * D;
@@ -838,7 +839,8 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       ++ahead;
     };
     ids_of(some, 0);
-    for (int i = 0; i < min(kDepth, tiles); ++i) request(i, __shfl_sync(htr::kFullWarp, some.id, i));
+    for (int i = 0; i < min(kDepth, tiles); ++i)
+      request(i, __shfl_sync(htr::kFullWarp, some.id, i), i == 0 && segment == 0 && warp == 0 && a.withhold == (int)blockIdx.x + 1);
     scales_of(some);
     then = some;
     Rows<T, D, NT> q;
@@ -851,7 +853,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       if (j == 0 && i) some = then;
       if (j == 0 && i + 32 < tiles) ids_of(then, i + 32);
       if (j == 8 && i + 24 < tiles) scales_of(then);
-      ok = __all_sync(htr::kFullWarp, bar_wait(smem_u32(&s_full[warp][get]), phase, &s_fail));
+      ok = __all_sync(htr::kFullWarp, bar_wait(smem_u32(&s_full[warp][get]), phase, &s_fail, kWarpSpinLimit));
       if (!ok) break;
       const int id = __shfl_sync(htr::kFullWarp, some.id, j);
       Tile<D> tile;
@@ -864,7 +866,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
         get = 0;
         phase ^= 1;
       }
-      if (i + kDepth < tiles) request(i + kDepth, __shfl_sync(htr::kFullWarp, j + kDepth < 32 ? some.id : then.id, (j + kDepth) & 31));
+      if (i + kDepth < tiles) request(i + kDepth, __shfl_sync(htr::kFullWarp, j + kDepth < 32 ? some.id : then.id, (j + kDepth) & 31), false);
       if (id >= 0) run.add(tile, q, first_at + i * kUnit, least, end, lane);
     }
     // ---- the warps' parts
@@ -885,6 +887,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
           *reinterpret_cast<float2*>(results(warp, row) + D / 8 * g + 2 * j) = make_float2(run.o[j][t][y], run.o[j][t][2 + y]);
       }
     __syncthreads();
+    const bool lost = *(volatile int*)&s_fail != 0;        // a wait ran out: this tile and those behind it in this run become NaN, by way of the sum
     const bool whole = u0 == 0 && u1 == x.units;
     float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPart;
     for (int z = tid; z < kRows * (D / 4); z += kAttThreads) {
@@ -902,6 +905,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
         l = fmaf(f, s_l[w][row], l);
         y.x = fmaf(f, v.x, y.x); y.y = fmaf(f, v.y, y.y); y.z = fmaf(f, v.z, y.z); y.w = fmaf(f, v.w, y.w);
       }
+      if (lost) l = __int_as_float(0x7FC00000);
       if (whole) {
         const float by = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing: zeros
         const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
@@ -922,7 +926,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
   }
   if (!ok) {                                               // a wait ran out: what is on its way arrives before the memory goes back
     for (; ahead > 0; --ahead) {
-      bar_wait(smem_u32(&s_full[warp][get]), phase, nullptr);
+      bar_wait(smem_u32(&s_full[warp][get]), phase, nullptr, kDrainLimit);
       if (++get == kDepth) {
         get = 0;
         phase ^= 1;
@@ -1021,6 +1025,8 @@ extern "C" {
 
 int htr_paged_last_cuda_error(void) { return t_last_cuda; }
 
+void htr_paged_attention_withhold(int block) { t_withhold = block < 0 ? 0 : block + 1; }
+
 int htr_page_plan(const int* lengths, const int* added, int requests, int* tables, int64_t table_stride, int table_width, int* free_pages, int pages,
                   const int* count, int page_size, int max_tokens, int* starts, int* positions, int* slots, int* seen, int* lengths_out,
                   int* count_out, int* status, htr_stream_t stream) {
@@ -1094,7 +1100,7 @@ int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts,
   int4* cuts = static_cast<int4*>(workspace);
   const AttentionArgs a = {q, starts, seen, tables, table_stride, table_width, requests, tokens, q_heads, kv_heads, q_heads / kv_heads, max_new,
                            static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), k_scale, v_scale, pages, shift,
-                           scale * 1.4426950408889634f, out, status, reinterpret_cast<float*>(cuts + attention_blocks(head_dim, attention_tiles(q_heads / kv_heads, max_new))), cuts};
+                           scale * 1.4426950408889634f, out, status, reinterpret_cast<float*>(cuts + attention_blocks(head_dim, attention_tiles(q_heads / kv_heads, max_new))), cuts, t_withhold};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (tc) return attention_tc_run(a, dtype, head_dim, workspace, st);
   return dtype == HTR_DTYPE_BF16 ? attention_of<__nv_bfloat16>(a, head_dim, max_new, st) : attention_of<__half>(a, head_dim, max_new, st);

@@ -164,7 +164,7 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     [starts[r], starts[r + 1]) of request r the i-th stands at position seen[r] - n + i and sees the cached positions up to its own; one that
     sees nothing gets zeros.  max_new: at least the largest n (tokens of a request beyond it are not computed).  scale: of the scores, 1 / sqrt(head_dim) by default.
     Returns `out`, or a new tensor like q; its rows behind starts[-1] are left as they are.  A table entry that is no page hides its
-    tokens (status 32).  Status 64: a wait inside the kernel ran out (about two seconds), and the results are not to be used.
+    tokens (status 32).  Status 64: a wait inside the kernel ran out (about two seconds); the rows that it concerns are NaN.
 
     Sums are float32.  A probability times the scale of its values' page is rounded to fp16: by 2^-11 of itself down to 2^-26 of the row's largest
     (18 nats), below by up to 2^-37 of that.  For bf16 that is less than the rounding of the output, for fp16 as much.  Where a request adds many

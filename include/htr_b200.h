@@ -320,14 +320,17 @@ int htr_paged_append(const void* qkv, int dtype, int64_t row_stride, const int* 
 /* out[t][head] = softmax(scale * q[t][head] . K) V over the cache, grouped-query and causal: of the tokens [starts[r], starts[r + 1]) of
  * request r the i-th stands at position seen[r] - n + i (n of them) and sees the positions up to its own; a token that sees nothing gets
  * zeros.  q and out [tokens][q_heads][head_dim], bf16 or fp16; rows behind starts[requests] are left as they are.  max_new: the largest
- * n.  A table entry that is no page hides its tokens (status 32).  Status 64: a wait inside the kernel ran out,
- * and the results are not to be used.  The workspace needs no preparation; its size is that for the current device. */
+ * n.  A table entry that is no page hides its tokens (status 32).  Status 64: a wait inside the kernel ran out (about two seconds); the
+ * rows that it concerns are NaN.  The workspace needs no preparation; its size is that for the current device. */
 size_t htr_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new,
                                            int table_width, int page_size);
 int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts, const int* seen, int requests, const int* tables,
                         int64_t table_stride, int table_width, const void* k_cache, const void* v_cache, const float* k_scale,
                         const float* v_scale, int pages, int page_size, int q_heads, int kv_heads, int head_dim, int max_new,
                         float scale, void* out, int* status, void* workspace, size_t workspace_bytes, htr_stream_t stream);
+/* Test hook: in the attention launches of this thread that follow, the first keys of thread block `block` never arrive, so that the bounded
+ * waits for them run out; block < 0: no longer. */
+void htr_paged_attention_withhold(int block);
 int htr_paged_last_cuda_error(void);
 
 /* One token per row of logits[rows][vocab] (rows row_stride elements apart, any of HTR_DTYPE_*; vocab <= 2^20) from a uniform number u[row] in

@@ -675,6 +675,33 @@ def test_queries_with_an_element_that_stands_out(dtype, D, adds, size):
 
 
 @gpu
+@pytest.mark.parametrize("D,have,adds,wide,block", ((128, [3000] * 12, [1] * 12, False, 60), (64, [900] * 30, [3] * 30, False, 100), (128, [1500] * 6, [100] * 6, True, 60),
+                                                    (64, [2500] * 9, [30] * 9, True, 75)))
+def test_rows_of_an_expired_wait_are_nan(D, have, adds, wide, block):
+    """The first keys of one thread block never arrive, so that bounded waits run out: the rows that it owes are NaN, the others as they are without, the
+    status word is set, and the next call is served again.  Single tokens, a few, tiles of 256 rows and twins of 120."""
+    from htr_b200 import _lib, paged
+
+    q, starts, seen, tables, cache = filled(torch.bfloat16, D, 16, 8, 2, have, adds)
+    if wide:
+        tables = widened(q, tables, cache)
+    status = ints([0])
+    want = paged.attention(q, starts, seen, tables, cache, max(adds), status=status)
+    assert int(status) == 0
+    for word in (status, None):
+        out = torch.full_like(q, 3.0)
+        _lib.lib.htr_paged_attention_withhold(block)
+        try:
+            paged.attention(q, starts, seen, tables, cache, max(adds), out=out, status=word)
+        finally:
+            _lib.lib.htr_paged_attention_withhold(-1)
+        lost = out.isnan().any(-1)
+        assert 0 < int(lost.sum()) < lost.numel() // 4 and out[lost].isnan().all() and torch.equal(out[~lost], want[~lost])
+    assert int(status) == 64
+    assert torch.equal(paged.attention(q, starts, seen, tables, cache, max(adds), status=status.zero_()), want) and int(status) == 0
+
+
+@gpu
 def test_the_workspace_is_sized_for_the_device_of_the_tensors(monkeypatch):
     """It depends on the device's number of SMs: asked for, as the launch is, with that device as the current one."""
     from htr_b200 import _lib, paged
