@@ -6,7 +6,9 @@
 // the running weight of the kept ones exceeds u times their sum.
 //
 // Borders decide about whole tokens, so weights are 64-bit integers, 2^42 exp(x) with exp in double: their sums are exact and do not
-// depend on who adds them, and a border can differ from that of real numbers only where u or p lies within 2^-42 of it.
+// depend on who adds them.  Each weight is off by up to 2^-43 of the largest when it is rounded (and 2^-44 before), so that a border lies
+// within vocab * 2^-42 of the largest weight of that of real numbers, and what weighs less than 2^-43 of it (29.8 temperatures below) is never chosen: 2^42
+// is the most that 2^20 weights and their multiples by 2^24 have room for.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -20,7 +20,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     are never chosen; a row that has no other gives token -1 and logprob NaN.
 
     Settings are None, one number for all rows, or a CUDA tensor of one value per row (float32; int32 for top_k).  Rows may be strided.
-    The choice is reproducible to the bit: weights are added as 64-bit integers."""
+    The choice is reproducible to the bit: weights are added as 64-bit integers, multiples of 2^-42 of the largest weight.  Borders are those of real
+    numbers to within vocab * 2^-42 of it, and a token below 2^-43 of it (29.8 temperatures) is never chosen.  No gradients."""
     both = _lib.host.sample(logits, u, temperature, top_k, top_p, min_p)     # the usual case; None: whatever it does not take
     if both is not None:
         return both

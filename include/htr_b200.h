@@ -338,7 +338,8 @@ int htr_paged_last_cuda_error(void);
  * (<= 0: all); the shortest beginning of those with at least top_p of their weight (>= 1: all); those with w >= min_p (<= 0: all); at
  * least one token.  The token is the first, by index, at which the running weight of the kept exceeds u times their sum, and
  * logprobs[row] (may be NULL) the logarithm of its share.  temperature <= 0: the largest logit's first index, 0.  A logit of -infinity
- * or NaN is never chosen; a row without another gives -1 and NaN.  Settings are arrays of one value per row, or NULL: 1, all, all, all. */
+ * or NaN is never chosen; a row without another gives -1 and NaN.  Weights are multiples of 2^-42 of the largest: borders are exact to within vocab
+ * times that, and less than half of it is never chosen.  Settings are arrays of one value per row, or NULL: 1, all, all, all. */
 int htr_sample(const void* logits, int dtype, int64_t row_stride, int rows, int vocab, const float* u, const float* temperature,
                const int* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs, htr_stream_t stream);
 int htr_sample_last_cuda_error(void);

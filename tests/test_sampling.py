@@ -145,6 +145,28 @@ def test_random_numbers_far_below_one(dtype, power):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("V", (1 << 20, 151936))
+@pytest.mark.parametrize("below", (20, 25, 28, 30, 40))
+def test_a_wide_tail_far_below_the_largest(dtype, V, below):
+    """One token, and all others `below` nats under it: weights are multiples of 2^-42, and borders within V * 2^-42 of their place."""
+    from htr_b200 import sampling
+
+    x = torch.zeros(6, V, device=DEV)
+    x[:, 0] = below
+    w, off = math.exp(-below), V * 2.0 ** -42
+    total = 1 + (V - 1) * w
+    u = np.float32([0.0, 0.5, 1 / total - 2 * off - 2.0 ** -23, (1 + 0.25 * V * w) / total, (1 + 0.75 * V * w) / total, 0.99999994])
+    tokens, logprobs = sampling.sample(x.to(dtype), torch.from_numpy(u).to(DEV))
+    for target, token, logprob in zip(u.astype(np.float64) * total, tokens.tolist(), logprobs.tolist()):
+        # the running weight passes the target at the token, but for the bound on both sides of it and on the total
+        assert (token == 0 or 1 + (token - 1) * w <= target + 2 * off) and 1 + token * w >= target - 2 * off
+        want = (-below if token else 0.0) - math.log(total)
+        assert abs(logprob - want) <= off + 2.0 ** -24 * abs(want) + 2.0 ** -50
+        assert token == 0 or below < 30                          # (0.41 of 2^-42 is none)
+
+
+@gpu
 def test_frequencies_follow_the_weights():
     from htr_b200 import sampling
 
