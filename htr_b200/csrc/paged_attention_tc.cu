@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         if (lane < 2) {
           s.ks[slot][2 * kw + lane] = ks;
           s.lv[slot][2 * kw + lane] = __log2f(vs);         // of a power of two: exact
-          s.inv[slot][2 * kw + lane] = __fdividef(1.f, vs);
+          s.inv[slot][2 * kw + lane] = __fdividef(kSumUnit, vs);
           s.real[slot][2 * kw + lane] = real;
         }
       };
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const bool whole = w.u0 == 0 && w.u1 == w.units;
       float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPartFloats<D>;
       const bool empty = l == 0.f;                         // a row that sees nothing: zeros
-      const float by = whole && !empty ? 1.f / l : 1.f;
+      const float by = whole && !empty ? kSumUnit / l : 1.f;
       const bool nan = *(volatile int*)&s.nan != 0;
       if (warp_has_rows) {
 #pragma unroll 1
@@ -845,7 +845,7 @@ __global__ void __launch_bounds__(512) paged_attention_tc_join_kernel(const Atte
     const auto part = [&](int i) { return tail + (size_t)i * 2 * kPartFloats<D>; };
     join_parts<4>(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
                [&](int i) { return reinterpret_cast<const float4*>(part(i) + (d * kRows + row) * 4); });
-    const float by = l == 0.f ? 0.f : 1.f / l;
+    const float by = l == 0.f ? 0.f : kSumUnit / l;
     const int i = row / a.group;
     T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + cut.y * x.per + i) * a.q_heads + (size_t)kvh * a.group + row - i * a.group) * D + 4 * d;
     *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};

@@ -77,6 +77,9 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 constexpr float kNone = -__builtin_huge_valf();
+// The sum of a row's probabilities in units of 2^7: terms of up to 2^15.5 under scales of values of 2^-100 stay finite for 2^19 of them (at 2^12, where they
+// begin, for 2^23), and the inverse of the largest scale, 2^119, is a normal number.
+constexpr float kSumUnit = 0.0078125f;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {

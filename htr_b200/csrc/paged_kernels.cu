@@ -608,7 +608,7 @@ struct Running {
         for (int t = 0; t < NT; ++t) mma_16816(s[t], a0, a1, a2, a3, rows.q[4 * i + j][t][0], rows.q[4 * i + j][t][1]);
       }
     }
-    const float lv = __log2f(x.vs), inv = __fdividef(1.f, x.vs);       // of a power of two: exact
+    const float lv = __log2f(x.vs), inv = __fdividef(kSumUnit, x.vs);  // of a power of two: exact
     const bool edge = at + 16 > least;
     bool grows = false;
 #pragma unroll
@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       }
       if (lost) l = __int_as_float(0x7FC00000);
       if (whole) {
-        const float by = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing: zeros
+        const float by = l == 0.f ? 0.f : kSumUnit / l;    // a row that sees nothing: zeros
         const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
         T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
         *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};
@@ -958,7 +958,7 @@ __global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const
     const auto part = [&](int i) { return tail + (size_t)i * 2 * kPart; };
     join_parts<8>(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
                [&](int i) { return reinterpret_cast<const float4*>(part(i) + row * D + d); });
-    const float by = l == 0.f ? 0.f : 1.f / l;
+    const float by = l == 0.f ? 0.f : kSumUnit / l;
     const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
     T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
     *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};

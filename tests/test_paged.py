@@ -654,6 +654,17 @@ def test_two_graphs_and_another_stream(adds, wide):
 
 
 @gpu
+@pytest.mark.parametrize("D,adds", ((64, 1), (128, 3), (64, 130), (128, 60)))
+@pytest.mark.parametrize("of_v", (-93, 125))
+def test_values_at_the_ends_of_the_range_over_a_long_sequence(D, adds, of_v):
+    """Scales of 2^-100 and 2^118, the ends of what `rope_append` gives (2^119 would be beyond bf16), over 150000 tokens of equal scores."""
+    q, starts, seen, tables, cache = filled(torch.bfloat16, D, 128, 4, 1, (150000,), (adds,))
+    q.zero_()
+    cache.v_scale.fill_(2.0 ** (of_v - 7))
+    check_attention(q, starts, seen, tables, cache, adds)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 @pytest.mark.parametrize("D,adds", ((128, 2), (64, 40), (128, 60)))
 @pytest.mark.parametrize("size", (8, 256, 4096))
