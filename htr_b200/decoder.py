@@ -440,6 +440,8 @@ class PackedDecoder:
             cache = self.paged_cache(R, sum(-(-(n + new_tokens) // page_size) for n in lens), page_size, max(lens) + new_tokens)
         elif cache.lengths.numel() != R or cache.cos is None or int(cache.lengths.max()) > 0:
             raise _lib.HTRError(f"generate_batch: the cache must be one of paged_cache for {R} requests, with none in it")
+        elif int(cache.status):
+            raise _lib.HTRError(f"generate_batch: the cache's status word still has what an earlier step left there ({int(cache.status)})")
         flat = [torch.as_tensor(p, dtype=torch.long).reshape(-1).to(dev) for p in prompts]
         every = torch.cat(flat)
         if int(every.min()) < 0 or int(every.max()) >= self.embed.shape[0]:

@@ -150,3 +150,18 @@ def test_generation_refuses():
     used.cos = None
     with pytest.raises(_lib.HTRError):
         model.forward_paged(torch.zeros(2, dtype=torch.long, device=DEV), plan, used, 1)
+
+
+def test_generation_does_not_answer_for_earlier_steps():
+    """A status word that an earlier step has set is refused before anything is done, and is not taken for this call's."""
+    from htr_b200 import _lib
+
+    model, prompts = a_model(), some_prompts((5, 20))
+    cache = model.paged_cache(2, 9, page_size=16)
+    cache.status.fill_(16)
+    with pytest.raises(_lib.HTRError, match="an earlier step"):
+        model.generate_batch(prompts, 4, cache=cache)
+    assert int(cache.status) == 16 and int(cache.count) == 9 and int(cache.lengths.max()) == 0
+    cache.status.zero_()
+    tokens, _ = model.generate_batch(prompts, 4, cache=cache)
+    assert (tokens >= 0).all()
