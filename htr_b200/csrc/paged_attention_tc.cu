@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   if (tid == 0) {
     s.fail = s.nan = 0;
     for (int i = 0; i < kRing; ++i) {
-      bar_init(smem_u32(&s.k_full[i]), 64);
+      bar_init(smem_u32(&s.k_full[i]), i == 0 && a.withhold == (int)blockIdx.x + 1 ? 65 : 64);      // (withheld: one arrival more than come)
       bar_init(smem_u32(&s.k_free[i]), 1);
       bar_init(smem_u32(&s.v_full[i]), 128);
       bar_init(smem_u32(&s.v_free[i]), 1);
@@ -328,7 +328,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         }
       };
       const auto announce_keys = [&](uint32_t n) {
-        if (n == 0 && kw == 0 && a.withhold == (int)blockIdx.x + 1) return;
         fence_async();
         bar_arrive(smem_u32(&s.k_full[n % kRing]));
       };
