@@ -18,9 +18,10 @@
 //   warps 12-13  keys (copies that pass no register) and scales, into a ring of four
 //   warp 14      (of 16) the products: Q K^T up to two units (a twin: four) before the P V that follow
 // What bounds it: per 256 rows and 64 tokens 1024 cycles of tensor pipe and as many of exponentials (16 a cycle and SM).  Measured, a prompt's second
-// 2048 tokens over 4096 (32 heads of 128 on 8, 103 GFLOP): 169 us, 610 TFLOP/s; 2650 cycles a unit, of which the exponentials of the two tiles
-// side by side take 1350, tensor memory to registers and back 600, the hand-over between roles 500; 12000 to begin and end an item (a unit
-// of 128 tokens with one hand-over, but the products of a tile in line with its softmax: 179 us).
+// 2048 tokens over 4096 (32 heads of 128 on 8, 103 GFLOP), in a chain of launches: 176 us, 587 TFLOP/s (fp16, with its third part of the queries, 189); a unit
+// takes 2650 cycles where no reference moves, of which the exponentials of the two tiles side by side take 1350, tensor memory to registers and back 600, the
+// hand-over between roles 500; 12000 to begin and end an item.  References that move cost 6 of the 176: with 2^4 in place of 2^12 below, 170.  (A unit of 128 tokens
+// with one hand-over, but the products of a tile in line with its softmax, took 179 where this took 165.)
 // Reference of a row's softmax: 2^12 under the largest term when it moves, and it moves when the sum of eight terms leaves the range of fp16 (eight
 // that are equal do not): terms down to 2^-26 of the largest keep all bits of fp16 (its step below that is 2^-24, of which P V sees at most a half each).
 // The scales of keys and values are powers of two per page: they enter the exponent (S * scale + log2 scale of the values - m) and leave
@@ -872,8 +873,8 @@ namespace htr {
 // The other kernel passes over the cache once per 16 rows; this one takes up to 128 of them for the same time, but begins and joins more slowly.
 // In the long run they are level at about 50 rows of 128 dimensions and 90 of 64; and below some 0.9e9 elements of scores times dimensions (of the
 // tables' whole width: lengths are not known here) the other is ahead.  Measured behind a flush of L2, us, the other / this one: 64 requests over
-// 2000, 2 heads of 128: 32 rows 48 / 67, 64 rows 79 / 67, 128 rows 140 / 69, 256 rows 261 / 81; of 64 dimensions: 64 rows 54 / 67, 128 rows 91 / 67,
-// 256 rows 167 / 77; one request over 8000, 2 heads of 128, 256 rows: 30 / 44; 9 over 5000: 64 rows 38 / 42, 128 rows 56 / 44.
+// 2000, 2 heads of 128: 32 rows 48 / 66, 48 rows 65 / 67, 64 rows 79 / 67, 128 rows 138 / 67, 256 rows 257 / 77; of 64 dimensions: 64 rows 54 / 63, 96 rows
+// 71 / 65, 128 rows 89 / 63, 256 rows 161 / 71; one request over 8000, 2 heads of 128, 256 rows: 30 / 42; 9 over 5000: 64 rows 38 / 42, 128 rows 56 / 42.
 bool attention_tc_serves(int tokens, int requests, int q_heads, int group, int max_new, long long width, int head_dim) {
   return requests <= kMaxRequests && group <= kRows && (long long)group * max_new * head_dim > 6144 &&
          (double)tokens * q_heads * (double)width * head_dim > 0.9e9;

@@ -25,8 +25,8 @@ thread_local int t_withhold = 0;                           // (htr_paged_attenti
 
 // ---- the plan of a step -----------------------------------------------------------------------------------------------------------
 //
-// What bounds it: nothing but latency (a few KB for a decode step), so it is one launch: 4.5 us for 32
-// requests of one token, 13 us for 1024 that add up to 200 each.  Every thread block scans all requests by
+// What bounds it: latency (a few KB for a decode step), so it is one launch: 4.5 us in a chain of launches for 32
+// requests of one token, and 13 us, most of it the scans below, for 1024 that add up to 200 each.  Every thread block scans all requests by
 // itself (at most 8192 of them, in shared memory) and then fills its share of the tokens by binary search: 20 times the additions of a
 // scan across thread blocks, and no waiting for one another.  The outputs may be the inputs' own buffers (lengths, count): the thread
 // blocks are one cluster, and nothing is written over before all of them have read.
@@ -265,8 +265,8 @@ constexpr int kAppendThreads = 256, kQueryHeads = 4;
 // begins one where the written token before it, up to a page back, is not of its page, and a slot that does not rise closes its page.  A prompt is bound by its bytes: a run stays in registers between the search for
 // its largest element and the rounding, and query rows are read four heads at a time, whose angles are the same.  A few tokens are
 // bound by latency: slots and positions, then rows, angles and the old scale at once, then the maximum.
-// What held a prompt back was the registers of a run, which for pages of 128 leave two thread blocks on an SM; for up to 64, half of them, four.
-// 4096 tokens of 32 heads of 128 on 8, pages of 64 (94 MB): 17.7 us, 5.3 TB/s (by the form for 128: 24.4).  8 tokens: 3.2 us (3.5).
+// What holds a prompt back is the registers of a run, which for pages of 128 leave two thread blocks on an SM; for up to 64, half of them, four.
+// 4096 tokens of 32 heads of 128 on 8 (94 MB), in a chain of launches: 15.8 us in pages of 64, 6.0 TB/s, and 18.7 in pages of 128.  8 tokens: 3.6 and 3.8 us.
 template <typename T, int D, int kMaxPage>
 __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_append_kernel(const AppendArgs a) {
   using R = Row<T, D>;
@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
 // there; of a tile that is cut every thread block leaves its part (maximum, sum, result) in the workspace, and a second launch joins them in the
 // order of the tokens.
 //
-// 64 requests of 10 to 16384 tokens, 32 heads of 128 on 8 (759 MB): 128 us, 5.9 TB/s.  With tiles in registers 172; with bank conflicts among the pieces of V 162;
-// in runs that count units alone 171; rows of V apart, by a copy for every two, 165.
+// 64 requests of 10 to 16384 tokens, 32 heads of 128 on 8 (759 MB): 128 us in a chain of launches, 5.9 TB/s (a call by itself 132 to 144).  Where it was tried, with
+// tiles in registers 172; with bank conflicts among the pieces of V 162; in runs that count units alone 171; rows of V apart, by a copy for every two, 165.
 //
 // Queries are fp16 under a power of two per row (bf16 keeps all its bits: 29 binades of normal fp16 below the row's largest element).
 // Probabilities are rounded to fp16, relative to the contribution that they make: the scale of the values' page is part of the exponent
@@ -492,8 +492,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8x8 matrix 
   return r;
 }
 constexpr int kAttWarps = 4, kAttThreads = kAttWarps * 32, kUnit = kAttWarps * 16;   // tokens of a unit
-// thread blocks per SM, by the registers that results and a tile need without spills (128 dimensions, 8 rows: four blocks instead of three 161 us, not 150,
-// at decode_64's sizes below)
+// thread blocks per SM, by the registers that results and a tile need without spills and by the rings (of 128 dimensions 64 KB: three at most)
 template <int D, int NT>
 constexpr int kAttBlocks = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
 constexpr int kDepth = 4;                                  // stages of a warp's ring

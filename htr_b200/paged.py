@@ -7,6 +7,7 @@
 
 Requests are rows: a step gives each of them as many tokens as it likes (none, one, a prompt), and the step's tokens stand one request
 after the other.  Nothing touches the host, so that a step can be captured in a CUDA graph.  Lengths, tables and slots are int32.
+No operator here has a gradient: results of inputs that require one do not.
 """
 import typing
 
@@ -78,7 +79,8 @@ def plan_step(lengths, new, tables, free, count, page_size, max_tokens, lengths_
     lengths [requests]: tokens that each request has in the cache; new [requests]: tokens that it adds (0: none; negative: it is over and its
     pages come back); tables [requests, pages of a request]; free [pages], of which the first count[0] are free.  A request that grows gets
     the pages it lacks, in the order of the requests: first those that came back in this step, then from the top of `free`.  `tables` and `free`
-    are updated in place.  Returns a StepPlan: starts (the first token of each request in the step), positions and slots of max_tokens tokens
+    are updated in place.  A page stands in one table and at one place of it: the pages of a request that is over come back whoever else has them.
+    Returns a StepPlan: starts (the first token of each request in the step), positions and slots of max_tokens tokens
     (-1: not served, and behind the last), seen (tokens in the cache after the step of a request that adds some, else 0), and the lengths
     and count after the step, in new tensors or in lengths_out / count_out (which may be lengths and count themselves).
 
@@ -168,7 +170,10 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
 
     Sums are float32.  A probability times the scale of its values' page is rounded to fp16: by 2^-11 of itself down to 2^-26 of the row's largest
     (18 nats), below by up to 2^-37 of that.  For bf16 that is less than the rounding of the output, for fp16 as much.  Where a request adds many
-    rows, elements of a query below 2^-9 (fp16: 2^-6) of its largest are held to 2^-17 of the largest."""
+    rows, elements of a query below 2^-9 (fp16: 2^-6) of its largest are held to 2^-17 of the largest.  Scales of the values of one request and head
+    that lie 2^110 or more apart lose the probabilities under the smaller ones.
+
+    Many rows a request are fast for up to 1024 requests and 256 query heads per key/value head; beyond, 16 rows at a time go over the cache."""
     what = "attention"
     y = _host.attention(q, starts, seen, tables, cache, max_new, scale, out, status)
     if y is not None:

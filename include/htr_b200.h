@@ -298,7 +298,7 @@ int htr_dec_rope_attention(const void* qkv, const int64_t* pos, const float* cos
  *
  * htr_page_plan: one step's tables and slots from lengths[requests] (tokens in the cache) and added[requests] (tokens that the step adds;
  * 0: none; negative: the request is over and its pages come back).  A request that grows gets the pages it lacks, in the order of the
- * requests, first from those that came back in this step, then from the top of free_pages[0..*count).  Outputs: starts[requests + 1] (first
+ * requests, first from those that came back in this step, then from the top of free_pages[0..*count).  No page stands in two tables.  Outputs: starts[requests + 1] (first
  * token of a request in the step's token arrays), positions and slots[max_tokens] (-1: not written, and behind the last token), seen[requests] (tokens
  * in the cache after the step of a request that adds some, else 0), lengths_out, *count_out; tables and free_pages are updated in place.
  * lengths_out and count_out may be lengths and count.  A request that cannot be served keeps its length, its tokens get -1:
