@@ -324,8 +324,10 @@ def check_runs(dtype, D, page, hkv, slots, positions, pages, rows, seed=0):
                 s = float(scale[id, h])
                 assert s == 2.0 ** (max(e, -12) if places[0] else e)
                 got = data[id, h].double() * s
-                bound = torch.maximum(2.0 ** -4 * new[tokens, h].abs(), torch.tensor(2.0 ** -10 * s, device=DEV)) * (1 + 2.0 ** -12)
-                assert ((got[places] - new[tokens, h]).abs() <= bound).all()
+                # half a step of e4m3 or of its subnormals, of the element as the float32 rotation gives it: off by d, three roundings of terms that are at
+                # most sqrt(2) * 448 * s in sum, 3 * 2^-24 * 634 * s < 2^-13 * s; in all (1 + 2^-4) * d more than half a step of the exact one
+                bound = torch.maximum(2.0 ** -4 * new[tokens, h].abs(), torch.tensor(2.0 ** -10 * s, device=DEV)) + 2.0 ** -12 * s
+                assert ((got[places] - new[tokens, h]).abs() <= bound).all(), float(((got[places] - new[tokens, h]).abs() / bound).max())
                 rest = [p for p in range(page) if p not in places]
                 early, late = [p for p in rest if p < places[0]], [p for p in rest if p > places[0]]
                 # the older ones keep their value, but for half a step of e4m3's subnormals; what lies behind the first place and is not written keeps its bytes
