@@ -19,7 +19,7 @@ DEV = torch.device("cuda:0")
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 FLOOR = 2.0 ** -100                                               # smallest scale
-LARGEST = 3.3895313892515355e38                                   # largest finite bf16
+LARGEST = 6.0 * 2.0 ** 119                                        # largest magnitude that is held
 THETA = 1.0e6
 
 
