@@ -12,6 +12,7 @@
 namespace htr {
 
 int paged_fail(int cuda_error);                            // keeps the error for htr_paged_last_cuda_error, HTR_ERR_CUDA
+int attention_withhold();                                  // what htr_paged_attention_withhold has set for this thread
 
 template <typename Kern, typename... Args>
 int paged_launch(Kern kern, dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t st, Args... args) {

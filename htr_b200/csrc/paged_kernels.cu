@@ -7,7 +7,7 @@
 // Why e4m3 under powers of two: a page fills token by token, and a later token may be larger than what its scale admits.  The scale
 // then grows and the older tokens are rescaled by a power of two, which keeps their three mantissa bits (only values that fall among
 // the subnormals, 2^-15 of the page's largest and less, are rounded again); 8-bit integers would be rounded anew every time.
-#include "paged_common.cuh"
+#include "paged_attention.cuh"
 
 namespace {
 
@@ -481,66 +481,13 @@ __global__ void __launch_bounds__(kAppendThreads, kMaxPage == 64 ? 4 : 2) rope_a
 // numbers: 2^-11 each at most, half of bf16's rounding of the output and a quarter of it, but as much as fp16's; smaller ones are off by up to 2^-37 of the largest.
 // (A token that takes nearly everything and whose values are zero leaves the result to terms that small: 2^-26 is 18 nats.)
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8x8 matrix of fp16, a row per four lanes
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-constexpr int kAttWarps = 4, kAttThreads = kAttWarps * 32, kUnit = kAttWarps * 16;   // tokens of a unit
+constexpr int kUnit = kAttWarps * 16;                      // tokens of a unit
 // thread blocks per SM, by the registers that results and a tile need without spills and by the rings (of 128 dimensions 64 KB: three at most)
 template <int D, int NT>
 constexpr int kAttBlocks = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
 constexpr int kDepth = 4;                                  // stages of a warp's ring
 template <int D>
 constexpr int kRingBytes = kDepth * 32 * D;                // of a warp
-
-// a row of queries as the right operand: fragments of rows g + 8 * tile, their scale (times that of the scores), for this lane's rows 2 c, 2 c + 1
-template <typename T, int D, int NT>
-struct Rows {
-  uint32_t q[D / 16][NT][2];
-  float scale[NT][2];
-  int end[NT][2];                                          // tokens that a row sees
-  __device__ __forceinline__ void load(const AttentionArgs& a, int start, int n, int seen, int row0, int kvh, int lane) {
-    const int g = lane >> 2, c = lane & 3, rows = n * a.group;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int row = row0 + 8 * t + g, i = row / a.group;
-      const bool ok = row < rows;
-      const T* src = static_cast<const T*>(a.q) + ((size_t)(start + i) * a.q_heads + (size_t)kvh * a.group + (row - i * a.group)) * D;
-      float v[D / 16][4], most = 0.f;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {                   // step k: dimensions 64 (k / 4) + 16 c + 4 (k % 4) ...
-        uint2 raw = {0, 0};
-        if (ok) raw = *reinterpret_cast<const uint2*>(src + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
-        const float2 lo = Half<T>::wide(raw.x), hi = Half<T>::wide(raw.y);
-        v[k][0] = lo.x; v[k][1] = lo.y; v[k][2] = hi.x; v[k][3] = hi.y;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[k][j]));
-      }
-      most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, 2));
-      const int e = query_exponent(most, 14);
-      const float up = exp2i(e);
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        q[k][t][0] = pack_half(v[k][0] * up, v[k][1] * up);
-        q[k][t][1] = pack_half(v[k][2] * up, v[k][3] * up);
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {                        // of the rows in which this lane holds scores
-        const int mine = 2 * c + y;
-        scale[t][y] = exp2i(-__shfl_sync(htr::kFullWarp, e, 4 * mine)) * a.scale;
-        const int at = row0 + 8 * t + mine;
-        end[t][y] = at < rows ? seen - n + at / a.group + 1 : 0;
-      }
-    }
-  }
-};
 
 // 16 tokens of keys and values of one page
 template <int D>
@@ -577,19 +524,12 @@ struct Tile {
   }
 };
 
-// running softmax of a warp: results O^T (dimension D/8 g + 2 j + i / 2, rows 2 c + i % 2), maximum and sum of this lane's rows
+// what a warp makes of its tokens
 template <int D, int NT>
-struct Running {
-  float o[D / 16][NT][4], m[NT][2], l[NT][2];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) o[j][t][0] = o[j][t][1] = o[j][t][2] = o[j][t][3] = 0.f;
-      m[t][0] = m[t][1] = kNone;
-      l[t][0] = l[t][1] = 0.f;
-    }
-  }
+struct Running : Results<D, NT> {
+  using Results<D, NT>::o;
+  using Results<D, NT>::m;
+  using Results<D, NT>::l;
   // 16 tokens from `at` on; `least`: tokens that every row sees, `end`: that some row sees
   template <typename R>
   __device__ __forceinline__ void add(Tile<D>& x, const R& rows, int at, int least, int end, int lane) {
@@ -622,20 +562,7 @@ struct Running {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float most = fmaxf(s[t][y], s[t][2 + y]);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(htr::kFullWarp, most, d));
-          const float now = fmaxf(m[t][y], most - 12.f);
-          const float keep = now == kNone ? 1.f : exp2_fast(m[t][y] - now);
-          m[t][y] = now;
-          l[t][y] *= keep;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            o[j][t][y] *= keep;
-            o[j][t][2 + y] *= keep;
-          }
-        }
+        for (int y = 0; y < 2; ++y) this->raise(t, y, fmaxf(s[t][y], s[t][2 + y]));
     }
     uint32_t p[NT][2];
 #pragma unroll
@@ -707,79 +634,36 @@ struct Running {
 
 // what an item costs besides its units (0: 171 us, 2: 133, 3: 128, 4: 128 at the sizes above)
 constexpr int kBegin = 3;
-// units of a request: every row tile and key/value head has as many as its tokens fill, at least one (which writes the zeros)
-struct Span {
-  int start, n, seen, rows, units;
-  long long total;
-  __device__ __forceinline__ Span(const AttentionArgs& a, int r, int tile_rows) {
-    start = max(a.starts[r], 0);
-    n = max(min(a.starts[r + 1], a.tokens) - start, 0);
-    seen = min(max(a.seen[r], 0), a.width << a.shift);
-    rows = min(n, a.max_new) * a.group;
-    units = max((seen + kUnit - 1) / kUnit, 1);
-    total = (long long)((rows + tile_rows - 1) / tile_rows) * (units + kBegin) * a.kv_heads;
-  }
-};
+using Work = Span<kUnit, kBegin>;
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attention_kernel(const AttentionArgs a) {
-  constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
-  constexpr int kRing = kRingBytes<D>;
+  constexpr int kRows = 8 * NT, kRing = kRingBytes<D>;
   static_assert(kRing >= kRows * (D + 4) * 4, "a warp's results lie where its tiles were");
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ unsigned long long s_full[kAttWarps][kDepth];
   __shared__ int s_fail;
-  __shared__ float s_m[kAttWarps][kRows], s_l[kAttWarps][kRows];
-  __shared__ long long s_sum[kAttWarps], s_at;
-  __shared__ int s_r;
+  __shared__ WarpParts<kRows> parts;
+  __shared__ Place place;
   pdl_enter();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     a.cuts[blockIdx.x] = {0, 0, 0, 0};
     s_fail = 0;
     for (int i = 0; i < kAttWarps * kDepth; ++i) bar_init(smem_u32(&s_full[0][i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const auto results = [&](int w, int row) { return reinterpret_cast<float*>(ring + w * kRing) + row * (D + 4); };
   // ---- this thread block's run of units
-  const int each = (a.requests + kAttThreads - 1) / kAttThreads, first = min(tid * each, a.requests), last = min(first + each, a.requests);
-  long long mine = 0;
-  for (int r = first; r < last; ++r) mine += Span(a, r, kRows).total;
-  long long sum = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(htr::kFullWarp, sum, o);
-    if (lane >= o) sum += x;
-  }
-  if (lane == 31) s_sum[warp] = sum;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < kAttWarps; ++w) {
-    if (w < warp) sum += s_sum[w];
-    total += s_sum[w];
-  }
-  const long long share = max((total + gridDim.x - 1) / gridDim.x, 1LL), from = blockIdx.x * share, to = min(from + share, total);
-  if (from >= to) return;
-  sum -= mine;
-  if (sum <= from && from < sum + mine) {
-    int r = first;
-    for (;; ++r) {
-      const long long x = Span(a, r, kRows).total;
-      if (from < sum + x) break;
-      sum += x;
-    }
-    s_r = r;
-    s_at = from - sum;
-  }
-  __syncthreads();
-  int r = s_r;
-  long long skip = s_at, left = to - from;
+  const Begin<Work> begin(a, kRows, &place);
+  if (begin.left <= 0) return;
+  const long long share = begin.share;
+  int r = begin.r;
+  long long skip = begin.skip, left = begin.left;
   bool bad = false, ok = true;
   int put = 0, get = 0, ahead = 0;                         // stages of this warp's ring, and how many tiles are on their way
   uint32_t phase = 0;
   for (int segment = 0; left > 0; ++segment) {
-    const Span x(a, r, kRows);
+    const Work x(a, r, kRows);
     if (skip >= x.total) {
       skip -= x.total;
       ++r;
@@ -842,7 +726,7 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       request(i, __shfl_sync(htr::kFullWarp, some.id, i), i == 0 && segment == 0 && warp == 0 && a.withhold == (int)blockIdx.x + 1);
     scales_of(some);
     then = some;
-    Rows<T, D, NT> q;
+    Rows<T, D, NT, 16> q;
     q.load(a, x.start, x.n, x.seen, row0, kvh, lane);
     Running<D, NT> run;
     run.clear();
@@ -868,56 +752,8 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
       if (i + kDepth < tiles) request(i + kDepth, __shfl_sync(htr::kFullWarp, j + kDepth < 32 ? some.id : then.id, (j + kDepth) & 31), false);
       if (id >= 0) run.add(tile, q, first_at + i * kUnit, least, end, lane);
     }
-    // ---- the warps' parts
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float l = run.l[t][y];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(htr::kFullWarp, l, o);
-        const int row = 8 * t + 2 * c + y;
-        if (g == 0) {
-          s_m[warp][row] = run.m[t][y];
-          s_l[warp][row] = l;
-        }
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-          *reinterpret_cast<float2*>(results(warp, row) + D / 8 * g + 2 * j) = make_float2(run.o[j][t][y], run.o[j][t][2 + y]);
-      }
-    __syncthreads();
-    const bool lost = *(volatile int*)&s_fail != 0;        // a wait ran out: this tile and those behind it in this run become NaN, by way of the sum
     const bool whole = u0 == 0 && u1 == x.units;
-    float* part = a.parts + ((size_t)blockIdx.x * 2 + (segment != 0)) * kPart;
-    for (int z = tid; z < kRows * (D / 4); z += kAttThreads) {
-      const int row = z / (D / 4), d = z % (D / 4) * 4;
-      if (row >= rows) continue;
-      float most = kNone;
-#pragma unroll
-      for (int w = 0; w < kAttWarps; ++w) most = fmaxf(most, s_m[w][row]);
-      float l = 0.f;
-      float4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < kAttWarps; ++w) {
-        const float f = most == kNone ? 1.f : exp2_fast(s_m[w][row] - most);
-        const float4 v = *reinterpret_cast<const float4*>(results(w, row) + d);
-        l = fmaf(f, s_l[w][row], l);
-        y.x = fmaf(f, v.x, y.x); y.y = fmaf(f, v.y, y.y); y.z = fmaf(f, v.z, y.z); y.w = fmaf(f, v.w, y.w);
-      }
-      if (lost) l = __int_as_float(0x7FC00000);
-      if (whole) {
-        const float by = l == 0.f ? 0.f : kSumUnit / l;    // a row that sees nothing: zeros
-        const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
-        T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
-        *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};
-      } else {
-        *reinterpret_cast<float4*>(part + row * D + d) = y;
-        if (d == 0) {
-          part[kRows * D + row] = most;
-          part[kRows * D + kRows + row] = l;
-        }
-      }
-    }
+    finish<T, D, NT, kRing>(a, run, ring, &parts, &s_fail, x, kvh, row0, rows, whole, segment != 0);
     if (!whole && u0 == 0 && tid == 0) {                   // it begins here and ends elsewhere: request, item, parts, place of the first
       const long long beyond = x.units - u1;
       a.cuts[blockIdx.x] = {r, item, 1 + (int)((beyond + share - 1) / share), segment != 0};
@@ -934,43 +770,6 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged_attent
     if (a.status && lane == 0) atomicOr(a.status, 64);
   }
   if (__any_sync(htr::kFullWarp, bad) && a.status && lane == 0) atomicOr(a.status, 32);
-}
-
-// Joins the parts of the tiles that were cut: kJoins thread blocks per run of the launch before, a thread per row and four dimensions, eight parts on their way.
-template <int D, int NT>
-constexpr int kJoins = 8 * NT * (D / 4) / kAttThreads;
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAttThreads) paged_attention_join_kernel(const AttentionArgs a) {
-  constexpr int kRows = 8 * NT, kPart = kRows * (D + 2);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  // (not before the wait: thread blocks of a next step's attention that found a place while this one's still ran cost it 35 us of 128)
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int4 cut = a.cuts[blockIdx.x];
-  if (cut.z == 0) return;
-  const Span x(a, cut.x, kRows);
-  const int kvh = cut.y % a.kv_heads, row0 = cut.y / a.kv_heads * kRows, rows = min(x.rows - row0, kRows);
-  const float *head = a.parts + ((size_t)blockIdx.x * 2 + cut.w) * kPart, *tail = a.parts + (size_t)blockIdx.x * 2 * kPart;
-  for (int z = blockIdx.y * kAttThreads + threadIdx.x; z < rows * (D / 4); z += kJoins<D, NT> * kAttThreads) {
-    const int row = z / (D / 4), d = z % (D / 4) * 4;
-    float m = head[kRows * D + row], l = head[kRows * D + kRows + row];
-    float4 y = *reinterpret_cast<const float4*>(head + row * D + d);
-    const auto part = [&](int i) { return tail + (size_t)i * 2 * kPart; };
-    join_parts<8>(cut.z, m, l, y, [&](int i) { return part(i) + kRows * D + row; }, [&](int i) { return part(i) + kRows * D + kRows + row; },
-               [&](int i) { return reinterpret_cast<const float4*>(part(i) + row * D + d); });
-    const float by = l == 0.f ? 0.f : kSumUnit / l;
-    const int i = (row0 + row) / a.group, h = row0 + row - i * a.group;
-    T* dst = static_cast<T*>(a.out) + ((size_t)(x.start + i) * a.q_heads + (size_t)kvh * a.group + h) * D + d;
-    *reinterpret_cast<uint2*>(dst) = {Half<T>::narrow(y.x * by, y.y * by), Half<T>::narrow(y.z * by, y.w * by)};
-  }
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// log2 of a page size that the kernels take, else -1
-int page_shift(int page_size) {
-  for (int s = 4; s <= 7; ++s)
-    if (page_size == 1 << s) return s;
-  return -1;
 }
 
 int attention_blocks(int head_dim, int tiles) {            // what the GPU holds at a time
@@ -990,7 +789,7 @@ int attention_run(const AttentionArgs& a, cudaStream_t st) {
   }
   if (e) return htr::paged_fail(e);
   const int rc = paged_launch(paged_attention_kernel<T, D, NT>, grid, block, 1, kBytes, st, a);
-  return rc != HTR_OK ? rc : paged_launch(paged_attention_join_kernel<T, D, NT>, dim3(grid.x, kJoins<D, NT>), block, 1, 0, st, a);
+  return rc != HTR_OK ? rc : paged_launch(paged_attention_join_kernel<T, D, NT, Work>, dim3(grid.x, kJoins<D, NT>), block, 1, 0, st, a);
 }
 
 template <typename T>
@@ -1017,6 +816,7 @@ int paged_fail(int cuda_error) {
   t_last_cuda = cuda_error;
   return HTR_ERR_CUDA;
 }
+int attention_withhold() { return t_withhold; }
 
 }  // namespace htr
 
