@@ -20,7 +20,8 @@ EXPORTS = ("htr_status_string", "htr_last_cuda_error", "htr_version", "htr_decod
            "htr_linear_workspace_bytes", "htr_linear_counter_bytes", "htr_linear", "htr_linear_ex", "htr_linear_peers", "htr_linear_grouped", "htr_linear_grouped_workspace_bytes", "htr_linear_routed", "htr_linear_static", "htr_linear_padded", "htr_linear_fused", "htr_linear_gemm", "htr_linear_gemm_peers", "htr_linear_gemm_workspace_bytes", "htr_linear_gemm_padded", "htr_linear_route_rows", "htr_route_plan_bytes", "htr_route_plan", "htr_linear_routed_gemm_workspace_bytes", "htr_linear_routed_gemm", "htr_linear_gemm_error_offset", "htr_gemm_withhold_tile", "htr_linear_gemm_shape", "htr_linear_gemm_last_cuda_error", "htr_dequant_w", "htr_viterbi", "htr_viterbi_workspace_bytes", "htr_viterbi_last_cuda_error", "htr_codebook_f32",
            "htr_linear_plan", "htr_set_gemv_kernel", "htr_linear_fault_offset", "htr_linear_peers_signal", "htr_linear_routed_peers", "htr_peer_wait", "htr_peer_barrier", "htr_moe_combine_peers", "htr_moe_weighted_sum", "htr_rank_sum", "htr_dec_add_rmsnorm", "htr_dec_rope_cache", "htr_dec_attention",
            "htr_dec_swiglu", "htr_dec_rope_attention", "htr_page_plan", "htr_paged_append", "htr_paged_attention",
-           "htr_paged_attention_workspace_bytes", "htr_paged_attention_withhold", "htr_paged_last_cuda_error", "htr_sample", "htr_sample_last_cuda_error")
+           "htr_paged_attention_workspace_bytes", "htr_paged_attention_withhold", "htr_paged_last_cuda_error",
+           "htr_paged4_append", "htr_paged4_unpack", "htr_paged4_attention", "htr_paged4_attention_workspace_bytes", "htr_rope_angles", "htr_sample", "htr_sample_last_cuda_error")
 
 
 class HTRError(RuntimeError):
@@ -85,6 +86,12 @@ def _load():
     lib.htr_paged_attention_workspace_bytes.argtypes = [i32] * 8
     lib.htr_paged_attention.argtypes = [vp, i32, i32, vp, vp, i32, vp, i64, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, ctypes.c_float, vp, vp, vp,
                                         sz, vp]
+    lib.htr_paged4_append.argtypes = [vp, i32, i64, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp]
+    lib.htr_paged4_unpack.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, vp, vp, i32, vp]
+    lib.htr_paged4_attention_workspace_bytes.restype = sz
+    lib.htr_paged4_attention_workspace_bytes.argtypes = [i32] * 8
+    lib.htr_paged4_attention.argtypes = lib.htr_paged_attention.argtypes
+    lib.htr_rope_angles.argtypes = [i64, i32, i32, *[ctypes.c_double] * 5, ctypes.c_float, vp, vp, vp]
     lib.htr_paged_attention_withhold.restype = None
     lib.htr_paged_attention_withhold.argtypes = [i32]
     lib.htr_sample.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
@@ -123,7 +130,7 @@ def check(status, what):
         msg = lib.htr_status_string(status).decode()
         if status == -7:
             code = (lib.htr_linear_gemm_last_cuda_error() if what.startswith(("htr_linear_gemm", "htr_route_plan", "htr_linear_routed_gemm")) else
-                    lib.htr_paged_last_cuda_error() if what.startswith("htr_page") else lib.htr_sample_last_cuda_error() if what == "htr_sample" else
+                    lib.htr_paged_last_cuda_error() if what.startswith(("htr_page", "htr_rope")) else lib.htr_sample_last_cuda_error() if what == "htr_sample" else
                     lib.htr_viterbi_last_cuda_error() if what.startswith(("htr_viterbi", "htr_codebook")) else lib.htr_last_cuda_error())
             msg += f" (cudaError {code})"
         raise HTRError(f"{what}: {msg}")

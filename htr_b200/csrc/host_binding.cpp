@@ -52,6 +52,11 @@ struct Entry {
   decltype(&htr_page_plan) page_plan;
   decltype(&htr_paged_append) paged_append;
   decltype(&htr_paged_attention) paged_attention;
+  decltype(&htr_paged4_append) paged4_append;
+  decltype(&htr_paged4_unpack) paged4_unpack;
+  decltype(&htr_paged4_attention) paged4_attention;
+  decltype(&htr_paged4_attention_workspace_bytes) paged4_attention_workspace_bytes;
+  decltype(&htr_rope_angles) rope_angles;
   decltype(&htr_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
   decltype(&htr_sample) sample;
 } g_lib = {};
@@ -545,23 +550,26 @@ bool table_of(const at::Tensor* t, const at::Device& dev, int64_t requests, int6
   return requests == 1 || t->stride(0) >= t->size(1);
 }
 
-// a layer's cache: (k, v, k_scale, v_scale)
+// a layer's cache: (k, v, k_scale, v_scale), in 8 bits with scales of pages or in 4 with scales of tokens
 struct Cache {
-  void *k, *v;
-  float *ks, *vs;
+  void *k, *v, *ks, *vs;
   int pages, heads, page, dim;
+  bool four;
 };
 bool cache_of(PyObject* o, const at::Device& dev, Cache* c) {
   if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
   const at::Tensor* t[4];
   for (int i = 0; i < 4; ++i)
-    if (!(t[i] = tensor(PyTuple_GET_ITEM(o, i))) || !plain(*t[i], dev, i < 2 ? at::kFloat8_e4m3fn : at::kFloat)) return false;
+    if (!(t[i] = tensor(PyTuple_GET_ITEM(o, i)))) return false;
+  const bool four = t[0]->scalar_type() == at::kByte;
+  for (int i = 0; i < 4; ++i)
+    if (!plain(*t[i], dev, i < 2 ? (four ? at::kByte : at::kFloat8_e4m3fn) : four ? at::kBFloat16 : at::kFloat)) return false;
   if (t[0]->dim() != 4 || t[1]->sizes() != t[0]->sizes() || t[0]->size(0) > (1 << 30) || t[0]->size(1) > (1 << 30)) return false;
   for (int i = 2; i < 4; ++i)
-    if (t[i]->dim() != 2 || t[i]->size(0) != t[0]->size(0) || t[i]->size(1) != t[0]->size(1)) return false;
+    if (t[i]->dim() != (four ? 3 : 2) || t[i]->size(0) != t[0]->size(0) || t[i]->size(1) != t[0]->size(1) || (four && t[i]->size(2) != t[0]->size(2))) return false;
   if (t[0]->size(2) > 128 || t[0]->size(3) > 128) return false;
-  *c = {t[0]->data_ptr(), t[1]->data_ptr(), t[2]->data_ptr<float>(), t[3]->data_ptr<float>(), (int)t[0]->size(0), (int)t[0]->size(1),
-        (int)t[0]->size(2), (int)t[0]->size(3)};
+  *c = {t[0]->data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), t[3]->data_ptr(), (int)t[0]->size(0), (int)t[0]->size(1),
+        (int)t[0]->size(2), (int)t[0]->size(3) * (four ? 2 : 1), four};
   return true;
 }
 
@@ -613,9 +621,9 @@ PyObject* py_plan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return all;
 }
 
-// rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status): the rotated queries
+// rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status, layout): the rotated queries
 PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 8) return none();
+  if (n != 9 || !PyUnicode_Check(a[8])) return none();
   const at::Tensor *x = tensor(a[0]), *pos = tensor(a[1]), *slots = tensor(a[2]), *cosv = tensor(a[3]), *sinv = tensor(a[4]);
   Cache c;
   int hq;
@@ -626,16 +634,23 @@ PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!cache_of(a[5], where, &c) || !int_of(a[6], &hq) || hq < 1 || cols != ((int64_t)hq + 2 * (int64_t)c.heads) * c.dim || T < 1 || T > (1 << 30)) return none();
   if (!vector_of(pos, where, at::kInt) || pos->numel() != T || !vector_of(slots, where, at::kInt) || slots->numel() != T || !cosv || !sinv ||
       !plain(*cosv, where, at::kFloat) || !plain(*sinv, where, at::kFloat) || cosv->dim() != 2 || cosv->sizes() != sinv->sizes() ||
-      cosv->size(1) != c.dim / 2 || cosv->size(0) > (1 << 30) || !optional_of(a[7], where, at::kInt, 1, &status))
+      cosv->size(1) > c.dim / 2 || (!c.four && cosv->size(1) != c.dim / 2) || cosv->size(0) > (1 << 30) || !optional_of(a[7], where, at::kInt, 1, &status))
     return none();
+  const bool halves = PyUnicode_CompareWithASCIIString(a[8], "half") == 0;
+  if (halves ? !c.four : PyUnicode_CompareWithASCIIString(a[8], "interleaved") != 0) return none();
   const int64_t stride = T == 1 ? cols : x->stride(0);
   const int dt = dtype_code(x->scalar_type()), dev = x->get_device();
   OnDevice on(dev);
   at::Tensor q = at::detail::empty_cuda({T, (int64_t)hq, (int64_t)c.dim}, x->scalar_type(), where, std::nullopt);
-  if (g_lib.paged_append(x->const_data_ptr(), dt, stride, pos->const_data_ptr<int>(), slots->const_data_ptr<int>(), (int)T, cosv->const_data_ptr<float>(),
-                         sinv->const_data_ptr<float>(), (int)cosv->size(0), hq, c.heads, c.dim, c.k, c.v, c.ks, c.vs, c.pages, c.page, q.data_ptr(),
-                         static_cast<int*>(status), c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
-    return none();
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev).stream();
+  const int rc =
+      c.four ? g_lib.paged4_append(x->const_data_ptr(), dt, stride, pos->const_data_ptr<int>(), slots->const_data_ptr<int>(), (int)T, cosv->const_data_ptr<float>(),
+                                   sinv->const_data_ptr<float>(), (int)cosv->size(0), 2 * (int)cosv->size(1), halves, hq, c.heads, c.dim, c.k, c.v, c.ks, c.vs,
+                                   c.pages, c.page, q.data_ptr(), static_cast<int*>(status), st)
+             : g_lib.paged_append(x->const_data_ptr(), dt, stride, pos->const_data_ptr<int>(), slots->const_data_ptr<int>(), (int)T, cosv->const_data_ptr<float>(),
+                                  sinv->const_data_ptr<float>(), (int)cosv->size(0), hq, c.heads, c.dim, c.k, c.v, static_cast<float*>(c.ks),
+                                  static_cast<float*>(c.vs), c.pages, c.page, q.data_ptr(), static_cast<int*>(status), st);
+  if (rc != HTR_OK) return none();
   return THPVariable_Wrap(std::move(q));
 }
 
@@ -668,14 +683,64 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!o || !plain(*o, where, q->scalar_type()) || o->sizes() != q->sizes()) return none();
     y = *o;
   }
-  const size_t need = g_lib.paged_attention_workspace_bytes((int)T, (int)R, (int)hq, c.heads, c.dim, most, (int)tables->size(1), c.page);
+  const size_t need = (c.four ? g_lib.paged4_attention_workspace_bytes : g_lib.paged_attention_workspace_bytes)((int)T, (int)R, (int)hq, c.heads, c.dim, most, (int)tables->size(1), c.page);
   if (need) work = at::detail::empty_cuda({(int64_t)need}, at::kByte, where, std::nullopt);
-  if (g_lib.paged_attention(q->const_data_ptr(), dt, (int)T, starts->const_data_ptr<int>(), seen->const_data_ptr<int>(), (int)R, tables->const_data_ptr<int>(),
-                            stride, (int)tables->size(1), c.k, c.v, c.ks, c.vs, c.pages, c.page, (int)hq, c.heads, c.dim, most, (float)scale, y.data_ptr(),
-                            static_cast<int*>(status), need ? work.data_ptr() : nullptr, need, c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev).stream();
+  const auto call = [&](auto entry, auto ks, auto vs) {
+    return entry(q->const_data_ptr(), dt, (int)T, starts->const_data_ptr<int>(), seen->const_data_ptr<int>(), (int)R, tables->const_data_ptr<int>(), stride,
+                 (int)tables->size(1), c.k, c.v, ks, vs, c.pages, c.page, (int)hq, c.heads, c.dim, most, (float)scale, y.data_ptr(),
+                 static_cast<int*>(status), need ? work.data_ptr() : nullptr, need, st);
+  };
+  if ((c.four ? call(g_lib.paged4_attention, c.ks, c.vs) : call(g_lib.paged_attention, static_cast<float*>(c.ks), static_cast<float*>(c.vs))) != HTR_OK)
     return none();
   if (a[7] != Py_None) return Py_NewRef(a[7]);
   return THPVariable_Wrap(std::move(y));
+}
+
+PyObject* pair_of(at::Tensor&& x, at::Tensor&& y) {
+  PyObject* both = PyTuple_New(2);
+  if (!both) return nullptr;
+  PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(x)));
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(y)));
+  return both;
+}
+
+// unpack(cache, pages, dtype): (keys, values)
+PyObject* py_unpack(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3 || !THPDtype_Check(a[2])) return none();
+  const at::Tensor* pages = tensor(a[1]);
+  Cache c;
+  if (!pages || !pages->is_cuda()) return none();
+  const at::Device where = pages->device();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[2])->scalar_type;
+  const int dt = dtype_code(type), dev = pages->get_device();
+  const int64_t count = pages->numel();
+  if (!cache_of(a[0], where, &c) || !c.four || !vector_of(pages, where, at::kInt) || dt < 0 || count > (1 << 30)) return none();
+  OnDevice on(dev);
+  at::Tensor out[2];
+  for (at::Tensor& t : out) t = at::detail::empty_cuda({count, (int64_t)c.heads, (int64_t)c.page, (int64_t)c.dim}, type, where, std::nullopt);
+  if (g_lib.paged4_unpack(c.k, c.v, c.ks, c.vs, c.pages, c.heads, c.page, c.dim, pages->const_data_ptr<int>(), (int)count, out[0].data_ptr(), out[1].data_ptr(), dt,
+                          c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+    return none();
+  return pair_of(std::move(out[0]), std::move(out[1]));
+}
+
+// rope_angles(rows, dim, theta, first, factor, original, low, high, magnitude, device index): (cosines, sines)
+PyObject* py_rope_angles(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int rows, dim, first, dev;
+  double theta, how[5];
+  if (n != 10 || !int_of(a[0], &rows) || !int_of(a[1], &dim) || !float_of(a[2], &theta) || !int_of(a[3], &first) || !int_of(a[9], &dev)) return none();
+  for (int i = 0; i < 5; ++i)
+    if (!float_of(a[4 + i], &how[i])) return none();
+  if (rows < 1 || dim < 2 || dim > 256 || dev < 0 || dev >= c10::cuda::device_count()) return none();
+  OnDevice on(dev);
+  const at::Device where(at::kCUDA, (c10::DeviceIndex)dev);
+  at::Tensor out[2];
+  for (at::Tensor& t : out) t = at::detail::empty_cuda({(int64_t)rows, (int64_t)(dim / 2)}, at::kFloat, where, std::nullopt);
+  if (g_lib.rope_angles(first, rows, dim, theta, how[0], how[1], how[2], how[3], (float)how[4], out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+                        c10::cuda::getCurrentCUDAStream(dev).stream()) != HTR_OK)
+    return none();
+  return pair_of(std::move(out[0]), std::move(out[1]));
 }
 
 // sample(logits, u, temperature, top_k, top_p, min_p): (tokens, logprobs); settings are tensors or None
@@ -754,8 +819,15 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   g_lib.paged_attention = reinterpret_cast<decltype(g_lib.paged_attention)>(at_name("htr_paged_attention"));
   g_lib.paged_attention_workspace_bytes =
       reinterpret_cast<decltype(g_lib.paged_attention_workspace_bytes)>(at_name("htr_paged_attention_workspace_bytes"));
+  g_lib.paged4_append = reinterpret_cast<decltype(g_lib.paged4_append)>(at_name("htr_paged4_append"));
+  g_lib.paged4_unpack = reinterpret_cast<decltype(g_lib.paged4_unpack)>(at_name("htr_paged4_unpack"));
+  g_lib.paged4_attention = reinterpret_cast<decltype(g_lib.paged4_attention)>(at_name("htr_paged4_attention"));
+  g_lib.paged4_attention_workspace_bytes =
+      reinterpret_cast<decltype(g_lib.paged4_attention_workspace_bytes)>(at_name("htr_paged4_attention_workspace_bytes"));
+  g_lib.rope_angles = reinterpret_cast<decltype(g_lib.rope_angles)>(at_name("htr_rope_angles"));
   g_lib.sample = reinterpret_cast<decltype(g_lib.sample)>(at_name("htr_sample"));
   if (!g_lib.page_plan || !g_lib.paged_append || !g_lib.paged_attention || !g_lib.paged_attention_workspace_bytes || !g_lib.sample ||
+      !g_lib.paged4_append || !g_lib.paged4_unpack || !g_lib.paged4_attention || !g_lib.paged4_attention_workspace_bytes || !g_lib.rope_angles ||
       !g_lib.linear_workspace_bytes || !g_lib.linear_gemm_workspace_bytes || !g_lib.add_rmsnorm || !g_lib.swiglu || !g_lib.rope_cache || !g_lib.attention || !g_lib.rope_attention || !g_lib.linear_routed || !g_lib.linear_routed_gemm || !g_lib.route_plan_bytes || !g_lib.route_plan || !g_lib.moe_weighted_sum ||
       !g_lib.linear_gemm_padded || !g_lib.route_rows || !g_lib.linear_ex || !g_lib.linear_gemm || !g_lib.linear_padded || !g_lib.linear_fused) {
     PyErr_SetString(PyExc_ImportError, "bind: an entry point of libhtr_b200 is missing");
@@ -789,6 +861,8 @@ PyMethodDef g_methods[] = {
     fast<py_plan_step>("plan_step"),
     fast<py_rope_append>("rope_append"),
     fast<py_attention>("attention"),
+    fast<py_unpack>("unpack"),
+    fast<py_rope_angles>("rope_angles"),
     fast<py_sample>("sample"),
     {"set_workspace", py_set_workspace, METH_VARARGS, nullptr},
     {"bind", py_bind, METH_O, nullptr},

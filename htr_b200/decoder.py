@@ -14,7 +14,7 @@ most 8 rows (decoding) fold the norms, the SwiGLU and the residual adds into the
 (`ops.linear_fused`) and, for a single token, the rotary embedding and cache write into the attention kernel: five launches
 per layer.  A decode step reads its position from a device tensor, so one CUDA graph captured once serves every step.
 
-Many sequences at once are served from a paged 8-bit cache (`paged.PagedCache`): `forward_paged` is one step of all of them, prompts and single
+Many sequences at once are served from a paged cache of 8 or 4 bits (`paged.PagedCache`): `forward_paged` is one step of all of them, prompts and single
 tokens together, and `generate_batch` runs prompts of different lengths to the end, its decoding steps a CUDA graph that plans the
 pages, appends, attends and samples (`sampling.sample`) without the host.
 """
@@ -23,7 +23,7 @@ import math
 
 import torch
 
-from . import _lib, ops, paged, sampling, wire
+from . import _lib, ops, paged, rotary, sampling, wire
 
 
 @dataclasses.dataclass
@@ -363,12 +363,17 @@ class PackedDecoder:
             raise _lib.HTRError(f"a decode step used a position outside the {self.cfg.max_len}-row caches (status {int(self.status.item())})")
         return out, ev[0].elapsed_time(ev[1]) * 1e-3, ev[1].elapsed_time(ev[2]) * 1e-3
 
-    def paged_cache(self, requests, pages, page_size=64, max_len=None):
+    def paged_cache(self, requests, pages, page_size=64, max_len=None, bits=8, **stretch):
         """A paged cache for this model: `pages` pages of `page_size` tokens shared by `requests` sequences of at most max_len tokens (as many as the
-        pages hold by default; not bound by cfg.max_len).  Beside the pages it holds the angles of max_len positions, 4 * head_dim bytes each."""
+        pages hold by default; not bound by cfg.max_len), in 8 or 4 bits.  Beside the pages it holds the angles of max_len positions, 4 * head_dim bytes each;
+        `stretch`: how `rotary.angles` lays them out for contexts longer than the model has learned (factor, original, low, high, magnitude)."""
         max_len = pages * page_size if max_len is None else max_len
-        cache = paged.PagedCache(self.cfg.layers, self.cfg.kv_heads, self.cfg.head_dim, pages, page_size, requests, max_len, self.device)
-        cache.cos, cache.sin = self._far_angles(cache.tables.shape[1] * page_size)
+        cache = paged.PagedCache(self.cfg.layers, self.cfg.kv_heads, self.cfg.head_dim, pages, page_size, requests, max_len, self.device, bits)
+        rows = cache.tables.shape[1] * page_size
+        if bits == 8 and not stretch:
+            cache.cos, cache.sin = self._far_angles(rows)
+        else:
+            cache.cos, cache.sin = rotary.angles(rows, self.cfg.head_dim, self.cfg.rope_theta, device=self.device, **stretch)
         return cache
 
     def forward_paged(self, ids, plan, cache, max_new):
@@ -426,18 +431,18 @@ class PackedDecoder:
 
     @torch.no_grad()
     def generate_batch(self, prompts, new_tokens, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0, eos=None, chunk=4096, page_size=64, cache=None,
-                       use_graph=True):
+                       use_graph=True, bits=8):
         """Continues all `prompts` (1-D tensors of ids, each at least one) by new_tokens tokens, or up to and with `eos`.
 
         The settings of `sampling.sample` are one for all or one per prompt (temperature 0: greedy).  Prompts go through in steps of at most `chunk`
         tokens, and then one token of each sequence a step (one CUDA graph).  `cache`: one of `paged_cache` with no sequence in it, and room for as
-        many as there are prompts; its pages come back at the end.  Returns (tokens [prompts, new_tokens], -1 behind an eos; their log-probabilities)."""
+        many as there are prompts; its pages come back at the end (without one: in `bits` bits).  Returns (tokens [prompts, new_tokens], -1 behind an eos; their log-probabilities)."""
         dev, R = self.device, len(prompts)
         lens = [int(p.numel()) for p in prompts]
         if min(lens, default=0) < 1 or new_tokens < 1 or chunk < 1:
             raise _lib.HTRError("generate_batch: wants at least one prompt of at least one token, new_tokens >= 1 and chunk >= 1")
         if cache is None:
-            cache = self.paged_cache(R, sum(-(-(n + new_tokens) // page_size) for n in lens), page_size, max(lens) + new_tokens)
+            cache = self.paged_cache(R, sum(-(-(n + new_tokens) // page_size) for n in lens), page_size, max(lens) + new_tokens, bits)
         elif cache.lengths.numel() != R or cache.cos is None or int(cache.lengths.max()) > 0:
             raise _lib.HTRError(f"generate_batch: the cache must be one of paged_cache for {R} requests, with none in it")
         elif int(cache.status):

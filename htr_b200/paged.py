@@ -1,8 +1,10 @@
-"""Many sequences in one paged 8-bit cache: the operators of a serving step between the packed linears.
+"""Many sequences in one paged cache of 8 or 4 bits: the operators of a serving step between the packed linears.
 
   plan_step     page tables, positions and slots of a step, built on the GPU from the requests' lengths
-  rope_append   rotary embedding, and the step's keys and values into the cache (e4m3, one power-of-two scale per page and head)
+  rope_append   rotary embedding, and the step's keys and values into the cache (e4m3, one power-of-two scale per page and head; or
+                e2m1, one bf16 scale per token and head, with a Hadamard transform of queries and keys)
   attention     grouped-query causal attention over the cache, from single tokens to prompts
+  unpack        pages of the 4-bit cache as keys and values
   PagedCache    the buffers that a server keeps: caches of all layers, page tables, free pages
 
 Requests are rows: a step gives each of them as many tokens as it likes (none, one, a prompt), and the step's tokens stand one request
@@ -13,7 +15,7 @@ import typing
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
@@ -24,6 +26,17 @@ _HALF = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 class LayerCache(typing.NamedTuple):
     """One layer's cache: k, v float8_e4m3fn [pages, kv_heads, page_size, head_dim]; k_scale, v_scale float32 [pages, kv_heads], powers of
     two.  The value of an element is element * scale."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+class LayerCache4(typing.NamedTuple):
+    """One layer's cache in 4 bits: k, v uint8 [pages, kv_heads, page_size, head_dim / 2], two e2m1 codes in a byte, the even dimension in its low half;
+    k_scale, v_scale bfloat16 [pages, kv_heads, page_size], between 2^-100 and 2^119 (NaN: so are the token's values).  The value of an element is
+    its code's (0, 0.5, 1, 1.5, 2, 3, 4, 6, and negative with the highest bit) * scale.  A key is held as H k / 8, H the Hadamard matrix of head_dim rows in
+    Sylvester's order; a query that meets it has to be H q * 8 / head_dim, as `rope_append` returns it."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -60,6 +73,27 @@ def _status(what, status, dev):
 
 
 def _cache(what, cache, dev):
+    """Pages, heads, page size, head dimensions of a layer's cache, and whether it is in 4 bits."""
+    if isinstance(cache, LayerCache4):
+        return *_cache4(what, cache, dev), True
+    return *_cache8(what, cache, dev), False
+
+
+def _cache4(what, cache, dev):
+    k, v, ks, vs = cache
+    if k.dtype != torch.uint8 or k.dim() != 4 or k.device != dev or not k.is_contiguous() or v.dtype != k.dtype or v.shape != k.shape or \
+            v.device != dev or not v.is_contiguous():
+        raise _lib.HTRError(f"{what}: k and v must be contiguous uint8 [pages, kv_heads, page_size, head_dim / 2] on {dev}")
+    pages, heads, page, dim = *k.shape[:3], 2 * k.shape[3]
+    if pages < 1 or heads < 1 or page not in PAGE_SIZES or dim not in HEAD_DIMS:
+        raise _lib.HTRError(f"{what}: pages of {PAGE_SIZES} tokens and heads of {HEAD_DIMS} are supported, got {page} and {dim}")
+    for s in (ks, vs):
+        if s.dtype != torch.bfloat16 or s.device != dev or tuple(s.shape) != (pages, heads, page) or not s.is_contiguous():
+            raise _lib.HTRError(f"{what}: scales must be contiguous bfloat16 [{pages}, {heads}, {page}] on {dev}")
+    return pages, heads, page, dim
+
+
+def _cache8(what, cache, dev):
     k, v, ks, vs = cache
     if k.dtype != torch.float8_e4m3fn or k.dim() != 4 or k.device != dev or not k.is_contiguous() or v.dtype != k.dtype or v.shape != k.shape or \
             v.device != dev or not v.is_contiguous():
@@ -117,11 +151,17 @@ def plan_step(lengths, new, tables, free, count, page_size, max_tokens, lengths_
     return StepPlan(starts, positions, slots, seen, lengths_out, count_out)
 
 
-def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None):
-    """Rotary embedding of a step's queries and keys, and its keys and values into one layer's cache.
+def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None, layout="interleaved"):
+    """Rotary embedding of a step's queries and keys, and its keys and values into one layer's cache (LayerCache or LayerCache4).
 
     qkv [tokens, (q_heads + 2 kv_heads) * head_dim] bf16 or fp16 (rows may be strided); positions, slots [tokens] as `plan_step` gives them; cos, sin
     float32 [rows, head_dim / 2], a row per position, for interleaved pairs.  Returns the rotated queries [tokens, q_heads, head_dim].
+
+    Into a cache of 4 bits, pairs may also be halves (layout "half": dimensions i and i + r / 2), and r, twice the columns of cos and sin, a part of the
+    head that is a multiple of 16: the first r dimensions are rotated.  The queries come back as H q * 8 / head_dim for the keys of such a cache (see
+    LayerCache4; fp16 ones whose sums leave its range become infinite).  A token's scale is bf16(largest / 6), its codes are the nearest, ties to the even code; infinities are held as
+    the largest value (6 * 2^119, or what the rest of a key's transform makes of them), and a row of a head that has a NaN is NaN as a whole.  A token whose slot does not lie above those of its page
+    among the page_size - 1 tokens before it is not written, and its query is zero (status 16).  What follows is of the cache of 8 bits.
 
     A page's scale is the smallest power of two (at least 2^-100) under which all of its tokens lie within e4m3 (448); it begins anew with the
     page's first place, and where a later token makes it grow the older ones are rescaled.  Infinities are held as the largest value, NaN as NaN.
@@ -129,14 +169,16 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None):
     The tokens of one page stand one after the other in rising slots, as `plan_step` lays them out, within page_size tokens of the step (tokens that are not
     written may lie between them); from a slot that does not rise on, that page's are not written (status 16)."""
     what = "rope_append"
-    q = _host.rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status)
+    q = _host.rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status, layout)
     if q is not None:
         return q
     if not qkv.is_cuda:
         raise _lib.HTRError("rope_append has no CPU path: tensors must live on a CUDA device")
     dev = qkv.device
-    pages, kv_heads, page, dim = _cache(what, cache, dev)
+    pages, kv_heads, page, dim, four = _cache(what, cache, dev)
     q_heads = int(q_heads)
+    if layout not in ("interleaved", "half") or (layout == "half" and not four):
+        raise _lib.HTRError(f"rope_append: layout is \"interleaved\", or for a cache of 4 bits \"half\", got {layout!r}")
     if qkv.dtype not in _HALF or qkv.dim() != 2 or q_heads < 1 or qkv.shape[1] != (q_heads + 2 * kv_heads) * dim:
         raise _lib.HTRError(f"rope_append: qkv must be bf16 or fp16 [tokens, {(q_heads + 2 * kv_heads) * dim}]")
     T = qkv.shape[0]
@@ -145,12 +187,20 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None):
     _int32(what, "positions", positions, dev, T)
     _int32(what, "slots", slots, dev, T)
     for t in (cos, sin):
-        if t.dtype != torch.float32 or t.device != dev or t.dim() != 2 or t.shape[1] != dim // 2 or t.shape != cos.shape or not t.is_contiguous():
-            raise _lib.HTRError(f"rope_append: cos and sin must be contiguous float32 [positions, {dim // 2}] on {dev}")
+        if t.dtype != torch.float32 or t.device != dev or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous() or \
+                (t.shape[1] not in range(8, dim // 2 + 1, 8) if four else t.shape[1] != dim // 2):
+            raise _lib.HTRError(f"rope_append: cos and sin must be contiguous float32 [positions, {'a multiple of 8 up to ' if four else ''}{dim // 2}] on {dev}")
     q = torch.empty((T, q_heads, dim), dtype=qkv.dtype, device=dev)
     if T == 0:
         return q
     with torch.cuda.device(dev):
+        if four:
+            rc = _lib.lib.htr_paged4_append(qkv.data_ptr(), _HALF[qkv.dtype], max(qkv.stride(0), qkv.shape[1]), positions.data_ptr(), slots.data_ptr(), T,
+                                            cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(layout == "half"), q_heads, kv_heads, dim,
+                                            *[t.data_ptr() for t in cache], pages, page, q.data_ptr(), _status(what, status, dev),
+                                            torch.cuda.current_stream(dev).cuda_stream)
+            _lib.check(rc, "htr_paged4_append")
+            return q
         rc = _lib.lib.htr_paged_append(qkv.data_ptr(), _HALF[qkv.dtype], max(qkv.stride(0), qkv.shape[1]), positions.data_ptr(), slots.data_ptr(), T,
                                        cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_heads, kv_heads, dim, cache[0].data_ptr(), cache[1].data_ptr(),
                                        cache[2].data_ptr(), cache[3].data_ptr(), pages, page, q.data_ptr(), _status(what, status, dev),
@@ -160,7 +210,7 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None):
 
 
 def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, status=None):
-    """Causal grouped-query attention of a step's tokens over one layer's cache.
+    """Causal grouped-query attention of a step's tokens over one layer's cache (LayerCache, or LayerCache4 with queries that `rope_append` made for it).
 
     q [tokens, q_heads, head_dim] bf16 or fp16; starts [requests + 1] and seen [requests] as `plan_step` gives them: of the n tokens
     [starts[r], starts[r + 1]) of request r the i-th stands at position seen[r] - n + i and sees the cached positions up to its own; one that
@@ -181,7 +231,7 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     if not q.is_cuda:
         raise _lib.HTRError("attention has no CPU path: tensors must live on a CUDA device")
     dev, R = q.device, seen.numel()
-    pages, kv_heads, page, dim = _cache(what, cache, dev)
+    pages, kv_heads, page, dim, four = _cache(what, cache, dev)
     if q.dtype not in _HALF or q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % kv_heads:
         raise _lib.HTRError(f"attention: q must be bf16 or fp16 [tokens, a multiple of {kv_heads} heads, {dim}]")
     T, q_heads = q.shape[:2]
@@ -200,31 +250,58 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
         return out
     most = min(int(max_new), T)
     with torch.cuda.device(dev):
-        need = _lib.lib.htr_paged_attention_workspace_bytes(T, R, q_heads, kv_heads, dim, most, tables.shape[1], page)      # (by the device's SMs)
+        need_of = _lib.lib.htr_paged4_attention_workspace_bytes if four else _lib.lib.htr_paged_attention_workspace_bytes
+        need = need_of(T, R, q_heads, kv_heads, dim, most, tables.shape[1], page)      # (by the device's SMs)
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rc = _lib.lib.htr_paged_attention(q.data_ptr(), _HALF[q.dtype], T, starts.data_ptr(), seen.data_ptr(), R, tables.data_ptr(), stride,
-                                          tables.shape[1], cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(), pages,
-                                          page, q_heads, kv_heads, dim, most, float(dim ** -0.5 if scale is None else scale), out.data_ptr(),
-                                          _status(what, status, dev), None if work is None else work.data_ptr(), need,
-                                          torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "htr_paged_attention")
+        entry = _lib.lib.htr_paged4_attention if four else _lib.lib.htr_paged_attention
+        rc = entry(q.data_ptr(), _HALF[q.dtype], T, starts.data_ptr(), seen.data_ptr(), R, tables.data_ptr(), stride, tables.shape[1], cache[0].data_ptr(),
+                   cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(), pages, page, q_heads, kv_heads, dim, most,
+                   float(dim ** -0.5 if scale is None else scale), out.data_ptr(), _status(what, status, dev), None if work is None else work.data_ptr(), need,
+                   torch.cuda.current_stream(dev).cuda_stream)
+        _lib.check(rc, "htr_paged4_attention" if four else "htr_paged_attention")
     return out
+
+
+def unpack(cache, pages, dtype=torch.bfloat16):
+    """The keys and values that pages of a LayerCache4 stand for: (k, v) [len(pages), kv_heads, page_size, head_dim] in dtype (bf16, fp16 or float32), rounded
+    once; keys are turned back (H k / 8 to k; float32 sums).  pages: int32; one that is none gives zeros."""
+    both = _host.unpack(cache, pages, dtype)
+    if both is not None:
+        return both
+    if not pages.is_cuda:
+        raise _lib.HTRError("unpack has no CPU path: tensors must live on a CUDA device")
+    dev = pages.device
+    if not isinstance(cache, LayerCache4):
+        raise _lib.HTRError("unpack: wants a LayerCache4")
+    count, kv_heads, page, dim = _cache4("unpack", cache, dev)
+    _int32("unpack", "pages", pages, dev, pages.numel())
+    if dtype not in ops._DTYPES:
+        raise _lib.HTRError("unpack: dtype must be bf16, fp16 or float32")
+    out = [torch.empty((pages.numel(), kv_heads, page, dim), dtype=dtype, device=dev) for _ in range(2)]
+    with torch.cuda.device(dev):
+        rc = _lib.lib.htr_paged4_unpack(*[t.data_ptr() for t in cache], count, kv_heads, page, dim, pages.data_ptr(), pages.numel(), out[0].data_ptr(),
+                                        out[1].data_ptr(), ops._DTYPES[dtype], torch.cuda.current_stream(dev).cuda_stream)
+        _lib.check(rc, "htr_paged4_unpack")
+    return tuple(out)
 
 
 class PagedCache:
     """What a server keeps from step to step: the caches of all layers, the requests' page tables and lengths, and the free pages."""
 
-    def __init__(self, layers, kv_heads, head_dim, pages, page_size, requests, max_len, device):
+    def __init__(self, layers, kv_heads, head_dim, pages, page_size, requests, max_len, device, bits=8):
         if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
             raise _lib.HTRError(f"PagedCache: pages of {PAGE_SIZES} tokens and heads of {HEAD_DIMS} are supported, got {page_size} and {head_dim}")
         if min(layers, kv_heads, pages, requests, max_len) < 1:
             raise _lib.HTRError("PagedCache: layers, kv_heads, pages, requests and max_len must be positive")
-        shape = (layers, pages, kv_heads, page_size, head_dim)
-        self.page_size, self.device = page_size, device
-        self.k = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
-        self.v = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
-        self.k_scale = torch.ones(shape[:3], dtype=torch.float32, device=device)
-        self.v_scale = torch.ones(shape[:3], dtype=torch.float32, device=device)
+        if bits not in (4, 8):
+            raise _lib.HTRError(f"PagedCache: 8 or 4 bits are supported, got {bits}")
+        shape = (layers, pages, kv_heads, page_size, head_dim * bits // 8)
+        self.page_size, self.device, self.bits = page_size, device, bits
+        self.k, self.v = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+        if bits == 8:
+            self.k, self.v = self.k.view(torch.float8_e4m3fn), self.v.view(torch.float8_e4m3fn)
+        scales = (shape[:3], torch.float32) if bits == 8 else (shape[:4], torch.bfloat16)
+        self.k_scale, self.v_scale = (torch.ones(scales[0], dtype=scales[1], device=device) for _ in range(2))
         self.tables = torch.full((requests, -(-max_len // page_size)), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
         self.free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device)       # page 0 is taken first
@@ -233,7 +310,7 @@ class PagedCache:
         self.cos = self.sin = None                            # angles of the positions, where a model lays them out (PackedDecoder.paged_cache)
 
     def layer(self, i):
-        return LayerCache(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i])
+        return (LayerCache if self.bits == 8 else LayerCache4)(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i])
 
     def plan(self, new, max_tokens):
         """`plan_step` on this cache's own buffers, which are updated in place: new [requests] int32, tokens that each adds (negative: it is over)."""

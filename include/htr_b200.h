@@ -333,6 +333,34 @@ int htr_paged_attention(const void* q, int dtype, int tokens, const int* starts,
 void htr_paged_attention_withhold(int block);
 int htr_paged_last_cuda_error(void);
 
+/* The same cache in 4 bits.  Keys and values [pages][kv_heads][page_size][head_dim / 2], two e2m1 codes in a byte, the even dimension in its low half, with
+ * bf16 scales [pages][kv_heads][page_size] (at least 2^-100, at most 2^119; NaN: so are the token's values).  Keys are held as H k / 8 (H: the head_dim x
+ * head_dim Hadamard matrix in Sylvester's order), so queries come as H q * 8 / head_dim, whose products with them are q k.
+ *
+ * htr_paged4_append: as htr_paged_append, into such a cache.  The first rotary_dim dimensions of a head (a multiple of 16) are rotated, angles cosv / sinv
+ * [angle_rows][rotary_dim / 2]; pairs are neighbours, or where `halves` is set dimensions i and i + rotary_dim / 2.  A token's scale is that of its largest
+ * element, bf16(largest / 6), its codes are the nearest, ties to the even code; infinities become the largest value, and with a NaN the whole row of a head
+ * is NaN.  A token with slot -1 is not written and its q row is zero; so is one whose slot or position lies outside, or whose slot does not lie above those of
+ * its page among the page_size - 1 tokens before it (status 16).  Tokens of one page lie within page_size tokens, as htr_page_plan lays them out.
+ * htr_paged4_unpack: the pages ids[count] as values [count][kv_heads][page_size][head_dim] of any HTR_DTYPE_*, keys turned back; a page that is none: zeros.
+ * htr_paged4_attention: as htr_paged_attention, with queries as htr_paged4_append gives them. */
+int htr_paged4_append(const void* qkv, int dtype, int64_t row_stride, const int* positions, const int* slots, int tokens, const float* cosv,
+                      const float* sinv, int angle_rows, int rotary_dim, int halves, int q_heads, int kv_heads, int head_dim, void* k_cache, void* v_cache,
+                      void* k_scale, void* v_scale, int pages, int page_size, void* q_out, int* status, htr_stream_t stream);
+int htr_paged4_unpack(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale, int pages, int kv_heads, int page_size, int head_dim,
+                      const int* ids, int count, void* k_out, void* v_out, int dtype, htr_stream_t stream);
+size_t htr_paged4_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new, int table_width, int page_size);
+int htr_paged4_attention(const void* q, int dtype, int tokens, const int* starts, const int* seen, int requests, const int* tables,
+                         int64_t table_stride, int table_width, const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                         int pages, int page_size, int q_heads, int kv_heads, int head_dim, int max_new, float scale, void* out, int* status,
+                         void* workspace, size_t workspace_bytes, htr_stream_t stream);
+/* Angles of the positions first ... first + rows - 1 for a rotary embedding of dim dimensions (even, at most 256): cosv and sinv [rows][dim / 2] = magnitude *
+ * cos and sin of position * theta^(-2 i / dim) * slow_i.  slow_i = 1 / factor where original is 0; else it is 1 for pairs that turn at least `high` times within
+ * `original` positions, 1 / factor for those that turn at most `low` times, and lies linearly between in between.  Positions are below 2^31; the error is some
+ * 2^-23 of magnitude, and 2^-53 of the angle. */
+int htr_rope_angles(int64_t first, int rows, int dim, double theta, double factor, double original, double low, double high, float magnitude,
+                    float* cosv, float* sinv, htr_stream_t stream);
+
 /* One token per row of logits[rows][vocab] (rows row_stride elements apart, any of HTR_DTYPE_*; vocab <= 2^20) from a uniform number u[row] in
  * [0, 1).  Tokens are ordered by logit, ties by index; w = exp((logit - largest) / temperature).  Kept is the shortest of: the first top_k
  * (<= 0: all); the shortest beginning of those with at least top_p of their weight (>= 1: all); those with w >= min_p (<= 0: all); at
