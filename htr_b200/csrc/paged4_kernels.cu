@@ -33,12 +33,6 @@ __device__ __forceinline__ uint32_t to_e2m1(const float (&v)[8]) {
       : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
-// a byte's two codes as fp16, each of the four
-__device__ __forceinline__ void from_e2m1(uint32_t w, uint32_t (&r)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
-}
 __device__ __forceinline__ float of_bf16(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
 // A row's D dimensions, 8 a lane, times the Hadamard matrix; by whole warps.
@@ -622,6 +616,7 @@ int htr_paged4_unpack(const void* k_cache, const void* v_cache, const void* k_sc
 
 size_t htr_paged4_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int max_new, int table_width, int page_size) {
   if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_new < 1 || table_width < 1 || page_shift(page_size) < 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  if (attention4_tc_serves(tokens, requests, q_heads, q_heads / kv_heads, max_new, (long long)table_width * page_size, head_dim)) return attention_tc_workspace(head_dim);
   const int tiles = attention_tiles(q_heads / kv_heads, max_new);
   const size_t rows = 8 * tiles;
   return attention_blocks(head_dim, tiles) * (2 * rows * (head_dim + 2) * sizeof(float) + sizeof(int4));
@@ -650,6 +645,7 @@ int htr_paged4_attention(const void* q, int dtype, int tokens, const int* starts
                      static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), static_cast<const float*>(k_scale),
                      static_cast<const float*>(v_scale), pages, shift, scale * 1.4426950408889634f, out, status, nullptr, cuts, attention_withhold()};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (attention4_tc_serves(tokens, requests, q_heads, a.group, max_new, (long long)table_width * page_size, head_dim)) return attention4_tc_run(a, dtype, head_dim, workspace, st);
   a.parts = reinterpret_cast<float*>(cuts + attention_blocks(head_dim, attention_tiles(a.group, max_new)));
   return dtype == HTR_DTYPE_BF16 ? attention_of<__nv_bfloat16>(a, head_dim, max_new, st) : attention_of<__half>(a, head_dim, max_new, st);
 }

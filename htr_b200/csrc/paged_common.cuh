@@ -64,6 +64,12 @@ __device__ __forceinline__ uint32_t from_e4m3(uint32_t two) {   // two e4m3 in t
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
   return r;
 }
+// a byte's two codes as fp16, each of the four
+__device__ __forceinline__ void from_e2m1(uint32_t w, uint32_t (&r)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+}
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {     // 0xFF where a byte is one of e4m3's NaN
   return __vcmpeq4(v & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
 }
@@ -173,5 +179,7 @@ __device__ __forceinline__ int query_exponent(float most, int top) {
 bool attention_tc_serves(int tokens, int requests, int q_heads, int group, int max_new, long long width, int head_dim);
 size_t attention_tc_workspace(int head_dim);
 int attention_tc_run(const AttentionArgs& a, int dtype, int head_dim, void* workspace, cudaStream_t st);
+bool attention4_tc_serves(int tokens, int requests, int q_heads, int group, int max_new, long long width, int head_dim);     // the same over the cache of 4 bits
+int attention4_tc_run(const AttentionArgs& a, int dtype, int head_dim, void* workspace, cudaStream_t st);
 
 }  // namespace htr

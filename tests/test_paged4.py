@@ -305,7 +305,7 @@ def filled(dtype, D, page, hq, hkv, have, adds, seed=0, pages=None, spread=0):
 def attend_exactly(q, starts, seen, tables, cache, scale):
     """In 64 bits: the result, and the sum of p |v|, to which the roundings of the probabilities are relative.  In it also 2^-27 of the largest p times scale for
     each code that a row sees: the kernels round p times scale to fp16, whose step ends at 2^-24, with the row's largest at 2^12 or more, so that half a step
-    is up to 2^-37 = 2^-10 * 2^-27 of that.  (A zero code of a token that takes nearly all leaves a result to terms that small.)"""
+    is up to 2^-37 = 2^-10 * 2^-27 of that.  (Where there are many rows, the scale is the largest of 16 neighbours.)  (A zero code of a token that takes nearly all leaves a result to terms that small.)"""
     hq, hkv, page, D = q.shape[1], cache.k.shape[1], cache.k.shape[2], q.shape[2]
     out, spread = torch.zeros(q.shape, dtype=torch.double, device=DEV), torch.zeros(q.shape, dtype=torch.double, device=DEV)
     for r in range(seen.numel()):
@@ -322,7 +322,8 @@ def attend_exactly(q, starts, seen, tables, cache, scale):
             v = torch.where(hide.all(0)[:, None], 0.0, v)
             vs = cache.v_scale[ids, h * hkv // hq].reshape(-1)[:n].double()
             code = (~hide).double() @ (v / vs[:, None]).abs().nan_to_num(0)
-            out[s:e, h], spread[s:e, h] = p @ v, p @ v.abs() + 2.0 ** -27 * (p * torch.where(hide, 0.0, vs)).amax(-1, keepdim=True) * code
+            near = torch.nn.functional.pad(vs.nan_to_num(0), (0, -n % 16)).view(-1, 16).amax(-1).repeat_interleave(16)[:n]
+            out[s:e, h], spread[s:e, h] = p @ v, p @ v.abs() + 2.0 ** -27 * (p * torch.where(hide, 0.0, near)).amax(-1, keepdim=True) * code
     return out, spread
 
 
