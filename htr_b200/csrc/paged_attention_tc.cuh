@@ -42,6 +42,8 @@ using namespace htr;
 
 constexpr int kThreads = 512, kTile = 128, kRows = 256, kUnit = 64, kGroups = kUnit / 16, kMaxRequests = 1024;
 constexpr int kTmemColumns = 512;                          // of a tile: S (P over it) at 0 and 64, O at 128
+template <int kBits>
+constexpr float kTopOf = kBits == 4 ? 4.f : 12.f;          // where a row's largest term lies when its reference moves
 constexpr int kRing = 4, kScales = 8;                      // units of keys and of values in shared memory; of their scales, read by all rows
 
 template <typename T, int D, int kBits>
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   if (tid == 0) {
     s.fail = s.nan = 0;
     for (int i = 0; i < kRing; ++i) {
-      bar_init(smem_u32(&s.k_full[i]), i == 0 && a.withhold == (int)blockIdx.x + 1 ? 65 : 64);      // (withheld: one arrival more than come)
+      bar_init(smem_u32(&s.k_full[i]), (kBits == 4 ? 128 : 64) + (i == 0 && a.withhold == (int)blockIdx.x + 1));      // (withheld: one arrival more than come)
       bar_init(smem_u32(&s.k_free[i]), 1);
       bar_init(smem_u32(&s.v_full[i]), 128);
       bar_init(smem_u32(&s.v_free[i]), 1);
@@ -326,98 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
     };
     Unit next;
     pages_of(next);
-    if constexpr (kBits == 4) {
-      // ---- widened: a warp takes 32 tokens of keys or 16 of values, a lane 32 dimensions of every kPer-th; the rows of a unit are fetched while the one before is written
-      constexpr int kTokens = keys ? 32 : 16, kPer = D == 128 ? 8 : 16, kPasses = kTokens / kPer;
-      const int first = keys ? 32 * kw : 16 * vw, in_pass = lane % kPer, piece = lane / kPer;
-      struct Rows {
-        uint4 v[kPasses];
-        uint16_t ks, vs;                                   // of token lane % kTokens
-      };
-      const auto rows_of = [&](const Unit& p, Rows& x) {   // (a page that is none is read as the first one and left aside later)
-        const auto row = [&](int token) {
-          const int id = keys && token >> 4 ? p.id[1] : p.id[0];
-          return ((((size_t)(valid(id) ? id : 0) * a.kv_heads + p.head) << a.shift) + ((p.at + first + token) & place_mask));
-        };
-#pragma unroll
-        for (int b = 0; b < kPasses; ++b)
-          x.v[b] = *reinterpret_cast<const uint4*>((keys ? a.k_cache : a.v_cache) + row(kPer * b + in_pass) * (D / 2) + 16 * piece);
-        const size_t at = row(lane % kTokens);
-        if (keys) x.ks = reinterpret_cast<const uint16_t*>(a.k_scale)[at];
-        x.vs = reinterpret_cast<const uint16_t*>(a.v_scale)[at];
-      };
-      // the exponent of the largest scale of a token's 16; `s`: 0 where there is none
-      const auto exponent = [&](float s) {
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) s = fmaxf(s, __shfl_xor_sync(kFullWarp, s, o));
-        return s > 0.f ? (int)(__float_as_uint(s) >> 23) - 127 : 0;
-      };
-      const auto write = [&](const Unit& p, const Rows& x, uint32_t n) {
-        const int mine = lane % kTokens, id = keys && mine >> 4 ? p.id[1] : p.id[0];
-        const bool real = valid(id), there = real && p.at + first + mine < p.end;
-        bad |= id != -1 && !real;                          // (-1: behind the last token)
-        const auto held = [&](float s) { return fminf(fmaxf(s, 7.888609052210118e-31f), 6.646139978924579e35f); };       // 2^-100 to 2^119
-        const float vs = __uint_as_float((uint32_t)x.vs << 16);
-        const bool nan_v = vs != vs;
-        const int ev = exponent(there && !nan_v ? held(vs) : 0.f);
-        float by;
-        if constexpr (keys) {
-          const float ks = __uint_as_float((uint32_t)x.ks << 16);
-          const bool nan_k = ks != ks;
-          const int ek = exponent(there && !nan_k ? held(ks) : 0.f);
-          by = !there ? 0.f : nan_k || nan_v ? __int_as_float(0x7FC00000) : held(ks) * exp2i(-ek);
-          if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.k_free, kRing, n - kRing));
-          if (!ok) return;
-          if ((lane & 15) == 0) {
-            const int slot = n % kScales, g = 2 * kw + (lane >> 4);
-            s.ks[slot][g] = exp2i(ek);
-            s.lv[slot][g] = (float)ev;
-            s.inv[slot][g] = exp2i(-ev) * kSumUnit;
-            s.real[slot][g] = real;
-          }
-        } else {
-          by = there && !nan_v ? held(vs) * exp2i(-ev) : 0.f;
-          if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.v_free, kRing, n - kRing));
-          if (!ok) return;
-        }
-        const uint32_t two = pack_half(by, by);
-        uint8_t* dst = smem + (keys ? Y::kK + (n % kRing) * Y::kKeys : Y::kV + (n % kRing) * Y::kValues);
-#pragma unroll
-        for (int b = 0; b < kPasses; ++b) {
-          const int token = kPer * b + in_pass;
-          const uint32_t scale = __shfl_sync(kFullWarp, two, token);
-          const uint32_t w[4] = {x.v[b].x, x.v[b].y, x.v[b].z, x.v[b].w};
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            uint32_t r[4];
-            from_e2m1(w[y], r);
-#pragma unroll
-            for (int z = 0; z < 4; ++z) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(r[z]) : "r"(scale));
-            *reinterpret_cast<uint4*>(dst + Y::template value<>(first + token, 4 * piece + y)) = {r[0], r[1], r[2], r[3]};
-          }
-        }
-        fence_async();
-        bar_arrive(smem_u32((keys ? s.k_full : s.v_full) + n % kRing));
-      };
-      Rows x[2];
-      Unit unit[2];
-      unit[0] = next;
-      if (count > 1) pages_of(next);
-      rows_of(unit[0], x[0]);
-      for (uint32_t n = 0; n < count && ok; n += 2) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (n + h >= count || !ok) break;
-          if (n + h + 1 < count) {
-            unit[h ^ 1] = next;
-            rows_of(unit[h ^ 1], x[h ^ 1]);
-            if (n + h + 2 < count) pages_of(next);
-          }
-          write(unit[h], x[h], n + h);
-        }
-      }
-      if (bad && a.status) atomicOr(a.status, 32);
-    } else if constexpr (keys) {
+    if constexpr (keys) {
       // ---- straight to their place; a unit is announced when the copies of the two after it are under way
       float ks = 0.f, vs = 1.f;
       bool real = false;
@@ -538,11 +449,126 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       }
     }
   };
+  // ================= keys and values of 4 bits (warps 8-13 and 15): 16 tokens of either are a piece of work, eight of which make a unit and go round
+  const auto feed4 = [&] {
+    constexpr int kFeeders = 7, kPer = D == 128 ? 8 : 16, kPasses = 16 / kPer;           // a lane has 32 dimensions of every kPer-th token
+    const int me = warp == 15 ? 6 : warp - 8, place_mask = (1 << a.shift) - 1, in_pass = lane % kPer, piece = lane / kPer;
+    const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
+    const auto held = [&](float s) { return fminf(fmaxf(s, 7.888609052210118e-31f), 6.646139978924579e35f); };           // 2^-100 to 2^119
+    const uint32_t pieces = 8 * (uint32_t)count;
+    bool ok = true, bad = false;
+    struct Piece {
+      int id, head, at, end;                               // at: its first token
+    };
+    struct Rows {
+      uint4 v[kPasses];
+      uint16_t ks, vs;                                     // of token lane % 16
+    };
+    Walk f(s, count);
+    f.look(a);
+    int fu = f.u0;
+    uint32_t fn = 0;                                       // the unit of the thread block that fu is
+    const auto page_of = [&](uint32_t n) {                 // pieces come in rising order
+      while (fn < n >> 3) {
+        ++fn;
+        if (++fu < f.u1) continue;
+        f.next(a);
+        f.look(a);
+        fu = f.u0;
+      }
+      Piece p;
+      p.at = fu * kUnit + 16 * (n & 3);
+      p.head = f.head;
+      p.end = f.end;
+      p.id = p.at < f.end ? (a.tables + f.r * a.table_stride)[p.at >> a.shift] : -1;
+      return p;
+    };
+    const auto rows_of = [&](const Piece& p, uint32_t n, Rows& x) {            // (a page that is none is read as the first one and left aside later)
+      const size_t row = ((((size_t)(valid(p.id) ? p.id : 0) * a.kv_heads + p.head) << a.shift) + (p.at & place_mask));
+      const uint8_t* src = (n & 4 ? a.v_cache : a.k_cache) + row * (D / 2) + in_pass * (D / 2) + 16 * piece;
+#pragma unroll
+      for (int b = 0; b < kPasses; ++b) x.v[b] = *reinterpret_cast<const uint4*>(src + kPer * b * (D / 2));
+      x.ks = reinterpret_cast<const uint16_t*>(a.k_scale)[row + (lane & 15)];
+      x.vs = reinterpret_cast<const uint16_t*>(a.v_scale)[row + (lane & 15)];
+    };
+    // the exponent of the largest scale of the 16; `s`: 0 where there is none
+    const auto exponent = [&](float s) {
+      const unsigned most = __reduce_max_sync(kFullWarp, __float_as_uint(s));
+      return most ? (int)(most >> 23) - 127 : 0;
+    };
+    const auto write = [&](const Piece& p, uint32_t piece_n, const Rows& x) {
+      const uint32_t n = piece_n >> 3;
+      const bool values = piece_n & 4, real = valid(p.id), there = real && p.at + (lane & 15) < p.end;
+      const int group = piece_n & 3;
+      bad |= p.id != -1 && !real;                          // (-1: behind the last token)
+      const float vs = __uint_as_float((uint32_t)x.vs << 16), ks = __uint_as_float((uint32_t)x.ks << 16);
+      const bool nan_v = vs != vs, nan_k = ks != ks;
+      const int ev = exponent(there && !nan_v ? held(vs) : 0.f);
+      float by;
+      if (values) {
+        by = there && !nan_v ? held(vs) * exp2i(-ev) : 0.f;
+        if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.v_free, kRing, n - kRing));
+        if (!ok) return;
+      } else {
+        const int ek = exponent(there && !nan_k ? held(ks) : 0.f);
+        by = !there ? 0.f : nan_k || nan_v ? __int_as_float(0x7FC00000) : held(ks) * exp2i(-ek);
+        if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.k_free, kRing, n - kRing));
+        if (!ok) return;
+        if (lane == 0) {
+          const int slot = n % kScales;
+          s.ks[slot][group] = exp2i(ek);
+          s.lv[slot][group] = (float)ev;
+          s.inv[slot][group] = exp2i(-ev) * kSumUnit;
+          s.real[slot][group] = real;
+        }
+      }
+      const uint32_t two = pack_half(by, by);
+      uint8_t* dst = smem + (values ? Y::kV + (n % kRing) * Y::kValues : Y::kK + (n % kRing) * Y::kKeys);
+#pragma unroll
+      for (int b = 0; b < kPasses; ++b) {
+        const uint32_t scale = __shfl_sync(kFullWarp, two, kPer * b + in_pass);
+        const uint32_t w[4] = {x.v[b].x, x.v[b].y, x.v[b].z, x.v[b].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          uint32_t r[4];
+          from_e2m1(w[y], r);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(r[z]) : "r"(scale));
+          *reinterpret_cast<uint4*>(dst + Y::template value<>(16 * group + kPer * b + in_pass, 4 * piece + y)) = {r[0], r[1], r[2], r[3]};
+        }
+      }
+      fence_async();
+      bar_arrive(smem_u32((values ? s.v_full : s.k_full) + n % kRing));
+    };
+    // the rows of a warp's next piece are fetched before those of one are written, the page of the piece after it before that.  (Two at a time, without the moves,
+    // were code that the softmax had to fetch its own again after: the prompt below took 339 us in place of 208.)
+    Piece one, next;
+    Rows x;
+    uint32_t n = me;
+    if (n < pieces) {
+      one = page_of(n);
+      rows_of(one, n, x);
+    }
+    if (n + kFeeders < pieces) next = page_of(n + kFeeders);
+#pragma unroll 1
+    for (; n < pieces && ok; n += kFeeders) {
+      const Piece now = one;
+      const Rows held_rows = x;
+      if (n + kFeeders < pieces) {
+        one = next;
+        rows_of(one, n + kFeeders, x);
+        if (n + 2 * kFeeders < pieces) next = page_of(n + 2 * kFeeders);
+      }
+      write(now, n, held_rows);
+    }
+    if (bad && a.status) atomicOr(a.status, 32);
+  };
   // registers of the four warpgroups: 2 * 160 + 2 * 96 = 4 * 128, what the launch has
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     if (count > 0) {
     // ================= softmax: a thread per row of tile x
+    constexpr float kTop = kTopOf<kBits>;
     const int x = warp >> 2, row = tid & (kTile - 1);
     const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), mine_at = lanes + 256 * x;
     bool ok = true;
@@ -697,18 +723,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
             float top = kNone;
 #pragma unroll
             for (int c = 0; c < kUnit; ++c) top = fmaxf(top, v[c]);
-            const bool moves = grows && top > kNone;
-            const float now = moves ? base + top - 12.f : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
+            const bool moves = (grows || (kBits == 4 && top > kTop)) && top > kNone;
+            const float now = moves ? base + top - kTop : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f, down = moves ? base - now : 0.f;
 #pragma unroll
             for (int c = 0; c < kUnit; ++c) v[c] += down;
             m = now;
             l *= f;
+            if (kBits == 4) exponentials();                // (the last unit's products are under way meanwhile)
             if (results) {
               ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));        // (S of this unit came before the results of the last one)
               fence_after();
               if (ok) follow(f);
             }
-            exponentials();
+            if (kBits == 8) exponentials();
           }
           l = fmaf(sum[0][0] + sum[0][1], inv.x, fmaf(sum[1][0] + sum[1][1], inv.y, fmaf(sum[2][0] + sum[2][1], inv.z, fmaf(sum[3][0] + sum[3][1], inv.w, l))));
           __syncwarp();
@@ -822,12 +849,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
     }
     if (lane == 0) s.finished[warp] = segment;
     }
-  } else if (warp < 12) {
+  } else if (kBits == 8 && warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (count > 0) feed(std::false_type{});
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    if (count > 0 && warp < 14) feed(std::true_type{});
+    if constexpr (kBits == 4) {
+      if (count > 0 && warp != 14) feed4();
+    } else {
+      if (count > 0 && warp < 14) feed(std::true_type{});
+    }
     if (count > 0 && warp == 14) {
     // ================= products: one thread, and as few instructions between two of them as can be (24 a unit, 50 to 60 cycles each to issue)
     if (elect_one()) {

@@ -303,9 +303,10 @@ def filled(dtype, D, page, hq, hkv, have, adds, seed=0, pages=None, spread=0):
 
 
 def attend_exactly(q, starts, seen, tables, cache, scale):
-    """In 64 bits: the result, and the sum of p |v|, to which the roundings of the probabilities are relative.  In it also 2^-27 of the largest p times scale for
-    each code that a row sees: the kernels round p times scale to fp16, whose step ends at 2^-24, with the row's largest at 2^12 or more, so that half a step
-    is up to 2^-37 = 2^-10 * 2^-27 of that.  (Where there are many rows, the scale is the largest of 16 neighbours.)  (A zero code of a token that takes nearly all leaves a result to terms that small.)"""
+    """In 64 bits: the result, and the sum of p |v|, to which the roundings of the probabilities are relative.  In it also 2^-19 of the largest p times scale for
+    each code that a row sees: the kernels round p times scale to fp16, whose step ends at 2^-24, with the row's largest at 2^4 or more, so that half a step
+    is up to 2^-29 = 2^-10 * 2^-19 of that.  (Where there are many rows, the scale is the largest of 16 neighbours.)  (A zero code of a token that takes nearly all
+    leaves a result to terms that small.)"""
     hq, hkv, page, D = q.shape[1], cache.k.shape[1], cache.k.shape[2], q.shape[2]
     out, spread = torch.zeros(q.shape, dtype=torch.double, device=DEV), torch.zeros(q.shape, dtype=torch.double, device=DEV)
     for r in range(seen.numel()):
@@ -323,7 +324,7 @@ def attend_exactly(q, starts, seen, tables, cache, scale):
             vs = cache.v_scale[ids, h * hkv // hq].reshape(-1)[:n].double()
             code = (~hide).double() @ (v / vs[:, None]).abs().nan_to_num(0)
             near = torch.nn.functional.pad(vs.nan_to_num(0), (0, -n % 16)).view(-1, 16).amax(-1).repeat_interleave(16)[:n]
-            out[s:e, h], spread[s:e, h] = p @ v, p @ v.abs() + 2.0 ** -27 * (p * torch.where(hide, 0.0, near)).amax(-1, keepdim=True) * code
+            out[s:e, h], spread[s:e, h] = p @ v, p @ v.abs() + 2.0 ** -19 * (p * torch.where(hide, 0.0, near)).amax(-1, keepdim=True) * code
     return out, spread
 
 
@@ -442,7 +443,7 @@ def test_table_entries_that_are_no_page_hide_their_tokens(adds, wide, page):
         hide = torch.arange(k.shape[0], device=DEV)[None] > torch.arange(k.shape[0] - n, k.shape[0], device=DEV)[:, None]
         hide[:, hidden] = True
         p = (q[:n, h].double() @ k.nan_to_num(0).T / 8).masked_fill(hide, float("-inf")).softmax(-1)
-        want, spread = p @ v.nan_to_num(0), p @ v.nan_to_num(0).abs() + 2.0 ** -27 * 6 * v.shape[0]      # (as in attend_exactly; scales are below 1)
+        want, spread = p @ v.nan_to_num(0), p @ v.nan_to_num(0).abs() + 2.0 ** -19 * 6 * v.shape[0]      # (as in attend_exactly; scales are below 1)
         assert ((got[:n, h].double() - want).abs() <= bound_of(q.dtype, want, spread)).all()
 
 
@@ -479,7 +480,7 @@ def test_queries_that_are_not_finite(bad, D, adds, wide):
 @pytest.mark.parametrize("spread", (0.0, 1.0))
 def test_a_token_that_takes_nearly_all_and_has_no_values(dtype, D, adds, R, nats, spread):
     """The first token's score lies `nats` above those of 16500 others, which are equal or differ by `spread`, and its values are zero: the result is made of
-    the others' probabilities, which have all their bits.  So many requests and heads (of the same pages) that one thread block goes over most of them."""
+    the others' probabilities.  So many requests and heads (of the same pages) that one thread block goes over most of them."""
     from htr_b200 import paged
 
     hkv, group = 8, 4
