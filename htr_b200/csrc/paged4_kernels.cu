@@ -55,6 +55,96 @@ __device__ __forceinline__ void hadamard(float (&v)[8], int lane) {
   }
 }
 
+// The same of 16 rows by one warp, as matrix products.  Of H = H_j x H_8 (d = 8 j + b) the H_j are products of 16 rows by 8 or 16 chunks j of 8 dimensions, for each
+// b; and the H_8, over b, are sums within a lane.  Lane (g, c) of the products' operand has rows g and g + 8 at kChunks chunks, and of their result too:
+// neighbouring ones (kChunks c + i), or every fourth (c + 4 i), whose 16-byte pieces lie side by side over the lanes.
+template <int D>
+constexpr int kChunks = D / 32;
+__device__ __forceinline__ int chunk_of(bool side_by_side, int chunks, int c, int i) { return side_by_side ? c + 4 * i : chunks * c + i; }
+// the right operand: (-1)^(bits of j_in & j_out) or, for rows that only move, j_in == j_out; `one`: 1 in the operand's type, two of them
+template <int D>
+struct Turn {
+  uint32_t b[D / 64][D / 64];                              // pair of chunks that come in; 8 rows of chunks that go out
+  __device__ __forceinline__ Turn(bool move, bool in_side, bool out_side, uint32_t one, int lane) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int p = 0; p < D / 64; ++p)
+#pragma unroll
+      for (int t = 0; t < D / 64; ++t) {
+        const int out = chunk_of(out_side, kChunks<D>, g >> 1, 2 * t + (g & 1));
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int in = chunk_of(in_side, kChunks<D>, c, 2 * p + e);
+          const uint32_t v = move ? (in == out ? one & 0xFFFFu : 0u) : (one & 0xFFFFu) ^ (__popc(in & out) & 1) << 15;
+          r |= v << (16 * e);
+        }
+        b[p][t] = r;
+      }
+  }
+};
+template <bool kBf16>
+__device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+  if constexpr (kBf16)
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b));
+  else
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b));
+}
+// the H_8 part: over the first index
+template <int kTiles>
+__device__ __forceinline__ void across(float (&v)[8][kTiles][4]) {
+#pragma unroll
+  for (int h = 1; h < 8; h *= 2)
+#pragma unroll
+    for (int b = 0; b < 8; ++b)
+      if (!(b & h))
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = v[b][t][i], y = v[b + h][t][i];
+            v[b][t][i] = x + y;
+            v[b + h][t][i] = x - y;
+          }
+}
+
+// the low halves of the bytes of x, the high ones of y
+__device__ __forceinline__ uint32_t low_of(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xE4;" : "=r"(r) : "r"(x), "r"(y), "n"(0x0F0F0F0Fu));
+  return r;
+}
+// the codes of two words, 8 each, as fp16 pairs (x's, y's) of the same place
+__device__ __forceinline__ void pairs_of(uint32_t x, uint32_t y, uint32_t (&r)[8]) {
+  uint32_t even[4], odd[4];
+  from_e2m1(low_of(x, y << 4), even);
+  from_e2m1(low_of(x >> 4, y), odd);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    r[2 * j] = even[j];
+    r[2 * j + 1] = odd[j];
+  }
+}
+
+// a row's scale from its largest magnitude (NaN stays), and what divides by it
+struct Scale {
+  float s, inv;
+  bool beyond;                                             // there is more than the scale admits
+  __device__ __forceinline__ explicit Scale(float most) {
+    s = most != most ? most : fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(most, 6.f))), kScaleLeast), kScaleMost);
+    inv = __fdiv_rn(1.f, s);
+    beyond = most > 6.f * kScaleMost;
+  }
+  // x / s, to the nearest where it is one of the values between two codes: a tie stays one
+  __device__ __forceinline__ float operator()(float x) const {
+    if (beyond) x = fminf(fmaxf(x, -6.f * kScaleMost), 6.f * kScaleMost);
+    const float y = x * inv;
+    return fmaf(fmaf(-y, s, x), inv, y);
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void widen(const uint4& raw, float (&v)[8]) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -85,20 +175,12 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 256, kMaxWindow = 64, kMaxPage = 128;
 
-// grid (windows of tokens, groups of kHeads heads of queries, keys and values as they stand in a row).  A thread holds 8 dimensions of a row, four pairs
-// of neighbours; in halves a pair's other element comes from another lane.
-// A token whose slot does not lie above those of its page in the page - 1 tokens before it is not written: every place has one writer.
-template <typename T, int D, int kHeads, bool kHalves>
-__global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const AppendArgs a) {
-  constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes, kWarps = kAppendThreads / 32;
-  __shared__ int s_slot[kMaxWindow + kMaxPage], s_pos[kMaxWindow];
-  __shared__ int s_bad[kMaxWindow];
-  pdl_enter();
-  const int tid = threadIdx.x, lane = tid % kLanes, row = tid / kLanes, page = 1 << a.shift;
-  const int t0 = blockIdx.x * a.window, n = min(a.window, a.tokens - t0), h0 = blockIdx.y * kHeads;
-  const T* qkv = static_cast<const T*>(a.qkv);
-  // ---- which of the tokens are written: slots of the window (from place `page` on) and of a page before it
-  for (int i = tid; i < page + n; i += kAppendThreads) {
+// Which of the tokens t0 ... t0 + n - 1 are written: s_slot their slots (from place `page` on, and of a page before them; -1: not valid), s_bad 0 for those that are
+// written, 2 for those that are not although their slot is not -1.  By all threads, which are in step after it.
+template <int kThreads>
+__device__ __forceinline__ void find_written(const AppendArgs& a, int t0, int n, int* s_slot, int* s_pos, int* s_bad) {
+  const int tid = threadIdx.x, page = 1 << a.shift;
+  for (int i = tid; i < page + n; i += kThreads) {
     const int t = t0 - page + i;
     const int slot = t >= 0 ? a.slots[t] : -1, pos = t >= 0 ? a.positions[t] : -1;
     const bool ok = slot >= 0 && slot < a.slots_total && pos >= 0 && pos < a.angle_rows;
@@ -110,7 +192,7 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
   }
   __syncthreads();
   if (t0 + n > 1)
-    for (int w = tid >> 5; w < n; w += kWarps) {
+    for (int w = tid >> 5; w < n; w += kThreads / 32) {
       const int slot = s_slot[page + w];
       bool bad = false;
       for (int i = 1 + (tid & 31); i < page; i += 32) {
@@ -121,8 +203,23 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
     }
   __syncthreads();
   if (a.status && blockIdx.y == 0)
-    for (int i = tid; i < n; i += kAppendThreads)
+    for (int i = tid; i < n; i += kThreads)
       if (s_bad[i] == 2) atomicOr(a.status, 16);
+}
+
+// grid (windows of tokens, groups of kHeads heads of queries, keys and values as they stand in a row).  A thread holds 8 dimensions of a row, four pairs
+// of neighbours; in halves a pair's other element comes from another lane.
+// A token whose slot does not lie above those of its page in the page - 1 tokens before it is not written: every place has one writer.
+template <typename T, int D, int kHeads, bool kHalves>
+__global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const AppendArgs a) {
+  constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes;
+  __shared__ int s_slot[kMaxWindow + kMaxPage], s_pos[kMaxWindow];
+  __shared__ int s_bad[kMaxWindow];
+  pdl_enter();
+  const int tid = threadIdx.x, lane = tid % kLanes, row = tid / kLanes, page = 1 << a.shift;
+  const int t0 = blockIdx.x * a.window, n = min(a.window, a.tokens - t0), h0 = blockIdx.y * kHeads;
+  const T* qkv = static_cast<const T*>(a.qkv);
+  find_written<kAppendThreads>(a, t0, n, s_slot, s_pos, s_bad);
   const bool first = 8 * lane < a.half, turned = 8 * lane < 2 * a.half;          // (halves) this lane's are the first of their pairs; they are rotated
   for (int w0 = 0; w0 < n; w0 += kRows) {
     const int w = min(w0 + row, n - 1), slot = s_slot[page + w];
@@ -194,16 +291,169 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
         const float x = __shfl_xor_sync(kFullWarp, most, o);
         most = most != most || x != x ? __int_as_float(0x7FC00000) : fmaxf(most, x);
       }
-      // (a row with a NaN: so are all of its values, by their scale)
-      const float scale = most != most ? most : fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(most, 6.f))), kScaleLeast), kScaleMost);
+      const Scale scale(most);                             // (a row with a NaN: so are all of its values, by their scale)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(v[j], scale);         // (divided, not by way of an inverse: a tie stays one)
+      for (int j = 0; j < 8; ++j) v[j] = scale(v[j]);
       if (!mine || !ok) continue;
       const bool values = h >= a.q_heads + a.kv_heads;
       const int head = h - a.q_heads - (values ? a.kv_heads : 0);
       const size_t place = (((size_t)(slot >> a.shift) * a.kv_heads + head) << a.shift) + (slot & (page - 1));
       *reinterpret_cast<uint32_t*>((values ? a.v_cache : a.k_cache) + place * (D / 2) + lane * 4) = to_e2m1(v);
-      if (lane == 0) (values ? a.v_scale : a.k_scale)[place] = (uint16_t)(__float_as_uint(scale) >> 16);
+      if (lane == 0) (values ? a.v_scale : a.k_scale)[place] = (uint16_t)(__float_as_uint(scale.s) >> 16);
+    }
+  }
+}
+
+// The same for many tokens: a warp takes 16 of them at a time, one head after the other, and transforms by matrix products.  The rotated elements enter as two
+// bf16 each, 16 bits in all: 2^-16 of an element at most, where queries are rounded to 2^-9 or 2^-12 of the result and keys to four bits.  (With three, 2^-24.)
+// An infinity among a row's elements makes all of the row NaN.
+constexpr int kRowsThreads = 128, kRowsTokens = 16, kRowsHeads = 16, kManyRows = 4096;
+
+template <typename T, int D, bool kHalves>
+__global__ void __launch_bounds__(kRowsThreads) rope_append4_rows_kernel(const AppendArgs a) {
+  constexpr int kWarps = kRowsThreads / 32, kTiles = D / 64;
+  __shared__ int s_slot[kRowsTokens + kMaxPage], s_pos[kRowsTokens], s_bad[kRowsTokens];
+  pdl_enter();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, page = 1 << a.shift;
+  const int t0 = blockIdx.x * kRowsTokens, n = min(kRowsTokens, a.tokens - t0);
+  const T* qkv = static_cast<const T*>(a.qkv);
+  find_written<kRowsThreads>(a, t0, n, s_slot, s_pos, s_bad);
+  const int last = min((int)(blockIdx.y + 1) * kRowsHeads, a.q_heads + 2 * a.kv_heads);
+  for (int h = blockIdx.y * kRowsHeads + warp; h < last; h += kWarps) {
+    const bool turns = h < a.q_heads + a.kv_heads, query = h < a.q_heads;
+    // rows g and g + 8; those behind the last are its
+    size_t row[2];
+    int w[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      w[r] = min(g + 8 * r, n - 1);
+      row[r] = (size_t)(t0 + w[r]) * a.row_stride + (size_t)h * D;
+    }
+    float v[8][kTiles][4];                                 // of dimension b of chunk 2 t + i % 2, row g + 8 (i / 2)
+    if (turns) {
+      const Turn<D> turn(false, true, query, D == 128 ? 0x3C003C00u : 0x3C803C80u, lane);        // 1 / D in bf16
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) v[b][t][0] = v[b][t][1] = v[b][t][2] = v[b][t][3] = 0.f;
+#pragma unroll
+      for (int p = 0; p < kTiles; ++p) {
+        uint32_t high[2][8], low[2][8];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const size_t angles = s_bad[w[r]] == 0 ? (size_t)s_pos[w[r]] * a.half : 0;
+          float x[2][8];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = 8 * chunk_of(true, kChunks<D>, c, 2 * p + e);
+            const uint4 raw = *reinterpret_cast<const uint4*>(qkv + row[r] + at);
+            widen<T>(raw, x[e]);
+            if (at >= 2 * a.half) continue;
+            if constexpr (kHalves) {
+              const bool first = at < a.half;
+              const uint4 raw2 = *reinterpret_cast<const uint4*>(qkv + row[r] + at + (first ? a.half : -a.half));
+              float y[8];
+              widen<T>(raw2, y);
+              const size_t from = angles + at - (first ? 0 : a.half);
+#pragma unroll
+              for (int z = 0; z < 8; z += 4) {
+                const float4 cs = *reinterpret_cast<const float4*>(a.cosv + from + z), sn = *reinterpret_cast<const float4*>(a.sinv + from + z);
+                const float k[4] = {cs.x, cs.y, cs.z, cs.w}, l[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[e][z + j] = x[e][z + j] * k[j] + (first ? -y[z + j] : y[z + j]) * l[j];
+              }
+            } else {
+              const size_t from = angles + at / 2;
+              const float4 cs = *reinterpret_cast<const float4*>(a.cosv + from), sn = *reinterpret_cast<const float4*>(a.sinv + from);
+              const float k[4] = {cs.x, cs.y, cs.z, cs.w}, l[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float y = x[e][2 * j], z = x[e][2 * j + 1];
+                x[e][2 * j] = y * k[j] - z * l[j];
+                x[e][2 * j + 1] = y * l[j] + z * k[j];
+              }
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            high[r][b] = Half<__nv_bfloat16>::narrow(x[0][b], x[1][b]);
+            const float2 held = Half<__nv_bfloat16>::wide(high[r][b]);
+            low[r][b] = Half<__nv_bfloat16>::narrow(x[0][b] - held.x, x[1][b] - held.y);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            mma_1688<true>(v[b][t], high[0][b], high[1][b], turn.b[p][t]);
+            mma_1688<true>(v[b][t], low[0][b], low[1][b], turn.b[p][t]);
+          }
+      }
+      across(v);
+      const float by = query ? 8.f : D / 8.f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[b][t][i] *= by;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int y = 0; y < kChunks<D>; ++y) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(qkv + row[r] + 8 * chunk_of(false, kChunks<D>, c, y));
+          float x[8];
+          widen<T>(raw, x);
+#pragma unroll
+          for (int b = 0; b < 8; ++b) v[b][y >> 1][2 * r + (y & 1)] = x[b];
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool mine = g + 8 * r < n, ok = s_bad[w[r]] == 0;
+      if (query) {
+#pragma unroll
+        for (int y = 0; y < kChunks<D>; ++y) {
+          const int t = y >> 1, i = 2 * r + (y & 1);
+          uint4 out = {Half<T>::narrow(v[0][t][i], v[1][t][i]), Half<T>::narrow(v[2][t][i], v[3][t][i]), Half<T>::narrow(v[4][t][i], v[5][t][i]), Half<T>::narrow(v[6][t][i], v[7][t][i])};
+          if (!ok) out = {0, 0, 0, 0};
+          if (mine) *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + ((size_t)(t0 + w[r]) * a.q_heads + h) * D + 8 * chunk_of(true, kChunks<D>, c, y)) = out;
+        }
+        continue;
+      }
+      float most = 0.f;
+      bool nan = false;
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int y = 0; y < kChunks<D>; ++y) {
+          const float x = v[b][y >> 1][2 * r + (y & 1)];
+          most = fmaxf(most, fabsf(x));
+          nan |= x != x;
+        }
+      if (nan) most = __int_as_float(0x7FC00000);
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        const float x = __shfl_xor_sync(kFullWarp, most, o);
+        most = most != most || x != x ? __int_as_float(0x7FC00000) : fmaxf(most, x);
+      }
+      const Scale scale(most);
+      uint32_t codes[kChunks<D>];
+#pragma unroll
+      for (int y = 0; y < kChunks<D>; ++y) {
+        float x[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) x[b] = scale(v[b][y >> 1][2 * r + (y & 1)]);
+        codes[y] = to_e2m1(x);
+      }
+      if (!mine || !ok) continue;
+      const int slot = s_slot[page + w[r]], head = h - a.q_heads - (turns ? 0 : a.kv_heads);
+      const size_t place = (((size_t)(slot >> a.shift) * a.kv_heads + head) << a.shift) + (slot & (page - 1));
+      uint8_t* to = (turns ? a.k_cache : a.v_cache) + place * (D / 2) + 4 * kChunks<D> * c;
+      if constexpr (D == 128) *reinterpret_cast<uint4*>(to) = {codes[0], codes[1], codes[2], codes[3]};
+      else *reinterpret_cast<uint2*>(to) = {codes[0], codes[1]};
+      if (c == 0) (turns ? a.k_scale : a.v_scale)[place] = (uint16_t)(__float_as_uint(scale.s) >> 16);
     }
   }
 }
@@ -218,7 +468,7 @@ struct UnpackArgs {
   void *k_out, *v_out;
 };
 
-constexpr int kUnpackThreads = 256;
+constexpr int kUnpackThreads = 128;
 
 template <typename T>
 __device__ __forceinline__ void put8(T* to, const float (&v)[8]) {
@@ -230,39 +480,62 @@ __device__ __forceinline__ void put8<float>(float* to, const float (&v)[8]) {
   *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// A thread block per page and head: its rows of keys, turned back (H H = D), and of values.  Bound by what it writes.
+// A warp takes 16 tokens of keys, which it turns back (H H = D), or of values, which pass through the same products only to lie side by side.  The sums are those of
+// codes, exact; one multiplication by the scale, and one rounding.  Bound by what it writes.
 template <typename T, int D>
-__global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArgs a) {
-  constexpr int kLanes = D / 8, kRows = kUnpackThreads / kLanes;
+__global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArgs a, long long pieces) {
+  constexpr int kTiles = D / 64;
   pdl_enter();
-  const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes, page = 1 << a.shift;
-  const int i = blockIdx.x / a.kv_heads, head = blockIdx.x - i * a.kv_heads, id = a.ids[i];
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const long long n = (long long)blockIdx.x * (kUnpackThreads / 32) + (threadIdx.x >> 5);        // piece: 16 tokens; keys and values in turns
+  if (n >= pieces) return;
+  const bool values = n & 1;
+  const long long sixteen = n >> 1;                        // of the output
+  const int unit = (int)(sixteen >> (a.shift - 4)), i = unit / a.kv_heads, head = unit - i * a.kv_heads, id = a.ids[i];
   const bool real = id >= 0 && id < a.pages;
-  const size_t from = ((size_t)(real ? id : 0) * a.kv_heads + head) << a.shift, to = (size_t)blockIdx.x << a.shift;
-#pragma unroll 4
-  for (int x = row; x < 2 * page; x += kRows) {            // (a multiple of kRows)
-    const bool values = x >= page;
-    const int place = x & (page - 1);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>((values ? a.v_cache : a.k_cache) + (from + place) * (D / 2) + lane * 4);
-    const float scale = of_bf16((values ? a.v_scale : a.k_scale)[from + place]);
-    uint32_t two[4];
-    from_e2m1(w, two);
-    float v[8];
+  const size_t from = (((size_t)(real ? id : 0) * a.kv_heads + head) << a.shift) + 16 * (sixteen & ((1 << (a.shift - 4)) - 1)), to = (size_t)sixteen * 16;
+  uint32_t w[2][kChunks<D>];
+  float scale[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = Half<__half>::wide(two[j]);
-      v[2 * j] = f.x * scale;
-      v[2 * j + 1] = f.y * scale;
+  for (int r = 0; r < 2; ++r) {
+    const size_t row = from + g + 8 * r;
+    const uint8_t* src = (values ? a.v_cache : a.k_cache) + row * (D / 2) + 4 * kChunks<D> * c;
+    if constexpr (D == 128) {
+      const uint4 x = *reinterpret_cast<const uint4*>(src);
+      w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(src);
+      w[r][0] = x.x; w[r][1] = x.y;
     }
-    if (!values) {                                         // (the same for a whole warp)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= 8.f / D;
-      hadamard<D>(v, lane);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = real ? v[j] : 0.f;
-    put8<T>(static_cast<T*>(values ? a.v_out : a.k_out) + (to + place) * D + lane * 8, v);
+    scale[r] = of_bf16((values ? a.v_scale : a.k_scale)[row]) * (values ? 1.f : 8.f / D);
   }
+  const Turn<D> turn(values, false, true, 0x3C003C00u, lane);
+  float v[8][kTiles][4];
+#pragma unroll
+  for (int b = 0; b < 8; ++b)
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) v[b][t][0] = v[b][t][1] = v[b][t][2] = v[b][t][3] = 0.f;
+#pragma unroll
+  for (int p = 0; p < kTiles; ++p) {
+    uint32_t x[2][8];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) pairs_of(w[r][2 * p], w[r][2 * p + 1], x[r]);
+#pragma unroll
+    for (int b = 0; b < 8; ++b)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) mma_1688<false>(v[b][t], x[0][b], x[1][b], turn.b[p][t]);
+  }
+  if (!values) across(v);
+  T* out = static_cast<T*>(values ? a.v_out : a.k_out);
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int y = 0; y < kChunks<D>; ++y) {
+      float x[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b) x[b] = real ? v[b][y >> 1][2 * r + (y & 1)] * scale[r] : 0.f;
+      put8<T>(out + (to + g + 8 * r) * D + 8 * chunk_of(true, kChunks<D>, c, y), x);
+    }
 }
 
 // ---- attention over the cache, few rows a request ---------------------------------------------------------------------------------
@@ -275,8 +548,8 @@ __global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArg
 //  * scales belong to tokens: those of keys multiply the scores, those of values enter the exponent (P' = 2^(s + log2 scale - m)) and the sum takes them out.
 // Row i of a half is its token i ^ (i >> 1 & 1): neighbouring lanes then read rows of both parities, which lie in different banks.
 
-constexpr int kTile = 32, kUnit = kAttWarps * kTile, kDepth = 4;
-constexpr int kBegin = 2;                                  // what an item costs besides its units
+constexpr int kTile = 32, kUnit = kAttWarps * kTile, kDepth = 3;
+constexpr int kBegin = 3;                                  // what an item costs besides its units
 using Work = Span<kUnit, kBegin>;
 template <int D, int NT>
 constexpr int kAttBlocks = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
@@ -290,10 +563,16 @@ struct Running : Results<D, NT> {
   using Results<D, NT>::o;
   using Results<D, NT>::m;
   using Results<D, NT>::l;
-  // a tile's tokens from `at` on; `least`: tokens that every row sees; `real`: halves that have a page
+  // a tile's tokens from `at` on; `least`: tokens that every row sees; `real`: halves that have a page; `read`: called when nothing of the stage is needed any more
   template <typename R, typename F>
-  __device__ __forceinline__ void add(const uint8_t* stage, const R& rows, int at, int least, unsigned real, int lane, F read) {
+  __device__ __forceinline__ void add(const uint8_t* stage, float4* wide, const R& rows, int at, int least, unsigned real, int lane, F read) {
     const int g = lane >> 2, c = lane & 3, pi = g ^ (g >> 1 & 1);
+    // scales of token `lane` of the tile
+    const uint16_t* scales = reinterpret_cast<const uint16_t*>(stage + 2 * kKeys<D>) + lane;
+    const float my_ks = of_bf16(scales[0]), vs = of_bf16(scales[kTile]);
+    const float held = fminf(fmaxf(vs, kScaleLeast), kScaleMost);      // (NaN: kScaleLeast, and the logarithm becomes NaN by what is added)
+    wide[lane] = make_float4(my_ks, __log2f(held) + (vs - vs), __fdividef(kSumUnit, held), 0.f);
+    __syncwarp();
     float s[2][NT][4], ks[2][2], lv[2][2], inv[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -310,11 +589,10 @@ struct Running : Results<D, NT> {
           const uint2 w = *reinterpret_cast<const uint2*>(stage + row * 32 + 8 * c);
           k[u][0] = w.x; k[u][1] = w.y;
         }
-        const uint16_t* scales = reinterpret_cast<const uint16_t*>(stage + 2 * kKeys<D>);
-        ks[h][u] = of_bf16(scales[row]);
-        const float vs = of_bf16(scales[kTile + row]), held = fminf(fmaxf(vs, kScaleLeast), kScaleMost);     // (NaN: kScaleLeast, and the logarithm stays NaN)
-        lv[h][u] = __log2f(vs != vs ? vs : held);
-        inv[h][u] = __fdividef(kSumUnit, held);
+        const float4 f = wide[row];
+        ks[h][u] = f.x;
+        lv[h][u] = f.y;
+        inv[h][u] = f.z;
       }
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
@@ -328,60 +606,79 @@ struct Running : Results<D, NT> {
         }
       }
     }
-    uint32_t v[2][4][D / 64];
+    float top[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int row = 16 * h + 8 * (x >> 1) + ((2 * c + (x & 1)) ^ (c & 1));
-        if constexpr (D == 128) {
-          const uint2 w = *reinterpret_cast<const uint2*>(stage + kKeys<D> + row * 64 + 8 * g);
-          v[h][x][0] = w.x; v[h][x][1] = w.y;
-        } else {
-          v[h][x][0] = *reinterpret_cast<const uint32_t*>(stage + kKeys<D> + row * 32 + 4 * g);
-        }
-      }
-    read();                                                // nothing of the stage is needed any more
-    const bool edge = at + kTile > least || real != 3;
-    bool grows = false;
+    for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = kNone;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                      // token pi + 8 (i / 2) of the half, row 2 c + i % 2
-          const float x = fmaf(s[h][t][i], rows.scale[t][i & 1] * ks[h][i >> 1], lv[h][i >> 1]);
-          s[h][t][i] = edge && (!(real >> h & 1) || at + 16 * h + pi + 8 * (i >> 1) >= rows.end[t][i & 1]) ? kNone : x;
-          grows |= s[h][t][i] > m[t][i & 1] + 15.5f;
-        }
+        for (int i = 0; i < 4; ++i) s[h][t][i] = fmaf(s[h][t][i], rows.scale[t][i & 1] * ks[h][i >> 1], lv[h][i >> 1]);
+    if (at + kTile > least || real != 3) {                 // tokens that some row does not see
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)                      // token pi + 8 (i / 2) of the half, row 2 c + i % 2
+            if (!(real >> h & 1) || at + 16 * h + pi + 8 * (i >> 1) >= rows.end[t][i & 1]) s[h][t][i] = kNone;
+    }
+    bool grows = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        top[t][y] = fmaxf(fmaxf(s[0][t][y], s[0][t][2 + y]), fmaxf(s[1][t][y], s[1][t][2 + y]));
+        grows |= top[t][y] > m[t][y] + 15.5f;
+      }
     if (__any_sync(kFullWarp, grows)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) this->raise(t, y, fmaxf(fmaxf(s[0][t][y], s[0][t][2 + y]), fmaxf(s[1][t][y], s[1][t][2 + y])));
+        for (int y = 0; y < 2; ++y) this->raise(t, y, top[t][y]);
     }
     uint32_t p[2][NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int t = 0; t < NT; ++t) {
+      const float base[2] = {m[t][0] == kNone ? 0.f : m[t][0], m[t][1] == kNone ? 0.f : m[t][1]};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int h = 0; h < 2; ++h) {
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = exp2_fast(s[h][t][i] - (m[t][i & 1] == kNone ? 0.f : m[t][i & 1]));
+          e[i] = exp2_fast(s[h][t][i] - base[i & 1]);
           l[t][i & 1] = fmaf(e[i], inv[h][i >> 1], l[t][i & 1]);
         }
         p[h][t][0] = transposed(pack_half(e[0], e[1]));
         p[h][t][1] = transposed(pack_half(e[2], e[3]));
       }
+    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[4][D / 64];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int row = 16 * h + 8 * (x >> 1) + ((2 * c + (x & 1)) ^ (c & 1));
+        if constexpr (D == 128) {
+          const uint2 w = *reinterpret_cast<const uint2*>(stage + kKeys<D> + row * 64 + 8 * g);
+          v[x][0] = w.x; v[x][1] = w.y;
+        } else {
+          v[x][0] = *reinterpret_cast<const uint32_t*>(stage + kKeys<D> + row * 32 + 4 * g);
+        }
+      }
+      if (h == 1) read();
 #pragma unroll
       for (int w = 0; w < D / 64; ++w) {
         // bytes of two tokens' codes of one dimension: even ones, odd ones
         constexpr uint32_t kLow = 0x0F0F0F0Fu;
-        const auto even = [&](int x) { return (v[h][x][w] & kLow) | ((v[h][x + 1][w] << 4) & ~kLow); };
-        const auto odd = [&](int x) { return ((v[h][x][w] >> 4) & kLow) | (v[h][x + 1][w] & ~kLow); };
+        const auto low_of = [&](uint32_t x, uint32_t y) {   // the low halves of the bytes of x, the high ones of y
+          uint32_t r;
+          asm("lop3.b32 %0, %1, %2, %3, 0xE4;" : "=r"(r) : "r"(x), "r"(y), "n"(kLow));
+          return r;
+        };
+        const auto even = [&](int x) { return low_of(v[x][w], v[x + 1][w] << 4); };
+        const auto odd = [&](int x) { return low_of(v[x][w] >> 4, v[x + 1][w]); };
         uint32_t a0[4], a1[4], a2[4], a3[4];
         from_e2m1(even(0), a0);
         from_e2m1(odd(0), a1);
@@ -392,34 +689,39 @@ struct Running : Results<D, NT> {
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma_16816(o[4 * w + j][t], a0[j], a1[j], a2[j], a3[j], p[h][t][0], p[h][t][1]);
       }
+    }
   }
 };
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged4_attention_kernel(const AttentionArgs a) {
   constexpr int kRows = 8 * NT, kRing = kDepth * kStage<D>;
   static_assert(kRing >= kRows * (D + 4) * 4, "a warp's results lie where its tiles were");
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ unsigned long long s_full[kAttWarps][kDepth];
-  __shared__ int s_fail;
   __shared__ WarpParts<kRows> parts;
   __shared__ Place place;
+  __shared__ float4 s_wide[kAttWarps][kTile];
+  __shared__ int s_fail;
   pdl_enter();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     a.cuts[blockIdx.x] = {0, 0, 0, 0};
     s_fail = 0;
-    for (int i = 0; i < kAttWarps * kDepth; ++i) bar_init(smem_u32(&s_full[0][i]), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   const Begin<Work> begin(a, kRows, &place);
   if (begin.left <= 0) return;
   const long long share = begin.share;
   int r = begin.r;
   long long skip = begin.skip, left = begin.left;
-  bool bad = false, ok = true;
-  int put = 0, get = 0, ahead = 0;                         // stages of this warp's ring, and how many tiles are on their way
-  uint32_t phase = 0;
+  bool bad = false;
+  uint8_t* const mine = ring + warp * kRing;
+  // where this lane's 16 bytes of a copy come from and go: of keys and values, and of the scales (lanes 0 to 7: of keys and of values, two lanes for a half)
+  const uint8_t *from_k = a.k_cache + 16 * lane, *from_v = a.v_cache + 16 * lane;
+  const uint8_t* from_scale = reinterpret_cast<const uint8_t*>(lane & 4 ? a.v_scale : a.k_scale) + 16 * (lane & 1);
   for (int segment = 0; left > 0; ++segment) {
     const Work x(a, r, kRows);
     if (skip >= x.total) {
@@ -439,84 +741,76 @@ __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged4_atten
     const int kvh = item % a.kv_heads, row0 = item / a.kv_heads * kRows, rows = min(x.rows - row0, kRows);
     const int last_token = (row0 + rows - 1) / a.group;
     const int least = max(x.seen - x.n + row0 / a.group + 1, 0), end = max(x.seen - x.n + last_token + 1, 0);
-    if (segment) {                                         // the results of the last tile have been read
-      __syncthreads();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    // ---- the tiles of this warp: kDepth are on their way.  Lane i holds the page of half i of 16 tiles, and of the 16 after them, which are fetched in time.
+    if (segment) __syncthreads();                          // the results of the last tile have been read
+    // ---- the tiles of this warp: kDepth are on their way.  Lane i holds the place of half i of 16 tiles, and of the 16 after them, which are fetched in time:
+    // in units of 16 tokens of a head, which are 8 D bytes of keys (int32 holds those of any memory).
     const int* table = a.tables + r * a.table_stride;
     const int stop = min(u1 * kUnit, end), first_at = u0 * kUnit + warp * kTile;
-    const int tiles = first_at < stop && ok ? (stop - first_at + kUnit - 1) / kUnit : 0;
+    const int tiles = first_at < stop ? (stop - first_at + kUnit - 1) / kUnit : 0;
     int some, then;
-    const auto ids_of = [&](int tile) {                    // -1: no page, or none of this warp's tokens
+    const auto places_of = [&](int tile) {                 // -1: no page, or none of this warp's tokens
       const int token = first_at + (tile + (lane >> 1)) * kUnit + 16 * (lane & 1);
       if (token >= stop) return -1;
       const int id = table[token >> a.shift];
       const bool real = id >= 0 && id < a.pages;           // no such page: its tokens are not seen
       bad |= !real;
-      return real ? id : -1;
+      return real ? ((id * a.kv_heads + kvh) << (a.shift - 4)) + ((token & ((1 << a.shift) - 1)) >> 4) : -1;
     };
-    const auto request = [&](int tile, int ids, int first, bool held) {        // by all lanes, of a stage that they have read; ids: of the tiles from `first` on
-      const int half = lane >> 2 & 1, kind = lane & 3, id = __shfl_sync(kFullWarp, ids, 2 * (tile - first) + half);
-      const unsigned real = __ballot_sync(kFullWarp, id >= 0);
-      const int halves = (real & 1) + (real >> 4 & 1);
-      if (!held) {
-        const uint32_t bar = smem_u32(&s_full[warp][put]), to = smem_u32(ring + warp * kRing + put * kStage<D>);
-        if (lane == 0) {
-          if (halves) bar_expect(bar, halves * (16 * D + 64));
-          else bar_arrive(bar);
-        }
-        __syncwarp();
-        if (lane < 8 && id >= 0) {                         // keys, values and their scales of both halves
-          const size_t at = (((size_t)id * a.kv_heads + kvh) << a.shift) + ((first_at + tile * kUnit + 16 * half) & ((1 << a.shift) - 1));
-          if (kind < 2) bulk_load(to + kind * kKeys<D> + half * 8 * D, (kind ? a.v_cache : a.k_cache) + at * (D / 2), 8 * D, bar);
-          else bulk_load(to + 2 * kKeys<D> + (kind - 2) * 2 * kTile + half * 32, reinterpret_cast<const uint16_t*>(kind == 2 ? a.k_scale : a.v_scale) + at, 32, bar);
+    // tile `tile` into the stage at `to`, by all lanes, which have read what was there.  What has no page stays what it was.
+    const auto request = [&](int tile, int places, uint8_t* to) {
+      const uint32_t stage = smem_u32(to) + 16 * lane;
+      int at[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        at[h] = __shfl_sync(kFullWarp, places, (2 * tile + h) & 31);
+        if (at[h] < 0) continue;
+        const uint8_t *k = from_k + (size_t)(unsigned)at[h] * (8 * D), *v = from_v + (size_t)(unsigned)at[h] * (8 * D);
+#pragma unroll
+        for (int y = 0; y < D / 64; ++y) {
+          copy16(stage + h * 8 * D + 512 * y, k + 512 * y);
+          copy16(stage + kKeys<D> + h * 8 * D + 512 * y, v + 512 * y);
         }
       }
-      if (++put == kDepth) put = 0;
-      ++ahead;
+      const int one = lane & 2 ? at[1] : at[0];
+      if (lane < 8 && one >= 0) copy16(stage + 2 * kKeys<D>, from_scale + (size_t)(unsigned)one * 32);
     };
-    some = then = ids_of(0);
-    for (int i = 0; i < min(kDepth, tiles); ++i) request(i, some, 0, i == 0 && segment == 0 && warp == 0 && a.withhold == (int)blockIdx.x + 1);
+    const auto done = [&] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    some = then = places_of(0);
+    for (int i = 0; i < kDepth; ++i) {
+      if (i < tiles) request(i, some, mine + i * kStage<D>);
+      done();
+    }
     Rows<T, D, NT, D / 4> q;
     q.load(a, x.start, x.n, x.seen, row0, kvh, lane);
     Running<D, NT> run;
     run.clear();
+    uint8_t* stage = mine;
+    unsigned real = 0;
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
-      const int j = i & 15;
-      if (j == 0 && i) some = then;
-      if (j == 0 && i + 16 < tiles) then = ids_of(i + 16);
-      ok = __all_sync(kFullWarp, bar_wait(smem_u32(&s_full[warp][get]), phase, &s_fail, kWarpSpinLimit));
-      if (!ok) break;
-      const unsigned real = __ballot_sync(kFullWarp, some >= 0) >> (2 * j) & 3;
-      const int at = first_at + i * kUnit;
-      run.add(ring + warp * kRing + get * kStage<D>, q, at, least, real, lane, [&] {
+      if ((i & 15) == 0) {
+        if (i) some = then;
+        if (i + 16 < tiles) then = places_of(i + 16);
+        real = __ballot_sync(kFullWarp, some >= 0);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      __syncwarp();
+      run.add(stage, s_wide[warp], q, first_at + i * kUnit, least, real & 3, lane, [&] {
         __syncwarp();
-        --ahead;
-        if (++get == kDepth) {
-          get = 0;
-          phase ^= 1;
-        }
-        if (i + kDepth < tiles) request(i + kDepth, j + kDepth < 16 ? some : then, i - j + (j + kDepth < 16 ? 0 : 16), false);
+        if (i + kDepth < tiles) request(i + kDepth, (i & 15) + kDepth < 16 ? some : then, stage);
+        done();
       });
+      real >>= 2;
+      stage += kStage<D>;
+      if (stage == mine + kRing) stage = mine;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     const bool whole = u0 == 0 && u1 == x.units;
     finish<T, D, NT, kRing>(a, run, ring, &parts, &s_fail, x, kvh, row0, rows, whole, segment != 0);
     if (!whole && u0 == 0 && tid == 0) {                   // it begins here and ends elsewhere: request, item, parts, place of the first
       const long long beyond = x.units - u1;
       a.cuts[blockIdx.x] = {r, item, 1 + (int)((beyond + share - 1) / share), segment != 0};
     }
-  }
-  if (!ok) {                                               // a wait ran out: what is on its way arrives before the memory goes back
-    for (; ahead > 0; --ahead) {
-      bar_wait(smem_u32(&s_full[warp][get]), phase, nullptr, kDrainLimit);
-      if (++get == kDepth) {
-        get = 0;
-        phase ^= 1;
-      }
-    }
-    if (a.status && lane == 0) atomicOr(a.status, 64);
   }
   if (__any_sync(kFullWarp, bad) && a.status && lane == 0) atomicOr(a.status, 32);
 }
@@ -548,21 +842,25 @@ int attention_of(const AttentionArgs& a, int head_dim, int max_new, cudaStream_t
 }
 
 template <typename T, int D>
-int append_of(const AppendArgs& a, bool halves, cudaStream_t st) {
-  const int heads = a.q_heads + 2 * a.kv_heads, windows = (a.tokens + a.window - 1) / a.window;
-  const dim3 block(kAppendThreads);
-  // few rows: a thread block for each head
-  if ((int64_t)windows * heads <= 4 * (int64_t)current_device_sms())
-    return halves ? paged_launch(rope_append4_kernel<T, D, 1, true>, dim3(windows, heads), block, 1, 0, st, a)
-                  : paged_launch(rope_append4_kernel<T, D, 1, false>, dim3(windows, heads), block, 1, 0, st, a);
-  return halves ? paged_launch(rope_append4_kernel<T, D, 4, true>, dim3(windows, (heads + 3) / 4), block, 1, 0, st, a)
-                : paged_launch(rope_append4_kernel<T, D, 4, false>, dim3(windows, (heads + 3) / 4), block, 1, 0, st, a);
+int append_of(AppendArgs a, bool halves, cudaStream_t st) {
+  const int heads = a.q_heads + 2 * a.kv_heads;
+  if ((int64_t)a.tokens * heads >= kManyRows) {
+    const dim3 grid((a.tokens + kRowsTokens - 1) / kRowsTokens, (heads + kRowsHeads - 1) / kRowsHeads);
+    return halves ? paged_launch(rope_append4_rows_kernel<T, D, true>, grid, dim3(kRowsThreads), 1, 0, st, a)
+                  : paged_launch(rope_append4_rows_kernel<T, D, false>, grid, dim3(kRowsThreads), 1, 0, st, a);
+  }
+  a.window = kAppendThreads / (D / 8);                     // what its rows hold at a time
+  const dim3 grid((a.tokens + a.window - 1) / a.window, heads);
+  return halves ? paged_launch(rope_append4_kernel<T, D, 1, true>, grid, dim3(kAppendThreads), 1, 0, st, a)
+                : paged_launch(rope_append4_kernel<T, D, 1, false>, grid, dim3(kAppendThreads), 1, 0, st, a);
 }
 
 template <typename T>
 int unpack_of(const UnpackArgs& a, int head_dim, int units, cudaStream_t st) {
-  return head_dim == 128 ? paged_launch(unpack4_kernel<T, 128>, dim3(units), dim3(kUnpackThreads), 1, 0, st, a)
-                         : paged_launch(unpack4_kernel<T, 64>, dim3(units), dim3(kUnpackThreads), 1, 0, st, a);
+  const long long pieces = ((long long)units << (a.shift - 4)) * 2;
+  const dim3 grid((unsigned)((pieces + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32)));
+  return head_dim == 128 ? paged_launch(unpack4_kernel<T, 128>, grid, dim3(kUnpackThreads), 1, 0, st, a, pieces)
+                         : paged_launch(unpack4_kernel<T, 64>, grid, dim3(kUnpackThreads), 1, 0, st, a, pieces);
 }
 
 }  // namespace
@@ -585,13 +883,8 @@ int htr_paged4_append(const void* qkv, int dtype, int64_t row_stride, const int*
   if (!aligned16(qkv) || !aligned16(cosv) || !aligned16(sinv) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_scale) || !aligned16(v_scale) ||
       !aligned16(q_out))
     return HTR_ERR_ALIGNMENT;
-  // tokens of a thread block: those that its rows hold at a time, and more where there are thread blocks enough
-  const int heads = q_heads + 2 * kv_heads, rows = kAppendThreads / (head_dim / 8);
-  int window = rows;
-  while (window < kMaxWindow && (int64_t)tokens * heads > (int64_t)window * current_device_sms() * 64) window *= 2;
   const AppendArgs a = {qkv, row_stride, positions, slots, tokens, cosv, sinv, angle_rows, rotary_dim / 2, q_heads, kv_heads, static_cast<uint8_t*>(k_cache),
-                        static_cast<uint8_t*>(v_cache), static_cast<uint16_t*>(k_scale), static_cast<uint16_t*>(v_scale), (int64_t)pages << shift, shift, window,
-                        q_out, status};
+                        static_cast<uint8_t*>(v_cache), static_cast<uint16_t*>(k_scale), static_cast<uint16_t*>(v_scale), (int64_t)pages << shift, shift, 0, q_out, status};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == HTR_DTYPE_BF16) return head_dim == 128 ? append_of<__nv_bfloat16, 128>(a, halves != 0, st) : append_of<__nv_bfloat16, 64>(a, halves != 0, st);
   return head_dim == 128 ? append_of<__half, 128>(a, halves != 0, st) : append_of<__half, 64>(a, halves != 0, st);

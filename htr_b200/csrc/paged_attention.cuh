@@ -66,6 +66,7 @@ template <int kUnit, int kBegin>
 struct Span {
   int start, n, seen, rows, units;
   long long total;
+  Span() = default;
   __device__ __forceinline__ Span(const AttentionArgs& a, int r, int tile_rows) {
     start = max(a.starts[r], 0);
     n = max(min(a.starts[r + 1], a.tokens) - start, 0);
