@@ -33,6 +33,9 @@ __device__ __forceinline__ uint32_t to_e2m1(const float (&v)[8]) {
       : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 __device__ __forceinline__ float of_bf16(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
 // A row's D dimensions, 8 a lane, times the Hadamard matrix; by whole warps.
@@ -83,14 +86,23 @@ struct Turn {
       }
   }
 };
-template <bool kBf16>
+__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b) {       // both halves of the sum against b
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b));
+}
 __device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
-  if constexpr (kBf16)
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b));
-  else
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b));
+}
+// two lanes of float32 arithmetic in one instruction
+__device__ __forceinline__ void turn2(float& x0, float& x1, float k0, float k1, float y0, float y1, float l0, float l1) {     // x k + y l
+  asm("{\n\t.reg .b64 x, k, y, l;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 k, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 l, {%6, %7};\n\tmul.rn.f32x2 x, x, k;\n\t"
+      "fma.rn.f32x2 x, y, l, x;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(x0), "+f"(x1) : "f"(k0), "f"(k1), "f"(y0), "f"(y1), "f"(l0), "f"(l1));
+}
+__device__ __forceinline__ float max_nan(float x, float y) {                                   // of magnitudes; a NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(x)), "f"(fabsf(y)));
+  return r;
 }
 // the H_8 part: over the first index
 template <int kTiles>
@@ -128,21 +140,23 @@ __device__ __forceinline__ void pairs_of(uint32_t x, uint32_t y, uint32_t (&r)[8
   }
 }
 
-// a row's scale from its largest magnitude (NaN stays), and what divides by it
+// a row's scale from its largest magnitude (NaN stays), and the division by it; elements come as x, and are x * by (a power of two)
 struct Scale {
-  float s, inv;
-  bool beyond;                                             // there is more than the scale admits
-  __device__ __forceinline__ explicit Scale(float most) {
+  float s, inv, less;
+  __device__ __forceinline__ explicit Scale(float most, float by = 1.f) {
+    most *= by;
     s = most != most ? most : fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(most, 6.f))), kScaleLeast), kScaleMost);
-    inv = __fdiv_rn(1.f, s);
-    beyond = most > 6.f * kScaleMost;
+    less = s * (1.f / by);
+    inv = __fdiv_rn(by, s);
   }
-  // x / s, to the nearest where it is one of the values between two codes: a tie stays one
+  // x * by / s, to the nearest where it is one of the values between two codes: a tie stays one
   __device__ __forceinline__ float operator()(float x) const {
-    if (beyond) x = fminf(fmaxf(x, -6.f * kScaleMost), 6.f * kScaleMost);
     const float y = x * inv;
-    return fmaf(fmaf(-y, s, x), inv, y);
+    return fmaf(fmaf(-y, less, x), inv, y);
   }
+  // there is more than the largest scale admits (an infinity, too): what an element is then taken for
+  __device__ __forceinline__ bool beyond(float most, float by = 1.f) const { return most * by > 6.f * kScaleMost; }
+  __device__ __forceinline__ float within(float x) const { return fminf(fmaxf(x, -6.f * less), 6.f * less); }
 };
 
 template <typename T>
@@ -279,19 +293,14 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
         continue;
       }
       float most = 0.f;
-      bool nan = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        most = fmaxf(most, fabsf(v[j]));
-        nan |= v[j] != v[j];
-      }
-      most = nan ? __int_as_float(0x7FC00000) : most;
+      for (int j = 0; j < 8; ++j) most = max_nan(most, v[j]);
 #pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) {
-        const float x = __shfl_xor_sync(kFullWarp, most, o);
-        most = most != most || x != x ? __int_as_float(0x7FC00000) : fmaxf(most, x);
-      }
+      for (int o = 1; o < kLanes; o <<= 1) most = max_nan(most, __shfl_xor_sync(kFullWarp, most, o));
       const Scale scale(most);                             // (a row with a NaN: so are all of its values, by their scale)
+      if (scale.beyond(most))
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = scale.within(v[j]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = scale(v[j]);
       if (!mine || !ok) continue;
@@ -307,31 +316,57 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
 // The same for many tokens: a warp takes 16 of them at a time, one head after the other, and transforms by matrix products.  The rotated elements enter as two
 // bf16 each, 16 bits in all: 2^-16 of an element at most, where queries are rounded to 2^-9 or 2^-12 of the result and keys to four bits.  (With three, 2^-24.)
 // An infinity among a row's elements makes all of the row NaN.
-constexpr int kRowsThreads = 128, kRowsTokens = 16, kRowsHeads = 16, kManyRows = 4096;
+constexpr int kRowsThreads = 128, kRowsTokens = 16, kRowsHeads = 8, kManyRows = 32768;
+
+// rows of tokens in shared memory, so far apart that lanes of two neighbouring tokens read different banks: elements, 64 bytes a piece; angles, 64 or (halves) 16 of 32
+template <int D>
+constexpr int kRowBytes = kRowsHeads * D * 2 + 64;
+template <int D, bool kHalves>
+constexpr int kAngleFloats = D / 2 + (kHalves ? 4 : 16);
+template <int D, bool kHalves>
+constexpr int kRowsSmem = kRowsTokens * (kRowBytes<D> + 8 * kAngleFloats<D, kHalves>);
 
 template <typename T, int D, bool kHalves>
-__global__ void __launch_bounds__(kRowsThreads) rope_append4_rows_kernel(const AppendArgs a) {
-  constexpr int kWarps = kRowsThreads / 32, kTiles = D / 64;
+__global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(const AppendArgs a) {
+  constexpr int kWarps = kRowsThreads / 32, kTiles = D / 64, kAngles = kAngleFloats<D, kHalves>;
+  extern __shared__ __align__(128) uint8_t rows_smem[];
+  float *cos_s = reinterpret_cast<float*>(rows_smem + kRowsTokens * kRowBytes<D>), *sin_s = cos_s + kRowsTokens * kAngles;
   __shared__ int s_slot[kRowsTokens + kMaxPage], s_pos[kRowsTokens], s_bad[kRowsTokens];
   pdl_enter();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, page = 1 << a.shift;
   const int t0 = blockIdx.x * kRowsTokens, n = min(kRowsTokens, a.tokens - t0);
-  const T* qkv = static_cast<const T*>(a.qkv);
+  const int h0 = blockIdx.y * kRowsHeads, heads = min(kRowsHeads, a.q_heads + 2 * a.kv_heads - h0);
+  {                                                        // all heads of the tokens are on their way while the slots are looked at
+    const uint8_t* from = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.qkv) + (size_t)t0 * a.row_stride + (size_t)h0 * D);
+    const int pieces = heads * D / 8;                      // of a token, 16 bytes each
+    for (int w = warp; w < n; w += kWarps)
+      for (int i = lane; i < pieces; i += 32) copy16(smem_u32(rows_smem + w * kRowBytes<D> + 16 * i), from + (size_t)w * a.row_stride * 2 + 16 * i);
+  }
   find_written<kRowsThreads>(a, t0, n, s_slot, s_pos, s_bad);
-  const int last = min((int)(blockIdx.y + 1) * kRowsHeads, a.q_heads + 2 * a.kv_heads);
-  for (int h = blockIdx.y * kRowsHeads + warp; h < last; h += kWarps) {
+  if (h0 < a.q_heads + a.kv_heads)
+    for (int w = warp; w < n; w += kWarps) {
+      const size_t at = s_bad[w] == 0 ? (size_t)s_pos[w] * a.half : 0;
+      for (int i = lane; i < a.half / 2; i += 32) {        // cosines, then sines
+        const int z = i < a.half / 4 ? i : i - a.half / 4;
+        copy16(smem_u32((i < a.half / 4 ? cos_s : sin_s) + w * kAngles + 4 * z), (i < a.half / 4 ? a.cosv : a.sinv) + at + 4 * z);
+      }
+    }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  for (int h = h0 + warp; h < h0 + heads; h += kWarps) {
     const bool turns = h < a.q_heads + a.kv_heads, query = h < a.q_heads;
     // rows g and g + 8; those behind the last are its
-    size_t row[2];
     int w[2];
+    const uint8_t* row[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       w[r] = min(g + 8 * r, n - 1);
-      row[r] = (size_t)(t0 + w[r]) * a.row_stride + (size_t)h * D;
+      row[r] = rows_smem + w[r] * kRowBytes<D> + (h - h0) * D * 2;
     }
     float v[8][kTiles][4];                                 // of dimension b of chunk 2 t + i % 2, row g + 8 (i / 2)
     if (turns) {
-      const Turn<D> turn(false, true, query, D == 128 ? 0x3C003C00u : 0x3C803C80u, lane);        // 1 / D in bf16
+      // queries times 8 / D, and keys times 1 / D, which their scale makes up for: so no finite ones add up to an infinity on the way
+      const Turn<D> turn(false, true, query, (D == 128 ? 0x3C003C00u : 0x3C803C80u) + (query ? 0x01800180u : 0), lane);
 #pragma unroll
       for (int b = 0; b < 8; ++b)
 #pragma unroll
@@ -341,30 +376,29 @@ __global__ void __launch_bounds__(kRowsThreads) rope_append4_rows_kernel(const A
         uint32_t high[2][8], low[2][8];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const size_t angles = s_bad[w[r]] == 0 ? (size_t)s_pos[w[r]] * a.half : 0;
+          const float *cs_at = cos_s + w[r] * kAngles, *sn_at = sin_s + w[r] * kAngles;
           float x[2][8];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int at = 8 * chunk_of(true, kChunks<D>, c, 2 * p + e);
-            const uint4 raw = *reinterpret_cast<const uint4*>(qkv + row[r] + at);
-            widen<T>(raw, x[e]);
+            widen<T>(*reinterpret_cast<const uint4*>(row[r] + 2 * at), x[e]);
             if (at >= 2 * a.half) continue;
             if constexpr (kHalves) {
               const bool first = at < a.half;
-              const uint4 raw2 = *reinterpret_cast<const uint4*>(qkv + row[r] + at + (first ? a.half : -a.half));
+              const int other = first ? at + a.half : at - a.half, angle = first ? at : other;
+              const uint32_t sign = first ? 0x80008000u : 0;
+              uint4 raw = *reinterpret_cast<const uint4*>(row[r] + 2 * other);
+              raw.x ^= sign; raw.y ^= sign; raw.z ^= sign; raw.w ^= sign;
               float y[8];
-              widen<T>(raw2, y);
-              const size_t from = angles + at - (first ? 0 : a.half);
+              widen<T>(raw, y);
 #pragma unroll
               for (int z = 0; z < 8; z += 4) {
-                const float4 cs = *reinterpret_cast<const float4*>(a.cosv + from + z), sn = *reinterpret_cast<const float4*>(a.sinv + from + z);
-                const float k[4] = {cs.x, cs.y, cs.z, cs.w}, l[4] = {sn.x, sn.y, sn.z, sn.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[e][z + j] = x[e][z + j] * k[j] + (first ? -y[z + j] : y[z + j]) * l[j];
+                const float4 cs = *reinterpret_cast<const float4*>(cs_at + angle + z), sn = *reinterpret_cast<const float4*>(sn_at + angle + z);
+                turn2(x[e][z], x[e][z + 1], cs.x, cs.y, y[z], y[z + 1], sn.x, sn.y);
+                turn2(x[e][z + 2], x[e][z + 3], cs.z, cs.w, y[z + 2], y[z + 3], sn.z, sn.w);
               }
             } else {
-              const size_t from = angles + at / 2;
-              const float4 cs = *reinterpret_cast<const float4*>(a.cosv + from), sn = *reinterpret_cast<const float4*>(a.sinv + from);
+              const float4 cs = *reinterpret_cast<const float4*>(cs_at + at / 2), sn = *reinterpret_cast<const float4*>(sn_at + at / 2);
               const float k[4] = {cs.x, cs.y, cs.z, cs.w}, l[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -384,27 +418,16 @@ __global__ void __launch_bounds__(kRowsThreads) rope_append4_rows_kernel(const A
 #pragma unroll
         for (int b = 0; b < 8; ++b)
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            mma_1688<true>(v[b][t], high[0][b], high[1][b], turn.b[p][t]);
-            mma_1688<true>(v[b][t], low[0][b], low[1][b], turn.b[p][t]);
-          }
+          for (int t = 0; t < kTiles; ++t) mma_16816_bf16(v[b][t], high[0][b], high[1][b], low[0][b], low[1][b], turn.b[p][t]);
       }
       across(v);
-      const float by = query ? 8.f : D / 8.f;
-#pragma unroll
-      for (int b = 0; b < 8; ++b)
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[b][t][i] *= by;
     } else {
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int y = 0; y < kChunks<D>; ++y) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(qkv + row[r] + 8 * chunk_of(false, kChunks<D>, c, y));
           float x[8];
-          widen<T>(raw, x);
+          widen<T>(*reinterpret_cast<const uint4*>(row[r] + 16 * chunk_of(false, kChunks<D>, c, y)), x);
 #pragma unroll
           for (int b = 0; b < 8; ++b) v[b][y >> 1][2 * r + (y & 1)] = x[b];
         }
@@ -413,32 +436,33 @@ __global__ void __launch_bounds__(kRowsThreads) rope_append4_rows_kernel(const A
     for (int r = 0; r < 2; ++r) {
       const bool mine = g + 8 * r < n, ok = s_bad[w[r]] == 0;
       if (query) {
+        if (!ok)
+#pragma unroll
+          for (int b = 0; b < 8; ++b)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) v[b][t][2 * r] = v[b][t][2 * r + 1] = 0.f;
 #pragma unroll
         for (int y = 0; y < kChunks<D>; ++y) {
           const int t = y >> 1, i = 2 * r + (y & 1);
-          uint4 out = {Half<T>::narrow(v[0][t][i], v[1][t][i]), Half<T>::narrow(v[2][t][i], v[3][t][i]), Half<T>::narrow(v[4][t][i], v[5][t][i]), Half<T>::narrow(v[6][t][i], v[7][t][i])};
-          if (!ok) out = {0, 0, 0, 0};
+          const uint4 out = {Half<T>::narrow(v[0][t][i], v[1][t][i]), Half<T>::narrow(v[2][t][i], v[3][t][i]), Half<T>::narrow(v[4][t][i], v[5][t][i]), Half<T>::narrow(v[6][t][i], v[7][t][i])};
           if (mine) *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + ((size_t)(t0 + w[r]) * a.q_heads + h) * D + 8 * chunk_of(true, kChunks<D>, c, y)) = out;
         }
         continue;
       }
       float most = 0.f;
-      bool nan = false;
 #pragma unroll
       for (int b = 0; b < 8; ++b)
 #pragma unroll
-        for (int y = 0; y < kChunks<D>; ++y) {
-          const float x = v[b][y >> 1][2 * r + (y & 1)];
-          most = fmaxf(most, fabsf(x));
-          nan |= x != x;
-        }
-      if (nan) most = __int_as_float(0x7FC00000);
+        for (int y = 0; y < kChunks<D>; ++y) most = max_nan(most, v[b][y >> 1][2 * r + (y & 1)]);
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        const float x = __shfl_xor_sync(kFullWarp, most, o);
-        most = most != most || x != x ? __int_as_float(0x7FC00000) : fmaxf(most, x);
-      }
-      const Scale scale(most);
+      for (int o = 1; o < 4; o <<= 1) most = max_nan(most, __shfl_xor_sync(kFullWarp, most, o));
+      const float by = turns ? D / 8.f : 1.f;
+      const Scale scale(most, by);
+      if (scale.beyond(most, by))
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+#pragma unroll
+          for (int y = 0; y < kChunks<D>; ++y) v[b][y >> 1][2 * r + (y & 1)] = scale.within(v[b][y >> 1][2 * r + (y & 1)]);
       uint32_t codes[kChunks<D>];
 #pragma unroll
       for (int y = 0; y < kChunks<D>; ++y) {
@@ -468,7 +492,7 @@ struct UnpackArgs {
   void *k_out, *v_out;
 };
 
-constexpr int kUnpackThreads = 128;
+constexpr int kUnpackThreads = 64;
 
 template <typename T>
 __device__ __forceinline__ void put8(T* to, const float (&v)[8]) {
@@ -507,7 +531,7 @@ __global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArg
       const uint2 x = *reinterpret_cast<const uint2*>(src);
       w[r][0] = x.x; w[r][1] = x.y;
     }
-    scale[r] = of_bf16((values ? a.v_scale : a.k_scale)[row]) * (values ? 1.f : 8.f / D);
+    scale[r] = real ? of_bf16((values ? a.v_scale : a.k_scale)[row]) * (values ? 1.f : 8.f / D) : 0.f;        // (codes are finite: zeros)
   }
   const Turn<D> turn(values, false, true, 0x3C003C00u, lane);
   float v[8][kTiles][4];
@@ -523,7 +547,7 @@ __global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArg
 #pragma unroll
     for (int b = 0; b < 8; ++b)
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) mma_1688<false>(v[b][t], x[0][b], x[1][b], turn.b[p][t]);
+      for (int t = 0; t < kTiles; ++t) mma_1688(v[b][t], x[0][b], x[1][b], turn.b[p][t]);
   }
   if (!values) across(v);
   T* out = static_cast<T*>(values ? a.v_out : a.k_out);
@@ -533,7 +557,7 @@ __global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArg
     for (int y = 0; y < kChunks<D>; ++y) {
       float x[8];
 #pragma unroll
-      for (int b = 0; b < 8; ++b) x[b] = real ? v[b][y >> 1][2 * r + (y & 1)] * scale[r] : 0.f;
+      for (int b = 0; b < 8; ++b) x[b] = v[b][y >> 1][2 * r + (y & 1)] * scale[r];
       put8<T>(out + (to + g + 8 * r) * D + 8 * chunk_of(true, kChunks<D>, c, y), x);
     }
 }
@@ -693,10 +717,6 @@ struct Running : Results<D, NT> {
   }
 };
 
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads, (kAttBlocks<D, NT>)) paged4_attention_kernel(const AttentionArgs a) {
   constexpr int kRows = 8 * NT, kRing = kDepth * kStage<D>;
@@ -841,13 +861,24 @@ int attention_of(const AttentionArgs& a, int head_dim, int max_new, cudaStream_t
   return head_dim == 128 ? attention_run<T, 128, 2>(a, st) : attention_run<T, 64, 2>(a, st);
 }
 
+template <typename T, int D, bool kHalves>
+int append_rows(const AppendArgs& a, dim3 grid, cudaStream_t st) {
+  static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
+  constexpr int kBytes = kRowsSmem<D, kHalves>;
+  int dev = 0, e = (int)cudaGetDevice(&dev);
+  if (kBytes > 40960 && !e && (dev < 0 || dev >= 64 || !allowed[dev])) {
+    e = (int)cudaFuncSetAttribute(rope_append4_rows_kernel<T, D, kHalves>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
+  }
+  return e ? paged_fail(e) : paged_launch(rope_append4_rows_kernel<T, D, kHalves>, grid, dim3(kRowsThreads), 1, kBytes, st, a);
+}
+
 template <typename T, int D>
 int append_of(AppendArgs a, bool halves, cudaStream_t st) {
   const int heads = a.q_heads + 2 * a.kv_heads;
   if ((int64_t)a.tokens * heads >= kManyRows) {
     const dim3 grid((a.tokens + kRowsTokens - 1) / kRowsTokens, (heads + kRowsHeads - 1) / kRowsHeads);
-    return halves ? paged_launch(rope_append4_rows_kernel<T, D, true>, grid, dim3(kRowsThreads), 1, 0, st, a)
-                  : paged_launch(rope_append4_rows_kernel<T, D, false>, grid, dim3(kRowsThreads), 1, 0, st, a);
+    return halves ? append_rows<T, D, true>(a, grid, st) : append_rows<T, D, false>(a, grid, st);
   }
   a.window = kAppendThreads / (D / 8);                     // what its rows hold at a time
   const dim3 grid((a.tokens + a.window - 1) / a.window, heads);

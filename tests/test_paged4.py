@@ -8,7 +8,7 @@ gpu = pytest.mark.gpu
 DEV = torch.device("cuda:0")
 LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 NAN = 0x7FC0
-MANY = 4096                                                  # rows (tokens times heads) from which on an append goes through matrix products
+MANY = 32768                                                 # rows (tokens times heads) from which on an append goes through matrix products
 
 
 def ints(v):
@@ -717,7 +717,8 @@ def turns(rows, dim, theta, first=0, factor=1.0, original=None, low=1.0, high=32
 @gpu
 @pytest.mark.parametrize("rows,dim,theta,how", ((1, 2, 1e4, {}), (1000, 128, 1e6, {}), (777, 96, 1e4, dict(first=131072)), (300, 6, 500.0, dict(factor=3.0)), (513, 256, 1e6, dict(first=999999)),
                                                 (4097, 64, 1e6, dict(factor=8.0, original=32768)), (100, 30, 1e4, dict(factor=4.0, original=2048, low=2.0, high=4.0, magnitude=1.3)),
-                                                (64, 128, 1e6, dict(first=2 ** 30))))
+                                                (64, 128, 1e6, dict(first=2 ** 30)),
+                                                (20011, 128, 1e6, dict(first=77)), (10007, 30, 1e4, dict(factor=4.0, original=2048, magnitude=0.8)), (9999, 256, 1e6, {}), (12345, 2, 1e4, {})))
 def test_angles(rows, dim, theta, how):
     from htr_b200 import rotary
 
@@ -725,7 +726,8 @@ def test_angles(rows, dim, theta, how):
     size = how.get("magnitude", 1.0)
     a = turns(rows, dim, theta, **{k: v for k, v in how.items() if k != "magnitude"})
     assert cos.shape == sin.shape == (rows, dim // 2) and cos.dtype == torch.float32
-    # sincospif is off by at most 2 steps of float32 (2^-24 of 1 each at most, twice), its correction, the factor and the result are rounded once each; and the angle
+    # sincospif is off by at most a step of float32 (2^-24), its correction and the factor are rounded once each (2^-25); where there are many rows the result is a product
+    # of two such complex numbers: each error times at most sqrt 2 for both parts of the other, and two roundings more: 2 * 1.42 * 2 + 1 < 7 times 2^-24.  And the angle
     # in 64 bits, once for the frequency (pow: 2 steps) and once for the product: 2^-51 of it, here and in the expectation
     far = torch.arange(how.get("first", 0), how.get("first", 0) + rows, dtype=torch.double)[:, None]
     bound = size * (7 * 2.0 ** -24 + 2 * 2.0 ** -51 * far)
@@ -742,7 +744,7 @@ def test_angles_are_those_of_the_decoder():
     model = PackedDecoder.__new__(PackedDecoder)
     model.cfg, model.device = DecoderConfig(), DEV
     for got, want in zip(rotary.angles(70000, 128, model.cfg.rope_theta, device=DEV), model._far_angles(70000)):
-        assert float((got - want).abs().max()) <= 8 * 2.0 ** -24
+        assert float((got - want).abs().max()) <= 8 * 2.0 ** -24   # (the bound of test_angles, and a rounding of the other)
 
 
 # ---- refusals -------------------------------------------------------------------------------------------------------
