@@ -725,14 +725,18 @@ PyObject* py_unpack(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return pair_of(std::move(out[0]), std::move(out[1]));
 }
 
-// rope_angles(rows, dim, theta, first, factor, original, low, high, magnitude, device index): (cosines, sines)
+// rope_angles(rows, dim, theta, first, factor, original, low, high, magnitude, device): (cosines, sines)
 PyObject* py_rope_angles(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  int rows, dim, first, dev;
+  int rows, dim, first;
   double theta, how[5];
-  if (n != 10 || !int_of(a[0], &rows) || !int_of(a[1], &dim) || !float_of(a[2], &theta) || !int_of(a[3], &first) || !int_of(a[9], &dev)) return none();
-  for (int i = 0; i < 5; ++i)
-    if (!float_of(a[4 + i], &how[i])) return none();
-  if (rows < 1 || dim < 2 || dim > 256 || dev < 0 || dev >= c10::cuda::device_count()) return none();
+  if (n != 10 || !int_of(a[0], &rows) || !int_of(a[1], &dim) || !float_of(a[2], &theta) || !int_of(a[3], &first) || !THPDevice_Check(a[9])) return none();
+  for (int i = 0; i < 5; ++i) {
+    if (i == 1 && a[4 + i] == Py_None) how[i] = 0;
+    else if (!float_of(a[4 + i], &how[i]) || (i == 1 && !(how[i] > 0))) return none();
+  }
+  const at::Device device = reinterpret_cast<THPDevice*>(a[9])->device;
+  if (rows < 1 || dim < 2 || dim > 256 || !device.is_cuda()) return none();
+  const int dev = device.has_index() ? device.index() : c10::cuda::current_device();
   OnDevice on(dev);
   const at::Device where(at::kCUDA, (c10::DeviceIndex)dev);
   at::Tensor out[2];

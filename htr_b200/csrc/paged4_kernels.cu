@@ -889,7 +889,9 @@ int append_of(AppendArgs a, bool halves, cudaStream_t st) {
 template <typename T>
 int unpack_of(const UnpackArgs& a, int head_dim, int units, cudaStream_t st) {
   const long long pieces = ((long long)units << (a.shift - 4)) * 2;
-  const dim3 grid((unsigned)((pieces + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32)));
+  const long long blocks = (pieces + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32);
+  if (blocks > 0x7FFFFFFF) return HTR_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)blocks);
   return head_dim == 128 ? paged_launch(unpack4_kernel<T, 128>, grid, dim3(kUnpackThreads), 1, 0, st, a, pieces)
                          : paged_launch(unpack4_kernel<T, 64>, grid, dim3(kUnpackThreads), 1, 0, st, a, pieces);
 }

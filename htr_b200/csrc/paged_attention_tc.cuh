@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const uint32_t n = piece_n >> 3;
       const bool values = piece_n & 4, real = valid(p.id), there = real && p.at + (lane & 15) < p.end;
       const int group = piece_n & 3;
-      bad |= p.id != -1 && !real;                          // (-1: behind the last token)
+      bad |= p.at < p.end && !real;
       const float vs = __uint_as_float((uint32_t)x.vs << 16), ks = __uint_as_float((uint32_t)x.ks << 16);
       const bool nan_v = vs != vs, nan_k = ks != ks;
       const int ev = exponent(there && !nan_v ? held(vs) : 0.f);

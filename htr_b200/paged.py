@@ -74,7 +74,7 @@ def _status(what, status, dev):
 
 def _cache(what, cache, dev):
     """Pages, heads, page size, head dimensions of a layer's cache, and whether it is in 4 bits."""
-    if isinstance(cache, LayerCache4):
+    if cache[0].dtype == torch.uint8:
         return *_cache4(what, cache, dev), True
     return *_cache8(what, cache, dev), False
 
@@ -275,8 +275,6 @@ def unpack(cache, pages, dtype=torch.bfloat16):
     if not pages.is_cuda:
         raise _lib.HTRError("unpack has no CPU path: tensors must live on a CUDA device")
     dev = pages.device
-    if not isinstance(cache, LayerCache4):
-        raise _lib.HTRError("unpack: wants a LayerCache4")
     count, kv_heads, page, dim = _cache4("unpack", cache, dev)
     _int32("unpack", "pages", pages, dev, pages.numel())
     if dtype not in ops._DTYPES:

@@ -333,18 +333,20 @@ def attend_exactly(q, starts, seen, tables, cache, scale):
     return out, spread
 
 
-def widened(q, tables, cache):
-    """The tables with so many more (unused) columns that many rows a request are taken to be much work: by their width, for lengths are not known on the host."""
-    page, width = cache.k.shape[2], tables.shape[1]
-    more = int(1.6e9 / (max(q.shape[0], 1) * q.shape[1] * q.shape[2] * page)) + 1 - width
-    return tables if more <= 0 else torch.cat([tables, torch.full((tables.shape[0], more), -1, dtype=torch.int32, device=tables.device)], 1)
+def many(q, tables, cache):
+    """The same call as one of much work, which goes by what the host knows: rows of queries behind the last token and (unused) columns of the tables.  Returns
+    q, tables and max_new."""
+    page, group, D = cache.k.shape[2], q.shape[1] // cache.k.shape[1], q.shape[2]
+    q = torch.cat([q, torch.ones_like(q[:1]).expand(max(24576 // (group * D) + 1 - q.shape[0], 0), -1, -1)])
+    more = int(1.6e9 / (q.shape[0] * q.shape[1] * D * page)) + 1 - tables.shape[1]
+    return q, tables if more <= 0 else torch.cat([tables, torch.full((tables.shape[0], more), -1, dtype=torch.int32, device=tables.device)], 1), q.shape[0]
 
 
-def check_attention(q, starts, seen, tables, cache, max_new, scale=None, **kw):
-    """By both kernels where there are many rows a request."""
-    if q.shape[1] // cache.k.shape[1] * min(max_new, q.shape[0]) * q.shape[2] > 2048:
-        check_one_attention(q, starts, seen, widened(q, tables, cache), cache, max_new, scale, **kw)
-    return check_one_attention(q, starts, seen, tables, cache, max_new, scale, **kw)
+def check_attention(q, starts, seen, tables, cache, max_new, scale=None, out=None):
+    """By both kernels."""
+    q2, tables2, most = many(q, tables, cache)
+    check_one_attention(q2, starts, seen, tables2, cache, most, scale)
+    return check_one_attention(q, starts, seen, tables, cache, max_new, scale, out=out)
 
 
 def bound_of(dtype, want, spread):
@@ -413,12 +415,11 @@ def test_a_nan_reaches_only_those_that_see_it(adds, wide, value):
     q, starts, seen, tables, cache = filled(torch.bfloat16, 128, 16, 8, 2, (40, 17), adds)
     from htr_b200 import paged
 
-    if wide:
-        tables = widened(q, tables, cache)
-    want = paged.attention(q, starts, seen, tables, cache, max(adds))
+    q, tables, most = many(q, tables, cache) if wide else (q, tables, max(adds))
+    want = paged.attention(q, starts, seen, tables, cache, most, out=torch.zeros_like(q))
     at, n = 40 + adds[0] - 2, adds[0]                            # the last token but one of request 0
     (cache.v_scale if value else cache.k_scale)[int(tables[0, at // 16]), 1, at % 16] = float("nan")
-    got = paged.attention(q, starts, seen, tables, cache, max(adds))
+    got = paged.attention(q, starts, seen, tables, cache, most, out=torch.zeros_like(q))
     hit = torch.zeros_like(got, dtype=torch.bool)
     hit[n - 2:n, 4:] = True
     assert torch.equal(got.isnan(), hit) and torch.equal(got[~hit], want[~hit])
@@ -431,14 +432,17 @@ def test_table_entries_that_are_no_page_hide_their_tokens(adds, wide, page):
     from htr_b200 import paged
 
     q, starts, seen, tables, cache = filled(torch.bfloat16, 64, page, 2, 1, (200, 64), adds)
-    if wide:
-        tables = widened(q, tables, cache)
-    status = ints([0])
-    full = paged.attention(q, starts, seen, tables, cache, max(adds), status=status).clone()
+    q, tables, most = many(q, tables, cache) if wide else (q, tables, max(adds))
+    status, total = ints([0]), int(starts[-1])
+    full = paged.attention(q, starts, seen, tables, cache, most, status=status)[:total].clone()
     assert int(status) == 0
     tables[0, 2], tables[1, :] = 1 << 30, -1
-    got = paged.attention(q, starts, seen, tables, cache, max(adds), status=status)
+    got = paged.attention(q, starts, seen, tables, cache, most, status=status)[:total]
     assert int(status) == 32 and torch.isfinite(got).all() and (got[int(starts[1]):] == 0).all() and not torch.equal(got, full)
+    alone, gap = tables.clone(), ints([0])                       # -1 in the place of a page, too
+    alone[0, 2], alone[1] = -1, alone[0]
+    paged.attention(q, starts, seen, alone, cache, most, status=gap)
+    assert int(gap) == 32
     # without the hidden tokens: request 0 alone, whose scores there are lower than anything that counts
     hidden = [t for t in range(int(seen[0])) if t // page == 2]
     n = int(starts[1])
@@ -468,11 +472,10 @@ def test_queries_that_are_not_finite(bad, D, adds, wide):
     from htr_b200 import paged
 
     q, starts, seen, tables, cache = filled(torch.bfloat16, D, 16, 8, 2, (40, 17), adds)
-    if wide:
-        tables = widened(q, tables, cache)
-    want = paged.attention(q, starts, seen, tables, cache, max(adds))
+    q, tables, most = many(q, tables, cache) if wide else (q, tables, max(adds))
+    want = paged.attention(q, starts, seen, tables, cache, most, out=torch.zeros_like(q))
     q[1, 5, 3] = bad
-    got = paged.attention(q, starts, seen, tables, cache, max(adds))
+    got = paged.attention(q, starts, seen, tables, cache, most, out=torch.zeros_like(q))
     hit = torch.zeros_like(got, dtype=torch.bool)
     hit[1, 5] = True
     assert torch.equal(got.isnan(), hit) and torch.equal(got[~hit], want[~hit])
@@ -502,7 +505,7 @@ def test_a_token_that_takes_nearly_all_and_has_no_values(dtype, D, adds, R, nats
     cache.k_scale[id, :, 0] = 16 * nats / 6 if nats != 15 else 40                     # (12, 15 and 18 times 16 / 6 are bf16's)
     cache.v[id, :, 0] = 0
     want, spread = attend_exactly(q, starts, seen, tables, cache, 1 / 16)
-    got = paged.attention(q.repeat(R, 1, 1), ints([adds * r for r in range(R + 1)]), seen.repeat(R), widened(q, tables, cache).repeat(R, 1), cache, adds, scale=1 / 16)
+    got = paged.attention(q.repeat(R, 1, 1), ints([adds * r for r in range(R + 1)]), seen.repeat(R), many(q, tables, cache)[1].repeat(R, 1), cache, adds * R, scale=1 / 16)
     off, bound = (got.double().view(R, *q.shape) - want).abs(), bound_of(dtype, want, spread)
     assert (off <= bound).all(), float((off / bound).max())
 
@@ -571,15 +574,18 @@ def test_two_graphs_and_another_stream(adds, wide):
     from htr_b200 import paged
 
     sets = [filled(torch.bfloat16, 128, 16, 8, 2, have, adds, seed=s) for s, have in enumerate(((3000, 1, 50), (40, 2500, 700)))]
+    most = max(adds)
     if wide:
-        sets = [(q, starts, seen, widened(q, tables, cache), cache) for q, starts, seen, tables, cache in sets]
-    want = [paged.attention(*x, max(adds)).clone() for x in sets]
+        sets = [(q2, starts, seen, tables2, cache) for q, starts, seen, tables, cache in sets for q2, tables2, most in (many(q, tables, cache),)]
+        most = sets[0][0].shape[0]
+    run = lambda x: paged.attention(*x, most, out=torch.zeros_like(x[0]))
+    want = [run(x).clone() for x in sets]
     graphs, outs = [], []
     for x in sets:
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            outs.append(paged.attention(*x, max(adds)))
+            outs.append(run(x))
         graphs.append(graph)
     streams = [torch.cuda.Stream() for _ in sets]
     torch.cuda.synchronize()
@@ -590,7 +596,7 @@ def test_two_graphs_and_another_stream(adds, wide):
         for graph, stream in zip(graphs, streams):
             with torch.cuda.stream(stream):
                 graph.replay()
-        eager = paged.attention(*sets[0], max(adds))
+        eager = run(sets[0])
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want)) and torch.equal(eager, want[0])
 
@@ -627,16 +633,16 @@ def test_rows_of_an_expired_wait_are_nan(D, have, adds, block):
     from htr_b200 import _lib, paged
 
     q, starts, seen, tables, cache = filled(torch.bfloat16, D, 16, 8, 2, have, adds)
-    tables = widened(q, tables, cache)
+    q, tables, most = many(q, tables, cache)
     status = ints([0])
-    want = paged.attention(q, starts, seen, tables, cache, max(adds), status=status)
+    want = paged.attention(q, starts, seen, tables, cache, most, out=torch.full_like(q, 3.0), status=status)
     assert int(status) == 0
     for word in (status, None):
         for one in range(block, block + 4):                      # (a thread block whose share is what an item costs besides its tokens has none)
             out = torch.full_like(q, 3.0)
             _lib.lib.htr_paged_attention_withhold(one)
             try:
-                paged.attention(q, starts, seen, tables, cache, max(adds), out=out, status=word)
+                paged.attention(q, starts, seen, tables, cache, most, out=out, status=word)
             finally:
                 _lib.lib.htr_paged_attention_withhold(-1)
             lost = out.isnan().any(-1)
@@ -644,7 +650,7 @@ def test_rows_of_an_expired_wait_are_nan(D, have, adds, block):
                 break
         assert 0 < int(lost.sum()) < lost.numel() // 4 and out[lost].isnan().all() and torch.equal(out[~lost], want[~lost])
     assert int(status) == 64
-    assert torch.equal(paged.attention(q, starts, seen, tables, cache, max(adds), status=status.zero_()), want) and int(status) == 0
+    assert torch.equal(paged.attention(q, starts, seen, tables, cache, most, out=torch.full_like(q, 3.0), status=status.zero_()), want) and int(status) == 0
 
 
 # ---- the operators in a row -----------------------------------------------------------------------------------------
