@@ -224,6 +224,7 @@ __device__ __forceinline__ void find_written(const AppendArgs& a, int t0, int n,
 // grid (windows of tokens, groups of kHeads heads of queries, keys and values as they stand in a row).  A thread holds 8 dimensions of a row, four pairs
 // of neighbours; in halves a pair's other element comes from another lane.
 // A token whose slot does not lie above those of its page in the page - 1 tokens before it is not written: every place has one writer.
+// Bound by latency: slots -> rows and angles -> sums over lanes.  8 tokens of 32 heads of 128 on 8 in a chain of launches: 2.6 us.
 template <typename T, int D, int kHeads, bool kHalves>
 __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const AppendArgs a) {
   constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes;
@@ -316,6 +317,9 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
 // The same for many tokens: a warp takes 16 of them at a time, one head after the other, and transforms by matrix products.  The rotated elements enter as two
 // bf16 each, 16 bits in all: 2^-16 of an element at most, where queries are rounded to 2^-9 or 2^-12 of the result and keys to four bits.  (With three, 2^-24.)
 // An infinity among a row's elements makes all of the row NaN.
+// Sums over lanes, four shuffles an element, were what bound the form above here: 65 us for 4096 tokens of 32 heads of 128 on 8 (94 MB) in a chain of launches.  With products
+// from registers 44, from shared memory, where all heads of 16 tokens are on their way at once, 33, and 28 (3.2 TB/s) with what a lane's chunks are known beforehand.
+// What bounds it now: 1200 instructions for 16 rows, at half of the issue slots.  The two forms are level at some 600 tokens of 48 heads (9.6 and 9.7 us; 1024: 17.2 and 11.5).
 constexpr int kRowsThreads = 128, kRowsTokens = 16, kRowsHeads = 8, kManyRows = 32768;
 
 // rows of tokens in shared memory, so far apart that lanes of two neighbouring tokens read different banks: elements, 64 bytes a piece; angles, 64 or (halves) 16 of 32
@@ -326,9 +330,11 @@ constexpr int kAngleFloats = D / 2 + (kHalves ? 4 : 16);
 template <int D, bool kHalves>
 constexpr int kRowsSmem = kRowsTokens * (kRowBytes<D> + 8 * kAngleFloats<D, kHalves>);
 
-template <typename T, int D, bool kHalves>
+// kFull: all of a head is rotated, and then a lane knows which of its chunks are the first of their pairs
+template <typename T, int D, bool kHalves, bool kFull>
 __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(const AppendArgs a) {
   constexpr int kWarps = kRowsThreads / 32, kTiles = D / 64, kAngles = kAngleFloats<D, kHalves>;
+  const int pairs = kFull ? D / 2 : a.half;
   extern __shared__ __align__(128) uint8_t rows_smem[];
   float *cos_s = reinterpret_cast<float*>(rows_smem + kRowsTokens * kRowBytes<D>), *sin_s = cos_s + kRowsTokens * kAngles;
   __shared__ int s_slot[kRowsTokens + kMaxPage], s_pos[kRowsTokens], s_bad[kRowsTokens];
@@ -345,10 +351,10 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
   find_written<kRowsThreads>(a, t0, n, s_slot, s_pos, s_bad);
   if (h0 < a.q_heads + a.kv_heads)
     for (int w = warp; w < n; w += kWarps) {
-      const size_t at = s_bad[w] == 0 ? (size_t)s_pos[w] * a.half : 0;
-      for (int i = lane; i < a.half / 2; i += 32) {        // cosines, then sines
-        const int z = i < a.half / 4 ? i : i - a.half / 4;
-        copy16(smem_u32((i < a.half / 4 ? cos_s : sin_s) + w * kAngles + 4 * z), (i < a.half / 4 ? a.cosv : a.sinv) + at + 4 * z);
+      const size_t at = s_bad[w] == 0 ? (size_t)s_pos[w] * pairs : 0;
+      for (int i = lane; i < pairs / 2; i += 32) {        // cosines, then sines
+        const int z = i < pairs / 4 ? i : i - pairs / 4;
+        copy16(smem_u32((i < pairs / 4 ? cos_s : sin_s) + w * kAngles + 4 * z), (i < pairs / 4 ? a.cosv : a.sinv) + at + 4 * z);
       }
     }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -382,10 +388,10 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
           for (int e = 0; e < 2; ++e) {
             const int at = 8 * chunk_of(true, kChunks<D>, c, 2 * p + e);
             widen<T>(*reinterpret_cast<const uint4*>(row[r] + 2 * at), x[e]);
-            if (at >= 2 * a.half) continue;
+            if (!kFull && at >= 2 * pairs) continue;
             if constexpr (kHalves) {
-              const bool first = at < a.half;
-              const int other = first ? at + a.half : at - a.half, angle = first ? at : other;
+              const bool first = kFull ? 2 * p + e < kChunks<D> / 2 : at < pairs;
+              const int other = first ? at + pairs : at - pairs, angle = first ? at : other;
               const uint32_t sign = first ? 0x80008000u : 0;
               uint4 raw = *reinterpret_cast<const uint4*>(row[r] + 2 * other);
               raw.x ^= sign; raw.y ^= sign; raw.z ^= sign; raw.w ^= sign;
@@ -505,7 +511,8 @@ __device__ __forceinline__ void put8<float>(float* to, const float (&v)[8]) {
 }
 
 // A warp takes 16 tokens of keys, which it turns back (H H = D), or of values, which pass through the same products only to lie side by side.  The sums are those of
-// codes, exact; one multiplication by the scale, and one rounding.  Bound by what it writes.
+// codes, exact; one multiplication by the scale, and one rounding.  Bound by what it writes: 901 pages of 64 tokens, 8 heads of 128 (297 MB) in 54 us in a chain of
+// launches, 5.5 TB/s.  (Sums over lanes: 78.  Warps that stay and fetch ahead: 87, their registers spill.)
 template <typename T, int D>
 __global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArgs a, long long pieces) {
   constexpr int kTiles = D / 64;
@@ -566,11 +573,20 @@ __global__ void __launch_bounds__(kUnpackThreads) unpack4_kernel(const UnpackArg
 //
 // As over the 8-bit cache (paged_kernels.cu): rows are query heads times tokens, the cache is the 16-row operand of m16n8k16, a warp takes tiles of the
 // cache for itself, work is cut evenly and joined.  What differs:
-//  * a tile has 32 tokens, in two halves that may lie in different pages;
+//  * a tile has 32 tokens, in two halves that may lie in different pages; what a tile costs besides its tokens is paid half as often;
+//  * tiles come by 16-byte asynchronous copies of all lanes.  (Eight bulk copies a tile, as halves, keys, values and scales lie apart, are issued lane by lane, 100 instructions:
+//    99 us where this took 86.)  No wait here depends on another thread but __syncwarp;
 //  * a byte is two neighbouring dimensions of a token, which is what a register of the keys' fragment holds; for values it has to be two neighbouring
 //    tokens of one dimension: two bitwise selections make such bytes of the words of two tokens;
 //  * scales belong to tokens: those of keys multiply the scores, those of values enter the exponent (P' = 2^(s + log2 scale - m)) and the sum takes them out.
+//    A lane makes these numbers for one token of the tile, and all fetch what they need from shared memory.
 // Row i of a half is its token i ^ (i >> 1 & 1): neighbouring lanes then read rows of both parities, which lie in different banks.
+//
+// 64 requests of 10 to 16384 tokens, 32 heads of 128 on 8 (392 MB): 80 us in a chain of launches, 4.9 TB/s; 64 of 16383 (1.1 GB): 192 us, 5.8 TB/s.  Two steps
+// of such a length differ by what their bytes take at 6.3 TB/s; the rest, some 16 us, is begin, end and join.  At the size above copies without products
+// take 67 us, products without copies 71: 434 instructions a tile at half of the issue slots, the conversions (two cycles each, with all other integer
+// instructions) at half of their pipe.  Tried without gain: four thread blocks on an SM (spills: 82 to 95), rings of two or four tiles, the first tiles of the next item
+// requested before the results of one are joined (82).
 
 constexpr int kTile = 32, kUnit = kAttWarps * kTile, kDepth = 3;
 constexpr int kBegin = 3;                                  // what an item costs besides its units
@@ -861,16 +877,16 @@ int attention_of(const AttentionArgs& a, int head_dim, int max_new, cudaStream_t
   return head_dim == 128 ? attention_run<T, 128, 2>(a, st) : attention_run<T, 64, 2>(a, st);
 }
 
-template <typename T, int D, bool kHalves>
+template <typename T, int D, bool kHalves, bool kFull>
 int append_rows(const AppendArgs& a, dim3 grid, cudaStream_t st) {
   static bool allowed[64] = {false};                       // shared memory beyond 48 KB: opted in once per device
   constexpr int kBytes = kRowsSmem<D, kHalves>;
   int dev = 0, e = (int)cudaGetDevice(&dev);
   if (kBytes > 40960 && !e && (dev < 0 || dev >= 64 || !allowed[dev])) {
-    e = (int)cudaFuncSetAttribute(rope_append4_rows_kernel<T, D, kHalves>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    e = (int)cudaFuncSetAttribute(rope_append4_rows_kernel<T, D, kHalves, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (!e && dev >= 0 && dev < 64) allowed[dev] = true;
   }
-  return e ? paged_fail(e) : paged_launch(rope_append4_rows_kernel<T, D, kHalves>, grid, dim3(kRowsThreads), 1, kBytes, st, a);
+  return e ? paged_fail(e) : paged_launch(rope_append4_rows_kernel<T, D, kHalves, kFull>, grid, dim3(kRowsThreads), 1, kBytes, st, a);
 }
 
 template <typename T, int D>
@@ -878,7 +894,8 @@ int append_of(AppendArgs a, bool halves, cudaStream_t st) {
   const int heads = a.q_heads + 2 * a.kv_heads;
   if ((int64_t)a.tokens * heads >= kManyRows) {
     const dim3 grid((a.tokens + kRowsTokens - 1) / kRowsTokens, (heads + kRowsHeads - 1) / kRowsHeads);
-    return halves ? append_rows<T, D, true>(a, grid, st) : append_rows<T, D, false>(a, grid, st);
+    if (2 * a.half == D) return halves ? append_rows<T, D, true, true>(a, grid, st) : append_rows<T, D, false, true>(a, grid, st);
+    return halves ? append_rows<T, D, true, false>(a, grid, st) : append_rows<T, D, false, false>(a, grid, st);
   }
   a.window = kAppendThreads / (D / 8);                     // what its rows hold at a time
   const dim3 grid((a.tokens + a.window - 1) / a.window, heads);

@@ -120,9 +120,17 @@ def test_cache_holds_what_was_appended(dtype, layout, D, page, hq, hkv, r):
 
 @gpu
 @pytest.mark.parametrize("layout", ("interleaved", "half"))
-@pytest.mark.parametrize("D,T", ((128, 1), (64, 1), (128, 700), (64, 1501)))
-def test_append_of_one_token_and_of_many(layout, D, T):
-    check_append(torch.bfloat16, D, 64, 12, 2, layout, D, [(T,)], slack_columns=8)
+@pytest.mark.parametrize("dtype,D,T,r", ((torch.bfloat16, 128, 1, 128), (torch.bfloat16, 64, 1, 64), (torch.bfloat16, 128, 700, 128), (torch.bfloat16, 64, 1501, 64),
+                                         (torch.bfloat16, 128, 2049, 128), (torch.float16, 64, 3001, 64), (torch.float16, 128, 2200, 48), (torch.bfloat16, 64, 2500, 32),
+                                         (torch.bfloat16, 128, 2100, 16), (torch.float16, 128, 2051, 128)))
+def test_append_of_one_token_and_of_many(dtype, layout, D, T, r):
+    check_append(dtype, D, 64, 12, 2, layout, r, [(T,)], slack_columns=8, pages=60)
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,T", ((1, 1, 11000), (3, 5, 2600), (33, 3, 900)))
+def test_heads_that_do_not_fill_a_thread_block(hq, hkv, T):
+    check_append(torch.bfloat16, 64, 128, hq, hkv, "half", 64, [(T // 2, T - T // 2)], pages=100)
 
 
 @gpu
