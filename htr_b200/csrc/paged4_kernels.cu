@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
         hadamard<D>(v, lane);
         const float by = h < a.q_heads ? 8.f : D / 8.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= by;
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] + (v[j] - v[j])) * by;        // (an infinity, which only an infinite element can have made, becomes NaN)
       }
       if (h < a.q_heads) {
         uint4 r = {Half<T>::narrow(v[0], v[1]), Half<T>::narrow(v[2], v[3]), Half<T>::narrow(v[4], v[5]), Half<T>::narrow(v[6], v[7])};

@@ -159,8 +159,9 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None, la
 
     Into a cache of 4 bits, pairs may also be halves (layout "half": dimensions i and i + r / 2), and r, twice the columns of cos and sin, a part of the
     head that is a multiple of 16: the first r dimensions are rotated.  The queries come back as H q * 8 / head_dim for the keys of such a cache (see
-    LayerCache4; fp16 ones whose sums leave its range become infinite).  A token's scale is bf16(largest / 6), its codes are the nearest, ties to the even code; infinities are held as
-    the largest value (6 * 2^119, or what the rest of a key's transform makes of them), and a row of a head that has a NaN is NaN as a whole.  A token whose slot does not lie above those of its page
+    LayerCache4; fp16 ones whose sums leave its range become infinite, and bf16 ones beyond 2^124 may).  A token's scale is bf16(largest / 6), its codes are the nearest, ties to
+    the even code; infinities among values are held as the largest value, 6 * 2^119, as is all that lies beyond it, and a row of a head that has a NaN is NaN as a whole, so
+    is one of queries or keys that has an infinity.  A token whose slot does not lie above those of its page
     among the page_size - 1 tokens before it is not written, and its query is zero (status 16).  What follows is of the cache of 8 bits.
 
     A page's scale is the smallest power of two (at least 2^-100) under which all of its tokens lie within e4m3 (448); it begins anew with the

@@ -189,6 +189,24 @@ def test_special_values_and_tokens_outside(layout, more):
 
 
 @gpu
+@pytest.mark.parametrize("layout", ("interleaved", "half"))
+@pytest.mark.parametrize("more", (0, MANY // 4))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_an_infinity_among_what_is_transformed_takes_its_row(dtype, layout, more):
+    from htr_b200 import paged
+
+    D, page = 128, 16
+    cache, (cos, sin) = empty_cache(1, 1, page, D), angles(32, D)
+    x = torch.ones(5 + more, 4 * D, dtype=dtype, device=DEV)
+    x[1, 5], x[2, D + 77], x[3, 2 * D], x[4, 3 * D - 1] = float("inf"), float("-inf"), float("-inf"), float("inf")
+    q = paged.rope_append(x, ints([0, 1, 2, 3, 4] + [0] * more), ints([0, 1, 2, 3, 4] + [-1] * more), cos, sin, cache, 2, layout=layout)
+    hit = torch.zeros(5 + more, 2, D, dtype=torch.bool, device=DEV)
+    hit[1, 0] = hit[2, 1] = True
+    assert torch.equal(q.isnan(), hit) and torch.isfinite(q[~hit]).all()
+    assert cache.k_scale[0, 0, :5].isnan().tolist() == [False, False, False, True, True] and torch.isfinite(cache.v_scale[0, 0, :5]).all()
+
+
+@gpu
 @pytest.mark.parametrize("page", (16, 64, 128))
 @pytest.mark.parametrize("D,hkv", ((128, 1), (64, 3), (64, 40), (128, 30)))
 def test_every_place_has_one_writer(page, D, hkv):
