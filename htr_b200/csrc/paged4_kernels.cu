@@ -223,7 +223,8 @@ __device__ __forceinline__ void find_written(const AppendArgs& a, int t0, int n,
 
 // grid (windows of tokens, groups of kHeads heads of queries, keys and values as they stand in a row).  A thread holds 8 dimensions of a row, four pairs
 // of neighbours; in halves a pair's other element comes from another lane.
-// A token whose slot does not lie above those of its page in the page - 1 tokens before it is not written: every place has one writer.
+// A token whose slot does not lie above those of its page in the page - 1 tokens before it is not written: every place has one writer, where the tokens of a
+// page lie within so many.
 // Bound by latency: slots -> rows and angles -> sums over lanes.  8 tokens of 32 heads of 128 on 8 in a chain of launches: 2.6 us.
 template <typename T, int D, int kHeads, bool kHalves>
 __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const AppendArgs a) {

@@ -134,7 +134,7 @@ extern "C" int htr_rope_angles(int64_t first, int rows, int dim, double theta, d
   if (rows < 0 || first < 0 || dim < 2 || dim % 2 || !(theta > 0) || !(factor > 0) || !(original >= 0) || !(low < high) || !std::isfinite(theta) ||
       !std::isfinite(factor) || !std::isfinite(original) || !std::isfinite(low) || !std::isfinite(high))
     return HTR_ERR_BAD_SHAPE;
-  if (dim > 2 * kMostPairs || first + rows > 0x7FFFFFFF || first > 0x7FFFFFFF) return HTR_ERR_TOO_LARGE;
+  if (dim > 2 * kMostPairs || first > 0x7FFFFFFF || first + rows > 0x7FFFFFFF) return HTR_ERR_TOO_LARGE;
   if (rows == 0) return HTR_OK;
   if (!cosv || !sinv) return HTR_ERR_NULL;
   constexpr double kPi = 3.14159265358979323846;

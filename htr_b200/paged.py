@@ -157,18 +157,20 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None, la
     qkv [tokens, (q_heads + 2 kv_heads) * head_dim] bf16 or fp16 (rows may be strided); positions, slots [tokens] as `plan_step` gives them; cos, sin
     float32 [rows, head_dim / 2], a row per position, for interleaved pairs.  Returns the rotated queries [tokens, q_heads, head_dim].
 
-    Into a cache of 4 bits, pairs may also be halves (layout "half": dimensions i and i + r / 2), and r, twice the columns of cos and sin, a part of the
-    head that is a multiple of 16: the first r dimensions are rotated.  The queries come back as H q * 8 / head_dim for the keys of such a cache (see
-    LayerCache4; fp16 ones whose sums leave its range become infinite, and bf16 ones beyond 2^124 may).  A token's scale is bf16(largest / 6), its codes are the nearest, ties to
-    the even code; infinities among values are held as the largest value, 6 * 2^119, as is all that lies beyond it, and a row of a head that has a NaN is NaN as a whole, so
-    is one of queries or keys that has an infinity.  A token whose slot does not lie above those of its page
-    among the page_size - 1 tokens before it is not written, and its query is zero (status 16).  What follows is of the cache of 8 bits.
-
-    A page's scale is the smallest power of two (at least 2^-100) under which all of its tokens lie within e4m3 (448); it begins anew with the
-    page's first place, and where a later token makes it grow the older ones are rescaled.  Infinities are held as the largest value, NaN as NaN.
     A token with slot -1 is not written and its query is zero; so is one whose slot or position lies outside the buffers (status 16).
     The tokens of one page stand one after the other in rising slots, as `plan_step` lays them out, within page_size tokens of the step (tokens that are not
-    written may lie between them); from a slot that does not rise on, that page's are not written (status 16)."""
+    written may lie between them).  In 8 bits, from a slot that does not rise on, that page's are not written; in 4, a token is not whose slot does not lie above
+    those of its page among the page_size - 1 tokens before it (status 16 both).  A slot that comes again farther on is the caller's to avoid: what it then holds may be
+    the codes of one token under the scale of the other.
+
+    8 bits: a page's scale is the smallest power of two (at least 2^-100) under which all of its tokens lie within e4m3 (448); it begins anew with the
+    page's first place, and where a later token makes it grow the older ones are rescaled.  Infinities are held as the largest value, NaN as NaN.
+
+    4 bits: pairs may also be halves (layout "half": dimensions i and i + r / 2), and r, twice the columns of cos and sin, a part of the
+    head that is a multiple of 16: the first r dimensions are rotated.  The queries come back as H q * 8 / head_dim for the keys of such a cache (see
+    LayerCache4; fp16 ones whose sums leave its range become infinite, and bf16 ones beyond 2^124 may).  A token's scale is bf16(largest / 6), its codes are the
+    nearest, ties to the even code.  Infinities among values are held as the largest value, 6 * 2^119, as is all that lies beyond it; a row of a head that has a NaN is
+    NaN as a whole, and so is one of queries or keys that has an infinity."""
     what = "rope_append"
     q = _host.rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status, layout)
     if q is not None:
