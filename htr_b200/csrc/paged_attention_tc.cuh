@@ -34,7 +34,8 @@
 // Seven warps (8-13, 15) feed both, 16 tokens at a time, by code that stands once and is not unrolled: twice and unrolled it drove the softmax out of the instruction cache
 // (339 us where this took 208).  The reference lies 2^4 under the largest term when it moves, and then for all rows of the warp whose largest lies higher: terms down to 2^-18 of the
 // largest keep all bits, smaller ones are off by up to 2^-29 of it.  Keys whose norms differ by token make references move, a move costs 3000 cycles, and with 2^12 every second unit of the
-// prompt above had one: 200 us, with 2^8 183, with 2^4 172 (2^0: 169; none: 146).  Two threads a row (16 softmax warps of 88 registers) took 186.
+// prompt above had one: 200 us, with 2^8 183, with 2^4 172 (2^0: 169; none: 146).  P goes to tensor memory before the
+// sums are looked at, and once more where a reference moves: 171.  Two threads a row (16 softmax warps of 88 registers) took 186, a thread for each kind of product 191.
 #pragma once
 #include <type_traits>
 
@@ -719,7 +720,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
               p[c] = pack_half(y, z);
             }
           };
+          const auto store = [&] {
+            tmem_store(scores, reinterpret_cast<const uint32_t (&)[16]>(p[0]));
+            tmem_store(scores + 16, reinterpret_cast<const uint32_t (&)[16]>(p[16]));
+          };
           exponentials();
+          if (kBits == 4) {                                // (on its way while it is looked at)
+            __syncwarp();
+            store();
+          }
           // a sum within the range of fp16: so is each of its terms
           const float most = fmaxf(fmaxf(fmaxf(sum[0][0], sum[0][1]), fmaxf(sum[1][0], sum[1][1])), fmaxf(fmaxf(sum[2][0], sum[2][1]), fmaxf(sum[3][0], sum[3][1])));
           const bool grows = m == kNone || most > 60000.f;
@@ -740,11 +749,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
               if (ok) follow(f);
             }
             if (kBits == 8) exponentials();
+            if (kBits == 4) {
+              tmem_stored();
+              store();
+            }
           }
           l = fmaf(sum[0][0] + sum[0][1], inv.x, fmaf(sum[1][0] + sum[1][1], inv.y, fmaf(sum[2][0] + sum[2][1], inv.z, fmaf(sum[3][0] + sum[3][1], inv.w, l))));
-          __syncwarp();
-          tmem_store(scores, reinterpret_cast<const uint32_t (&)[16]>(p[0]));
-          tmem_store(scores + 16, reinterpret_cast<const uint32_t (&)[16]>(p[16]));
+          if (kBits == 8) {
+            __syncwarp();
+            store();
+          }
           tmem_stored();
         }
         fence_before();
