@@ -86,9 +86,21 @@ struct Turn {
       }
   }
 };
-__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b) {       // both halves of the sum against b
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b));
+// float32 as two of tf32, which have 11 significant bits and are cut off: 2^-20 of an element is left over at most (`b`: a pair of bf16, exact in tf32)
+struct Tf32 {
+  uint32_t high, low;
+  __device__ __forceinline__ explicit Tf32(float x) {
+    high = __float_as_uint(x) & 0xFFFFE000u;
+    low = __float_as_uint(x - __uint_as_float(high));
+  }
+};
+__device__ __forceinline__ void mma_1688_tf32(float (&d)[4], const Tf32& a0, const Tf32& a1, const Tf32& a2, const Tf32& a3, uint32_t b) {
+  const auto part = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b << 16), "r"(b & 0xFFFF0000u));
+  };
+  part(a0.low, a1.low, a2.low, a3.low);
+  part(a0.high, a1.high, a2.high, a3.high);
 }
 __device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
@@ -316,11 +328,12 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
 }
 
 // The same for many tokens: a warp takes 16 of them at a time, one head after the other, and transforms by matrix products.  The rotated elements enter as two
-// bf16 each, 16 bits in all: 2^-16 of an element at most, where queries are rounded to 2^-9 or 2^-12 of the result and keys to four bits.  (With three, 2^-24.)
+// tf32 each, which leave 2^-20 of an element at most.  (Two bf16, 2^-16, in half of the products took 28 us where this takes 30, but a code that lies next to a tie then comes
+// out as its neighbour often enough to show: 5e-4 of the norm of fp16 keys, whose own rounding is 2e-4.)
 // An infinity among a row's elements makes all of the row NaN.
 // Sums over lanes, four shuffles an element, were what bound the form above here: 65 us for 4096 tokens of 32 heads of 128 on 8 (94 MB) in a chain of launches.  With products
-// from registers 44, from shared memory, where all heads of 16 tokens are on their way at once, 33, and 28 (3.2 TB/s) with what a lane's chunks are known beforehand.
-// What bounds it now: 1200 instructions for 16 rows, at half of the issue slots.  The two forms are level at some 600 tokens of 48 heads (9.6 and 9.7 us; 1024: 17.2 and 11.5).
+// from registers 44, from shared memory, where all heads of 16 tokens are on their way at once, 33, and 28 with what a lane's chunks are known beforehand.
+// What bounds it now (3.0 TB/s): some 1200 instructions for 16 rows, at half of the issue slots.  The two forms are level at some 600 tokens of 48 heads (9.6 and 9.7 us; 1024: 17.2 and 11.5).
 constexpr int kRowsThreads = 128, kRowsTokens = 16, kRowsHeads = 8, kManyRows = 32768;
 
 // rows of tokens in shared memory, so far apart that lanes of two neighbouring tokens read different banks: elements, 64 bytes a piece; angles, 64 or (halves) 16 of 32
@@ -380,15 +393,14 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
         for (int t = 0; t < kTiles; ++t) v[b][t][0] = v[b][t][1] = v[b][t][2] = v[b][t][3] = 0.f;
 #pragma unroll
       for (int p = 0; p < kTiles; ++p) {
-        uint32_t high[2][8], low[2][8];
+        float x[2][2][8];                                  // rows, chunks of the pair
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float *cs_at = cos_s + w[r] * kAngles, *sn_at = sin_s + w[r] * kAngles;
-          float x[2][8];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int at = 8 * chunk_of(true, kChunks<D>, c, 2 * p + e);
-            widen<T>(*reinterpret_cast<const uint4*>(row[r] + 2 * at), x[e]);
+            widen<T>(*reinterpret_cast<const uint4*>(row[r] + 2 * at), x[r][e]);
             if (!kFull && at >= 2 * pairs) continue;
             if constexpr (kHalves) {
               const bool first = kFull ? 2 * p + e < kChunks<D> / 2 : at < pairs;
@@ -401,31 +413,27 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
 #pragma unroll
               for (int z = 0; z < 8; z += 4) {
                 const float4 cs = *reinterpret_cast<const float4*>(cs_at + angle + z), sn = *reinterpret_cast<const float4*>(sn_at + angle + z);
-                turn2(x[e][z], x[e][z + 1], cs.x, cs.y, y[z], y[z + 1], sn.x, sn.y);
-                turn2(x[e][z + 2], x[e][z + 3], cs.z, cs.w, y[z + 2], y[z + 3], sn.z, sn.w);
+                turn2(x[r][e][z], x[r][e][z + 1], cs.x, cs.y, y[z], y[z + 1], sn.x, sn.y);
+                turn2(x[r][e][z + 2], x[r][e][z + 3], cs.z, cs.w, y[z + 2], y[z + 3], sn.z, sn.w);
               }
             } else {
               const float4 cs = *reinterpret_cast<const float4*>(cs_at + at / 2), sn = *reinterpret_cast<const float4*>(sn_at + at / 2);
               const float k[4] = {cs.x, cs.y, cs.z, cs.w}, l[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float y = x[e][2 * j], z = x[e][2 * j + 1];
-                x[e][2 * j] = y * k[j] - z * l[j];
-                x[e][2 * j + 1] = y * l[j] + z * k[j];
+                const float y = x[r][e][2 * j], z = x[r][e][2 * j + 1];
+                x[r][e][2 * j] = y * k[j] - z * l[j];
+                x[r][e][2 * j + 1] = y * l[j] + z * k[j];
               }
             }
           }
-#pragma unroll
-          for (int b = 0; b < 8; ++b) {
-            high[r][b] = Half<__nv_bfloat16>::narrow(x[0][b], x[1][b]);
-            const float2 held = Half<__nv_bfloat16>::wide(high[r][b]);
-            low[r][b] = Half<__nv_bfloat16>::narrow(x[0][b] - held.x, x[1][b] - held.y);
-          }
         }
 #pragma unroll
-        for (int b = 0; b < 8; ++b)
+        for (int b = 0; b < 8; ++b) {
+          const Tf32 a0(x[0][0][b]), a1(x[1][0][b]), a2(x[0][1][b]), a3(x[1][1][b]);
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) mma_16816_bf16(v[b][t], high[0][b], high[1][b], low[0][b], low[1][b], turn.b[p][t]);
+          for (int t = 0; t < kTiles; ++t) mma_1688_tf32(v[b][t], a0, a1, a2, a3, turn.b[p][t]);
+        }
       }
       across(v);
     } else {

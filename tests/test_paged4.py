@@ -94,8 +94,9 @@ def check_append(dtype, D, page, hq, hkv, layout, r, steps, size=1.0, pages=40, 
         c, s = (t.double()[torch.tensor(pos, device=DEV)] for t in (cos, sin))
         z = rotated(y[:, :hq + hkv], c, s, layout) @ H
         # float32: three roundings of a rotation, then log2 D of each sum, each relative to at most the sum of all magnitudes (of which a rotated pair has up to
-        # sqrt 2 times as much); where there are many rows, their elements enter as two bf16, the second of which rounds what the first leaves (2^-8) to 2^-8 of it
-        noise = ((3 + math.log2(D)) * 2.0 ** -24 + (2.0 ** -16 if T * (hq + 2 * hkv) >= MANY else 0)) * 2 ** 0.5 * y[:, :hq + hkv].abs().sum(-1)
+        # sqrt 2 times as much); where there are many rows, their elements enter as two tf32, the second of which cuts what the first leaves (2^-10) at
+        # 2^-10 of it, and the matrix unit adds up in four steps, each cut at 2^-22 of the largest or finer
+        noise = ((3 + math.log2(D)) * 2.0 ** -24 + (2.0 ** -19 if T * (hq + 2 * hkv) >= MANY else 0)) * 2 ** 0.5 * y[:, :hq + hkv].abs().sum(-1)
         want = z[:, :hq] * 8 / D
         bound = torch.finfo(dtype).eps / 2 * want.abs() + noise[:, :hq, None] * 8 / D * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
         assert ((q.double() - want).abs() <= bound).all(), float(((q.double() - want).abs() / bound).max())
