@@ -29,8 +29,11 @@
 // runs of units of (request, item, head), each as many as its last token sees.
 // Over the cache of 4 bits everything is fp16: a code times its token's scale (2 and 8 significant bits) is, exactly, under a power of two for each 16
 // tokens of keys and of values, which takes the place of a page's scale; the warps that feed keys and values widen both on their way.  A row of Q is one part
-// of fp16 (28 binades), for the same tensor pipe as bf16's two of e4m3.  Tokens whose scale lies below 2^-13 of the largest of their 16 are off by up to 2^-25 of
-// that, and probabilities are relative to what they would be under it.  A value whose scale is NaN is a zero, and its key NaN, which reaches those that see it.
+// of fp16 (28 binades), for the same tensor pipe as bf16's two of e4m3.  A value whose scale is NaN is a zero, and its key NaN, which reaches those that see it.
+// Where the scales of 16 keys lie more than 13 binades apart, or those of 16 values more than 4, each of the tokens keeps its own: codes are widened as they are, and the scale
+// multiplies the scores or enters the exponent and the sum token by token.  The power of two comes from all 16, and a row need not see all of them: so keys and values are exact
+// whatever lies beside them, and what a token's neighbours, seen or not, can do to its probability is to take less than five binades from the bits below.  A unit
+// with such tokens takes some two times as long: the prompt above 384 us where every unit has one, 180 where one page in 64 has; and that they are looked for costs it 3 us of 176.
 // Seven warps (8-13, 15) feed both, 16 tokens at a time, by code that stands once and is not unrolled: twice and unrolled it drove the softmax out of the instruction cache
 // (339 us where this took 208).  The reference lies 2^4 under the largest term when it moves, and then for all rows of the warp whose largest lies higher: terms down to 2^-18 of the
 // largest keep all bits, smaller ones are off by up to 2^-29 of it.  Keys whose norms differ by token make references move, a move costs 3000 cycles, and with 2^12 every second unit of the
@@ -50,6 +53,7 @@ constexpr int kTmemColumns = 512;                          // of a tile: S (P ov
 template <int kBits>
 constexpr float kTopOf = kBits == 4 ? 4.f : 12.f;          // where a row's largest term lies when its reference moves
 constexpr int kRing = 4, kScales = 8;                      // units of keys and of values in shared memory; of their scales, read by all rows
+constexpr int kKeySpread = 13, kValueSpread = 4;           // binades between the scales of 16 tokens of 4 bits from which on each token keeps its own
 
 template <typename T, int D, int kBits>
 struct Layout {                                            // bytes of the operands
@@ -154,7 +158,7 @@ struct Shared {
   uint32_t tmem;
   int fail, nan;
   alignas(16) float ks[kScales][kGroups], lv[kScales][kGroups], inv[kScales][kGroups];     // of the 16-token groups of a unit: scales; log2 and inverse of those of the values
-  unsigned char real[kScales][kGroups];                    // groups that have a page
+  unsigned char real[kScales][kGroups];                    // 1: groups that have a page; 2: whose tokens keep their own scales
   float twin_m[kTile], twin_l[kTile];
   int finished[8];                                         // items of the run that the rows of a warp are through with
 };
@@ -199,6 +203,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   uint8_t* smem = raw_smem + (-smem_u32(raw_smem) & 1023);
   __shared__ Shared s;
+  // of tokens that keep their own scales, as ks, lv and inv
+  constexpr int kOwn = kBits == 4 ? kScales : 1;
+  __shared__ __align__(16) float own_ks[kOwn][kUnit], own_lv[kOwn][kUnit], own_inv[kOwn][kUnit];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* fail = &s.fail;
@@ -459,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
     constexpr int kFeeders = 7, kPer = D == 128 ? 8 : 16, kPasses = 16 / kPer;           // a lane has 32 dimensions of every kPer-th token
     const int me = warp == 15 ? 6 : warp - 8, place_mask = (1 << a.shift) - 1, in_pass = lane % kPer, piece = lane / kPer;
     const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
-    const auto held = [&](float s) { return fminf(fmaxf(s, 7.888609052210118e-31f), 6.646139978924579e35f); };           // 2^-100 to 2^119
+    const auto held = [&](float s) { return fminf(fmaxf(s, 7.888609052210118e-31f), 6.646139978924579e35f); };           // 2^-100 to 2^119 (NaN: 2^-100)
     const uint32_t pieces = 8 * (uint32_t)count;
     bool ok = true, bad = false;
     struct Piece {
@@ -509,22 +516,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const float vs = __uint_as_float((uint32_t)x.vs << 16), ks = __uint_as_float((uint32_t)x.ks << 16);
       const bool nan_v = vs != vs, nan_k = ks != ks;
       const int ev = exponent(there && !nan_v ? held(vs) : 0.f);
+      const bool own_v = __any_sync(kFullWarp, there && !nan_v && held(vs) < exp2i(ev - kValueSpread));      // (ev >= -100)
       float by;
       if (values) {
-        by = there && !nan_v ? held(vs) * exp2i(-ev) : 0.f;
+        by = there && !nan_v ? own_v ? 1.f : held(vs) * exp2i(-ev) : 0.f;
         if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.v_free, kRing, n - kRing));
         if (!ok) return;
       } else {
         const int ek = exponent(there && !nan_k ? held(ks) : 0.f);
-        by = !there ? 0.f : nan_k || nan_v ? __int_as_float(0x7FC00000) : held(ks) * exp2i(-ek);
+        const bool own_k = __any_sync(kFullWarp, there && !nan_k && held(ks) < exp2i(ek - kKeySpread));
+        by = !there ? 0.f : nan_k || nan_v ? __int_as_float(0x7FC00000) : own_k ? 1.f : held(ks) * exp2i(-ek);
         if (n >= kRing) ok = __all_sync(kFullWarp, ring(s.k_free, kRing, n - kRing));
         if (!ok) return;
+        const int slot = n % kScales;
         if (lane == 0) {
-          const int slot = n % kScales;
           s.ks[slot][group] = exp2i(ek);
           s.lv[slot][group] = (float)ev;
           s.inv[slot][group] = exp2i(-ev) * kSumUnit;
-          s.real[slot][group] = real;
+          s.real[slot][group] = real | (own_k || own_v ? 2 : 0);
+        }
+        if ((own_k || own_v) && lane < 16) {               // (what is not there is masked)
+          own_ks[slot][16 * group + lane] = own_k ? held(ks) : exp2i(ek);
+          own_lv[slot][16 * group + lane] = own_v ? __log2f(held(vs)) : (float)ev;
+          own_inv[slot][16 * group + lane] = own_v ? __fdividef(kSumUnit, held(vs)) : exp2i(-ev) * kSumUnit;
         }
       }
       const uint32_t two = pack_half(by, by);
@@ -680,6 +694,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
       const uint32_t step = w.twin ? 2 : 1;                // of this tile's units
       n += w.twin ? x : 0;
       int u = w.u0 + (w.twin ? x : 0);
+      // a unit with tokens that keep their own scales: as below, in less code and more time
+      const auto by_token = [&](uint32_t scores, int slot, unsigned real, int at) {
+        uint32_t raw[32];
+        float v[32];
+        const auto terms = [&](int h, float base) {
+          __syncwarp();
+          tmem_load(scores + 32 * h, raw);
+          tmem_loaded(raw);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int g = 2 * h + (c >> 4), t = 32 * h + c;
+            const bool own = real >> (8 * g) & 2;
+            const float ks = own ? own_ks[slot][t] : s.ks[slot][g], lv = own ? own_lv[slot][t] : s.lv[slot][g];
+            v[c] = at + t >= row_end || !(real >> (8 * g) & 1) ? kNone : fmaf(__uint_as_float(raw[c]), row_scale * ks, lv - base);
+          }
+        };
+        float top = kNone;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          terms(h, 0.f);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) top = fmaxf(top, v[c]);
+        }
+        const bool moves = m == kNone ? top > kNone : top - m > kTop;
+        if (__any_sync(kFullWarp, moves)) {
+          const float now = moves ? top - kTop : m, f = moves && m != kNone ? exp2_fast(m - now) : 1.f;
+          m = now;
+          l *= f;
+          if (results) {
+            ok = __all_sync(kFullWarp, turn(s.pv_done, x, done - 1));
+            fence_after();
+            if (ok) follow(f);
+          }
+        }
+        const float base = m == kNone ? 0.f : m;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {                      // P goes over scores that have been read: 16 columns of the first 32 each time
+          terms(h, base);
+          uint32_t p[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const int g = 2 * h + (c >> 4), t = 32 * h + c;
+            const bool own = real >> (8 * g) & 2;
+            const float y = exp2_fast(v[c]), z = exp2_fast(v[c + 1]);
+            l = fmaf(y, own ? own_inv[slot][t] : s.inv[slot][g], fmaf(z, own ? own_inv[slot][t + 1] : s.inv[slot][g], l));
+            p[c >> 1] = pack_half(y, z);
+          }
+          __syncwarp();
+          tmem_store(scores + 16 * h, p);
+          tmem_stored();
+        }
+      };
       for (; u < w.u1 && ok; u += step, n += step) {
         // (the scales were there before the keys, the keys before the scores)
         ok = __all_sync(kFullWarp, turn(s.s_full, x, done));
@@ -688,6 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
         const int at = u * kUnit, slot = n % kScales;
         const uint32_t scores = mine_at + 64 * (done & 1);
         if (warp_has_rows) {
+          do {
           uint32_t raw[2][32];
           tmem_load(scores, raw[0]);
           tmem_load(scores + 32, raw[1]);
@@ -705,6 +772,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
 #pragma unroll
             for (int c = 16 * g; c < 16 * g + 16; c += 2) fma2(v[c], v[c + 1], raw[c >> 5][c & 31], raw[c >> 5][(c & 31) + 1], by[g], add[g]);
           if (at + kUnit > w.least || real != 0x01010101u) {
+            if (kBits == 4 && (real & 0x02020202u)) {      // (asked here, where most units do not come by: before the terms a prompt took 178 us where it takes 176)
+              by_token(scores, slot, real, at);
+              break;
+            }
 #pragma unroll
             for (int c = 0; c < kUnit; ++c)
               if (at + c >= row_end || !(real >> (8 * (c >> 4)) & 1)) v[c] = kNone;
@@ -760,6 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
             store();
           }
           tmem_stored();
+          } while (false);
         }
         fence_before();
         bar_arrive(smem_u32(&s.p_full[2 * x + (done & 1)]));

@@ -226,9 +226,9 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     rows, elements of a query below 2^-9 (fp16: 2^-6) of its largest are held to 2^-17 of the largest.  Scales of the values of one request and head
     that lie 2^110 or more apart lose the probabilities under the smaller ones.
 
-    Over a cache of 4 bits it is the scale of the value (where a request adds many rows, the largest of 16 neighbours), and fp16 holds 2^-11 down to
-    2^-18 of the row's largest (12 nats), below by up to 2^-29 of that; queries are held to 28 binades, and keys and values exactly (many rows: to 2^-25 of the
-    largest scale of 16 neighbours).
+    Over a cache of 4 bits it is the scale of the value (where a request adds many rows, the largest of 16 neighbours, seen or not, as far as it lies less than 2^5
+    above), and fp16 holds 2^-11 down to 2^-18 of the row's largest (12 nats), below by up to 2^-29 of that; queries are held to 28 binades, and keys and values exactly.
+    Many rows take up to about twice as long over neighbours whose scales differ by more (keys: 2^13).
 
     Many rows a request are fast for up to 1024 requests and 256 query heads per key/value head; beyond, 16 rows at a time go over the cache."""
     what = "attention"

@@ -452,6 +452,65 @@ def test_a_nan_reaches_only_those_that_see_it(adds, wide, value):
     assert torch.equal(got.isnan(), hit) and torch.equal(got[~hit], want[~hit])
 
 
+def attend_by_scales(q, starts, seen, tables, cache, scale, wide):
+    """As attend_exactly, with the bound of either kernel from what a row sees alone: half a step of fp16, 2^-25, for each code under a probability times the scale of
+    its value, of which the row's largest lies at 2^4 or more: 2^-29 of that; where there are many rows (`wide`), the scale is one that lies less than 2^5 higher."""
+    want, mass, floor = (torch.zeros(q.shape, dtype=torch.double, device=DEV) for _ in range(3))
+    hq, hkv, D = q.shape[1], cache.k.shape[1], q.shape[2]
+    for r in range(seen.numel()):
+        s, e, n = int(starts[r]), int(starts[r + 1]), int(seen[r])
+        ids = tables[r, :-(-n // cache.k.shape[2])].long()
+        hide = torch.arange(n, device=DEV)[None] > torch.arange(n - (e - s), n, device=DEV)[:, None]
+        for h in range(hq):
+            g = h * hkv // hq
+            k, v = (values(c[ids, g], f[ids, g]).reshape(-1, D)[:n] for c, f in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+            vs = cache.v_scale[ids, g].reshape(-1)[:n].double()
+            p = (q[s:e, h].double() @ k.T * scale).masked_fill(hide, float("-inf")).softmax(-1)
+            want[s:e, h], mass[s:e, h] = p @ v, p @ v.abs()
+            floor[s:e, h] = 2.0 ** (-24 if wide else -29) * (p * vs).amax(-1, keepdim=True) * ((~hide).double() @ (v / vs[:, None]).abs())
+    return want, mass + 2.0 ** 10 * floor                    # (bound_of takes 2^-10 of it)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,adds,wide", ((128, (3, 1), False), (64, (9, 2), False), (128, (100, 1), True), (64, (95, 33), True), (128, (30, 1), True)))
+@pytest.mark.parametrize("above", (6, 12, 20, 30, 119))
+@pytest.mark.parametrize("value", (False, True))
+def test_tokens_that_a_row_does_not_see_do_not_reach_it(dtype, D, adds, wide, above, value):
+    """The scale of a later token's key or value lies far above those of its neighbours: rows that do not see it stay within the bound of what they see."""
+    from htr_b200 import paged
+
+    q, starts, seen, tables, cache = filled(dtype, D, 16, 8, 2, (40, 17), adds)
+    at, n = 40 + adds[0] - 2, adds[0] - 2                        # the last token but one of request 0; rows before it
+    (cache.v_scale if value else cache.k_scale)[int(tables[0, at // 16]), :, at % 16] = 2.0 ** above
+    want, spread = attend_by_scales(q, starts, seen, tables, cache, D ** -0.5, wide)
+    q2, tables2, most = many(q, tables, cache) if wide else (q, tables, max(adds))
+    got = paged.attention(q2, starts, seen, tables2, cache, most)
+    for rows in (slice(0, n), slice(int(starts[1]), int(starts[2]))):
+        off, bound = (got[rows].double() - want[rows]).abs(), bound_of(dtype, want, spread)[rows]
+        assert (off <= bound).all(), float((off / bound).max())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,adds,wide", ((128, (2, 1), False), (64, (60, 1), True), (128, (100, 7), True)))
+@pytest.mark.parametrize("above", (8, 14, 18, 25, 60))
+def test_keys_beside_much_larger_ones(dtype, D, adds, wide, above):
+    """Each seventh key is many times its neighbours, in two dimensions in which the queries have nothing: what the neighbours' scores are does not change."""
+    from htr_b200 import paged
+
+    q, starts, seen, tables, cache = filled(dtype, D, 32, 8, 2, (300, 33), adds)
+    q[..., 6:8] = 0
+    cache.k[:, :, 3::7] = 0
+    cache.k[:, :, 3::7, 3] = 0x77
+    cache.k_scale[:, :, 3::7] = 2.0 ** above
+    want, spread = attend_by_scales(q, starts, seen, tables, cache, D ** -0.5, wide)
+    q2, tables2, most = many(q, tables, cache) if wide else (q, tables, max(adds))
+    got, n = paged.attention(q2, starts, seen, tables2, cache, most), q.shape[0]
+    off, bound = (got[:n].double() - want).abs(), bound_of(dtype, want, spread)
+    assert (off <= bound).all(), float((off / bound).max())
+
+
 @gpu
 @pytest.mark.parametrize("adds,wide", (((1, 1), False), ((60, 1), False), ((60, 1), True)))
 @pytest.mark.parametrize("page", (16, 64))
