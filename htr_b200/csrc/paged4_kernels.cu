@@ -16,6 +16,9 @@ namespace {
 
 using namespace htr;
 
+// Elements are rotated as 1 / 16 of what they are or less, and transformed as 1 / (16 D): a row of finite ones then stays finite under angles whose magnitude is up to 8 (a pair
+// adds up to at most sqrt 2 times its length, which is sqrt 2 times the larger element, and D / 2 pairs to at most D times the largest).
+constexpr float kDown = 0.0625f;                           // (besides 1 / D; of many tokens the angles are multiplied: 0.9 us of the 31 below)
 constexpr float kScaleLeast = 7.888609052210118e-31f, kScaleMost = 6.646139978924579e35f;          // 2^-100, 2^119
 
 __device__ __forceinline__ void pdl_enter() {
@@ -276,6 +279,8 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
       float v[8];
       widen<T>(raw[i], v);
       if (h < a.q_heads + a.kv_heads) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= kDown / D;
         if constexpr (kHalves) {
           const int other = lane + (turned ? first ? a.half / 8 : -a.half / 8 : 0);
           const float sign = first ? -1.f : 1.f;
@@ -292,13 +297,10 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const Appe
             v[2 * j + 1] = x * sn[j] + y * cs[j];
           }
         }
-        // (so that no finite ones add up to an infinity on the way)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= 1.f / D;
         hadamard<D>(v, lane);
-        const float by = h < a.q_heads ? 8.f : D / 8.f;
+        const float by = (h < a.q_heads ? 8.f : D / 8.f) / kDown;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (v[j] + (v[j] - v[j])) * by;        // (an infinity, which only an infinite element can have made, becomes NaN)
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] + (v[j] - v[j])) * by;        // (an infinity here, which only an infinite element or angle can have made, becomes NaN)
       }
       if (h < a.q_heads) {
         uint4 r = {Half<T>::narrow(v[0], v[1]), Half<T>::narrow(v[2], v[3]), Half<T>::narrow(v[4], v[5]), Half<T>::narrow(v[6], v[7])};
@@ -372,6 +374,13 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
       }
     }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (h0 < a.q_heads + a.kv_heads)                         // angles times kDown, by the threads that fetched them
+    for (int w = warp; w < n; w += kWarps)
+      for (int i = lane; i < pairs / 2; i += 32) {
+        float4* const at = reinterpret_cast<float4*>((i < pairs / 4 ? cos_s : sin_s - pairs) + w * kAngles + 4 * i);
+        const float4 f = *at;
+        *at = make_float4(f.x * kDown, f.y * kDown, f.z * kDown, f.w * kDown);
+      }
   __syncthreads();
   for (int h = h0 + warp; h < h0 + heads; h += kWarps) {
     const bool turns = h < a.q_heads + a.kv_heads, query = h < a.q_heads;
@@ -385,8 +394,8 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
     }
     float v[8][kTiles][4];                                 // of dimension b of chunk 2 t + i % 2, row g + 8 (i / 2)
     if (turns) {
-      // queries times 8 / D, and keys times 1 / D, which their scale makes up for: so no finite ones add up to an infinity on the way
-      const Turn<D> turn(false, true, query, (D == 128 ? 0x3C003C00u : 0x3C803C80u) + (query ? 0x01800180u : 0), lane);
+      // times 1 / D, which with kDown of the angles the scale of keys makes up for; queries times 8 / D / kDown
+      const Turn<D> turn(false, true, query, (D == 128 ? 0x3C003C00u : 0x3C803C80u) + (query ? 0x03800380u : 0), lane);
 #pragma unroll
       for (int b = 0; b < 8; ++b)
 #pragma unroll
@@ -401,7 +410,11 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
           for (int e = 0; e < 2; ++e) {
             const int at = 8 * chunk_of(true, kChunks<D>, c, 2 * p + e);
             widen<T>(*reinterpret_cast<const uint4*>(row[r] + 2 * at), x[r][e]);
-            if (!kFull && at >= 2 * pairs) continue;
+            if (!kFull && at >= 2 * pairs) {
+#pragma unroll
+              for (int b = 0; b < 8; ++b) x[r][e][b] *= kDown;
+              continue;
+            }
             if constexpr (kHalves) {
               const bool first = kFull ? 2 * p + e < kChunks<D> / 2 : at < pairs;
               const int other = first ? at + pairs : at - pairs, angle = first ? at : other;
@@ -471,7 +484,7 @@ __global__ void __launch_bounds__(kRowsThreads, 4) rope_append4_rows_kernel(cons
         for (int y = 0; y < kChunks<D>; ++y) most = max_nan(most, v[b][y >> 1][2 * r + (y & 1)]);
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) most = max_nan(most, __shfl_xor_sync(kFullWarp, most, o));
-      const float by = turns ? D / 8.f : 1.f;
+      const float by = turns ? D / 8.f / kDown : 1.f;
       const Scale scale(most, by);
       if (scale.beyond(most, by))
 #pragma unroll

@@ -340,7 +340,7 @@ int htr_paged_last_cuda_error(void);
  * htr_paged4_append: as htr_paged_append, into such a cache.  The first rotary_dim dimensions of a head (a multiple of 16) are rotated, angles cosv / sinv
  * [angle_rows][rotary_dim / 2]; pairs are neighbours, or where `halves` is set dimensions i and i + rotary_dim / 2.  A token's scale is that of its largest
  * element, bf16(largest / 6), its codes are the nearest, ties to the even code; infinities of values become the largest value, and with a NaN the whole row of a head
- * is NaN, as is one of queries or keys with an infinity.  A token with slot -1 is not written and its q row is zero; so is one whose slot or position lies outside, or whose slot does not lie above those of
+ * is NaN, as is one of queries or keys with an infinity (finite keys stay so under angles of a magnitude up to 8).  A token with slot -1 is not written and its q row is zero; so is one whose slot or position lies outside, or whose slot does not lie above those of
  * its page among the page_size - 1 tokens before it (status 16).  Tokens of one page lie within page_size tokens, as htr_page_plan lays them out.
  * htr_paged4_unpack: the pages ids[count] as values [count][kv_heads][page_size][head_dim] of any HTR_DTYPE_*, keys turned back; a page that is none: zeros.
  * htr_paged4_attention: as htr_paged_attention, with queries as htr_paged4_append gives them. */

@@ -208,6 +208,38 @@ def test_an_infinity_among_what_is_transformed_takes_its_row(dtype, layout, more
 
 
 @gpu
+@pytest.mark.parametrize("layout", ("interleaved", "half"))
+@pytest.mark.parametrize("more", (0, MANY // 3))
+@pytest.mark.parametrize("D,r", ((64, 64), (128, 128), (128, 48)))
+@pytest.mark.parametrize("size", (0.5 ** 0.5, 5.0))
+def test_finite_pairs_whose_rotation_leaves_float32(layout, more, D, r, size):
+    """Two elements of 3e38 that turn by 45 degrees make one of 4e38 (and more under angles with a magnitude): rows of keys stay finite, at most 6 * 2^119, and
+    so do queries that come back within bf16."""
+    from htr_b200 import paged
+
+    cache = empty_cache(1, 1, 16, D)
+    cos = torch.full((1, r // 2), size, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(D + r)
+    x = torch.randn(6, 3 * D, device=DEV, generator=g)
+    i, j = (4, 5) if layout == "interleaved" else (4, 4 + r // 2)
+    x[0, i] = x[0, j] = 1e38                                     # of a query
+    x[1, i], x[1, j] = -1e38, 1e38
+    x[2, D + i] = x[2, D + j] = 3e38                             # of a key
+    x[3, D:2 * D] = x[3, D:2 * D].sign() * 3e38
+    x[4, D:2 * D] = 3e38
+    x[5, D + i] = x[5, D + j] = 2e36
+    x = torch.cat([x, x[:1].expand(more, -1)]).bfloat16()
+    q = paged.rope_append(x, ints([0] * (6 + more)), ints([*range(6)] + [-1] * more), cos, cos.clone(), cache, 1, layout=layout)[:6]
+    y = x[:6].double().view(6, 3, D)
+    z = rotated(y[:, :2], cos.double().expand(6, -1), cos.double().expand(6, -1), layout) @ sylvester(D)
+    # as in check_append, but that a pair grows by up to sqrt 2 times size
+    noise = ((3 + math.log2(D)) * 2.0 ** -24 + (2.0 ** -19 if (6 + more) * 3 >= MANY else 0)) * 2 ** 0.5 * max(size, 1.0) * y[:, :2].abs().sum(-1)
+    want = z[:, 0] * 8 / D
+    assert ((q[:, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() + noise[:, :1] * 8 / D * 1.01).all()
+    check_rows(cache.k[0, :, :6].transpose(0, 1), cache.k_scale[0, :, :6].transpose(0, 1), (z[:, 1:] / 8).clamp(-6 * 2.0 ** 119, 6 * 2.0 ** 119), noise[:, 1:] / 8)
+
+
+@gpu
 @pytest.mark.parametrize("page", (16, 64, 128))
 @pytest.mark.parametrize("D,hkv", ((128, 1), (64, 3), (64, 40), (128, 30)))
 def test_every_place_has_one_writer(page, D, hkv):
