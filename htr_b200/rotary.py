@@ -9,10 +9,12 @@ def angles(rows, dim, theta=1.0e6, first=0, factor=1.0, original=None, low=1.0, 
 
     Pair i turns by theta^(-2 i / dim) a position.  For contexts longer than a model has learned, `factor` slows the pairs down: all of them, or where
     `original` (the positions that it learned) is given, those that turn at most `low` times within it by the whole factor, those that turn `high` times and more not at
-    all, and between them by a share that lies linearly in their turns.  Cosines and sines are multiplied by `magnitude` (it sharpens the scores by its
+    all, and between them by a share that lies linearly in their turns (not in the pair's index between two rounded borders, as some models have it: between the borders those have
+    other frequencies).  Cosines and sines are multiplied by `magnitude` (it sharpens the scores by its
     square, as far as the rotated part of a head goes).
 
-    Angles are taken in 64 bits; the result is off by some 2^-23 of magnitude."""
+    Angles are taken in 64 bits.  A result is off by at most 7 * 2^-24 of magnitude, and by what the roundings of the frequency and the angle make, 2^-51 of the angle.  Tables of many rows
+    (64 a multiprocessor and more) are products of two angles' cosines and sines, in float32: the last bits of a position depend on which table it stands in."""
     both = _lib.host.rope_angles(rows, dim, theta, first, factor, original, low, high, magnitude, device)    # the usual case; None: whatever it does not take
     if both is not None:
         return both
