@@ -18,8 +18,7 @@ using namespace htr;
 
 // Elements are rotated as 1 / 16 of what they are or less, and transformed as 1 / (16 D): a row of finite ones then stays finite under angles whose magnitude is up to 8 (a pair
 // adds up to at most sqrt 2 times its length, which is sqrt 2 times the larger element, and D / 2 pairs to at most D times the largest).
-constexpr float kDown = 0.0625f;                           // (besides 1 / D; of many tokens the angles are multiplied: 0.9 us of the 31 below)
-constexpr float kScaleLeast = 7.888609052210118e-31f, kScaleMost = 6.646139978924579e35f;          // 2^-100, 2^119
+constexpr float kDown = 0.0625f;                           // (besides 1 / D; of many tokens the angles are multiplied: 1 us of the 33 below)
 
 __device__ __forceinline__ void pdl_enter() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -197,12 +196,14 @@ struct AppendArgs {
   uint8_t *k_cache, *v_cache;
   uint16_t *k_scale, *v_scale;
   long long slots_total;
-  int shift, window;
+  int shift;
   void* q_out;
   int* status;
 };
 
-constexpr int kAppendThreads = 256, kMaxWindow = 64, kMaxPage = 128;
+constexpr int kAppendThreads = 256, kMaxPage = 128;
+template <int D>
+constexpr int kAppendTokens = kAppendThreads / (D / 8);    // of a thread block
 
 // Which of the tokens t0 ... t0 + n - 1 are written: s_slot their slots (from place `page` on, and of a page before them; -1: not valid), s_bad 0 for those that are
 // written, 2 for those that are not although their slot is not -1.  By all threads, which are in step after it.
@@ -236,106 +237,97 @@ __device__ __forceinline__ void find_written(const AppendArgs& a, int t0, int n,
       if (s_bad[i] == 2) atomicOr(a.status, 16);
 }
 
-// grid (windows of tokens, groups of kHeads heads of queries, keys and values as they stand in a row).  A thread holds 8 dimensions of a row, four pairs
+// grid (kAppendTokens tokens each, heads of queries, keys and values as they stand in a row).  A thread holds 8 dimensions of a row, four pairs
 // of neighbours; in halves a pair's other element comes from another lane.
 // A token whose slot does not lie above those of its page in the page - 1 tokens before it is not written: every place has one writer, where the tokens of a
 // page lie within so many.
-// Bound by latency: slots -> rows and angles -> sums over lanes.  8 tokens of 32 heads of 128 on 8 in a chain of launches: 2.6 us.
-template <typename T, int D, int kHeads, bool kHalves>
+// Bound by latency: slots -> rows and angles -> sums over lanes.  8 tokens of 32 heads of 128 on 8 in a chain of launches: 2.5 us.
+template <typename T, int D, bool kHalves>
 __global__ void __launch_bounds__(kAppendThreads) rope_append4_kernel(const AppendArgs a) {
-  constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes;
-  __shared__ int s_slot[kMaxWindow + kMaxPage], s_pos[kMaxWindow];
-  __shared__ int s_bad[kMaxWindow];
+  constexpr int kLanes = D / 8, kTokens = kAppendTokens<D>;
+  __shared__ int s_slot[kTokens + kMaxPage], s_pos[kTokens], s_bad[kTokens];
   pdl_enter();
   const int tid = threadIdx.x, lane = tid % kLanes, row = tid / kLanes, page = 1 << a.shift;
-  const int t0 = blockIdx.x * a.window, n = min(a.window, a.tokens - t0), h0 = blockIdx.y * kHeads;
-  const T* qkv = static_cast<const T*>(a.qkv);
+  const int t0 = blockIdx.x * kTokens, n = min(kTokens, a.tokens - t0), h = blockIdx.y;
   find_written<kAppendThreads>(a, t0, n, s_slot, s_pos, s_bad);
   const bool first = 8 * lane < a.half, turned = 8 * lane < 2 * a.half;          // (halves) this lane's are the first of their pairs; they are rotated
-  for (int w0 = 0; w0 < n; w0 += kRows) {
-    const int w = min(w0 + row, n - 1), slot = s_slot[page + w];
-    const bool mine = w0 + row < n, ok = s_bad[w] == 0;
-    const size_t t = t0 + w;
-    uint4 raw[kHeads];
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i)
-      if (h0 + i < a.q_heads + 2 * a.kv_heads) raw[i] = *reinterpret_cast<const uint4*>(qkv + t * a.row_stride + (size_t)(h0 + i) * D + lane * 8);
+  const int w = min(row, n - 1), slot = s_slot[page + w];
+  const bool mine = row < n, ok = s_bad[w] == 0;
+  const size_t t = t0 + w;
+  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.qkv) + t * a.row_stride + (size_t)h * D + lane * 8);
+  float v[8];
+  if (h < a.q_heads + a.kv_heads) {
     constexpr int kAngles = kHalves ? 8 : 4;
     float cs[kAngles], sn[kAngles];
-    if (h0 < a.q_heads + a.kv_heads) {
-      const int from = !turned ? 0 : kHalves ? 8 * lane - (first ? 0 : a.half) : 4 * lane;
-      const size_t at = (ok ? (size_t)s_pos[w] * a.half : 0) + from;
+    const int from = !turned ? 0 : kHalves ? 8 * lane - (first ? 0 : a.half) : 4 * lane;
+    const size_t at = (ok ? (size_t)s_pos[w] * a.half : 0) + from;
 #pragma unroll
-      for (int j = 0; j < kAngles; j += 4) {
-        const float4 c = *reinterpret_cast<const float4*>(a.cosv + at + j), s = *reinterpret_cast<const float4*>(a.sinv + at + j);
-        cs[j] = c.x; cs[j + 1] = c.y; cs[j + 2] = c.z; cs[j + 3] = c.w;
-        sn[j] = s.x; sn[j + 1] = s.y; sn[j + 2] = s.z; sn[j + 3] = s.w;
+    for (int j = 0; j < kAngles; j += 4) {
+      const float4 c = *reinterpret_cast<const float4*>(a.cosv + at + j), s = *reinterpret_cast<const float4*>(a.sinv + at + j);
+      cs[j] = c.x; cs[j + 1] = c.y; cs[j + 2] = c.z; cs[j + 3] = c.w;
+      sn[j] = s.x; sn[j + 1] = s.y; sn[j + 2] = s.z; sn[j + 3] = s.w;
+    }
+    widen<T>(raw, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= kDown / D;
+    if constexpr (kHalves) {
+      const int other = lane + (turned ? first ? a.half / 8 : -a.half / 8 : 0);
+      const float sign = first ? -1.f : 1.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float p = __shfl_sync(kFullWarp, v[j], other, kLanes);
+        if (turned) v[j] = v[j] * cs[j] + sign * p * sn[j];
+      }
+    } else if (turned) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = v[2 * j], y = v[2 * j + 1];
+        v[2 * j] = x * cs[j] - y * sn[j];
+        v[2 * j + 1] = x * sn[j] + y * cs[j];
       }
     }
+    hadamard<D>(v, lane);
+    const float by = (h < a.q_heads ? 8.f : D / 8.f) / kDown;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int h = h0 + i;
-      if (h >= a.q_heads + 2 * a.kv_heads) break;
-      float v[8];
-      widen<T>(raw[i], v);
-      if (h < a.q_heads + a.kv_heads) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= kDown / D;
-        if constexpr (kHalves) {
-          const int other = lane + (turned ? first ? a.half / 8 : -a.half / 8 : 0);
-          const float sign = first ? -1.f : 1.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float p = __shfl_sync(kFullWarp, v[j], other, kLanes);
-            if (turned) v[j] = v[j] * cs[j] + sign * p * sn[j];
-          }
-        } else if (turned) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = v[2 * j], y = v[2 * j + 1];
-            v[2 * j] = x * cs[j] - y * sn[j];
-            v[2 * j + 1] = x * sn[j] + y * cs[j];
-          }
-        }
-        hadamard<D>(v, lane);
-        const float by = (h < a.q_heads ? 8.f : D / 8.f) / kDown;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (v[j] + (v[j] - v[j])) * by;        // (an infinity here, which only an infinite element or angle can have made, becomes NaN)
-      }
-      if (h < a.q_heads) {
-        uint4 r = {Half<T>::narrow(v[0], v[1]), Half<T>::narrow(v[2], v[3]), Half<T>::narrow(v[4], v[5]), Half<T>::narrow(v[6], v[7])};
-        if (!ok) r = {0, 0, 0, 0};
-        if (mine) *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (t * a.q_heads + h) * D + lane * 8) = r;
-        continue;
-      }
-      float most = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max_nan(most, v[j]);
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) most = max_nan(most, __shfl_xor_sync(kFullWarp, most, o));
-      const Scale scale(most);                             // (a row with a NaN: so are all of its values, by their scale)
-      if (scale.beyond(most))
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = scale.within(v[j]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = scale(v[j]);
-      if (!mine || !ok) continue;
-      const bool values = h >= a.q_heads + a.kv_heads;
-      const int head = h - a.q_heads - (values ? a.kv_heads : 0);
-      const size_t place = (((size_t)(slot >> a.shift) * a.kv_heads + head) << a.shift) + (slot & (page - 1));
-      *reinterpret_cast<uint32_t*>((values ? a.v_cache : a.k_cache) + place * (D / 2) + lane * 4) = to_e2m1(v);
-      if (lane == 0) (values ? a.v_scale : a.k_scale)[place] = (uint16_t)(__float_as_uint(scale.s) >> 16);
-    }
+    for (int j = 0; j < 8; ++j) v[j] = (v[j] + (v[j] - v[j])) * by;            // (an infinity here, which only an infinite element or angle can have made, becomes NaN)
+  } else {
+    widen<T>(raw, v);
   }
+  if (h < a.q_heads) {
+    uint4 r = {Half<T>::narrow(v[0], v[1]), Half<T>::narrow(v[2], v[3]), Half<T>::narrow(v[4], v[5]), Half<T>::narrow(v[6], v[7])};
+    if (!ok) r = {0, 0, 0, 0};
+    if (mine) *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (t * a.q_heads + h) * D + lane * 8) = r;
+    return;
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = max_nan(most, v[j]);
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) most = max_nan(most, __shfl_xor_sync(kFullWarp, most, o));
+  const Scale scale(most);                                 // (a row with a NaN: so are all of its values, by their scale)
+  if (scale.beyond(most))
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = scale.within(v[j]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = scale(v[j]);
+  if (!mine || !ok) return;
+  const bool values = h >= a.q_heads + a.kv_heads;
+  const int head = h - a.q_heads - (values ? a.kv_heads : 0);
+  const size_t place = (((size_t)(slot >> a.shift) * a.kv_heads + head) << a.shift) + (slot & (page - 1));
+  *reinterpret_cast<uint32_t*>((values ? a.v_cache : a.k_cache) + place * (D / 2) + lane * 4) = to_e2m1(v);
+  if (lane == 0) (values ? a.v_scale : a.k_scale)[place] = (uint16_t)(__float_as_uint(scale.s) >> 16);
 }
 
 // The same for many tokens: a warp takes 16 of them at a time, one head after the other, and transforms by matrix products.  The rotated elements enter as two
-// tf32 each, which leave 2^-20 of an element at most.  (Two bf16, 2^-16, in half of the products took 28 us where this takes 30, but a code that lies next to a tie then comes
+// tf32 each, which leave 2^-20 of an element at most.  (Two bf16, 2^-16, in half of the products took 28 us where this then took 30, but a code that lies next to a tie then comes
 // out as its neighbour often enough to show: 5e-4 of the norm of fp16 keys, whose own rounding is 2e-4.)
 // An infinity among a row's elements makes all of the row NaN.
-// Sums over lanes, four shuffles an element, were what bound the form above here: 65 us for 4096 tokens of 32 heads of 128 on 8 (94 MB) in a chain of launches.  With products
+// Sums over lanes, four shuffles an element, were what bound the form above here, then 65 us (now 53) for 4096 tokens of 32 heads of 128 on 8 (94 MB) in a chain of launches.  With products
 // from registers 44, from shared memory, where all heads of 16 tokens are on their way at once, 33, and 28 with what a lane's chunks are known beforehand.
-// What bounds it now (3.0 TB/s): some 1200 instructions for 16 rows, at half of the issue slots.  The two forms are level at some 600 tokens of 48 heads (9.6 and 9.7 us; 1024: 17.2 and 11.5).
+// Now 33 in either layout (2.9 TB/s; with the tf32 parts and the range of finite pairs).  What bounds it: some 1200 instructions for 16 rows, at half of the issue slots.  Of 128
+// dimensions it holds 128 registers and spills 64 to 116 bytes a thread (halves, whole heads of bf16: 64 stored, 88 loaded; interleaved parts of heads: 4); of 64 none.
+// The two forms are about level at 32768 rows, for heads of either size.  us, few / many, a launch of another kernel between two: 700 tokens of 48 heads of 128 11.7 / 10.6, 900 14.2 / 12.9, 500 of
+// 80 13.6 / 12.9; 700 of 48 of 64 8.4 / 7.6.  In a chain of its own: 600 of 48 of 128 9.5 / 12.4, 900 13.1 / 13.4, 1200 16.5 / 13.3; of 64 700 7.2 / 7.9, 1200 11.0 / 8.6.
 constexpr int kRowsThreads = 128, kRowsTokens = 16, kRowsHeads = 8, kManyRows = 32768;
 
 // rows of tokens in shared memory, so far apart that lanes of two neighbouring tokens read different banks: elements, 64 bytes a piece; angles, 64 or (halves) 16 of 32
@@ -733,12 +725,6 @@ struct Running : Results<D, NT> {
 #pragma unroll
       for (int w = 0; w < D / 64; ++w) {
         // bytes of two tokens' codes of one dimension: even ones, odd ones
-        constexpr uint32_t kLow = 0x0F0F0F0Fu;
-        const auto low_of = [&](uint32_t x, uint32_t y) {   // the low halves of the bytes of x, the high ones of y
-          uint32_t r;
-          asm("lop3.b32 %0, %1, %2, %3, 0xE4;" : "=r"(r) : "r"(x), "r"(y), "n"(kLow));
-          return r;
-        };
         const auto even = [&](int x) { return low_of(v[x][w], v[x + 1][w] << 4); };
         const auto odd = [&](int x) { return low_of(v[x][w] >> 4, v[x + 1][w]); };
         uint32_t a0[4], a1[4], a2[4], a3[4];
@@ -912,17 +898,16 @@ int append_rows(const AppendArgs& a, dim3 grid, cudaStream_t st) {
 }
 
 template <typename T, int D>
-int append_of(AppendArgs a, bool halves, cudaStream_t st) {
+int append_of(const AppendArgs& a, bool halves, cudaStream_t st) {
   const int heads = a.q_heads + 2 * a.kv_heads;
   if ((int64_t)a.tokens * heads >= kManyRows) {
     const dim3 grid((a.tokens + kRowsTokens - 1) / kRowsTokens, (heads + kRowsHeads - 1) / kRowsHeads);
     if (2 * a.half == D) return halves ? append_rows<T, D, true, true>(a, grid, st) : append_rows<T, D, false, true>(a, grid, st);
     return halves ? append_rows<T, D, true, false>(a, grid, st) : append_rows<T, D, false, false>(a, grid, st);
   }
-  a.window = kAppendThreads / (D / 8);                     // what its rows hold at a time
-  const dim3 grid((a.tokens + a.window - 1) / a.window, heads);
-  return halves ? paged_launch(rope_append4_kernel<T, D, 1, true>, grid, dim3(kAppendThreads), 1, 0, st, a)
-                : paged_launch(rope_append4_kernel<T, D, 1, false>, grid, dim3(kAppendThreads), 1, 0, st, a);
+  const dim3 grid((a.tokens + kAppendTokens<D> - 1) / kAppendTokens<D>, heads);
+  return halves ? paged_launch(rope_append4_kernel<T, D, true>, grid, dim3(kAppendThreads), 1, 0, st, a)
+                : paged_launch(rope_append4_kernel<T, D, false>, grid, dim3(kAppendThreads), 1, 0, st, a);
 }
 
 template <typename T>
@@ -956,7 +941,7 @@ int htr_paged4_append(const void* qkv, int dtype, int64_t row_stride, const int*
       !aligned16(q_out))
     return HTR_ERR_ALIGNMENT;
   const AppendArgs a = {qkv, row_stride, positions, slots, tokens, cosv, sinv, angle_rows, rotary_dim / 2, q_heads, kv_heads, static_cast<uint8_t*>(k_cache),
-                        static_cast<uint8_t*>(v_cache), static_cast<uint16_t*>(k_scale), static_cast<uint16_t*>(v_scale), (int64_t)pages << shift, shift, 0, q_out, status};
+                        static_cast<uint8_t*>(v_cache), static_cast<uint16_t*>(k_scale), static_cast<uint16_t*>(v_scale), (int64_t)pages << shift, shift, q_out, status};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == HTR_DTYPE_BF16) return head_dim == 128 ? append_of<__nv_bfloat16, 128>(a, halves != 0, st) : append_of<__nv_bfloat16, 64>(a, halves != 0, st);
   return head_dim == 128 ? append_of<__half, 128>(a, halves != 0, st) : append_of<__half, 64>(a, halves != 0, st);

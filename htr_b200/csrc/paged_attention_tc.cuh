@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const A
     constexpr int kFeeders = 7, kPer = D == 128 ? 8 : 16, kPasses = 16 / kPer;           // a lane has 32 dimensions of every kPer-th token
     const int me = warp == 15 ? 6 : warp - 8, place_mask = (1 << a.shift) - 1, in_pass = lane % kPer, piece = lane / kPer;
     const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
-    const auto held = [&](float s) { return fminf(fmaxf(s, 7.888609052210118e-31f), 6.646139978924579e35f); };           // 2^-100 to 2^119 (NaN: 2^-100)
+    const auto held = [&](float s) { return fminf(fmaxf(s, kScaleLeast), kScaleMost); };         // (NaN: kScaleLeast)
     const uint32_t pieces = 8 * (uint32_t)count;
     bool ok = true, bad = false;
     struct Piece {

@@ -64,6 +64,7 @@ __device__ __forceinline__ uint32_t from_e4m3(uint32_t two) {   // two e4m3 in t
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
   return r;
 }
+constexpr float kScaleLeast = 7.888609052210118e-31f, kScaleMost = 6.646139978924579e35f;          // of codes of 4 bits: 2^-100, 2^119
 // a byte's two codes as fp16, each of the four
 __device__ __forceinline__ void from_e2m1(uint32_t w, uint32_t (&r)[4]) {
   asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"

@@ -168,7 +168,8 @@ def rope_append(qkv, positions, slots, cos, sin, cache, q_heads, status=None, la
 
     4 bits: pairs may also be halves (layout "half": dimensions i and i + r / 2), and r, twice the columns of cos and sin, a part of the
     head that is a multiple of 16: the first r dimensions are rotated.  The queries come back as H q * 8 / head_dim for the keys of such a cache (see
-    LayerCache4; fp16 ones whose sums leave its range become infinite, and rows of bf16 ones beyond 2^124 may become infinite or NaN).  A token's scale is bf16(largest / 6), its codes are the
+    LayerCache4; sums are float32, and where tokens times heads reach 32768, of elements that are cut at 2^-20 of what they are: the code of an element beside a tie may depend
+    on how many tokens the step has; fp16 ones whose sums leave its range become infinite, and rows of bf16 ones beyond 2^124 may become infinite or NaN).  A token's scale is bf16(largest / 6), its codes are the
     nearest, ties to the even code.  Infinities among values are held as the largest value, 6 * 2^119, as is all that lies beyond it; a row of a head that has a NaN is
     NaN as a whole, and so is one of queries or keys that has an infinity; finite keys stay so under cosines and sines of a magnitude up to 8."""
     what = "rope_append"
