@@ -36,9 +36,9 @@
 // with such tokens takes some two times as long: the prompt above 384 us where every unit has one, 180 where one page in 64 has; and that they are looked for costs it 3 us of 176.
 // Seven warps (8-13, 15) feed both, 16 tokens at a time, by code that stands once and is not unrolled: twice and unrolled it drove the softmax out of the instruction cache
 // (339 us where this took 208).  The reference lies 2^4 under the largest term when it moves, and then for all rows of the warp whose largest lies higher: terms down to 2^-18 of the
-// largest keep all bits, smaller ones are off by up to 2^-29 of it.  Keys whose norms differ by token make references move, a move costs 3000 cycles, and with 2^12 every second unit of the
+// largest keep all bits, smaller ones are off by up to 2^-29 of it.  Keys whose norms differ by token make references move, a move costs 1900 cycles, and with 2^12 every second unit of the
 // prompt above had one: 200 us, with 2^8 183, with 2^4 172 (2^0: 169; none: 146).  P goes to tensor memory before the
-// sums are looked at, and once more where a reference moves: 171.  Two threads a row (16 softmax warps of 88 registers) took 186, a thread for each kind of product 191.
+// sums are looked at, and once more where a reference moves: 171 (these without scales of tokens, with which it is 176).  Two threads a row (16 softmax warps of 88 registers) took 186, a thread for each kind of product 191.
 #pragma once
 #include <type_traits>
 

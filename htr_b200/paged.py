@@ -231,7 +231,8 @@ def attention(q, starts, seen, tables, cache, max_new, scale=None, out=None, sta
     above), and fp16 holds 2^-11 down to 2^-18 of the row's largest (12 nats), below by up to 2^-29 of that; queries are held to 28 binades, and keys and values exactly.
     Many rows take up to about twice as long over neighbours whose scales differ by more (keys: 2^13).
 
-    Many rows a request are fast for up to 1024 requests and 256 query heads per key/value head; beyond, 16 rows at a time go over the cache."""
+    Many rows a request are fast for up to 1024 requests and 256 query heads per key/value head; beyond, 16 rows at a time go over the cache.  Which kernel serves goes by max_new and
+    the tables' width for all requests of a call: a piece of a prompt and many single tokens are faster in calls of their own."""
     what = "attention"
     y = _host.attention(q, starts, seen, tables, cache, max_new, scale, out, status)
     if y is not None:

@@ -13,7 +13,7 @@ def angles(rows, dim, theta=1.0e6, first=0, factor=1.0, original=None, low=1.0, 
     other frequencies).  Cosines and sines are multiplied by `magnitude` (it sharpens the scores by its
     square, as far as the rotated part of a head goes).
 
-    Angles are taken in 64 bits.  A result is off by at most 7 * 2^-24 of magnitude, and by what the roundings of the frequency and the angle make, 2^-51 of the angle.  Tables of many rows
+    Angles are taken in 64 bits.  A result is off by at most 7 * 2^-24 of magnitude, and by what the roundings of the frequency and the angle make, some 2^-51 of the angle.  Tables of many rows
     (64 a multiprocessor and more) are products of two angles' cosines and sines, in float32: the last bits of a position depend on which table it stands in."""
     both = _lib.host.rope_angles(rows, dim, theta, first, factor, original, low, high, magnitude, device)    # the usual case; None: whatever it does not take
     if both is not None:

@@ -357,7 +357,7 @@ int htr_paged4_attention(const void* q, int dtype, int tokens, const int* starts
 /* Angles of the positions first ... first + rows - 1 for a rotary embedding of dim dimensions (even, at most 256): cosv and sinv [rows][dim / 2] = magnitude *
  * cos and sin of position * theta^(-2 i / dim) * slow_i.  slow_i = 1 / factor where original is 0; else it is 1 for pairs that turn at least `high` times within
  * `original` positions, 1 / factor for those that turn at most `low` times, and lies linearly (in turns) between in between.  Positions are below 2^31; the error is
- * at most 7 * 2^-24 of magnitude, and 2^-51 of the angle; from 64 rows a multiprocessor on the last bits of a position depend on the table's first row. */
+ * at most 7 * 2^-24 of magnitude, and some 2^-51 of the angle; from 64 rows a multiprocessor on the last bits of a position depend on the table's first row. */
 int htr_rope_angles(int64_t first, int rows, int dim, double theta, double factor, double original, double low, double high, float magnitude,
                     float* cosv, float* sinv, htr_stream_t stream);
 

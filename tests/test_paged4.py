@@ -651,6 +651,33 @@ def test_lengths_of_all_kinds_in_one_step(D, page, hq, hkv, most, seed):
     check_attention(*filled(torch.bfloat16, D, page, hq, hkv, have, adds, seed=seed), max_new=most)
 
 
+def source(name):
+    import os
+
+    return open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "htr_b200", "csrc", name)).read()
+
+
+def test_sizes_that_the_tests_choose_kernels_by():
+    """MANY and what `many` fills up to are the borders that the sources have."""
+    import re
+
+    assert int(re.search(r"kManyRows = (\d+);", source("paged4_kernels.cu"))[1]) == MANY
+    rule = re.search(r"max_new \* head_dim > (\d+) &&\s*\(double\)tokens \* q_heads \* \(double\)width \* head_dim > ([\d.e]+);", source("paged4_attention_tc.cu"))
+    assert int(rule[1]) == 24576 and float(rule[2]) <= 1.6e9
+
+
+@gpu
+@pytest.mark.parametrize("D,page,adds", ((128, 16, (3, 1)), (64, 64, (100, 1)), (128, 64, (517,)), (64, 16, (1, 1))))
+def test_either_kernel_is_the_one_that_is_meant(D, page, adds):
+    """Their workspaces differ: that of many rows has two parts of 256 rows for each multiprocessor."""
+    from htr_b200 import _lib
+
+    q, starts, seen, tables, cache = filled(torch.bfloat16, D, page, 8, 2, (40, 17)[:len(adds)], adds)
+    sms = torch.cuda.get_device_properties(DEV).multi_processor_count
+    need = lambda q, tables, most: _lib.lib.htr_paged4_attention_workspace_bytes(q.shape[0], seen.numel(), 8, 2, D, most, tables.shape[1], page)
+    assert need(*many(q, tables, cache)) == sms * (2 * 256 * (D + 2) * 4 + 16) != need(q, tables, max(adds))
+
+
 @gpu
 def test_attention_of_many_requests():
     adds = [1] * 1100
