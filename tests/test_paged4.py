@@ -525,6 +525,26 @@ def test_tokens_that_a_row_does_not_see_do_not_reach_it(dtype, D, adds, wide, ab
 
 @gpu
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("D,hq,have,adds", ((128, 8, (3000, 100, 0, 700), (150, 3, 70, 40)), (64, 8, (2000, 33, 5, 900), (130, 300, 1, 64)), (64, 2, (5000, 17), (500, 3))))
+def test_scales_of_all_sizes_over_long_sequences(dtype, D, hq, have, adds):
+    """Scales of 19 binades, so that nearly all groups of 16 keep those of their tokens, by both kernels; parts of cut tiles and twins among them."""
+    from htr_b200 import paged
+
+    q, starts, seen, tables, cache = filled(dtype, D, 32, hq, 2, have, adds, spread=9)
+    scale = 2.0 ** -9 * D ** -0.5                                # (scores as elsewhere: up to about 40 in sum)
+    for wide in (False, True):
+        want, spread = attend_by_scales(q, starts, seen, tables, cache, scale, wide)
+        q2, tables2, most = many(q, tables, cache) if wide else (q, tables, 1 + 16 // (hq // 2))
+        bound = bound_of(dtype, want, spread)
+        for r, n in enumerate(adds if wide else [min(a, most) for a in adds]):
+            rows = slice(int(starts[r]), int(starts[r]) + n)
+            if wide or n == adds[r]:
+                off = (paged.attention(q2, starts, seen, tables2, cache, most, scale=scale)[rows].double() - want[rows]).abs()
+                assert (off <= bound[rows]).all(), (r, float((off / bound[rows]).max()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
 @pytest.mark.parametrize("D,adds,wide", ((128, (2, 1), False), (64, (60, 1), True), (128, (100, 7), True)))
 @pytest.mark.parametrize("above", (8, 14, 18, 25, 60))
 def test_keys_beside_much_larger_ones(dtype, D, adds, wide, above):
